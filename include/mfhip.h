@@ -296,6 +296,149 @@ int mfh_pack_planes(int batch, const float *planes, uint64_t *masks,
 int mfh_debug_quantize_fp8(int rows, int cols, const float *w, uint8_t *codes,
                            float *scale);
 
+/* ---- Learning from the policy ------------------------------------------
+ *
+ * Losses on rows of policy logits with their gradients, and the clipping of a
+ * net's gradients, for programs that train the nets this library evaluates.
+ * No counterpart in the reference.  The logits and move lists are the device
+ * arrays of mfh_net_eval_priors_device.  Every call enqueues kernels on
+ * `stream` (a hipStream_t; NULL is the default stream of the device),
+ * allocates nothing, keeps nothing between calls and copies nothing to the
+ * host, so it can be captured into a HIP graph; only mfh_grad_set_create and
+ * _destroy cannot.  Calls do not order each other: two that share an output
+ * or a workspace are ordered by the caller.  Array arguments are device
+ * memory of one device, in one allocation each; a pointer that is not
+ * (host memory, another device's, another device's stream) is rejected with
+ * MFH_ERR_INVALID.  Offsets, indices and actions are read on the device:
+ * offsets outside their array are clamped to it. */
+
+enum { MFH_DTYPE_F32 = 0, MFH_DTYPE_BF16 = 1, MFH_DTYPE_F16 = 2 };
+
+/* rows of logits over a vocabulary, each with the softmax
+ *   p_k = exp((x_k - max x) / softmax_temp) / sum
+ * over the row's entries k: its moves d_move_indices[d_move_offsets[r] ..
+ * d_move_offsets[r + 1]), as in mfh_net_eval_priors_device (0..256 per row,
+ * vocab <= 32768; an index outside the vocabulary reads logit 0; an index
+ * listed twice counts twice), or all columns when d_move_offsets is NULL.  A
+ * logit of -inf takes its entry out; a row with no entry left gives zeros
+ * everywhere.  The row's action is the move played (or the token written):
+ * a column among its entries, anything else (-1) for none. */
+typedef struct {
+  const void *d_logits;
+  int64_t stride; /* elements from one row to the next, >= vocab */
+  int64_t rows;   /* >= 0 */
+  int32_t vocab;  /* 1 .. 2^30 */
+  int32_t dtype;  /* MFH_DTYPE_*: of the logits, reference logits and gradient */
+  const int32_t *d_move_offsets; /* [rows + 1], or NULL */
+  const int16_t *d_move_indices; /* [n_moves], NULL without offsets */
+  int64_t n_moves;
+  const int32_t *d_actions; /* [rows], or NULL: no row has one */
+  float softmax_temp;       /* > 0 */
+  int32_t device;           /* HIP device ordinal, -1 = the logits' device */
+} mfh_policy_rows;
+
+/* Clipped policy loss of each row, with l = ln p_action,
+ *   rho = exp(l - old_logp), A = advantage:
+ *   loss = weight (-min(rho A, clip(rho, 1 - clip_low, 1 + clip_high) A)
+ *                  + kl_coef KL(p || q) - entropy_coef H(p)),
+ * q the softmax of the reference logits over the same entries and
+ * temperature.  The first term is 0 in rows without an action or with
+ * d_advantage NULL; d_old_logp NULL is the row's own l (rho = 1).  A row of
+ * weight 0 is not read and gives zeros.  The gradient of the sum of all
+ * losses (old_logp, advantage, weight and q held fixed) goes to d_grad, every
+ * column of every row (0 outside the row's entries); at rho on a bound the
+ * unclipped branch counts.  Where q lacks an entry that p has, KL is infinite
+ * and the row's gradient not finite.  kl, entropy and logp (l, 0 without an action) are
+ * not weighted.  Any output may be NULL.  d_grad may be d_logits or
+ * d_ref_logits with the same stride, and overlaps neither otherwise. */
+typedef struct {
+  const float *d_old_logp;  /* [rows] */
+  const float *d_advantage; /* [rows] */
+  const float *d_weight;    /* [rows], NULL: 1 */
+  const void *d_ref_logits; /* NULL: no KL term (kl_coef must be 0) */
+  int64_t ref_stride;
+  float clip_low, clip_high; /* >= 0; infinity leaves that side open */
+  float kl_coef, entropy_coef;
+  float *d_loss, *d_logp, *d_kl, *d_entropy; /* [rows] */
+  void *d_grad;
+  int64_t grad_stride;
+} mfh_policy_loss;
+int mfh_policy_loss_device(const mfh_policy_rows *rows, const mfh_policy_loss *loss,
+                           void *stream);
+
+/* Preference loss of pairs of sequences.  Sequence j is the rows
+ * d_seq_offsets[j] .. d_seq_offsets[j + 1] (non-decreasing); pair i prefers
+ * sequence 2i to 2i + 1.  s_j is the sum (with `average` the mean, 0 of
+ * nothing) of ln p_action - ref_logp over its rows with an action, and with
+ * D = s_2i - s_2i+1 and h = beta D:
+ *   SIGMOID: -(1 - label_smoothing) ln sig(h) - label_smoothing ln sig(-h)
+ *   HINGE:   max(0, 1 - h)
+ *   SQUARE:  (D - 1 / (2 beta))^2
+ * times the pair's weight (a pair of weight 0 gives a loss, margin and
+ * gradient of 0).  margin is h.  logp
+ * is ln p_action, 0 without an action.  The gradient of the sum of all losses
+ * goes to the sequences' rows of d_grad, every column.  Rows before the first
+ * sequence or behind the last are neither read nor written.  Any output may
+ * be NULL; d_grad may be d_logits with the same stride.  d_workspace holds
+ * mfh_preference_loss_workspace_bytes(rows) bytes, 8-byte aligned. */
+enum { MFH_PREFERENCE_SIGMOID = 0, MFH_PREFERENCE_HINGE = 1, MFH_PREFERENCE_SQUARE = 2 };
+typedef struct {
+  const int32_t *d_seq_offsets; /* [2 pairs + 1] */
+  int64_t pairs;                /* >= 0 */
+  const float *d_ref_logp;      /* [rows], NULL: 0 */
+  const float *d_weight;        /* [pairs], NULL: 1 */
+  int32_t kind;                 /* MFH_PREFERENCE_* */
+  int32_t average;              /* 0 or 1 */
+  float beta;                   /* > 0 */
+  float label_smoothing;        /* 0 .. 0.5, SIGMOID only */
+  float *d_loss, *d_margin;     /* [pairs] */
+  float *d_logp;                /* [rows] */
+  void *d_grad;
+  int64_t grad_stride;
+  void *d_workspace;
+  uint64_t workspace_bytes;
+} mfh_preference_loss;
+int mfh_preference_loss_workspace_bytes(int64_t rows, uint64_t *bytes);
+int mfh_preference_loss_device(const mfh_policy_rows *rows, const mfh_preference_loss *loss,
+                               void *stream);
+
+/* A net's gradients: tensors of their own addresses, sizes and types, laid
+ * out once.  The set holds the list, not the memory: it is never written
+ * after creation, so calls on one set may run at once.  dst receives the
+ * scaled gradients: src itself, memory of its own, or NULL for a tensor that
+ * counts in the norm only.  No dst may overlap another tensor's src or dst,
+ * nor its own src in part.  device -1 is the device of the first tensor (the current one without
+ * any).  Waits for the device only in _destroy. */
+typedef struct {
+  const void *src;
+  void *dst;
+  uint64_t count; /* elements, 0 allowed */
+  int32_t dtype;  /* MFH_DTYPE_* */
+} mfh_grad_tensor;
+typedef struct mfh_grad_set mfh_grad_set;
+int mfh_grad_set_create(const mfh_grad_tensor *tensors, int n_tensors, int device,
+                        mfh_grad_set **out);
+void mfh_grad_set_destroy(mfh_grad_set *set);
+
+/* Bytes of the d_workspace (8-byte aligned) of the two calls below. */
+int mfh_grad_workspace_bytes(const mfh_grad_set *set, uint64_t *bytes);
+
+/* d_sumsq[1] = the sum of the squares of every gradient, in 64 bits and in an
+ * order that depends on the set alone. */
+int mfh_grad_norm_device(const mfh_grad_set *set, double *d_sumsq, void *d_workspace,
+                         uint64_t workspace_bytes, void *stream);
+
+/* dst = src * min(1, max_norm / sqrt(*d_sumsq)), rounded once; a sum that is
+ * NaN makes every dst NaN.  For gradients spread over several processes, whose
+ * sums the caller adds up in between. */
+int mfh_grad_scale_device(const mfh_grad_set *set, const double *d_sumsq, float max_norm,
+                          void *stream);
+
+/* Both in one call.  d_norm[1] (NULL to skip) receives the norm before
+ * clipping. */
+int mfh_grad_clip_device(const mfh_grad_set *set, float max_norm, float *d_norm,
+                         void *d_workspace, uint64_t workspace_bytes, void *stream);
+
 /* ---- Network files (no device needed) ----------------------------------
  *
  * A reader for the reference's `.pb` / `.pb.gz` network files

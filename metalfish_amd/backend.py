@@ -22,6 +22,8 @@ LIB_PATH = os.path.join(_PKG, "libmfhip.so")
 MFH_OK = 0
 PRECISION = {"bf16": 0, "bf16x2": 1, "bf16x2_gemm": 2, "fp8": 3, "bf16x2_fp8lo": 4}
 WEIGHTS = {"bf16": 0, "fp8": 1}
+DTYPE = {"f32": 0, "bf16": 1, "f16": 2}
+PREFERENCE = {"sigmoid": 0, "hinge": 1, "square": 2}
 ACTIVATION = {"default": 0, "mish": 1, "relu": 2, "none": 3, "tanh": 4, "sigmoid": 5,
               "selu": 6, "swish": 7, "relu_2": 8}
 
@@ -37,7 +39,11 @@ EXPORTS = ("mfh_net_create", "mfh_net_destroy", "mfh_net_eval", "mfh_net_eval_pl
            "mfh_net_eval_priors", "mfh_net_eval_priors_device",
            "mfh_net_eval_device_moves_left", "mfh_net_eval_device_noalloc",
            "mfh_debug_encoder_layer", "mfh_debug_skinny_gemm", "mfh_debug_gemm_fp8",
-           "mfh_debug_quantize_rows_e4m3", "mfh_debug_gemm_lo8")
+           "mfh_debug_quantize_rows_e4m3", "mfh_debug_gemm_lo8",
+           "mfh_policy_loss_device", "mfh_preference_loss_workspace_bytes",
+           "mfh_preference_loss_device", "mfh_grad_set_create", "mfh_grad_set_destroy",
+           "mfh_grad_workspace_bytes", "mfh_grad_norm_device", "mfh_grad_scale_device",
+           "mfh_grad_clip_device")
 FORMAT_FIELDS = ("input", "output", "network", "policy", "value", "moves_left",
                  "default_activation", "smolgen_activation", "ffn_activation", "input_embedding")
 
@@ -68,6 +74,40 @@ class MfhCapabilities(ctypes.Structure):
                 ("max_batch_size", ctypes.c_int), ("device", ctypes.c_int),
                 ("device_name", ctypes.c_char * 64), ("arch_name", ctypes.c_char * 32),
                 ("weight_bytes", ctypes.c_uint64), ("workspace_bytes", ctypes.c_uint64)]
+
+
+class MfhPolicyRows(ctypes.Structure):
+    _fields_ = [("d_logits", ctypes.c_void_p), ("stride", ctypes.c_int64),
+                ("rows", ctypes.c_int64), ("vocab", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("d_move_offsets", ctypes.c_void_p), ("d_move_indices", ctypes.c_void_p),
+                ("n_moves", ctypes.c_int64), ("d_actions", ctypes.c_void_p),
+                ("softmax_temp", ctypes.c_float), ("device", ctypes.c_int32)]
+
+
+class MfhPolicyLoss(ctypes.Structure):
+    _fields_ = [("d_old_logp", ctypes.c_void_p), ("d_advantage", ctypes.c_void_p),
+                ("d_weight", ctypes.c_void_p), ("d_ref_logits", ctypes.c_void_p),
+                ("ref_stride", ctypes.c_int64), ("clip_low", ctypes.c_float),
+                ("clip_high", ctypes.c_float), ("kl_coef", ctypes.c_float),
+                ("entropy_coef", ctypes.c_float), ("d_loss", ctypes.c_void_p),
+                ("d_logp", ctypes.c_void_p), ("d_kl", ctypes.c_void_p),
+                ("d_entropy", ctypes.c_void_p), ("d_grad", ctypes.c_void_p),
+                ("grad_stride", ctypes.c_int64)]
+
+
+class MfhPreferenceLoss(ctypes.Structure):
+    _fields_ = [("d_seq_offsets", ctypes.c_void_p), ("pairs", ctypes.c_int64),
+                ("d_ref_logp", ctypes.c_void_p), ("d_weight", ctypes.c_void_p),
+                ("kind", ctypes.c_int32), ("average", ctypes.c_int32), ("beta", ctypes.c_float),
+                ("label_smoothing", ctypes.c_float), ("d_loss", ctypes.c_void_p),
+                ("d_margin", ctypes.c_void_p), ("d_logp", ctypes.c_void_p),
+                ("d_grad", ctypes.c_void_p), ("grad_stride", ctypes.c_int64),
+                ("d_workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
+
+
+class MfhGradTensor(ctypes.Structure):
+    _fields_ = [("src", ctypes.c_void_p), ("dst", ctypes.c_void_p), ("count", ctypes.c_uint64),
+                ("dtype", ctypes.c_int32)]
 
 
 _lib = None
@@ -124,6 +164,15 @@ def lib():
             "mfh_net_eval_device_moves_left": ([vp, i, vp, vp, vp, vp, vp, vp], i),
             "mfh_net_eval_device_noalloc": ([vp, i, vp, vp, vp, vp, vp], i),
             "mfh_debug_encoder_layer": ([vp, i, i, i, vp, vp, ctypes.POINTER(ctypes.c_float)], i),
+            "mfh_policy_loss_device": ([vp, vp, vp], i),
+            "mfh_preference_loss_workspace_bytes": ([ctypes.c_int64, ctypes.POINTER(u64)], i),
+            "mfh_preference_loss_device": ([vp, vp, vp], i),
+            "mfh_grad_set_create": ([vp, i, i, ctypes.POINTER(vp)], i),
+            "mfh_grad_set_destroy": ([vp], None),
+            "mfh_grad_workspace_bytes": ([vp, ctypes.POINTER(u64)], i),
+            "mfh_grad_norm_device": ([vp, vp, vp, u64, vp], i),
+            "mfh_grad_scale_device": ([vp, vp, ctypes.c_float, vp], i),
+            "mfh_grad_clip_device": ([vp, ctypes.c_float, vp, vp, u64, vp], i),
         }
         for name, (args, res) in sig.items():
             fn = getattr(L, name)
@@ -544,6 +593,108 @@ def create_network(spec, weights, max_batch=256, device=-1, precision="bf16x2",
                       smolgen_activation=spec.smolgen_activation, max_batch=max_batch,
                       device=device, precision=precision, weights_dtype=weights_dtype,
                       fused_layernorm=fused_layernorm)
+
+
+def policy_rows(d_logits, rows, vocab, dtype="f32", stride=None, d_move_offsets=None,
+                d_move_indices=None, n_moves=0, d_actions=None, softmax_temp=1.0, device=-1):
+    """Rows of policy logits in device memory (pointers are device addresses)
+    for the losses below: [rows, vocab] of ``dtype`` "f32", "bf16" or "f16",
+    ``stride`` elements apart (vocab), with the move lists of
+    ``eval_priors_device`` (int32 offsets [rows + 1], int16 indices
+    [n_moves]) or, without, a softmax over all columns; ``d_actions`` int32
+    [rows], -1 for none.  Holds addresses only: it may be kept for as long as
+    the buffers are."""
+    return MfhPolicyRows(d_logits, vocab if stride is None else stride, rows, vocab, DTYPE[dtype],
+                         d_move_offsets, d_move_indices, n_moves, d_actions, softmax_temp, device)
+
+
+def policy_loss_device(rows, d_old_logp=None, d_advantage=None, d_weight=None, d_ref_logits=None,
+                       ref_stride=None, clip_low=0.2, clip_high=0.2, kl_coef=0.0,
+                       entropy_coef=0.0, d_loss=None, d_logp=None, d_kl=None, d_entropy=None,
+                       d_grad=None, grad_stride=None, stream=None):
+    """Clipped policy loss with a divergence from a reference policy and an
+    entropy term, per row of ``rows`` (``policy_rows``), and its gradient with
+    respect to the logits (mfh_policy_loss_device).  Strides default to the
+    vocabulary; outputs left None are not written."""
+    v = rows.vocab
+    a = MfhPolicyLoss(d_old_logp, d_advantage, d_weight, d_ref_logits,
+                      v if ref_stride is None else ref_stride, clip_low, clip_high, kl_coef,
+                      entropy_coef, d_loss, d_logp, d_kl, d_entropy, d_grad,
+                      v if grad_stride is None else grad_stride)
+    _check(lib().mfh_policy_loss_device(ctypes.addressof(rows), ctypes.addressof(a), stream),
+           "mfh_policy_loss_device")
+
+
+def preference_loss_workspace_bytes(rows: int) -> int:
+    """Bytes of device memory a preference loss over ``rows`` rows works in."""
+    n = ctypes.c_uint64(0)
+    _check(lib().mfh_preference_loss_workspace_bytes(rows, ctypes.byref(n)),
+           "mfh_preference_loss_workspace_bytes")
+    return n.value
+
+
+def preference_loss_device(rows, pairs, d_seq_offsets, kind="sigmoid", beta=0.1,
+                           label_smoothing=0.0, average=False, d_ref_logp=None, d_weight=None,
+                           d_loss=None, d_margin=None, d_logp=None, d_grad=None,
+                           grad_stride=None, d_workspace=None, workspace_bytes=0, stream=None):
+    """Loss of ``pairs`` pairs of sequences of ``rows`` by their
+    log-probability ratios, the first of each preferred, and its gradient
+    with respect to the logits (mfh_preference_loss_device).  ``d_seq_offsets``
+    int32 [2 pairs + 1]; ``kind`` "sigmoid", "hinge" or "square"."""
+    a = MfhPreferenceLoss(d_seq_offsets, pairs, d_ref_logp, d_weight, PREFERENCE[kind],
+                          1 if average else 0, beta, label_smoothing, d_loss, d_margin, d_logp,
+                          d_grad, rows.vocab if grad_stride is None else grad_stride, d_workspace,
+                          workspace_bytes)
+    _check(lib().mfh_preference_loss_device(ctypes.addressof(rows), ctypes.addressof(a), stream),
+           "mfh_preference_loss_device")
+
+
+class GradSet:
+    """The gradients of a net, laid out once: ``tensors`` is a list of (src,
+    dst, count, dtype) with device addresses; dst is src (in place), memory
+    of its own, or None for a tensor that counts in the norm only.  Norm and
+    clipping run over all of them in two launches."""
+
+    def __init__(self, tensors, device=-1):
+        self._h = None
+        arr = (MfhGradTensor * max(1, len(tensors)))()
+        for j, (src, dst, count, dtype) in enumerate(tensors):
+            arr[j] = MfhGradTensor(src, dst, count, DTYPE[dtype])
+        handle = ctypes.c_void_p()
+        _check(lib().mfh_grad_set_create(arr, len(tensors), device, ctypes.byref(handle)),
+               "mfh_grad_set_create")
+        self._h = handle
+        n = ctypes.c_uint64(0)
+        _check(lib().mfh_grad_workspace_bytes(self._h, ctypes.byref(n)),
+               "mfh_grad_workspace_bytes")
+        self.workspace_bytes = n.value
+
+    def close(self):
+        if self._h:
+            lib().mfh_grad_set_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def norm_device(self, d_sumsq, d_workspace, workspace_bytes, stream=None):
+        """float64 *d_sumsq = the sum of all squares (mfh_grad_norm_device)."""
+        _check(lib().mfh_grad_norm_device(self._h, d_sumsq, d_workspace, workspace_bytes, stream),
+               "mfh_grad_norm_device")
+
+    def scale_device(self, d_sumsq, max_norm, stream=None):
+        """dst = src * min(1, max_norm / sqrt(*d_sumsq)) (mfh_grad_scale_device)."""
+        _check(lib().mfh_grad_scale_device(self._h, d_sumsq, max_norm, stream),
+               "mfh_grad_scale_device")
+
+    def clip_device(self, max_norm, d_norm, d_workspace, workspace_bytes, stream=None):
+        """Both in one call; float32 *d_norm (or None) receives the norm before
+        clipping (mfh_grad_clip_device)."""
+        _check(lib().mfh_grad_clip_device(self._h, max_norm, d_norm, d_workspace, workspace_bytes,
+                                          stream), "mfh_grad_clip_device")
 
 
 class WeightsFile:

@@ -35,6 +35,7 @@
 #include "../host/policy_tables.h"
 #include "../host/weights_file.h"
 #include "mfh_kernels.h"
+#include "mfh_status.h"
 
 // Device memory of mfh_net_eval_device_noalloc: the workspace of one small
 // forward (activations, split-K partials, smolgen bias) for callers that
@@ -44,14 +45,20 @@
 constexpr size_t kScratchBytes = size_t(64) << 20;
 static __device__ __align__(256) unsigned char scratch[kScratchBytes];
 
-namespace {
+namespace mfh {
 
-thread_local std::string g_last_error;
+static thread_local std::string g_last_error;
 
 int SetError(int code, const std::string &msg) {
   g_last_error = msg;
   return code;
 }
+
+}  // namespace mfh
+
+namespace {
+
+using mfh::SetError;
 
 #define MFH_HIP_CHECK(expr)                                                    \
   do {                                                                         \
@@ -2397,7 +2404,7 @@ int CheckMovesLeftOut(const mfh_net *net, const float *moves_left, const char *f
 
 extern "C" {
 
-const char *mfh_last_error(void) { return g_last_error.c_str(); }
+const char *mfh_last_error(void) { return mfh::g_last_error.c_str(); }
 
 int mfh_device_count(int *count) {
   if (!count)

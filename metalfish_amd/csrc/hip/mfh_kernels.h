@@ -485,4 +485,81 @@ hipError_t LaunchValueHead(const float *hidden, int parts, const float *b1,
                            const float *b2, int mode, float *out,
                            hipStream_t stream, std::string *err);
 
+// Element types of the losses and of the gradient clipping (MFH_DTYPE_*).
+enum DType : int { DT_F32 = 0, DT_BF16 = 1, DT_F16 = 2 };
+inline int DTypeBytes(int dtype) { return dtype == DT_F32 ? 4 : 2; }
+
+// Rows of policy logits with a loss and its gradient.  One launch computes,
+// per row, the softmax statistics over the row's entries (moves or columns)
+// and whichever outputs are set:
+//   * loss, logp, kl, entropy and the gradient of the clipped policy loss;
+//   * mark: ln p of the action, or kNoAction, for the preference loss;
+//   * with coef: the gradient coef[row] (1[k = action] - p_k) / temperature
+//     alone, of the preference loss.
+constexpr float kNoAction = 1.0f;  // no log-probability is positive
+struct RowLossParams {
+  const void *x = nullptr;  // logits
+  std::int64_t ldx = 0;
+  const void *y = nullptr;  // reference logits
+  std::int64_t ldy = 0;
+  void *g = nullptr;  // gradient
+  std::int64_t ldg = 0;
+  std::int64_t rows = 0;
+  int vocab = 0;
+  int dtype = DT_F32;
+  const std::int32_t *offsets = nullptr;  // null: every column is an entry
+  const std::int16_t *indices = nullptr;
+  std::int64_t n_moves = 0;
+  const std::int32_t *actions = nullptr;
+  float inv_temp = 1.f;
+  const float *old_logp = nullptr, *advantage = nullptr, *weight = nullptr;
+  float ratio_low = 0.f, ratio_high = 0.f;  // bounds of the clipped ratio
+  float kl_coef = 0.f, entropy_coef = 0.f;
+  float *loss = nullptr, *logp = nullptr, *kl = nullptr, *entropy = nullptr;
+  float *mark = nullptr;
+  const float *coef = nullptr;
+  // Rows outside [seq_offsets[0], seq_offsets[n_seq]) are left alone.
+  const std::int32_t *seq_offsets = nullptr;
+  std::int64_t n_seq = 0;
+  std::int64_t row0 = 0;  // set by LaunchRowLoss: first row of the launch
+};
+hipError_t LaunchRowLoss(const RowLossParams &p, hipStream_t stream, std::string *err);
+
+// One workgroup per pair of sequences: sums of (mark - ref_logp) over their
+// rows in 64 bits and a fixed order, the pair's loss and margin, and each
+// row's gradient coefficient (0 without an action) and log-probability.
+struct PairLossParams {
+  const std::int32_t *seq_offsets = nullptr;
+  std::int64_t pairs = 0, rows = 0;
+  const float *mark = nullptr, *ref_logp = nullptr, *weight = nullptr;
+  int kind = 0;
+  bool average = false;
+  float beta = 0.f, smoothing = 0.f;
+  float *loss = nullptr, *margin = nullptr, *logp = nullptr, *coef = nullptr;
+};
+hipError_t LaunchPairLoss(const PairLossParams &p, hipStream_t stream, std::string *err);
+
+// A part of one gradient tensor, at most kGradChunk elements: a unit of work
+// of the norm and of the scaling.  dst may be null (norm only).
+constexpr int kGradChunk = 16384;
+struct GradChunk {
+  const void *src;
+  void *dst;
+  std::int32_t count;
+  std::int32_t dtype;
+};
+// Workgroups of the norm: one 64-bit partial sum each.  A function of the
+// number of chunks alone, so the order of the sum is the set's.
+int GradNormGroups(std::int64_t chunks);
+hipError_t LaunchGradSumsq(const GradChunk *chunks, std::int64_t n_chunks, double *partials,
+                           hipStream_t stream, std::string *err);
+// *sumsq = the partials' sum.
+hipError_t LaunchGradSum(const double *partials, int n, double *sumsq, hipStream_t stream,
+                         std::string *err);
+// Scales by min(1, max_norm / sqrt(sum of the n partials)); norm (optional)
+// receives the square root.
+hipError_t LaunchGradScale(const GradChunk *chunks, std::int64_t n_chunks, const double *partials,
+                           int n, float max_norm, float *norm, hipStream_t stream,
+                           std::string *err);
+
 }  // namespace mfh
