@@ -20,6 +20,7 @@
 struct mfh_grad_set {
   int device = 0;
   std::int64_t n_chunks = 0;
+  bool past = false;                 // too large for the caches
   mfh::GradChunk *chunks = nullptr;  // device memory, read only
 };
 
@@ -448,8 +449,9 @@ int mfh_grad_set_create(const mfh_grad_tensor *tensors, int n_tensors, int devic
       add(t.src, false);
       if (t.dst)
         add(t.dst, true);
-      for (uint64_t at = 0; at < t.count; at += mfh::kGradChunk) {
-        const uint64_t n = std::min<uint64_t>(mfh::kGradChunk, t.count - at);
+      const uint64_t most = mfh::kGradChunkBytes / es;
+      for (uint64_t at = 0; at < t.count; at += most) {
+        const uint64_t n = std::min<uint64_t>(most, t.count - at);
         chunks.push_back({static_cast<const char *>(t.src) + at * es,
                           t.dst ? static_cast<char *>(t.dst) + at * es : nullptr,
                           static_cast<std::int32_t>(n), t.dtype});
@@ -501,6 +503,10 @@ int mfh_grad_set_create(const mfh_grad_tensor *tensors, int n_tensors, int devic
     auto set = std::make_unique<mfh_grad_set>();
     set->device = dev;
     set->n_chunks = static_cast<std::int64_t>(chunks.size());
+    std::int64_t total = 0;
+    for (const mfh::GradChunk &c : chunks)
+      total += static_cast<std::int64_t>(c.count) * mfh::DTypeBytes(c.dtype);
+    set->past = total > mfh::kGradCachedBytes;
     if (!chunks.empty()) {
       const size_t bytes = chunks.size() * sizeof(mfh::GradChunk);
       e = hipMalloc(reinterpret_cast<void **>(&set->chunks), bytes);
@@ -559,7 +565,7 @@ int mfh_grad_norm_device(const mfh_grad_set *set, double *d_sumsq, void *d_works
       return rc;
     std::string err;
     double *partials = static_cast<double *>(d_workspace);
-    hipError_t e = mfh::LaunchGradSumsq(set->chunks, set->n_chunks, partials, st, &err);
+    hipError_t e = mfh::LaunchGradSumsq(set->chunks, set->n_chunks, set->past, partials, st, &err);
     if (e == hipSuccess)
       e = mfh::LaunchGradSum(partials, groups, d_sumsq, st, &err);
     return e == hipSuccess ? MFH_OK : HipError(fn, err.empty() ? "launch" : err.c_str(), e);
@@ -585,8 +591,8 @@ int mfh_grad_scale_device(const mfh_grad_set *set, const double *d_sumsq, float 
     if (rc != MFH_OK)
       return rc;
     std::string err;
-    const hipError_t e = mfh::LaunchGradScale(set->chunks, set->n_chunks, d_sumsq, 1, max_norm,
-                                              nullptr, st, &err);
+    const hipError_t e = mfh::LaunchGradScale(set->chunks, set->n_chunks, set->past, d_sumsq,
+                                              1, max_norm, nullptr, st, &err);
     return e == hipSuccess ? MFH_OK : HipError(fn, err.empty() ? "launch" : err.c_str(), e);
   } catch (const std::exception &e) {
     return Invalid(fn, e.what());
@@ -614,10 +620,10 @@ int mfh_grad_clip_device(const mfh_grad_set *set, float max_norm, float *d_norm,
       return rc;
     std::string err;
     double *partials = static_cast<double *>(d_workspace);
-    hipError_t e = mfh::LaunchGradSumsq(set->chunks, set->n_chunks, partials, st, &err);
+    hipError_t e = mfh::LaunchGradSumsq(set->chunks, set->n_chunks, set->past, partials, st, &err);
     if (e == hipSuccess)
-      e = mfh::LaunchGradScale(set->chunks, set->n_chunks, partials, groups, max_norm, d_norm, st,
-                               &err);
+      e = mfh::LaunchGradScale(set->chunks, set->n_chunks, set->past, partials, groups,
+                               max_norm, d_norm, st, &err);
     return e == hipSuccess ? MFH_OK : HipError(fn, err.empty() ? "launch" : err.c_str(), e);
   } catch (const std::exception &e) {
     return Invalid(fn, e.what());

@@ -539,9 +539,13 @@ struct PairLossParams {
 };
 hipError_t LaunchPairLoss(const PairLossParams &p, hipStream_t stream, std::string *err);
 
-// A part of one gradient tensor, at most kGradChunk elements: a unit of work
-// of the norm and of the scaling.  dst may be null (norm only).
-constexpr int kGradChunk = 16384;
+// A part of one gradient tensor, at most kGradChunkBytes: a unit of work of
+// the norm and of the scaling.  dst may be null (norm only).
+constexpr int kGradChunkBytes = 16384;
+// Sets above this many bytes are read and written past the caches
+// (non-temporal); below, each XCD's L2 still holds the chunks that it read for
+// the norm when it scales them (a workgroup takes the same chunks).
+constexpr std::int64_t kGradCachedBytes = std::int64_t(16) << 20;
 struct GradChunk {
   const void *src;
   void *dst;
@@ -551,15 +555,16 @@ struct GradChunk {
 // Workgroups of the norm: one 64-bit partial sum each.  A function of the
 // number of chunks alone, so the order of the sum is the set's.
 int GradNormGroups(std::int64_t chunks);
-hipError_t LaunchGradSumsq(const GradChunk *chunks, std::int64_t n_chunks, double *partials,
-                           hipStream_t stream, std::string *err);
+hipError_t LaunchGradSumsq(const GradChunk *chunks, std::int64_t n_chunks,
+                           bool past, double *partials, hipStream_t stream,
+                           std::string *err);
 // *sumsq = the partials' sum.
 hipError_t LaunchGradSum(const double *partials, int n, double *sumsq, hipStream_t stream,
                          std::string *err);
 // Scales by min(1, max_norm / sqrt(sum of the n partials)); norm (optional)
 // receives the square root.
-hipError_t LaunchGradScale(const GradChunk *chunks, std::int64_t n_chunks, const double *partials,
-                           int n, float max_norm, float *norm, hipStream_t stream,
-                           std::string *err);
+hipError_t LaunchGradScale(const GradChunk *chunks, std::int64_t n_chunks,
+                           bool past, const double *partials, int n, float max_norm,
+                           float *norm, hipStream_t stream, std::string *err);
 
 }  // namespace mfh
