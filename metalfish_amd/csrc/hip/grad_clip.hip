@@ -48,11 +48,6 @@ __device__ __forceinline__ std::uint32_t Round(float f) {
     return __builtin_bit_cast(std::uint16_t, static_cast<_Float16>(f));
 }
 
-// The addresses of a chunk come out of memory; without the address space every
-// access through them would be a flat one (which also counts as an LDS access).
-#define MFH_GLOBAL __attribute__((address_space(1)))
-#define MFH_CONSTANT __attribute__((address_space(4)))
-
 template <int DT>
 using Bits = std::conditional_t<DT == DT_F32, std::uint32_t, std::uint16_t>;
 template <int DT>

@@ -122,6 +122,12 @@ __device__ __forceinline__ unsigned Lo8Pack4(float a, float b, float c, float d)
 // direct global->LDS load builtin takes.
 #define MFH_LDS_PTR(p) ((__attribute__((address_space(3))) void *)(p))
 
+// Address spaces of global memory and of memory that no kernel running at the
+// time writes.  A pointer that comes out of memory or a condition is generic
+// without them, and every access through it a flat one.
+#define MFH_GLOBAL __attribute__((address_space(1)))
+#define MFH_CONSTANT __attribute__((address_space(4)))
+
 // Sum of the split-K partials x[0], x[stride], ..., x[(parts - 1) * stride]
 // added in that order (a fixed order, whatever the launch shape), with the
 // loads of each run of B parts issued together: partials written by

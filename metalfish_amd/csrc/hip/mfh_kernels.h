@@ -521,7 +521,7 @@ struct RowLossParams {
   // Rows outside [seq_offsets[0], seq_offsets[n_seq]) are left alone.
   const std::int32_t *seq_offsets = nullptr;
   std::int64_t n_seq = 0;
-  std::int64_t row0 = 0;  // set by LaunchRowLoss: first row of the launch
+  std::int64_t row0 = 0, end = 0;  // set by LaunchRowLoss: the rows of one launch
 };
 hipError_t LaunchRowLoss(const RowLossParams &p, hipStream_t stream, std::string *err);
 

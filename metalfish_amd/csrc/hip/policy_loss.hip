@@ -21,8 +21,16 @@ namespace mfh {
 namespace {
 
 constexpr float kLog2e = 1.44269504f;
+constexpr float kLog2eLow = 1.92596299e-8f;  // log2(e) - kLog2e
 constexpr float kLn2 = 0.69314718f;
 constexpr int kMaxMoves = 256;
+#ifndef LOOPG
+#define LOOPG 256
+#endif
+#ifndef MIDW
+#define MIDW 8
+#endif
+constexpr double kPastBytes = 32e6;
 
 // 16 bytes of a row at any element's alignment (global memory takes
 // unaligned vector accesses on gfx950).
@@ -80,6 +88,60 @@ template <> struct Elem<DT_F16> {
 // exp2 on v_exp_f32: 1 ulp, results below 2^-126 are 0.
 __device__ __forceinline__ float Exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// Rows of an array of elements, in global memory.
+template <int DT> using Row = MFH_GLOBAL typename Elem<DT>::T *;
+template <int DT> using ConstRow = const MFH_GLOBAL typename Elem<DT>::T *;
+template <int DT>
+__device__ __forceinline__ ConstRow<DT> RowOf(const void *p, std::int64_t row, std::int64_t stride) {
+  return (ConstRow<DT>)p + row * stride;
+}
+template <int DT>
+__device__ __forceinline__ Row<DT> RowOf(void *p, std::int64_t row, std::int64_t stride) {
+  return (Row<DT>)p + row * stride;
+}
+
+// A row's vectors, through the caches or (PAST, large calls) past them.
+template <int DT, bool PAST>
+__device__ __forceinline__ u32x4 LoadVec(ConstRow<DT> p) {
+  const auto *v = (const MFH_GLOBAL typename Elem<DT>::V *)p;
+  if constexpr (PAST)
+    return __builtin_nontemporal_load(v);
+  else
+    return *v;
+}
+template <int DT, bool PAST>
+__device__ __forceinline__ void StoreVec(Row<DT> p, u32x4 value) {
+  auto *v = (MFH_GLOBAL typename Elem<DT>::V *)p;
+  if constexpr (PAST)
+    __builtin_nontemporal_store(static_cast<typename Elem<DT>::V>(value), v);
+  else
+    *v = value;
+}
+
+// Row scalars, on the vector unit's own exponential, logarithm and reciprocal
+// (1 ulp each): every wave computes them for its one row, so their length
+// counts.
+__device__ __forceinline__ float Rcp(float x) { return __builtin_amdgcn_rcpf(x); }
+__device__ __forceinline__ float Log2(float x) { return __builtin_amdgcn_logf(x); }
+
+// e^x: x log2(e) in two parts, the lower one applied to first order.
+__device__ __forceinline__ float Exp(float x) {
+  const float h = x * kLog2e;
+  const float l = __builtin_fmaf(x, kLog2e, -h) + x * kLog2eLow;
+  const float r = Exp2(h);
+  // l is NaN where h is infinite, and r then is 0 or infinite.
+  return r > 0.f && r < __builtin_inff() ? r + r * (l * kLn2) : r;
+}
+
+// ln(1 + z) for z >= 0: 2 atanh(s), s = z / (2 + z) <= 1/5, by its series below
+// z = 1/2 (the first term left out is 3e-10 of the sum).
+__device__ __forceinline__ float Log1p(float z) {
+  if (!(z < 0.5f))
+    return Log2(1.f + z) * kLn2;
+  const float s = z * Rcp(2.f + z), q = s * s;
+  return 2.f * s * (1.f + q * (1.f / 3 + q * (1.f / 5 + q * (1.f / 7 + q * (1.f / 9 + q / 11)))));
+}
+
 // Reductions over a wave on the data-parallel paths of the vector unit (six
 // dependent instructions; a shuffle through LDS is several times that), the
 // result in every lane.
@@ -111,26 +173,26 @@ __device__ __forceinline__ float WaveMax(float v) {
   return LastLane(v);
 }
 
-// The same over the first W lanes (W = 4 or 16), which hold one value of each
+// The same over the first W lanes (4, 8 or 16), which hold one value of each
 // wave.
 template <int W>
 __device__ __forceinline__ float LanesSum(float v) {
   v += Dpp<kRowShr + 1, 0xF>(0.f, v);
   v += Dpp<kRowShr + 2, 0xF>(0.f, v);
-  if constexpr (W == 16) {
+  if constexpr (W >= 8)
     v += Dpp<kRowShr + 4, 0xF>(0.f, v);
+  if constexpr (W >= 16)
     v += Dpp<kRowShr + 8, 0xF>(0.f, v);
-  }
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), W - 1));
 }
 template <int W>
 __device__ __forceinline__ float LanesMax(float v) {
   v = fmaxf(v, Dpp<kRowShr + 1, 0xF>(v, v));
   v = fmaxf(v, Dpp<kRowShr + 2, 0xF>(v, v));
-  if constexpr (W == 16) {
+  if constexpr (W >= 8)
     v = fmaxf(v, Dpp<kRowShr + 4, 0xF>(v, v));
+  if constexpr (W >= 16)
     v = fmaxf(v, Dpp<kRowShr + 8, 0xF>(v, v));
-  }
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), W - 1));
 }
 
@@ -182,9 +244,9 @@ __device__ __forceinline__ RowStats Stats(float m, const float (&sums)[3], float
   RowStats r;
   r.m = m;
   r.empty = sums[0] == 0.f;
-  const float sum = r.empty ? 1.f : sums[0], inv = 1.f / sum;
-  r.log_sum = logf(sum);
-  r.log2_sum = r.log_sum * kLog2e;
+  const float sum = r.empty ? 1.f : sums[0], inv = Rcp(sum);
+  r.log2_sum = Log2(sum);
+  r.log_sum = r.log2_sum * kLn2;
   r.mean_z = sums[1] * kLn2 * inv;
   r.mean_d = sums[2] * inv_temp * inv;
   return r;
@@ -263,7 +325,7 @@ __device__ __forceinline__ float KlTerm(const Coefs &k, float p, float u, float 
 // KL from the sum of its terms; infinite where the reference lacks what the
 // policy plays (E_p d is, and no term then means anything).
 __device__ __forceinline__ float KlOf(float terms, float mean_d) {
-  return mean_d == __builtin_inff() ? mean_d : log1pf(terms);
+  return mean_d == __builtin_inff() ? mean_d : Log1p(terms);
 }
 
 // The gradient of N entries without the action's own term, and their part of
@@ -302,15 +364,30 @@ __device__ __forceinline__ bool WantsKl(const RowLossParams &a) {
   return a.kl || (a.loss && a.kl_coef != 0.f);
 }
 
+// A row's scalar inputs, loaded together before anything waits on one.
+struct RowInputs {
+  float weight;  // 0: the row is not read
+  int action;
+  float advantage, old_logp;
+};
+__device__ __forceinline__ RowInputs Inputs(const RowLossParams &a, std::int64_t row) {
+  RowInputs r;
+  r.weight = a.coef ? a.coef[row] : a.weight ? a.weight[row] : 1.f;
+  r.action = a.actions ? a.actions[row] : -1;
+  r.advantage = a.advantage ? a.advantage[row] : 0.f;
+  r.old_logp = a.old_logp ? a.old_logp[row] : 0.f;
+  return r;
+}
+
 // The first term of the loss and its derivative by ln p_a.
 struct Surrogate {
   float loss, slope;
 };
-__device__ __forceinline__ Surrogate Clipped(const RowLossParams &a, std::int64_t row, float logp) {
-  const float adv = a.advantage[row];
-  const float ratio = a.old_logp ? expf(logp - a.old_logp[row]) : 1.f;
-  const float plain = ratio * adv;
-  const float bounded = fminf(fmaxf(ratio, a.ratio_low), a.ratio_high) * adv;
+__device__ __forceinline__ Surrogate Clipped(const RowLossParams &a, const RowInputs &in,
+                                             float logp) {
+  const float ratio = a.old_logp ? Exp(logp - in.old_logp) : 1.f;
+  const float plain = ratio * in.advantage;
+  const float bounded = fminf(fmaxf(ratio, a.ratio_low), a.ratio_high) * in.advantage;
   // The unclipped branch on ties and for NaN.
   return bounded < plain ? Surrogate{-bounded, 0.f} : Surrogate{-plain, -plain};
 }
@@ -321,9 +398,9 @@ struct RowResult {
   RowGrad grad;
   float logp, surrogate, entropy;
 };
-__device__ __forceinline__ RowResult Evaluate(const RowLossParams &a, std::int64_t row, float w,
+__device__ __forceinline__ RowResult Evaluate(const RowLossParams &a, const RowInputs &in,
                                               const RowStats &st, bool acted, float xa) {
-  RowResult r{{w * a.inv_temp, 0.f, 0.f, 0.f}, 0.f, 0.f, 0.f};
+  RowResult r{{in.weight * a.inv_temp, 0.f, 0.f, 0.f}, 0.f, 0.f, 0.f};
   if (acted)
     r.logp = (xa - st.m) * a.inv_temp - st.log_sum;
   if (a.coef) {
@@ -331,7 +408,7 @@ __device__ __forceinline__ RowResult Evaluate(const RowLossParams &a, std::int64
     return r;
   }
   if (acted && a.advantage) {
-    const Surrogate s = Clipped(a, row, r.logp);
+    const Surrogate s = Clipped(a, in, r.logp);
     r.surrogate = s.loss;
     r.grad.slope = s.slope;
   }
@@ -382,19 +459,13 @@ __device__ __forceinline__ bool OutsideSequences(const RowLossParams &a, std::in
   return a.seq_offsets && (row < a.seq_offsets[0] || row >= a.seq_offsets[a.n_seq]);
 }
 
-// The factor on a row's outputs; 0: the row is not read.
-__device__ __forceinline__ float RowWeight(const RowLossParams &a, std::int64_t row) {
-  return a.coef ? a.coef[row] : a.weight ? a.weight[row] : 1.f;
-}
-
 // Zeros in a whole gradient row, by `threads` threads.
 template <int DT>
-__device__ __forceinline__ void ZeroRow(typename Elem<DT>::T *g, int n, int thread, int threads) {
+__device__ __forceinline__ void ZeroRow(Row<DT> g, int n, int thread, int threads) {
   using E = Elem<DT>;
   const int vecs = n / E::kPerVec;
   for (int v = thread; v < vecs; v += threads)
-    *reinterpret_cast<typename E::V *>(g + static_cast<std::int64_t>(v) * E::kPerVec) =
-        u32x4{0, 0, 0, 0};
+    StoreVec<DT, false>(g + static_cast<std::int64_t>(v) * E::kPerVec, u32x4{0, 0, 0, 0});
   const int t = vecs * E::kPerVec + thread;
   if (thread < E::kPerVec && t < n)
     g[t] = 0;
@@ -411,14 +482,75 @@ __device__ __forceinline__ void Unpack(u32x4 v, float (&x)[Elem<DT>::kPerVec]) {
     x[i] = Elem<DT>::Get(v, i);
 }
 
+template <int DT, bool REF, bool GUARD>
+__device__ __forceinline__ void AddVec(u32x4 xr, u32x4 yr, float m, float c, float (&sums)[3]) {
+  constexpr int VE = Elem<DT>::kPerVec;
+  float xs[VE], ys[VE] = {};
+  Unpack<DT>(xr, xs);
+  if constexpr (REF)
+    Unpack<DT>(yr, ys);
+#pragma unroll
+  for (int i = 0; i < VE; ++i)
+    AddStats<REF, GUARD>(xs[i], ys[i], m, c, sums);
+}
+
+// Four entries at a time: eight would hold more registers.
+template <int DT, bool REF, bool GUARD>
+__device__ __forceinline__ u32x4 FinishVec(const Coefs &k, bool want_kl, u32x4 xr, u32x4 yr,
+                                           float &kl) {
+  using E = Elem<DT>;
+  constexpr int VE = E::kPerVec;
+  float f[VE];
+#pragma unroll
+  for (int h = 0; h < VE; h += 4) {
+    float xs[4], ys[4] = {}, part[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      xs[i] = E::Get(xr, h + i);
+      if constexpr (REF)
+        ys[i] = E::Get(yr, h + i);
+    }
+    FinishEntries<4, REF, GUARD>(k, want_kl, xs, ys, kl, part);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      f[h + i] = part[i];
+  }
+  return E::Pack(f);
+}
+
+// The elements behind the last whole vector, and the action's own term, by the
+// thread that wrote its column.
+template <int DT, bool REF, bool GUARD>
+__device__ __forceinline__ void FinishRest(const Coefs &k, bool want_kl, bool want_grad, Row<DT> g,
+                                           const RowGrad &grad, int act, float xa, float ya,
+                                           const float (&xt)[1], const float (&yt)[1], int vecs,
+                                           bool has_rest, int threads, int tid, float &kl) {
+  using E = Elem<DT>;
+  constexpr int VE = E::kPerVec;
+  float ft[1];
+  if (has_rest) {
+    FinishEntries<1, REF, GUARD>(k, want_kl, xt, yt, kl, ft);
+    if (want_grad)
+      g[vecs * VE + tid] = E::Round(ft[0]);
+  }
+  const int v = act / VE;
+  if (want_grad && act >= 0 && tid == (v < vecs ? v % threads : act - vecs * VE)) {
+    float none = 0.f;
+    const float xs[1] = {xa}, ys[1] = {ya};
+    FinishEntries<1, REF, GUARD>(k, false, xs, ys, none, ft);
+    g[act] = E::Round(ft[0] + grad.scale * grad.slope);
+  }
+}
+
+#define MFH_INLINE __attribute__((always_inline))
+
 // A whole row in the registers of W waves, NV vectors of 16 bytes a lane; the
 // elements behind the last whole vector, one to a lane, in a register more.
 // Three passes over the registers: maximum, sums, gradient with KL.  Four rows
 // to a workgroup where a wave has one to itself.
-template <int DT, int W, int NV, bool REF>
+template <int DT, int W, int NV, bool REF, bool PAST>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void DenseRowKernel(RowLossParams a) {
   using E = Elem<DT>;
-  using T = typename E::T;
   constexpr int VE = E::kPerVec;
   __shared__ float red[W][4];
   const int tid = W == 1 ? threadIdx.x & 63 : threadIdx.x;
@@ -426,22 +558,23 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void DenseRowKernel(RowLossP
   if constexpr (W == 1)
     row = row * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   row += a.row0;
-  if (row >= a.rows || OutsideSequences(a, row))
+  if (row >= a.end || OutsideSequences(a, row))
     return;
   const int n = a.vocab, vecs = n / VE, rest = n - vecs * VE;
-  const T *x = static_cast<const T *>(a.x) + row * a.ldx;
-  const T *y = REF ? static_cast<const T *>(a.y) + row * a.ldy : nullptr;
-  T *g = a.g ? static_cast<T *>(a.g) + row * a.ldg : nullptr;
-  const float w = RowWeight(a, row);
-  if (w == 0.f) {
+  const ConstRow<DT> x = RowOf<DT>(a.x, row, a.ldx);
+  const ConstRow<DT> y = RowOf<DT>(a.y, row, a.ldy);
+  const Row<DT> g = RowOf<DT>(a.g, row, a.ldg);
+  const bool want_grad = a.g != nullptr;
+  const RowInputs in = Inputs(a, row);
+  if (in.weight == 0.f) {
     if (tid == 0)
       WriteZeros(a, row);
-    if (g)
+    if (want_grad)
       ZeroRow<DT>(g, n, tid, 64 * W);
     return;
   }
-  const int act = a.actions ? a.actions[row] : -1;
-  bool acted = act >= 0 && act < n;
+  const int act = in.action;
+  const bool acted = act >= 0 && act < n;
   const float xa = acted ? E::One(x[act]) : 0.f;
   const float ya = REF && acted ? E::One(y[act]) : 0.f;
   u32x4 xr[NV], yr[REF ? NV : 1];
@@ -449,14 +582,14 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void DenseRowKernel(RowLossP
   for (int j = 0; j < NV; ++j) {
     const int v = j * 64 * W + tid;
     if (v < vecs)
-      xr[j] = *reinterpret_cast<const typename E::V *>(x + v * VE);
+      xr[j] = LoadVec<DT, PAST>(x + v * VE);
   }
   if constexpr (REF) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int v = j * 64 * W + tid;
       if (v < vecs)
-        yr[j] = *reinterpret_cast<const typename E::V *>(y + v * VE);
+        yr[j] = LoadVec<DT, PAST>(y + v * VE);
     }
   }
   const bool has_rest = tid < rest;
@@ -478,7 +611,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void DenseRowKernel(RowLossP
 
   const float c = a.inv_temp * kLog2e;
   float sums[3];
-  const auto sum = [&](auto guard) {
+  const auto sum = [&](auto guard) MFH_INLINE {
     constexpr bool GUARD = decltype(guard)::value;
     sums[0] = sums[1] = sums[2] = 0.f;
 #pragma unroll
@@ -486,15 +619,8 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void DenseRowKernel(RowLossP
       Repack(xr[j]);
       if (REF)
         Repack(yr[REF ? j : 0]);
-      if (j * 64 * W + tid < vecs) {
-        float xs[VE], ys[VE] = {};
-        Unpack<DT>(xr[j], xs);
-        if constexpr (REF)
-          Unpack<DT>(yr[j], ys);
-#pragma unroll
-        for (int i = 0; i < VE; ++i)
-          AddStats<REF, GUARD>(xs[i], ys[i], m, c, sums);
-      }
+      if (j * 64 * W + tid < vecs)
+        AddVec<DT, REF, GUARD>(xr[j], yr[REF ? j : 0], m, c, sums);
     }
     if (has_rest)
       AddStats<REF, GUARD>(xt[0], yt[0], m, c, sums);
@@ -508,16 +634,16 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void DenseRowKernel(RowLossP
   if (st.empty) {
     if (tid == 0)
       WriteZeros(a, row);
-    if (g)
+    if (want_grad)
       ZeroRow<DT>(g, n, tid, 64 * W);
     return;
   }
-  const RowResult res = Evaluate(a, row, w, st, acted, xa);
+  const RowResult res = Evaluate(a, in, st, acted, xa);
   const bool want_kl = REF && WantsKl(a);
   float kl[1] = {0.f};
-  if (g || want_kl) {
+  if (want_grad || want_kl) {
     const Coefs k = CoefsOf(st, res.grad, a.inv_temp);
-    const auto finish = [&](auto guard) {
+    const auto finish = [&](auto guard) MFH_INLINE {
       constexpr bool GUARD = decltype(guard)::value;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
@@ -526,29 +652,13 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void DenseRowKernel(RowLossP
           Repack(yr[REF ? j : 0]);
         const int v = j * 64 * W + tid;
         if (v < vecs) {
-          float xs[VE], ys[VE] = {}, f[VE];
-          Unpack<DT>(xr[j], xs);
-          if constexpr (REF)
-            Unpack<DT>(yr[j], ys);
-          FinishEntries<VE, REF, GUARD>(k, want_kl, xs, ys, kl[0], f);
-          if (g)
-            *reinterpret_cast<typename E::V *>(g + v * VE) = E::Pack(f);
+          const u32x4 f = FinishVec<DT, REF, GUARD>(k, want_kl, xr[j], yr[REF ? j : 0], kl[0]);
+          if (want_grad)
+            StoreVec<DT, PAST>(g + v * VE, f);
         }
       }
-      float ft[1];
-      if (has_rest) {
-        FinishEntries<1, REF, GUARD>(k, want_kl, xt, yt, kl[0], ft);
-        if (g)
-          g[vecs * VE + tid] = E::Round(ft[0]);
-      }
-      // The action's own term, by the thread that wrote its column.
-      const int v = act / VE;
-      if (g && acted && tid == (v < vecs ? v % (64 * W) : act - vecs * VE)) {
-        float none = 0.f;
-        const float xs[1] = {xa}, ys[1] = {ya};
-        FinishEntries<1, REF, GUARD>(k, false, xs, ys, none, ft);
-        g[act] = E::Round(ft[0] + res.grad.scale * res.grad.slope);
-      }
+      FinishRest<DT, REF, GUARD>(k, want_kl, want_grad, g, res.grad, acted ? act : -1, xa, ya, xt,
+                                 yt, vecs, has_rest, 64 * W, tid, kl[0]);
     };
     if (guarded)
       finish(std::true_type{});
@@ -560,35 +670,25 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void DenseRowKernel(RowLossP
     }
   }
   if (tid == 0)
-    WriteRow(a, row, w, acted, res, kl[0]);
+    WriteRow(a, row, in.weight, acted, res, kl[0]);
 }
 
-// Rows longer than the registers hold: one pass for the statistics with a
-// running maximum per lane, a second for KL and the gradient, from the end of
-// the row backwards (its last part is nearest in the caches).
+// A row that is not in registers, by a workgroup of 16 waves: one pass for the
+// statistics with a running maximum per lane, a second for KL and the
+// gradient, from the end of the row backwards (its last part is nearest in the
+// caches).
 template <int DT, bool REF>
-__global__ __launch_bounds__(1024) void LongRowKernel(RowLossParams a) {
+__device__ __forceinline__ void StreamRow(const RowLossParams &a, std::int64_t row,
+                                          const RowInputs &in, float (*red)[4]) {
   using E = Elem<DT>;
-  using T = typename E::T;
   constexpr int VE = E::kPerVec, W = 16, kThreads = 64 * W;
-  __shared__ float red[W][4];
-  const std::int64_t row = a.row0 + blockIdx.x;
-  if (OutsideSequences(a, row))
-    return;
   const int tid = threadIdx.x;
   const int n = a.vocab, vecs = n / VE, rest = n - vecs * VE;
-  const T *x = static_cast<const T *>(a.x) + row * a.ldx;
-  const T *y = REF ? static_cast<const T *>(a.y) + row * a.ldy : nullptr;
-  T *g = a.g ? static_cast<T *>(a.g) + row * a.ldg : nullptr;
-  const float w = RowWeight(a, row);
-  if (w == 0.f) {
-    if (tid == 0)
-      WriteZeros(a, row);
-    if (g)
-      ZeroRow<DT>(g, n, tid, kThreads);
-    return;
-  }
-  const int act = a.actions ? a.actions[row] : -1;
+  const ConstRow<DT> x = RowOf<DT>(a.x, row, a.ldx);
+  const ConstRow<DT> y = RowOf<DT>(a.y, row, a.ldy);
+  const Row<DT> g = RowOf<DT>(a.g, row, a.ldg);
+  const bool want_grad = a.g != nullptr;
+  const int act = in.action;
   const bool acted = act >= 0 && act < n;
   const float xa = acted ? E::One(x[act]) : 0.f;
   const float ya = REF && acted ? E::One(y[act]) : 0.f;
@@ -600,7 +700,7 @@ __global__ __launch_bounds__(1024) void LongRowKernel(RowLossParams a) {
   float m = xt[0], sums[3] = {0.f, 0.f, 0.f};
   // Sums over the old maximum as sums over the new: e and t of each term fall
   // by the same step.
-  const auto rescale = [&](float from, float to) {
+  const auto rescale = [&](float from, float to) MFH_INLINE {
     if (sums[0] == 0.f)
       return;
     const float step = (from - to) * c, f = Exp2(step);
@@ -611,23 +711,19 @@ __global__ __launch_bounds__(1024) void LongRowKernel(RowLossParams a) {
   if (has_rest)
     AddStats<REF, true>(xt[0], yt[0], m == -__builtin_inff() ? 0.f : m, c, sums);
   for (int v = tid; v < vecs; v += kThreads) {
-    float xs[VE], ys[VE] = {};
-    Unpack<DT>(*reinterpret_cast<const typename E::V *>(x + static_cast<std::int64_t>(v) * VE), xs);
+    const u32x4 xr = LoadVec<DT, false>(x + static_cast<std::int64_t>(v) * VE);
+    u32x4 yr = {};
     if constexpr (REF)
-      Unpack<DT>(*reinterpret_cast<const typename E::V *>(y + static_cast<std::int64_t>(v) * VE),
-                 ys);
+      yr = LoadVec<DT, false>(y + static_cast<std::int64_t>(v) * VE);
     float top = m;
 #pragma unroll
     for (int i = 0; i < VE; ++i)
-      top = fmaxf(top, xs[i]);
+      top = fmaxf(top, E::Get(xr, i));
     if (top > m) {
       rescale(m, top);
       m = top;
     }
-    const float from = m == -__builtin_inff() ? 0.f : m;
-#pragma unroll
-    for (int i = 0; i < VE; ++i)
-      AddStats<REF, true>(xs[i], ys[i], from, c, sums);
+    AddVec<DT, REF, true>(xr, yr, m == -__builtin_inff() ? 0.f : m, c, sums);
   }
   float top = GroupMax<W>(m, red);
   top = top == -__builtin_inff() ? 0.f : top;
@@ -638,135 +734,258 @@ __global__ __launch_bounds__(1024) void LongRowKernel(RowLossParams a) {
   if (st.empty) {
     if (tid == 0)
       WriteZeros(a, row);
-    if (g)
+    if (want_grad)
       ZeroRow<DT>(g, n, tid, kThreads);
     return;
   }
-  const RowResult res = Evaluate(a, row, w, st, acted, xa);
+  const RowResult res = Evaluate(a, in, st, acted, xa);
   const bool want_kl = REF && WantsKl(a);
   float kl[1] = {0.f};
-  if (g || want_kl) {
+  if (want_grad || want_kl) {
     const Coefs k = CoefsOf(st, res.grad, a.inv_temp);
-    const int steps = (vecs + kThreads - 1) / kThreads;
-    for (int j = steps - 1; j >= 0; --j) {
+    for (int j = (vecs - 1) / kThreads; j >= 0; --j) {
       const std::int64_t v = static_cast<std::int64_t>(j) * kThreads + tid;
       if (v >= vecs)
         continue;
-      float xs[VE], ys[VE] = {}, f[VE];
-      Unpack<DT>(*reinterpret_cast<const typename E::V *>(x + v * VE), xs);
+      const u32x4 xr = LoadVec<DT, false>(x + v * VE);
+      u32x4 yr = {};
       if constexpr (REF)
-        Unpack<DT>(*reinterpret_cast<const typename E::V *>(y + v * VE), ys);
-      FinishEntries<VE, REF, true>(k, want_kl, xs, ys, kl[0], f);
-      if (g)
-        *reinterpret_cast<typename E::V *>(g + v * VE) = E::Pack(f);
+        yr = LoadVec<DT, false>(y + v * VE);
+      const u32x4 f = FinishVec<DT, REF, true>(k, want_kl, xr, yr, kl[0]);
+      if (want_grad)
+        StoreVec<DT, true>(g + v * VE, f);
     }
-    float ft[1];
-    if (has_rest) {
-      FinishEntries<1, REF, true>(k, want_kl, xt, yt, kl[0], ft);
-      if (g)
-        g[vecs * VE + tid] = E::Round(ft[0]);
-    }
-    const int v = act / VE;
-    if (g && acted && tid == (v < vecs ? v % kThreads : act - vecs * VE)) {
-      float none = 0.f;
-      const float xs[1] = {xa}, ys[1] = {ya};
-      FinishEntries<1, REF, true>(k, false, xs, ys, none, ft);
-      g[act] = E::Round(ft[0] + res.grad.scale * res.grad.slope);
-    }
+    FinishRest<DT, REF, true>(k, want_kl, want_grad, g, res.grad, acted ? act : -1, xa, ya, xt, yt,
+                              vecs, has_rest, kThreads, tid, kl[0]);
     if (want_kl) {
       GroupSum<W>(kl, red);
       kl[0] = KlOf(kl[0], st.mean_d);
     }
   }
   if (tid == 0)
-    WriteRow(a, row, w, acted, res, kl[0]);
+    WriteRow(a, row, in.weight, acted, res, kl[0]);
 }
 
-// A row's legal moves, one wave per row and four rows per workgroup, at most
-// four entries a lane.  The gradient row is zeros but for the entries: the
-// zeros are written while the logits are on their way, the entries over them
-// afterwards (a wave's stores reach an address in order).  A move listed twice
-// adds up: a bit per column finds such rows, where the first of equal entries
-// writes for all.
+// Rows longer than the registers hold.
 template <int DT, bool REF>
-__global__ __launch_bounds__(256) void MovesRowKernel(RowLossParams a) {
-  using E = Elem<DT>;
-  using T = typename E::T;
-  constexpr int NE = kMaxMoves / 64;
-  extern __shared__ std::uint32_t seen_all[];
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const std::int64_t row = a.row0 + static_cast<std::int64_t>(blockIdx.x) * 4 + wave;
-  if (row >= a.rows || OutsideSequences(a, row))
+__global__ __launch_bounds__(1024) void StreamRowKernel(RowLossParams a) {
+  __shared__ float red[16][4];
+  const std::int64_t row = a.row0 + blockIdx.x;
+  if (OutsideSequences(a, row))
     return;
-  const int n = a.vocab, words = (n + 31) / 32;
-  std::uint32_t *seen = seen_all + wave * words;
-  T *g = a.g ? static_cast<T *>(a.g) + row * a.ldg : nullptr;
-  const float w = RowWeight(a, row);
-  if (w == 0.f) {
-    if (lane == 0)
-      WriteZeros(a, row);
-    if (g)
-      ZeroRow<DT>(g, n, lane, 64);
+  const RowInputs in = Inputs(a, row);
+  if (in.weight != 0.f) {
+    StreamRow<DT, REF>(a, row, in, red);
     return;
   }
-  std::int64_t start = a.offsets[row], count = a.offsets[row + 1];
-  start = start < 0 ? 0 : start > a.n_moves ? a.n_moves : start;
-  count = (count > a.n_moves ? a.n_moves : count) - start;
-  const int moves = count < 0 ? 0 : count > kMaxMoves ? kMaxMoves : static_cast<int>(count);
-  const int act = a.actions ? a.actions[row] : -1;
-  const T *x = static_cast<const T *>(a.x) + row * a.ldx;
-  const T *y = REF ? static_cast<const T *>(a.y) + row * a.ldy : nullptr;
+  if (threadIdx.x == 0)
+    WriteZeros(a, row);
+  if (a.g)
+    ZeroRow<DT>(RowOf<DT>(a.g, row, a.ldg), a.vocab, threadIdx.x, 1024);
+}
 
+// Rows that fill the registers of 16 waves, so that a CU holds one workgroup
+// and its loads, passes and stores would follow one another.  A workgroup takes
+// row after row (every gridDim.x-th), and as the last pass is done with a
+// vector of the present row it loads the next row's into its registers.  All
+// rows take the same way through the loop, so that there is one such place:
+// rows of weight 0 or none compute nothing of use and store nothing, and rows
+// that need the guards are streamed.  At least 4 * 1024 vectors a row.
+template <int DT, int NV, bool REF>
+__global__ __launch_bounds__(1024) void LoopRowKernel(RowLossParams a) {
+  using E = Elem<DT>;
+  constexpr int VE = E::kPerVec, W = 16, kThreads = 64 * W;
+  __shared__ float red[W][4];
+  const int tid = threadIdx.x;
+  const int n = a.vocab, vecs = n / VE, rest = n - vecs * VE;
+  const bool has_rest = tid < rest;
+  const bool want_grad = a.g != nullptr;
+  const bool want_kl = REF && WantsKl(a);
+  const float c = a.inv_temp * kLog2e;
+
+  u32x4 xr[NV], yr[REF ? NV : 1];
+  // Vector j of a row; some vector of it where the row has fewer, and the
+  // row's first where there is nothing to read (`live` 0).
+  const auto load = [&](std::int64_t r, int j, int live) MFH_INLINE {
+    int v = j * kThreads + tid;
+    v = (v < vecs ? v : tid) * live;
+    xr[j] = LoadVec<DT, true>(RowOf<DT>(a.x, r, a.ldx) + v * VE);
+    if constexpr (REF)
+      yr[j] = LoadVec<DT, true>(RowOf<DT>(a.y, r, a.ldy) + v * VE);
+  };
+  const auto alive = [&](std::int64_t r) MFH_INLINE {
+    return r < a.end && !OutsideSequences(a, r) && Inputs(a, r).weight != 0.f;
+  };
+  std::int64_t row = a.row0 + blockIdx.x;
+  bool live = alive(row);
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+    load(row, j, live);
+  while (row < a.end) {
+    const std::int64_t next = row + gridDim.x;
+    const bool next_live = alive(next);
+    const std::int64_t next_row = next < a.end ? next : row;
+    const ConstRow<DT> x = RowOf<DT>(a.x, row, a.ldx);
+    const ConstRow<DT> y = RowOf<DT>(a.y, row, a.ldy);
+    const Row<DT> g = RowOf<DT>(a.g, row, a.ldg);
+    const RowInputs in = Inputs(a, row);
+    const int act = in.action;
+    const bool acted = act >= 0 && act < n;
+    const float xa = acted ? E::One(x[act]) : 0.f;
+    const float ya = REF && acted ? E::One(y[act]) : 0.f;
+    const float xt[1] = {has_rest ? E::One(x[vecs * VE + tid]) : -__builtin_inff()};
+    const float yt[1] = {REF && has_rest ? E::One(y[vecs * VE + tid]) : 0.f};
+    float m = -__builtin_inff();
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (j * kThreads + tid < vecs) {
+        float xs[VE];
+        Unpack<DT>(xr[j], xs);
+#pragma unroll
+        for (int i = 0; i < VE; ++i)
+          m = fmaxf(m, xs[i]);
+      }
+    m = GroupMax<W>(fmaxf(m, xt[0]), red);
+    m = m == -__builtin_inff() ? 0.f : m;
+    float sums[3] = {0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      Repack(xr[j]);
+      if (REF)
+        Repack(yr[REF ? j : 0]);
+      if (j * kThreads + tid < vecs)
+        AddVec<DT, REF, false>(xr[j], yr[REF ? j : 0], m, c, sums);
+    }
+    if (has_rest)
+      AddStats<REF, false>(xt[0], yt[0], m, c, sums);
+    GroupSum<W>(sums, red);
+    // A sum of 0 has a NaN beside it (0 times the -inf of its logits), as a
+    // row that needs the guards does.
+    const bool stream = live && NeedsGuard(sums), here = live && !stream;
+    if (stream) {
+      StreamRow<DT, REF>(a, row, in, red);
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        asm volatile("" : "=v"(xr[j]));  // no longer needed
+        if (REF)
+          asm volatile("" : "=v"(yr[REF ? j : 0]));
+      }
+    }
+    const RowStats st = Stats(m, sums, a.inv_temp);
+    const RowResult res = Evaluate(a, in, st, acted, xa);
+    const Coefs k = CoefsOf(st, res.grad, a.inv_temp);
+    float kl[1] = {0.f};
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      Repack(xr[j]);
+      if (REF)
+        Repack(yr[REF ? j : 0]);
+      const int v = j * kThreads + tid;
+      if (v < vecs && (want_grad || want_kl)) {
+        const u32x4 f = FinishVec<DT, REF, false>(k, want_kl, xr[j], yr[REF ? j : 0], kl[0]);
+        if (want_grad && here)
+          StoreVec<DT, true>(g + v * VE, f);
+      }
+      // Not earlier: the present row's vector is in the registers.
+      __builtin_amdgcn_sched_barrier(0);
+      load(next_row, j, next_live);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (here) {
+      FinishRest<DT, REF, false>(k, want_kl, want_grad, g, res.grad, acted ? act : -1, xa, ya, xt,
+                                 yt, vecs, has_rest, kThreads, tid, kl[0]);
+      if (want_kl) {
+        GroupSum<W>(kl, red);
+        kl[0] = KlOf(kl[0], st.mean_d);
+      }
+      if (tid == 0)
+        WriteRow(a, row, in.weight, acted, res, kl[0]);
+    } else if (!live && !OutsideSequences(a, row)) {
+      if (tid == 0)
+        WriteZeros(a, row);
+      if (want_grad)
+        ZeroRow<DT>(g, n, tid, kThreads);
+    }
+    row = next;
+    live = next_live;
+  }
+}
+
+// The entries of one row, NE a lane: columns (-1 outside the vocabulary, where
+// the logit is 0, and behind the list) and logits.
+template <int NE> struct Entries {
   int col[NE];
-  float xv[NE], yv[NE];
+  float x[NE], y[NE];
+};
+
+template <int NE>
+__device__ __forceinline__ void LoadColumns(const RowLossParams &a, std::int64_t start, int moves,
+                                            Entries<NE> &e) {
 #pragma unroll
   for (int r = 0; r < NE; ++r) {
-    const int i = r * 64 + lane;
-    col[r] = -1;
+    const int i = r * 64 + (threadIdx.x & 63);
+    e.col[r] = -1;
     if (i < moves) {
       const int k = a.indices[start + i];
-      col[r] = k >= 0 && k < n ? k : -1;
+      e.col[r] = k >= 0 && k < a.vocab ? k : -1;
     }
   }
+}
+
+template <int DT, bool REF, int NE>
+__device__ __forceinline__ void LoadLogits(const RowLossParams &a, std::int64_t row, int moves,
+                                           Entries<NE> &e) {
+  using E = Elem<DT>;
+  using T = typename E::T;
+  const ConstRow<DT> x = RowOf<DT>(a.x, row, a.ldx);
+  const ConstRow<DT> y = RowOf<DT>(a.y, row, a.ldy);
 #pragma unroll
   for (int r = 0; r < NE; ++r) {
-    const bool in = r * 64 + lane < moves, inside = col[r] >= 0;
-    xv[r] = inside ? E::One(x[col[r]]) : in ? 0.f : -__builtin_inff();
+    const bool listed = r * 64 + static_cast<int>(threadIdx.x & 63) < moves;
+    const bool inside = e.col[r] >= 0;
+    e.x[r] = inside ? E::One(x[e.col[r]]) : listed ? 0.f : -__builtin_inff();
+    e.y[r] = 0.f;
     if constexpr (REF)
-      yv[r] = inside ? E::One(y[col[r]]) : in ? 0.f : -__builtin_inff();
+      e.y[r] = inside ? E::One(y[e.col[r]]) : listed ? 0.f : -__builtin_inff();
   }
-  bool twice = false;
-  if (g) {
-    ZeroRow<DT>(g, n, lane, 64);
-    for (int i = lane; i < words; i += 64)
-      seen[i] = 0;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-    for (int r = 0; r < NE; ++r) {
-      if (r * 64 >= moves)
-        break;
-      bool again = false;
-      if (col[r] >= 0) {
-        const std::uint32_t bit = 1u << (col[r] & 31);
-        again = atomicOr(seen + (col[r] >> 5), bit) & bit;
-      }
-      twice = twice || __any(again);
-    }
-  }
+}
+
+// One row's legal moves by one wave.  The gradient row is put together in LDS,
+// part_cols columns at a time, and written once, in whole vectors: zeros, and
+// each entry's value in its column.  A move listed twice adds up: each entry
+// first leaves its number in its column, and where one finds another's, the
+// first of equal entries counts them and writes for all.
+template <int DT, bool REF, bool PAST, int NE>
+__device__ __forceinline__ void MovesRow(const RowLossParams &a, std::int64_t row,
+                                         const RowInputs &in, const Entries<NE> &entries,
+                                         unsigned char *lds, int part_cols) {
+  using E = Elem<DT>;
+  using T = typename E::T;
+  constexpr int VE = E::kPerVec;
+  const int lane = threadIdx.x & 63;
+  const int n = a.vocab, act = in.action;
+  const Row<DT> g = RowOf<DT>(a.g, row, a.ldg);
+  const bool want_grad = a.g != nullptr;
+  T *buf = reinterpret_cast<T *>(lds);
+  const auto clear = [&](int cols) {
+    for (int v = lane; v * VE < cols; v += 64)
+      *reinterpret_cast<u32x4 *>(buf + v * VE) = u32x4{0, 0, 0, 0};
+  };
+  const int(&col)[NE] = entries.col;
+  const float(&xv)[NE] = entries.x;
+  const float(&yv)[NE] = entries.y;
+  if (want_grad)
+    clear(n < part_cols ? n : part_cols);
   // The entry of the action (the first of equal ones).
   bool acted = false;
-  float xa = 0.f;
-  float m = -__builtin_inff();
+  float xa = 0.f, m = xv[0];
 #pragma unroll
   for (int r = 0; r < NE; ++r) {
-    if (r * 64 >= moves)
-      break;
     m = fmaxf(m, xv[r]);
     const unsigned long long hit = __ballot(act >= 0 && col[r] == act);
     if (hit && !acted) {
       acted = true;
-      xa = __shfl(xv[r], __ffsll(hit) - 1);
+      xa = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(xv[r]), __ffsll(hit) - 1));
     }
   }
   m = WaveMax(m);
@@ -774,108 +993,172 @@ __global__ __launch_bounds__(256) void MovesRowKernel(RowLossParams a) {
   const float c = a.inv_temp * kLog2e;
   float sums[3] = {0.f, 0.f, 0.f};
 #pragma unroll
-  for (int r = 0; r < NE; ++r) {
-    if (r * 64 >= moves)
-      break;
-    AddStats<REF, true>(xv[r], REF ? yv[r] : 0.f, m, c, sums);
-  }
-  GroupSum<1>(sums, nullptr);
+  for (int r = 0; r < NE; ++r)
+    AddStats<REF, true>(xv[r], yv[r], m, c, sums);
+  sums[0] = WaveSum(sums[0]);
+  sums[1] = WaveSum(sums[1]);
+  if constexpr (REF)
+    sums[2] = WaveSum(sums[2]);
   const RowStats st = Stats(m, sums, a.inv_temp);
-  if (st.empty) {
-    if (lane == 0)
-      WriteZeros(a, row);
-    return;  // the gradient's zeros are written
-  }
-  const RowResult res = Evaluate(a, row, w, st, acted, xa);
+  const RowResult res = Evaluate(a, in, st, acted, xa);
   const bool want_kl = REF && WantsKl(a);
-  float kl[1] = {0.f};
-  if (g || want_kl) {
+  float kl = 0.f, f[NE] = {};
+  if (!st.empty && (want_grad || want_kl)) {
     const Coefs k = CoefsOf(st, res.grad, a.inv_temp);
-    float f[NE];
 #pragma unroll
     for (int r = 0; r < NE; ++r) {
-      if (r * 64 >= moves)
-        break;
-      const float xs[1] = {xv[r]}, ys[1] = {REF ? yv[r] : 0.f};
+      const float xs[1] = {xv[r]}, ys[1] = {yv[r]};
       float ft[1];
-      FinishEntries<1, REF, true>(k, want_kl, xs, ys, kl[0], ft);
+      FinishEntries<1, REF, true>(k, want_kl, xs, ys, kl, ft);
       f[r] = ft[0];
     }
-    if (g) {
+    if (want_kl)
+      kl = KlOf(WaveSum(kl), st.mean_d);
+  }
+  if (lane == 0) {
+    if (st.empty)
+      WriteZeros(a, row);
+    else
+      WriteRow(a, row, in.weight, acted, res, kl);
+  }
+  if (!want_grad)
+    return;
+  for (int p0 = 0; p0 < n; p0 += part_cols) {
+    const int cols = n - p0 < part_cols ? n - p0 : part_cols;
+    if (p0 > 0)
+      clear(cols);
+    if (!st.empty) {
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      if (!twice) {
+      bool other = false;
 #pragma unroll
-        for (int r = 0; r < NE; ++r) {
-          if (r * 64 >= moves)
-            break;
-          if (col[r] >= 0)
-            g[col[r]] = E::Round(col[r] == act ? f[r] + res.grad.scale * res.grad.slope : f[r]);
-        }
-      } else {
-        for (int r = 0; r * 64 < moves; ++r) {
+      for (int r = 0; r < NE; ++r)
+        if (col[r] >= p0 && col[r] < p0 + cols)
+          buf[col[r] - p0] = static_cast<T>(r * 64 + lane);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+      for (int r = 0; r < NE; ++r)
+        if (col[r] >= p0 && col[r] < p0 + cols)
+          other = other || buf[col[r] - p0] != static_cast<T>(r * 64 + lane);
+      const bool twice = __any(other);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+      for (int r = 0; r < NE; ++r) {
+        float value = f[r];
+        bool writes = col[r] >= p0 && col[r] < p0 + cols;
+        if (twice) {
           float times = 0.f;
-          bool first = true;
-          const int mine = r == 0 ? col[0] : r == 1 ? col[1] : r == 2 ? col[2] : col[3];
-          const float value = r == 0 ? f[0] : r == 1 ? f[1] : r == 2 ? f[2] : f[3];
-          for (int i = 0; i < moves; ++i) {
-            const int q = i >> 6;
-            const int other =
-                __shfl(q == 0 ? col[0] : q == 1 ? col[1] : q == 2 ? col[2] : col[3], i & 63);
-            if (other == mine) {
-              times += 1.f;
-              first = first && i >= r * 64 + lane;
+#pragma unroll
+          for (int q = 0; q < NE; ++q)
+#pragma unroll 1
+            for (int i = 0; i < 64; ++i) {
+              const int same = __builtin_amdgcn_readlane(col[q], i);
+              if (same == col[r]) {
+                times += 1.f;
+                writes = writes && q * 64 + i >= r * 64 + lane;
+              }
             }
-          }
-          if (mine >= 0 && first)
-            g[mine] = E::Round(mine == act ? times * value + res.grad.scale * res.grad.slope
-                                           : times * value);
+          value *= times;
         }
+        if (writes)
+          buf[col[r] - p0] =
+              E::Round(col[r] == act ? value + res.grad.scale * res.grad.slope : value);
       }
     }
-    if (want_kl) {
-      GroupSum<1>(kl, nullptr);
-      kl[0] = KlOf(kl[0], st.mean_d);
-    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const int vecs = cols / VE;
+    for (int v = lane; v < vecs; v += 64)
+      StoreVec<DT, PAST>(g + p0 + v * VE, *reinterpret_cast<const u32x4 *>(buf + v * VE));
+    const int t = vecs * VE + lane;
+    if (lane < VE && t < cols)
+      g[p0 + t] = buf[t];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
-  if (lane == 0)
-    WriteRow(a, row, w, acted, res, kl[0]);
 }
 
-template <int DT, bool REF, int W, int NV>
+// Four waves to a workgroup, each with a row of its own.  A row of up to 64
+// moves, as nearly all have, takes one entry a lane.  (Four rows a wave, their
+// lists and logits loaded together, took 20 % longer at 20000 rows and 60 % at
+// 1000: the waves hide each other's loads.)
+constexpr int kPartBytes = 8192;  // of each wave's LDS
+template <int DT, bool REF, bool PAST>
+__global__ __launch_bounds__(256) void MovesRowKernel(RowLossParams a, int part_cols) {
+  using T = typename Elem<DT>::T;
+  extern __shared__ u32x4 parts[];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const std::int64_t row = a.row0 + static_cast<std::int64_t>(blockIdx.x) * 4 + wave;
+  if (row >= a.end || OutsideSequences(a, row))
+    return;
+  const RowInputs in = Inputs(a, row);
+  std::int64_t start = a.offsets[row], count = a.offsets[row + 1];
+  if (in.weight == 0.f) {
+    if ((threadIdx.x & 63) == 0)
+      WriteZeros(a, row);
+    if (a.g)
+      ZeroRow<DT>(RowOf<DT>(a.g, row, a.ldg), a.vocab, threadIdx.x & 63, 64);
+    return;
+  }
+  start = start < 0 ? 0 : start > a.n_moves ? a.n_moves : start;
+  count = (count > a.n_moves ? a.n_moves : count) - start;
+  const int moves = count < 0 ? 0 : count > kMaxMoves ? kMaxMoves : static_cast<int>(count);
+  unsigned char *lds = reinterpret_cast<unsigned char *>(parts) +
+                       static_cast<size_t>(wave) * part_cols * sizeof(T);
+  if (moves <= 64) {
+    Entries<1> e;
+    LoadColumns(a, start, moves, e);
+    LoadLogits<DT, REF>(a, row, moves, e);
+    MovesRow<DT, REF, PAST>(a, row, in, e, lds, part_cols);
+  } else {
+    Entries<kMaxMoves / 64> e;
+    LoadColumns(a, start, moves, e);
+    LoadLogits<DT, REF>(a, row, moves, e);
+    MovesRow<DT, REF, PAST>(a, row, in, e, lds, part_cols);
+  }
+}
+
+template <int DT, bool REF, bool PAST, int W, int NV>
 void LaunchDense(const RowLossParams &p, unsigned rows, hipStream_t s) {
-  if constexpr (W == 1)
-    hipLaunchKernelGGL((DenseRowKernel<DT, 1, NV, REF>), dim3((rows + 3) / 4), dim3(256), 0, s, p);
-  else
-    hipLaunchKernelGGL((DenseRowKernel<DT, W, NV, REF>), dim3(rows), dim3(64 * W), 0, s, p);
+  hipLaunchKernelGGL((DenseRowKernel<DT, W, NV, REF, PAST>), dim3(W == 1 ? (rows + 3) / 4 : rows),
+                     dim3(W == 1 ? 256 : 64 * W), 0, s, p);
 }
 
-template <int DT, bool REF>
+template <int DT, bool REF, bool PAST>
 void LaunchRows(const RowLossParams &p, unsigned rows, hipStream_t s) {
   constexpr int VE = Elem<DT>::kPerVec;
-  constexpr int WIDE = VE == 4 ? 8 : 4;  // vectors of a lane that hold 2048 columns
   if (p.offsets) {
-    const unsigned bits = 4 * ((p.vocab + 31) / 32) * sizeof(std::uint32_t);
-    hipLaunchKernelGGL((MovesRowKernel<DT, REF>), dim3((rows + 3) / 4), dim3(256), p.g ? bits : 0,
-                       s, p);
+    // A part is a whole number of vectors.
+    constexpr int ES = 16 / VE;
+    const int whole = (p.vocab + VE - 1) / VE * VE;
+    const int part = whole < kPartBytes / ES ? whole : kPartBytes / ES;
+    hipLaunchKernelGGL((MovesRowKernel<DT, REF, PAST>), dim3((rows + 3) / 4), dim3(256),
+                       p.g ? 4 * part * ES : 0, s, p, part);
     return;
   }
   const int vecs = p.vocab / VE;
   if (vecs <= 64)
-    LaunchDense<DT, REF, 1, 1>(p, rows, s);
+    LaunchDense<DT, REF, PAST, 1, 1>(p, rows, s);
   else if (vecs <= 128)
-    LaunchDense<DT, REF, 1, 2>(p, rows, s);
-  else if (vecs <= 64 * WIDE / 2)
-    LaunchDense<DT, REF, 1, WIDE / 2>(p, rows, s);
-  else if (vecs <= 64 * WIDE)
-    LaunchDense<DT, REF, 1, WIDE>(p, rows, s);
-  else if (vecs <= 256 * 4)
-    LaunchDense<DT, REF, 4, 4>(p, rows, s);
-  else if (vecs <= 1024 * 4)
-    LaunchDense<DT, REF, 16, 4>(p, rows, s);
-  else if (vecs <= 1024 * 8)
-    LaunchDense<DT, REF, 16, 8>(p, rows, s);
+    LaunchDense<DT, REF, PAST, 1, 2>(p, rows, s);
+  else if (vecs <= 256)
+    LaunchDense<DT, REF, PAST, 1, 4>(p, rows, s);
+  else if (vecs <= 512)
+    LaunchDense<DT, REF, PAST, 4, 2>(p, rows, s);
+  else if (vecs <= 1024)
+    LaunchDense<DT, REF, PAST, 4, 4>(p, rows, s);
+  else if (vecs <= 4096)
+    LaunchDense<DT, REF, PAST, MIDW, 64 / MIDW>(p, rows, s);
+  else if (vecs <= 8192)
+    hipLaunchKernelGGL((LoopRowKernel<DT, 8, REF>), dim3(rows < LOOPG ? rows : LOOPG), dim3(1024),
+                       0, s, p);
   else
-    hipLaunchKernelGGL((LongRowKernel<DT, REF>), dim3(rows), dim3(1024), 0, s, p);
+    hipLaunchKernelGGL((StreamRowKernel<DT, REF>), dim3(rows), dim3(1024), 0, s, p);
+}
+
+template <int DT>
+void LaunchRowsOf(const RowLossParams &p, bool past, unsigned rows, hipStream_t s) {
+  if (p.y)
+    past ? LaunchRows<DT, true, true>(p, rows, s) : LaunchRows<DT, true, false>(p, rows, s);
+  else
+    past ? LaunchRows<DT, false, true>(p, rows, s) : LaunchRows<DT, false, false>(p, rows, s);
 }
 
 // Sum over the 256 threads of a workgroup, in a fixed order.
@@ -968,19 +1251,19 @@ hipError_t LaunchRowLoss(const RowLossParams &p, hipStream_t stream, std::string
     return hipErrorInvalidValue;
   }
   RowLossParams q = p;
+  const double arrays = 1.0 + (p.y != nullptr) + (p.g != nullptr);
+  const bool past = arrays * p.rows * p.vocab * DTypeBytes(p.dtype) > kPastBytes;
   // A launch holds fewer than 2^32 threads.
   constexpr std::int64_t kRows = std::int64_t(1) << 21;
   for (q.row0 = 0; q.row0 < p.rows; q.row0 += kRows) {
-    const unsigned rows =
-        static_cast<unsigned>(p.rows - q.row0 < kRows ? p.rows - q.row0 : kRows);
-    switch (p.dtype * 2 + (p.y ? 1 : 0)) {
-    case 2 * DT_F32: LaunchRows<DT_F32, false>(q, rows, stream); break;
-    case 2 * DT_F32 + 1: LaunchRows<DT_F32, true>(q, rows, stream); break;
-    case 2 * DT_BF16: LaunchRows<DT_BF16, false>(q, rows, stream); break;
-    case 2 * DT_BF16 + 1: LaunchRows<DT_BF16, true>(q, rows, stream); break;
-    case 2 * DT_F16: LaunchRows<DT_F16, false>(q, rows, stream); break;
-    default: LaunchRows<DT_F16, true>(q, rows, stream); break;
-    }
+    q.end = p.rows - q.row0 < kRows ? p.rows : q.row0 + kRows;
+    const unsigned rows = static_cast<unsigned>(q.end - q.row0);
+    if (p.dtype == DT_F32)
+      LaunchRowsOf<DT_F32>(q, past, rows, stream);
+    else if (p.dtype == DT_BF16)
+      LaunchRowsOf<DT_BF16>(q, past, rows, stream);
+    else
+      LaunchRowsOf<DT_F16>(q, past, rows, stream);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess)
       return e;
