@@ -24,12 +24,7 @@ constexpr float kLog2e = 1.44269504f;
 constexpr float kLog2eLow = 1.92596299e-8f;  // log2(e) - kLog2e
 constexpr float kLn2 = 0.69314718f;
 constexpr int kMaxMoves = 256;
-#ifndef LOOPG
-#define LOOPG 256
-#endif
-#ifndef MIDW
-#define MIDW 8
-#endif
+constexpr unsigned kCus = 256;
 constexpr double kPastBytes = 32e6;
 
 // 16 bytes of a row at any element's alignment (global memory takes
@@ -229,6 +224,57 @@ __device__ __forceinline__ float GroupMax(float v, float (*red)[4]) {
   return v;
 }
 
+// Sums over a row's entries: of e, of e log2(e), of e d with d = x - y; and the
+// least d.
+struct Sums {
+  float e = 0.f, et = 0.f, ed = 0.f, least = __builtin_inff();
+};
+
+// One entry's part, t = log2(e).  GUARD: an entry whose e is 0 adds nothing,
+// also where its logits are infinite.  Rows without such entries are summed
+// without the guard, and again with it if a sum comes out NaN (0 times
+// infinity): it costs two of nine instructions.
+template <bool REF, bool GUARD>
+__device__ __forceinline__ void AddStats(float x, float y, float m, float c, Sums &s) {
+  const float t = (x - m) * c, e = Exp2(t);
+  s.e += e;
+  s.et += GUARD && e == 0.f ? 0.f : e * t;
+  if constexpr (REF) {
+    const float d = x - y;
+    s.ed += GUARD && e == 0.f ? 0.f : e * d;
+    s.least = fminf(s.least, d);
+  }
+}
+
+// Over the W waves of a workgroup, in one exchange.
+template <int W, bool REF> __device__ __forceinline__ void GroupSums(Sums &s, float (*red)[4]) {
+  s.e = WaveSum(s.e);
+  s.et = WaveSum(s.et);
+  if constexpr (REF) {
+    s.ed = WaveSum(s.ed);
+    s.least = -WaveMax(-s.least);
+  }
+  if constexpr (W > 1) {
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0)
+      *reinterpret_cast<f32x4 *>(red[threadIdx.x >> 6]) = f32x4{s.e, s.et, s.ed, s.least};
+    __syncthreads();
+    const f32x4 v = *reinterpret_cast<const f32x4 *>(red[threadIdx.x & (W - 1)]);
+    s.e = LanesSum<W>(v[0]);
+    s.et = LanesSum<W>(v[1]);
+    if constexpr (REF) {
+      s.ed = LanesSum<W>(v[2]);
+      s.least = -LanesMax<W>(-v[3]);
+    }
+  }
+}
+
+// A NaN, or an entry so far below the reference (u < -60) that exp(-u) may
+// overflow.
+template <bool REF> __device__ __forceinline__ bool NeedsGuard(const Sums &s, float inv_temp) {
+  return s.et != s.et || s.ed != s.ed || (REF && !(s.least * inv_temp - s.ed / s.e * inv_temp > -60.f));
+}
+
 // What a row's scalars come to, from its statistics.
 struct RowStats {
   float m;         // maximum (0 where every entry is masked)
@@ -239,34 +285,16 @@ struct RowStats {
   bool empty;      // no entry left
 };
 
-// sums: of e, of e log2(e) and of e (x - y).
-__device__ __forceinline__ RowStats Stats(float m, const float (&sums)[3], float inv_temp) {
+__device__ __forceinline__ RowStats Stats(float m, const Sums &sums, float inv_temp) {
   RowStats r;
   r.m = m;
-  r.empty = sums[0] == 0.f;
-  const float sum = r.empty ? 1.f : sums[0], inv = Rcp(sum);
+  r.empty = sums.e == 0.f;
+  const float sum = r.empty ? 1.f : sums.e, inv = Rcp(sum);
   r.log2_sum = Log2(sum);
   r.log_sum = r.log2_sum * kLn2;
-  r.mean_z = sums[1] * kLn2 * inv;
-  r.mean_d = sums[2] * inv_temp * inv;
+  r.mean_z = sums.et * kLn2 * inv;
+  r.mean_d = sums.ed * inv_temp * inv;
   return r;
-}
-
-// One entry's part of the statistics, t = log2(e).  GUARD: an entry whose e is
-// 0 adds nothing, also where its logits are infinite.  Rows without such
-// entries are summed without the guard, and again with it if a sum comes out
-// NaN (0 times infinity): it costs two of nine instructions.
-template <bool REF, bool GUARD>
-__device__ __forceinline__ void AddStats(float x, float y, float m, float c, float (&s)[3]) {
-  const float t = (x - m) * c, e = Exp2(t);
-  s[0] += e;
-  s[1] += GUARD && e == 0.f ? 0.f : e * t;
-  if constexpr (REF)
-    s[2] += GUARD && e == 0.f ? 0.f : e * (x - y);
-}
-
-__device__ __forceinline__ bool NeedsGuard(const float (&s)[3]) {
-  return s[1] != s[1] || s[2] != s[2];
 }
 
 // Coefficients of one row's gradient
@@ -294,18 +322,17 @@ __device__ __forceinline__ Coefs CoefsOf(const RowStats &st, const RowGrad &g, f
   return k;
 }
 
-// (exp(-u) - 1 + u) / u^2 for |u| <= 2: its interpolation of degree 8 in the
-// Chebyshev nodes there, 1.6e-7 from it relative (3.0e-7 with the roundings).
-__device__ __forceinline__ float KlSeries(float u) {
-  float r = 0x1.3cbf98p-22f;
-  r = r * u - 0x1.91528cp-19f;
-  r = r * u + 0x1.9f1d2ap-16f;
-  r = r * u - 0x1.9e9c00p-13f;
-  r = r * u + 0x1.6c1b2ap-10f;
-  r = r * u - 0x1.1117bcp-7f;
-  r = r * u + 0x1.55554ap-5f;
-  r = r * u - 0x1.555536p-3f;
-  return r * u + 0x1.000000p-1f;
+// exp(-u) - 1 + u for u > -60: its series for |u| < 1/4 (the first term left out
+// is 1.2e-8 of the sum), where the difference would cancel.
+__device__ __forceinline__ float Phi(float u) {
+  const float e = Exp2(-u * kLog2e);
+  float r = -1.f / 5040;
+  r = r * u + 1.f / 720;
+  r = r * u - 1.f / 120;
+  r = r * u + 1.f / 24;
+  r = r * u - 1.f / 6;
+  r = r * u + 0.5f;
+  return fabsf(u) < 0.25f ? u * u * r : (e - 1.f) + u;
 }
 
 // p (exp(-u) - 1 + u), the term of KL, for any u; ym: the reference logit less
@@ -317,9 +344,7 @@ __device__ __forceinline__ float KlTerm(const Coefs &k, float p, float u, float 
     const float q = Exp2(ym * k.c + k.kl_shift);
     return p == 0.f ? q : q - p * (1.f - u);
   }
-  if (p == 0.f)
-    return 0.f;
-  return fabsf(u) <= 2.f ? p * u * u * KlSeries(u) : p * (Exp2(-u * kLog2e) - 1.f + u);
+  return p == 0.f ? 0.f : p * Phi(u);
 }
 
 // KL from the sum of its terms; infinite where the reference lacks what the
@@ -329,11 +354,11 @@ __device__ __forceinline__ float KlOf(float terms, float mean_d) {
 }
 
 // The gradient of N entries without the action's own term, and their part of
-// KL.  The terms of KL take the series unless an entry of the wave needs more.
+// KL.  GUARD: as for the sums, and any u.
 template <int N, bool REF, bool GUARD>
 __device__ __forceinline__ void FinishEntries(const Coefs &k, bool want_kl, const float (&x)[N],
                                               const float (&y)[N], float &kl, float (&f)[N]) {
-  float p[N], u[N], top = 0.f;
+  float p[N], u[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const float xm = x[i] - k.m;
@@ -341,27 +366,28 @@ __device__ __forceinline__ void FinishEntries(const Coefs &k, bool want_kl, cons
     float v = k.a * xm + k.d;
     if constexpr (REF) {
       u[i] = (x[i] - y[i]) * k.inv_temp - k.mean_d;
-      top = fmaxf(top, fabsf(u[i]));
       v = k.b * u[i] + v;
     }
     f[i] = GUARD && p[i] == 0.f ? 0.f : p[i] * v;
   }
   if (REF && want_kl) {
-    if (GUARD || __any(!(top <= 2.f))) {
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        kl += KlTerm(k, p[i], u[i], y[i] - k.m);
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        kl += p[i] * (u[i] * u[i]) * KlSeries(u[i]);
-    }
+    for (int i = 0; i < N; ++i)
+      kl += GUARD ? KlTerm(k, p[i], u[i], y[i] - k.m) : p[i] * Phi(u[i]);
   }
 }
 
 // Whether the divergence itself is asked for (its gradient needs no KL).
 __device__ __forceinline__ bool WantsKl(const RowLossParams &a) {
   return a.kl || (a.loss && a.kl_coef != 0.f);
+}
+
+// Element i of an input array, i the same in the whole wave, by a scalar load:
+// a vector load would be waited for behind every row load and store that the
+// wave has on its way.  No kernel writes the array while this one runs (an
+// output that is d_old_logp has each row's value read before it is written).
+template <class T> __device__ __forceinline__ T Uniform(const T *p, std::int64_t i) {
+  return ((const MFH_CONSTANT T *)p)[i];
 }
 
 // A row's scalar inputs, loaded together before anything waits on one.
@@ -372,10 +398,10 @@ struct RowInputs {
 };
 __device__ __forceinline__ RowInputs Inputs(const RowLossParams &a, std::int64_t row) {
   RowInputs r;
-  r.weight = a.coef ? a.coef[row] : a.weight ? a.weight[row] : 1.f;
-  r.action = a.actions ? a.actions[row] : -1;
-  r.advantage = a.advantage ? a.advantage[row] : 0.f;
-  r.old_logp = a.old_logp ? a.old_logp[row] : 0.f;
+  r.weight = a.coef ? Uniform(a.coef, row) : a.weight ? Uniform(a.weight, row) : 1.f;
+  r.action = a.actions ? Uniform(a.actions, row) : -1;
+  r.advantage = a.advantage ? Uniform(a.advantage, row) : 0.f;
+  r.old_logp = a.old_logp ? Uniform(a.old_logp, row) : 0.f;
   return r;
 }
 
@@ -456,7 +482,8 @@ __device__ __forceinline__ void WriteZeros(const RowLossParams &a, std::int64_t 
 }
 
 __device__ __forceinline__ bool OutsideSequences(const RowLossParams &a, std::int64_t row) {
-  return a.seq_offsets && (row < a.seq_offsets[0] || row >= a.seq_offsets[a.n_seq]);
+  return a.seq_offsets &&
+         (row < Uniform(a.seq_offsets, 0) || row >= Uniform(a.seq_offsets, a.n_seq));
 }
 
 // Zeros in a whole gradient row, by `threads` threads.
@@ -483,7 +510,7 @@ __device__ __forceinline__ void Unpack(u32x4 v, float (&x)[Elem<DT>::kPerVec]) {
 }
 
 template <int DT, bool REF, bool GUARD>
-__device__ __forceinline__ void AddVec(u32x4 xr, u32x4 yr, float m, float c, float (&sums)[3]) {
+__device__ __forceinline__ void AddVec(u32x4 xr, u32x4 yr, float m, float c, Sums &sums) {
   constexpr int VE = Elem<DT>::kPerVec;
   float xs[VE], ys[VE] = {};
   Unpack<DT>(xr, xs);
@@ -552,7 +579,7 @@ template <int DT, int W, int NV, bool REF, bool PAST>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void DenseRowKernel(RowLossParams a) {
   using E = Elem<DT>;
   constexpr int VE = E::kPerVec;
-  __shared__ float red[W][4];
+  __shared__ __align__(16) float red[W][4];
   const int tid = W == 1 ? threadIdx.x & 63 : threadIdx.x;
   std::int64_t row = blockIdx.x;
   if constexpr (W == 1)
@@ -610,10 +637,10 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void DenseRowKernel(RowLossP
   m = m == -__builtin_inff() ? 0.f : m;
 
   const float c = a.inv_temp * kLog2e;
-  float sums[3];
+  Sums sums;
   const auto sum = [&](auto guard) MFH_INLINE {
     constexpr bool GUARD = decltype(guard)::value;
-    sums[0] = sums[1] = sums[2] = 0.f;
+    sums = Sums{};
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       Repack(xr[j]);
@@ -624,10 +651,10 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void DenseRowKernel(RowLossP
     }
     if (has_rest)
       AddStats<REF, GUARD>(xt[0], yt[0], m, c, sums);
-    GroupSum<W>(sums, red);
+    GroupSums<W, REF>(sums, red);
   };
   sum(std::false_type{});
-  const bool guarded = NeedsGuard(sums);
+  const bool guarded = NeedsGuard<REF>(sums, a.inv_temp);
   if (guarded)
     sum(std::true_type{});
   const RowStats st = Stats(m, sums, a.inv_temp);
@@ -697,16 +724,17 @@ __device__ __forceinline__ void StreamRow(const RowLossParams &a, std::int64_t r
   const float yt[1] = {REF && has_rest ? E::One(y[vecs * VE + tid]) : 0.f};
 
   const float c = a.inv_temp * kLog2e;
-  float m = xt[0], sums[3] = {0.f, 0.f, 0.f};
+  float m = xt[0];
+  Sums sums;
   // Sums over the old maximum as sums over the new: e and t of each term fall
   // by the same step.
   const auto rescale = [&](float from, float to) MFH_INLINE {
-    if (sums[0] == 0.f)
+    if (sums.e == 0.f)
       return;
     const float step = (from - to) * c, f = Exp2(step);
-    sums[1] = f == 0.f ? 0.f : f * (sums[1] + sums[0] * step);
-    sums[0] *= f;
-    sums[2] = f == 0.f ? 0.f : f * sums[2];
+    sums.et = f == 0.f ? 0.f : f * (sums.et + sums.e * step);
+    sums.e *= f;
+    sums.ed = f == 0.f ? 0.f : f * sums.ed;
   };
   if (has_rest)
     AddStats<REF, true>(xt[0], yt[0], m == -__builtin_inff() ? 0.f : m, c, sums);
@@ -729,7 +757,7 @@ __device__ __forceinline__ void StreamRow(const RowLossParams &a, std::int64_t r
   top = top == -__builtin_inff() ? 0.f : top;
   rescale(m, top);
   m = top;
-  GroupSum<W>(sums, red);
+  GroupSums<W, REF>(sums, red);
   const RowStats st = Stats(m, sums, a.inv_temp);
   if (st.empty) {
     if (tid == 0)
@@ -769,7 +797,7 @@ __device__ __forceinline__ void StreamRow(const RowLossParams &a, std::int64_t r
 // Rows longer than the registers hold.
 template <int DT, bool REF>
 __global__ __launch_bounds__(1024) void StreamRowKernel(RowLossParams a) {
-  __shared__ float red[16][4];
+  __shared__ __align__(16) float red[16][4];
   const std::int64_t row = a.row0 + blockIdx.x;
   if (OutsideSequences(a, row))
     return;
@@ -790,12 +818,13 @@ __global__ __launch_bounds__(1024) void StreamRowKernel(RowLossParams a) {
 // vector of the present row it loads the next row's into its registers.  All
 // rows take the same way through the loop, so that there is one such place:
 // rows of weight 0 or none compute nothing of use and store nothing, and rows
-// that need the guards are streamed.  At least 4 * 1024 vectors a row.
+// that need the guards are streamed.  NV: the vectors of a lane, the last
+// one filled for some lane.
 template <int DT, int NV, bool REF>
 __global__ __launch_bounds__(1024) void LoopRowKernel(RowLossParams a) {
   using E = Elem<DT>;
   constexpr int VE = E::kPerVec, W = 16, kThreads = 64 * W;
-  __shared__ float red[W][4];
+  __shared__ __align__(16) float red[W][4];
   const int tid = threadIdx.x;
   const int n = a.vocab, vecs = n / VE, rest = n - vecs * VE;
   const bool has_rest = tid < rest;
@@ -804,20 +833,46 @@ __global__ __launch_bounds__(1024) void LoopRowKernel(RowLossParams a) {
   const float c = a.inv_temp * kLog2e;
 
   u32x4 xr[NV], yr[REF ? NV : 1];
-  // Vector j of a row; some vector of it where the row has fewer, and the
-  // row's first where there is nothing to read (`live` 0).
-  const auto load = [&](std::int64_t r, int j, int live) MFH_INLINE {
-    int v = j * kThreads + tid;
-    v = (v < vecs ? v : tid) * live;
-    xr[j] = LoadVec<DT, true>(RowOf<DT>(a.x, r, a.ldx) + v * VE);
+  // This lane's place among vectors j * kThreads on: NV is such that all are
+  // there but for the last j, where the lanes behind the end share its last.
+  // The same address arithmetic every time, from one register and the row's
+  // uniform address (addresses kept for all j would be spilled, and the wait
+  // for one to come back would be one for every load on its way).
+  const auto place = [&](int j) MFH_INLINE {
+    int lane = tid;
+    asm volatile("" : "+v"(lane));
+    const int end = vecs - j * kThreads - 1;
+    return (j < NV - 1 || lane < end ? lane : end) * VE;
+  };
+  const auto filled = [&](int j) MFH_INLINE { return j < NV - 1 || j * kThreads + tid < vecs; };
+  // Vector j of a row; the row's first ones where there is nothing to read.
+  const auto load = [&](std::int64_t r, int j, bool live) MFH_INLINE {
+    const int from = live ? j * kThreads * VE : 0, at = live ? place(j) : 0;
+    xr[j] = LoadVec<DT, true>(RowOf<DT>(a.x, r, a.ldx) + from + at);
     if constexpr (REF)
-      yr[j] = LoadVec<DT, true>(RowOf<DT>(a.y, r, a.ldy) + v * VE);
+      yr[j] = LoadVec<DT, true>(RowOf<DT>(a.y, r, a.ldy) + from + at);
   };
   const auto alive = [&](std::int64_t r) MFH_INLINE {
     return r < a.end && !OutsideSequences(a, r) && Inputs(a, r).weight != 0.f;
   };
+  // The action's logits and the elements behind the last vector (some logit of
+  // the row where there is none), as they are: a conversion would wait.
+  struct Few {
+    typename E::T xa, ya, xt, yt;
+  };
+  const auto load_few = [&](std::int64_t r, int act) MFH_INLINE {
+    const ConstRow<DT> x = RowOf<DT>(a.x, r, a.ldx), y = RowOf<DT>(a.y, r, a.ldy);
+    const int at = act >= 0 && act < n ? act : 0, last = has_rest ? vecs * VE + tid : 0;
+    Few f{x[at], 0, x[last], 0};
+    if constexpr (REF) {
+      f.ya = y[at];
+      f.yt = y[last];
+    }
+    return f;
+  };
   std::int64_t row = a.row0 + blockIdx.x;
   bool live = alive(row);
+  Few few = load_few(row, Inputs(a, row).action);
 #pragma unroll
   for (int j = 0; j < NV; ++j)
     load(row, j, live);
@@ -825,20 +880,18 @@ __global__ __launch_bounds__(1024) void LoopRowKernel(RowLossParams a) {
     const std::int64_t next = row + gridDim.x;
     const bool next_live = alive(next);
     const std::int64_t next_row = next < a.end ? next : row;
-    const ConstRow<DT> x = RowOf<DT>(a.x, row, a.ldx);
-    const ConstRow<DT> y = RowOf<DT>(a.y, row, a.ldy);
     const Row<DT> g = RowOf<DT>(a.g, row, a.ldg);
     const RowInputs in = Inputs(a, row);
     const int act = in.action;
     const bool acted = act >= 0 && act < n;
-    const float xa = acted ? E::One(x[act]) : 0.f;
-    const float ya = REF && acted ? E::One(y[act]) : 0.f;
-    const float xt[1] = {has_rest ? E::One(x[vecs * VE + tid]) : -__builtin_inff()};
-    const float yt[1] = {REF && has_rest ? E::One(y[vecs * VE + tid]) : 0.f};
+    const Few next_few = load_few(next_row, Inputs(a, next_row).action);
+    const float xa = E::One(few.xa), ya = REF ? E::One(few.ya) : 0.f;
+    const float xt[1] = {has_rest ? E::One(few.xt) : -__builtin_inff()};
+    const float yt[1] = {REF && has_rest ? E::One(few.yt) : 0.f};
     float m = -__builtin_inff();
 #pragma unroll
     for (int j = 0; j < NV; ++j)
-      if (j * kThreads + tid < vecs) {
+      if (filled(j)) {
         float xs[VE];
         Unpack<DT>(xr[j], xs);
 #pragma unroll
@@ -847,21 +900,21 @@ __global__ __launch_bounds__(1024) void LoopRowKernel(RowLossParams a) {
       }
     m = GroupMax<W>(fmaxf(m, xt[0]), red);
     m = m == -__builtin_inff() ? 0.f : m;
-    float sums[3] = {0.f, 0.f, 0.f};
+    Sums sums;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       Repack(xr[j]);
       if (REF)
         Repack(yr[REF ? j : 0]);
-      if (j * kThreads + tid < vecs)
+      if (filled(j))
         AddVec<DT, REF, false>(xr[j], yr[REF ? j : 0], m, c, sums);
     }
     if (has_rest)
       AddStats<REF, false>(xt[0], yt[0], m, c, sums);
-    GroupSum<W>(sums, red);
+    GroupSums<W, REF>(sums, red);
     // A sum of 0 has a NaN beside it (0 times the -inf of its logits), as a
     // row that needs the guards does.
-    const bool stream = live && NeedsGuard(sums), here = live && !stream;
+    const bool stream = live && NeedsGuard<REF>(sums, a.inv_temp), here = live && !stream;
     if (stream) {
       StreamRow<DT, REF>(a, row, in, red);
 #pragma unroll
@@ -880,11 +933,10 @@ __global__ __launch_bounds__(1024) void LoopRowKernel(RowLossParams a) {
       Repack(xr[j]);
       if (REF)
         Repack(yr[REF ? j : 0]);
-      const int v = j * kThreads + tid;
-      if (v < vecs && (want_grad || want_kl)) {
+      if (filled(j) && (want_grad || want_kl)) {
         const u32x4 f = FinishVec<DT, REF, false>(k, want_kl, xr[j], yr[REF ? j : 0], kl[0]);
         if (want_grad && here)
-          StoreVec<DT, true>(g + v * VE, f);
+          StoreVec<DT, true>(g + j * kThreads * VE + place(j), f);
       }
       // Not earlier: the present row's vector is in the registers.
       __builtin_amdgcn_sched_barrier(0);
@@ -908,6 +960,7 @@ __global__ __launch_bounds__(1024) void LoopRowKernel(RowLossParams a) {
     }
     row = next;
     live = next_live;
+    few = next_few;
   }
 }
 
@@ -991,14 +1044,11 @@ __device__ __forceinline__ void MovesRow(const RowLossParams &a, std::int64_t ro
   m = WaveMax(m);
   m = m == -__builtin_inff() ? 0.f : m;
   const float c = a.inv_temp * kLog2e;
-  float sums[3] = {0.f, 0.f, 0.f};
+  Sums sums;
 #pragma unroll
   for (int r = 0; r < NE; ++r)
     AddStats<REF, true>(xv[r], yv[r], m, c, sums);
-  sums[0] = WaveSum(sums[0]);
-  sums[1] = WaveSum(sums[1]);
-  if constexpr (REF)
-    sums[2] = WaveSum(sums[2]);
+  GroupSums<1, REF>(sums, nullptr);
   const RowStats st = Stats(m, sums, a.inv_temp);
   const RowResult res = Evaluate(a, in, st, acted, xa);
   const bool want_kl = REF && WantsKl(a);
@@ -1089,7 +1139,7 @@ __global__ __launch_bounds__(256) void MovesRowKernel(RowLossParams a, int part_
   if (row >= a.end || OutsideSequences(a, row))
     return;
   const RowInputs in = Inputs(a, row);
-  std::int64_t start = a.offsets[row], count = a.offsets[row + 1];
+  std::int64_t start = Uniform(a.offsets, row), count = Uniform(a.offsets, row + 1);
   if (in.weight == 0.f) {
     if ((threadIdx.x & 63) == 0)
       WriteZeros(a, row);
@@ -1121,6 +1171,12 @@ void LaunchDense(const RowLossParams &p, unsigned rows, hipStream_t s) {
                      dim3(W == 1 ? 256 : 64 * W), 0, s, p);
 }
 
+template <int DT, bool REF, int NV>
+void LaunchLoop(const RowLossParams &p, unsigned rows, hipStream_t s) {
+  hipLaunchKernelGGL((LoopRowKernel<DT, NV, REF>), dim3(rows < kCus ? rows : kCus), dim3(1024), 0,
+                     s, p);
+}
+
 template <int DT, bool REF, bool PAST>
 void LaunchRows(const RowLossParams &p, unsigned rows, hipStream_t s) {
   constexpr int VE = Elem<DT>::kPerVec;
@@ -1145,10 +1201,15 @@ void LaunchRows(const RowLossParams &p, unsigned rows, hipStream_t s) {
   else if (vecs <= 1024)
     LaunchDense<DT, REF, PAST, 4, 4>(p, rows, s);
   else if (vecs <= 4096)
-    LaunchDense<DT, REF, PAST, MIDW, 64 / MIDW>(p, rows, s);
+    LaunchDense<DT, REF, PAST, 8, 8>(p, rows, s);
+  else if (vecs <= 5120)
+    LaunchLoop<DT, REF, 5>(p, rows, s);
+  else if (vecs <= 6144)
+    LaunchLoop<DT, REF, 6>(p, rows, s);
+  else if (vecs <= 7168)
+    LaunchLoop<DT, REF, 7>(p, rows, s);
   else if (vecs <= 8192)
-    hipLaunchKernelGGL((LoopRowKernel<DT, 8, REF>), dim3(rows < LOOPG ? rows : LOOPG), dim3(1024),
-                       0, s, p);
+    LaunchLoop<DT, REF, 8>(p, rows, s);
   else
     hipLaunchKernelGGL((StreamRowKernel<DT, REF>), dim3(rows), dim3(1024), 0, s, p);
 }
