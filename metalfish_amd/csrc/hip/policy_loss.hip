@@ -332,7 +332,10 @@ __device__ __forceinline__ float Phi(float u) {
   r = r * u + 1.f / 24;
   r = r * u - 1.f / 6;
   r = r * u + 0.5f;
-  return fabsf(u) < 0.25f ? u * u * r : (e - 1.f) + u;
+  float near = u * u * r, far = (e - 1.f) + u;
+  // Both, and a select: as a branch for each entry it took a fifth longer.
+  asm volatile("" : "+v"(near), "+v"(far));
+  return fabsf(u) < 0.25f ? near : far;
 }
 
 // p (exp(-u) - 1 + u), the term of KL, for any u; ym: the reference logit less
