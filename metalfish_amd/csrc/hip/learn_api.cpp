@@ -378,38 +378,25 @@ int mfh_preference_loss_device(const mfh_policy_rows *rows, const mfh_preference
     rc = Enter(fn, rows->device, ptrs, st, &on);
     if (rc != MFH_OK)
       return rc;
-    p.seq_offsets = loss->d_seq_offsets;
-    p.n_seq = 2 * loss->pairs;
-    float *mark = static_cast<float *>(loss->d_workspace);
-    float *coef = mark + rows->rows;
+    p.g = loss->d_grad;
+    p.ldg = loss->grad_stride;
+    mfh::PairLossParams q;
+    q.seq_offsets = loss->d_seq_offsets;
+    q.pairs = loss->pairs;
+    q.rows = rows->rows;
+    q.mark = static_cast<float *>(loss->d_workspace);
+    q.coef = q.mark + rows->rows;
+    q.ref_logp = loss->d_ref_logp;
+    q.weight = loss->d_weight;
+    q.kind = loss->kind;
+    q.average = loss->average != 0;
+    q.beta = loss->beta;
+    q.smoothing = loss->label_smoothing;
+    q.loss = loss->d_loss;
+    q.margin = loss->d_margin;
+    q.logp = loss->d_logp;
     std::string err;
-    p.mark = mark;
-    hipError_t e = mfh::LaunchRowLoss(p, st, &err);
-    if (e == hipSuccess) {
-      mfh::PairLossParams q;
-      q.seq_offsets = loss->d_seq_offsets;
-      q.pairs = loss->pairs;
-      q.rows = rows->rows;
-      q.mark = mark;
-      q.ref_logp = loss->d_ref_logp;
-      q.weight = loss->d_weight;
-      q.kind = loss->kind;
-      q.average = loss->average != 0;
-      q.beta = loss->beta;
-      q.smoothing = loss->label_smoothing;
-      q.loss = loss->d_loss;
-      q.margin = loss->d_margin;
-      q.logp = loss->d_logp;
-      q.coef = loss->d_grad ? coef : nullptr;
-      e = mfh::LaunchPairLoss(q, st, &err);
-    }
-    if (e == hipSuccess && loss->d_grad) {
-      p.mark = nullptr;
-      p.coef = coef;
-      p.g = loss->d_grad;
-      p.ldg = loss->grad_stride;
-      e = mfh::LaunchRowLoss(p, st, &err);
-    }
+    const hipError_t e = mfh::LaunchPreference(p, q, st, &err);
     return e == hipSuccess ? MFH_OK : HipError(fn, err.empty() ? "launch" : err.c_str(), e);
   } catch (const std::exception &e) {
     return Invalid(fn, e.what());

@@ -525,19 +525,24 @@ struct RowLossParams {
 };
 hipError_t LaunchRowLoss(const RowLossParams &p, hipStream_t stream, std::string *err);
 
-// One workgroup per pair of sequences: sums of (mark - ref_logp) over their
-// rows in 64 bits and a fixed order, the pair's loss and margin, and each
-// row's gradient coefficient (0 without an action) and log-probability.
+// Pairs of sequences of rows: marks of all rows; per pair the sums of (mark -
+// ref_logp) over its rows, in 64 bits and a fixed order, its loss and margin,
+// and each row's log-probability and gradient coefficient (0 without an
+// action); the gradient of all rows (rows.g).  Short lines of moves take one
+// launch, others three (two without a gradient).  mark and coef: workspace,
+// one value a row each.
 struct PairLossParams {
   const std::int32_t *seq_offsets = nullptr;
   std::int64_t pairs = 0, rows = 0;
-  const float *mark = nullptr, *ref_logp = nullptr, *weight = nullptr;
+  float *mark = nullptr;
+  const float *ref_logp = nullptr, *weight = nullptr;
   int kind = 0;
   bool average = false;
   float beta = 0.f, smoothing = 0.f;
   float *loss = nullptr, *margin = nullptr, *logp = nullptr, *coef = nullptr;
 };
-hipError_t LaunchPairLoss(const PairLossParams &p, hipStream_t stream, std::string *err);
+hipError_t LaunchPreference(const RowLossParams &rows, const PairLossParams &pairs,
+                            hipStream_t stream, std::string *err);
 
 // A part of one gradient tensor, at most kGradChunkBytes: a unit of work of
 // the norm and of the scaling.  dst may be null (norm only).

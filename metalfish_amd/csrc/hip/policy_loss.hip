@@ -24,7 +24,7 @@ constexpr float kLog2e = 1.44269504f;
 constexpr float kLog2eLow = 1.92596299e-8f;  // log2(e) - kLog2e
 constexpr float kLn2 = 0.69314718f;
 constexpr int kMaxMoves = 256;
-constexpr unsigned kCus = 256;
+constexpr unsigned kCus = 256, kFewRows = 1024;
 constexpr double kPastBytes = 32e6;
 
 // 16 bytes of a row at any element's alignment (global memory takes
@@ -992,7 +992,6 @@ template <int DT, bool REF, int NE>
 __device__ __forceinline__ void LoadLogits(const RowLossParams &a, std::int64_t row, int moves,
                                            Entries<NE> &e) {
   using E = Elem<DT>;
-  using T = typename E::T;
   const ConstRow<DT> x = RowOf<DT>(a.x, row, a.ldx);
   const ConstRow<DT> y = RowOf<DT>(a.y, row, a.ldy);
 #pragma unroll
@@ -1128,20 +1127,11 @@ __device__ __forceinline__ void MovesRow(const RowLossParams &a, std::int64_t ro
   }
 }
 
-// Four waves to a workgroup, each with a row of its own.  A row of up to 64
-// moves, as nearly all have, takes one entry a lane.  (Four rows a wave, their
-// lists and logits loaded together, took 20 % longer at 20000 rows and 60 % at
-// 1000: the waves hide each other's loads.)
-constexpr int kPartBytes = 8192;  // of each wave's LDS
+// A row by its list, by one wave.  Up to 64 moves, as nearly all rows have,
+// take one entry a lane.
 template <int DT, bool REF, bool PAST>
-__global__ __launch_bounds__(256) void MovesRowKernel(RowLossParams a, int part_cols) {
-  using T = typename Elem<DT>::T;
-  extern __shared__ u32x4 parts[];
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const std::int64_t row = a.row0 + static_cast<std::int64_t>(blockIdx.x) * 4 + wave;
-  if (row >= a.end || OutsideSequences(a, row))
-    return;
-  const RowInputs in = Inputs(a, row);
+__device__ __forceinline__ void ListedRow(const RowLossParams &a, std::int64_t row,
+                                          const RowInputs &in, unsigned char *lds, int part_cols) {
   std::int64_t start = Uniform(a.offsets, row), count = Uniform(a.offsets, row + 1);
   if (in.weight == 0.f) {
     if ((threadIdx.x & 63) == 0)
@@ -1153,8 +1143,6 @@ __global__ __launch_bounds__(256) void MovesRowKernel(RowLossParams a, int part_
   start = start < 0 ? 0 : start > a.n_moves ? a.n_moves : start;
   count = (count > a.n_moves ? a.n_moves : count) - start;
   const int moves = count < 0 ? 0 : count > kMaxMoves ? kMaxMoves : static_cast<int>(count);
-  unsigned char *lds = reinterpret_cast<unsigned char *>(parts) +
-                       static_cast<size_t>(wave) * part_cols * sizeof(T);
   if (moves <= 64) {
     Entries<1> e;
     LoadColumns(a, start, moves, e);
@@ -1166,6 +1154,31 @@ __global__ __launch_bounds__(256) void MovesRowKernel(RowLossParams a, int part_
     LoadLogits<DT, REF>(a, row, moves, e);
     MovesRow<DT, REF, PAST>(a, row, in, e, lds, part_cols);
   }
+}
+
+// Four waves to a workgroup, each with a row of its own.  (Four rows a wave,
+// their lists and logits loaded together, took 20 % longer at 20000 rows and
+// 60 % at 1000: the waves hide each other's loads.)
+constexpr int kPartBytes = 8192;  // of each wave's LDS
+template <int DT, bool REF, bool PAST>
+__global__ __launch_bounds__(256) void MovesRowKernel(RowLossParams a, int part_cols) {
+  extern __shared__ u32x4 parts[];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const std::int64_t row = a.row0 + static_cast<std::int64_t>(blockIdx.x) * 4 + wave;
+  if (row >= a.end || OutsideSequences(a, row))
+    return;
+  ListedRow<DT, REF, PAST>(a, row, Inputs(a, row),
+                           reinterpret_cast<unsigned char *>(parts) +
+                               static_cast<size_t>(wave) * part_cols *
+                                   sizeof(typename Elem<DT>::T),
+                           part_cols);
+}
+
+// Columns of a part of a row in LDS: a whole number of vectors.
+template <int DT> int PartCols(int vocab) {
+  constexpr int VE = Elem<DT>::kPerVec, most = kPartBytes / (16 / VE);
+  const int whole = (vocab + VE - 1) / VE * VE;
+  return whole < most ? whole : most;
 }
 
 template <int DT, bool REF, bool PAST, int W, int NV>
@@ -1184,17 +1197,16 @@ template <int DT, bool REF, bool PAST>
 void LaunchRows(const RowLossParams &p, unsigned rows, hipStream_t s) {
   constexpr int VE = Elem<DT>::kPerVec;
   if (p.offsets) {
-    // A part is a whole number of vectors.
-    constexpr int ES = 16 / VE;
-    const int whole = (p.vocab + VE - 1) / VE * VE;
-    const int part = whole < kPartBytes / ES ? whole : kPartBytes / ES;
+    const int part = PartCols<DT>(p.vocab);
     hipLaunchKernelGGL((MovesRowKernel<DT, REF, PAST>), dim3((rows + 3) / 4), dim3(256),
-                       p.g ? 4 * part * ES : 0, s, p, part);
+                       p.g ? 4 * part * sizeof(typename Elem<DT>::T) : 0, s, p, part);
     return;
   }
   const int vecs = p.vocab / VE;
   if (vecs <= 64)
     LaunchDense<DT, REF, PAST, 1, 1>(p, rows, s);
+  else if (vecs <= 256 && rows <= kFewRows)
+    LaunchDense<DT, REF, PAST, 4, 1>(p, rows, s);
   else if (vecs <= 128)
     LaunchDense<DT, REF, PAST, 1, 2>(p, rows, s);
   else if (vecs <= 256)
@@ -1203,6 +1215,8 @@ void LaunchRows(const RowLossParams &p, unsigned rows, hipStream_t s) {
     LaunchDense<DT, REF, PAST, 4, 2>(p, rows, s);
   else if (vecs <= 1024)
     LaunchDense<DT, REF, PAST, 4, 4>(p, rows, s);
+  else if (vecs <= 2048)
+    LaunchDense<DT, REF, PAST, 8, 4>(p, rows, s);
   else if (vecs <= 4096)
     LaunchDense<DT, REF, PAST, 8, 8>(p, rows, s);
   else if (vecs <= 5120)
@@ -1225,84 +1239,153 @@ void LaunchRowsOf(const RowLossParams &p, bool past, unsigned rows, hipStream_t 
     past ? LaunchRows<DT, false, true>(p, rows, s) : LaunchRows<DT, false, false>(p, rows, s);
 }
 
-// Sum over the 256 threads of a workgroup, in a fixed order.
-__device__ double GroupSum64(double v, double *red) {
+// Sum over the W waves of a workgroup, in a fixed order.
+template <int W> __device__ __forceinline__ double GroupSum64(double v, double *red) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1)
     v += __shfl_xor(v, o, 64);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0)
-    red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return (red[0] + red[1]) + (red[2] + red[3]);
+  if constexpr (W > 1) {
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0)
+      red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = red[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w)
+      v += red[w];
+  }
+  return v;
 }
 
-__global__ __launch_bounds__(256) void PairLossKernel(PairLossParams a) {
-  __shared__ double red[4];
-  __shared__ float share[2];
-  const std::int64_t pair = blockIdx.x;
-  const float w = a.weight ? a.weight[pair] : 1.f;
-  std::int64_t begin[2], end[2];
-  double sum[2], count[2];
-  for (int s = 0; s < 2; ++s) {
-    std::int64_t b = a.seq_offsets[2 * pair + s], e = a.seq_offsets[2 * pair + s + 1];
-    b = b < 0 ? 0 : b > a.rows ? a.rows : b;
-    e = e < b ? b : e > a.rows ? a.rows : e;
-    begin[s] = b;
-    end[s] = e;
-    double t = 0.0, c = 0.0;
-    for (std::int64_t r = b + threadIdx.x; r < e; r += 256) {
-      const float l = a.mark[r];
-      if (l != kNoAction) {
-        t += a.ref_logp ? static_cast<double>(l) - a.ref_logp[r] : static_cast<double>(l);
-        c += 1.0;
-      }
+// A pair's loss from the marks of its rows, by W waves; the coefficients of
+// the gradients of its two sequences' rows.
+struct PairResult {
+  std::int64_t begin, middle, end;  // rows of the two sequences
+  float share[2];
+};
+template <int W>
+__device__ __forceinline__ PairResult PairLoss(const PairLossParams &a, std::int64_t pair,
+                                               double *red) {
+  PairResult r;
+  const float w = a.weight ? Uniform(a.weight, pair) : 1.f;
+  std::int64_t at[3];
+#pragma unroll
+  for (int s = 0; s < 3; ++s) {
+    at[s] = Uniform(a.seq_offsets, 2 * pair + s);
+    at[s] = at[s] < 0 ? 0 : at[s] > a.rows ? a.rows : at[s];
+  }
+  r.begin = at[0];
+  r.middle = at[1] < at[0] ? at[0] : at[1];
+  r.end = at[2] < r.middle ? r.middle : at[2];
+  double sum[2] = {0.0, 0.0}, count[2] = {0.0, 0.0};
+  for (std::int64_t i = r.begin + threadIdx.x; i < r.end; i += 64 * W) {
+    const float l = a.mark[i];
+    const double ref = a.ref_logp ? static_cast<double>(a.ref_logp[i]) : 0.0;
+    const int s = i >= r.middle;
+    if (l != kNoAction) {
+      sum[s] += l - ref;
+      count[s] += 1.0;
     }
-    sum[s] = GroupSum64(t, red);
-    count[s] = GroupSum64(c, red);
+  }
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    sum[s] = GroupSum64<W>(sum[s], red);
+    if (a.average) {
+      count[s] = GroupSum64<W>(count[s], red);
+      if (count[s] > 0.0)
+        sum[s] /= count[s];
+    }
+  }
+  const double beta = a.beta, diff = sum[0] - sum[1], h = beta * diff;
+  double loss, slope;  // slope: by the difference of the two sums
+  if (a.kind == 0) {
+    // ln(1 + e^-h) and ln(1 + e^h) = ln(1 + e^-|h|) + max(0, -+h); sig(h)
+    // from the same exponential.
+    const double eps = a.smoothing, tail = exp(-fabs(h)), base = log1p(tail);
+    const double small = tail / (1.0 + tail), sig = h >= 0.0 ? 1.0 - small : small;
+    loss = base + (1.0 - eps) * fmax(-h, 0.0) + eps * fmax(h, 0.0);
+    if (h != h)
+      loss = h;
+    slope = beta * (eps * sig - (1.0 - eps) * (h >= 0.0 ? small : 1.0 - small));
+  } else if (a.kind == 1) {
+    loss = h < 1.0 ? 1.0 - h : h >= 1.0 ? 0.0 : h;
+    slope = h < 1.0 ? -beta : h >= 1.0 ? 0.0 : h;
+  } else {
+    const double off = diff - 0.5 / beta;
+    loss = off * off;
+    slope = 2.0 * off;
   }
   if (threadIdx.x == 0) {
-    for (int s = 0; s < 2; ++s)
-      if (a.average && count[s] > 0.0)
-        sum[s] /= count[s];
-    const double beta = a.beta, diff = sum[0] - sum[1], h = beta * diff;
-    double loss, slope;  // slope: by the difference of the two sums
-    if (a.kind == 0) {
-      // ln(1 + e^-h) and ln(1 + e^h) = ln(1 + e^-|h|) + max(0, -+h); sig(h)
-      // from the same exponential.
-      const double eps = a.smoothing, tail = exp(-fabs(h)), base = log1p(tail);
-      const double sig = h >= 0.0 ? 1.0 / (1.0 + tail) : tail / (1.0 + tail);
-      const double not_sig = h >= 0.0 ? tail / (1.0 + tail) : 1.0 / (1.0 + tail);
-      loss = base + (1.0 - eps) * fmax(-h, 0.0) + eps * fmax(h, 0.0);
-      if (h != h)
-        loss = h;
-      slope = beta * (eps * sig - (1.0 - eps) * not_sig);
-    } else if (a.kind == 1) {
-      loss = h < 1.0 ? 1.0 - h : h >= 1.0 ? 0.0 : h;
-      slope = h < 1.0 ? -beta : h >= 1.0 ? 0.0 : h;
-    } else {
-      const double r = diff - 0.5 / beta;
-      loss = r * r;
-      slope = 2.0 * r;
-    }
     if (a.loss)
       a.loss[pair] = w == 0.f ? 0.f : static_cast<float>(w * loss);
     if (a.margin)
       a.margin[pair] = w == 0.f ? 0.f : static_cast<float>(h);
-    for (int s = 0; s < 2; ++s) {
-      const double c = a.average && count[s] > 0.0 ? slope / count[s] : slope;
-      share[s] = w == 0.f ? 0.f : static_cast<float>(w * (s == 0 ? c : -c));
-    }
+  }
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const double c = a.average && count[s] > 0.0 ? slope / count[s] : slope;
+    r.share[s] = w == 0.f ? 0.f : static_cast<float>(w * (s == 0 ? c : -c));
+  }
+  return r;
+}
+
+template <int W> __global__ __launch_bounds__(64 * W) void PairLossKernel(PairLossParams a) {
+  __shared__ double red[W];
+  const PairResult r = PairLoss<W>(a, blockIdx.x, red);
+  for (std::int64_t i = r.begin + threadIdx.x; i < r.end; i += 64 * W) {
+    const float l = a.mark[i];
+    const bool acted = l != kNoAction;
+    if (a.coef)
+      a.coef[i] = acted ? r.share[i >= r.middle] : 0.f;
+    if (a.logp)
+      a.logp[i] = acted ? l : 0.f;
+  }
+}
+
+// A few short lines of moves in one launch: a workgroup takes a pair, its waves
+// the pair's rows in turn; marks through the workspace as in the three
+// launches.  Up to 8 rows a pair on average (one a wave) and 512 pairs: 16
+// pairs of 2 rows 6.4 us (9.4 in three launches), 256 pairs of about 5 rows 8.1
+// (11.3); 1024 pairs of 2 rows 15.1 (12.8), 128 pairs of 60 rows 50 (25).
+constexpr int kPairWaves = 8, kFewPairs = 512;
+template <int DT>
+__global__ __launch_bounds__(64 * kPairWaves) void PairMovesKernel(RowLossParams a,
+                                                                   PairLossParams q,
+                                                                   int part_cols) {
+  extern __shared__ u32x4 parts[];
+  __shared__ double red[kPairWaves];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  unsigned char *lds = reinterpret_cast<unsigned char *>(parts) +
+                       static_cast<size_t>(wave) * part_cols * sizeof(typename Elem<DT>::T);
+  const std::int64_t pair = blockIdx.x;
+  std::int64_t from = Uniform(q.seq_offsets, 2 * pair), to = Uniform(q.seq_offsets, 2 * pair + 2);
+  from = from < 0 ? 0 : from;
+  to = to > q.rows ? q.rows : to;
+  RowLossParams marks = a;
+  marks.g = nullptr;
+  for (std::int64_t row = from + wave; row < to; row += kPairWaves) {
+    RowInputs in = Inputs(marks, row);
+    ListedRow<DT, false, false>(marks, row, in, lds, part_cols);
   }
   __syncthreads();
-  for (int s = 0; s < 2; ++s)
-    for (std::int64_t r = begin[s] + threadIdx.x; r < end[s]; r += 256) {
-      const bool acted = a.mark[r] != kNoAction;
-      if (a.coef)
-        a.coef[r] = acted ? share[s] : 0.f;
-      if (a.logp)
-        a.logp[r] = acted ? a.mark[r] : 0.f;
-    }
+  const PairResult r = PairLoss<kPairWaves>(q, pair, red);
+  RowLossParams grads = a;
+  grads.mark = nullptr;
+  grads.coef = q.mark;  // not read: the coefficient is at hand
+  for (std::int64_t row = r.begin + wave; row < r.end; row += kPairWaves) {
+    const float l = q.mark[row];
+    const bool acted = l != kNoAction;
+    if (q.logp && lane == 0)
+      q.logp[row] = acted ? l : 0.f;
+    if (!a.g)
+      continue;
+    RowInputs in{};
+    in.weight = __int_as_float(__builtin_amdgcn_readfirstlane(
+        __float_as_int(acted ? r.share[row >= r.middle] : 0.f)));
+    in.action = a.actions ? Uniform(a.actions, row) : -1;
+    ListedRow<DT, false, false>(grads, row, in, lds, part_cols);
+  }
 }
 
 }  // namespace
@@ -1335,15 +1418,56 @@ hipError_t LaunchRowLoss(const RowLossParams &p, hipStream_t stream, std::string
   return hipSuccess;
 }
 
-hipError_t LaunchPairLoss(const PairLossParams &p, hipStream_t stream, std::string *err) {
-  if (p.pairs < 0 || p.pairs > (1 << 23) || (p.pairs > 0 && (!p.seq_offsets || (p.rows > 0 && !p.mark)))) {
+template <int DT>
+static void LaunchPairMoves(const RowLossParams &p, const PairLossParams &q, hipStream_t s) {
+  const int part = PartCols<DT>(p.vocab);
+  hipLaunchKernelGGL(PairMovesKernel<DT>, dim3(static_cast<unsigned>(q.pairs)),
+                     dim3(64 * kPairWaves),
+                     p.g ? kPairWaves * part * sizeof(typename Elem<DT>::T) : 0, s, p, q, part);
+}
+
+hipError_t LaunchPreference(const RowLossParams &rows, const PairLossParams &pairs,
+                            hipStream_t stream, std::string *err) {
+  if (pairs.pairs < 0 || pairs.pairs > (1 << 23) ||
+      (pairs.pairs > 0 && (!pairs.seq_offsets || (pairs.rows > 0 && !pairs.mark))) ||
+      (rows.g && !pairs.coef)) {
     if (err)
-      *err = "pair_loss: needs 0 <= pairs <= 2^23, offsets and log-probabilities";
+      *err = "preference: needs 0 <= pairs <= 2^23, offsets and a workspace";
     return hipErrorInvalidValue;
   }
-  if (p.pairs > 0)
-    hipLaunchKernelGGL(PairLossKernel, dim3(static_cast<unsigned>(p.pairs)), dim3(256), 0, stream, p);
-  return hipGetLastError();
+  if (pairs.pairs == 0)
+    return hipSuccess;
+  if (rows.offsets && pairs.pairs <= kFewPairs && rows.rows <= kPairWaves * pairs.pairs) {
+    RowLossParams p = rows;
+    p.mark = pairs.mark;
+    if (p.dtype == DT_F32)
+      LaunchPairMoves<DT_F32>(p, pairs, stream);
+    else if (p.dtype == DT_BF16)
+      LaunchPairMoves<DT_BF16>(p, pairs, stream);
+    else
+      LaunchPairMoves<DT_F16>(p, pairs, stream);
+    return hipGetLastError();
+  }
+  RowLossParams p = rows;
+  p.g = nullptr;
+  p.mark = pairs.mark;
+  p.seq_offsets = pairs.seq_offsets;
+  p.n_seq = 2 * pairs.pairs;
+  hipError_t e = LaunchRowLoss(p, stream, err);
+  if (e != hipSuccess)
+    return e;
+  const dim3 grid(static_cast<unsigned>(pairs.pairs));
+  if (pairs.rows <= 256 * pairs.pairs)
+    hipLaunchKernelGGL(PairLossKernel<1>, grid, dim3(64), 0, stream, pairs);
+  else
+    hipLaunchKernelGGL(PairLossKernel<4>, grid, dim3(256), 0, stream, pairs);
+  e = hipGetLastError();
+  if (e != hipSuccess || !rows.g)
+    return e;
+  p.g = rows.g;
+  p.mark = nullptr;
+  p.coef = pairs.coef;
+  return LaunchRowLoss(p, stream, err);
 }
 
 }  // namespace mfh

@@ -28,6 +28,7 @@ class DeviceBuffers:
         self.hip.hipDeviceSynchronize.argtypes = []
         self.ptrs = []
         self.streams = []
+        self.graphs = []
 
     def alloc(self, nbytes):
         p = ctypes.c_void_p()
@@ -65,8 +66,30 @@ class DeviceBuffers:
         else:
             assert self.hip.hipStreamSynchronize(stream) == 0
 
+    def capture(self, stream, calls):
+        """What `calls()` enqueues on the stream as a HIP graph: a function that
+        launches it there."""
+        h = self.hip
+        graph, run = ctypes.c_void_p(), ctypes.c_void_p()
+        assert h.hipStreamBeginCapture(ctypes.c_void_p(stream), 0) == 0
+        try:
+            calls()
+        finally:
+            rc = h.hipStreamEndCapture(ctypes.c_void_p(stream), ctypes.byref(graph))
+        assert rc == 0
+        assert h.hipGraphInstantiate(ctypes.byref(run), graph, None, None, ctypes.c_size_t(0)) == 0
+        self.graphs.append((graph, run))
+
+        def launch():
+            assert h.hipGraphLaunch(run, ctypes.c_void_p(stream)) == 0
+        return launch
+
     def free(self):
         self.sync()
+        for graph, run in self.graphs:
+            self.hip.hipGraphExecDestroy(run)
+            self.hip.hipGraphDestroy(graph)
+        self.graphs = []
         for p in self.ptrs:
             self.hip.hipFree(p)
         for s in self.streams:

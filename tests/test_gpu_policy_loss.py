@@ -140,6 +140,71 @@ def test_whole_rows_of_the_policy(dev, dtype, rows):
     check(batch, got, ref, 0.2, 0.05, **sc, rows=range(0, rows, max(1, rows // 60)))
 
 
+@pytest.mark.parametrize("dtype,vocab", [("f32", 20003), ("f32", 28001), ("bf16", 40009),
+                                         ("bf16", 65535), ("f16", 50021)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_more_long_rows_than_the_card_runs_at_once(dev, dtype, vocab, in_place):
+    """Rows that a workgroup takes one after another, the next one's logits
+    loaded ahead: among them rows of weight 0 (with NaN), rows with nothing
+    left, masked rows, rows far below their reference, and the last row."""
+    rng = np.random.default_rng(vocab)
+    rows = 600
+    x = rng.standard_normal((rows, vocab), dtype=np.float32) * 2
+    ref = x + 0.3 * rng.standard_normal((rows, vocab), dtype=np.float32)
+    actions = rng.integers(0, vocab, rows)
+    actions[5], actions[300] = vocab - 1, -1
+    special = {1: "masked", 3: "empty", 257: "masked", 258: "far", 259: "nan", 400: "empty",
+               511: "masked", 513: "far", 599: "masked"}
+    weight = rng.uniform(0.5, 1.5, rows).astype(np.float32)
+    for b, kind in special.items():
+        actions[b] = 7
+        if kind == "masked":
+            x[b, 100:] = ref[b, 100:] = -np.inf
+        elif kind == "empty":
+            x[b] = -np.inf
+        elif kind == "far":
+            x[b, 50:60] -= 90.0
+        else:
+            x[b], weight[b] = np.nan, 0.0
+    weight[[2, 255, 598]] = 0.0
+    batch = lg.Batch(dev, x, dtype, None, actions, pad=vocab % 3)
+    sc = dict(advantage=rng.normal(size=rows).astype(np.float32), weight=weight)
+    got = lg.policy(batch, ref=ref, kl_coef=0.3, entropy_coef=0.1, in_place=in_place, **sc, **CLIP)
+    some = sorted({0, 5, 256, 300, 512, 597, 2, 255, 598, *special, *range(20, 600, 97)})
+    refv = lu.from_bits(lu.to_bits(ref[some], dtype), dtype)
+    part = lg.Batch.__new__(lg.Batch)
+    part.dev, part.dtype, part.moves, part.temp = dev, dtype, None, 1.0
+    part.values, part.actions = batch.values[some], actions[some]
+    part.rows, part.vocab = len(some), vocab
+    check(part, {k: v[some] for k, v in got.items()}, refv, 0.3, 0.1,
+          advantage=sc["advantage"][some], weight=weight[some])
+
+
+def test_rows_of_several_launches(dev):
+    """More rows than one launch takes (2^21)."""
+    rows = (1 << 21) + 5
+    rng = np.random.default_rng(2)
+    x = rng.standard_normal((rows, 2), dtype=np.float32)
+    d_x, d_a = dev.put(x), dev.put((np.arange(rows) % 2).astype(np.int32))
+    logp, grad = lg.Column(dev, rows), dev.put(np.zeros_like(x))
+    adv = dev.put(np.ones(rows, np.float32))
+    off = dev.put((2 * np.arange(rows + 1)).astype(np.int32))
+    idx = dev.put(np.tile(np.array([0, 1], np.int16), rows))
+    d = (x[:, 1] - x[:, 0]).astype(np.float64) * np.where(np.arange(rows) % 2, 1, -1)
+    want = -np.logaddexp(0, -d)
+    for kw in ({}, dict(d_move_offsets=off, d_move_indices=idx, n_moves=2 * rows)):
+        r = backend.policy_rows(d_x, rows, 2, d_actions=d_a, **kw)
+        backend.policy_loss_device(r, d_advantage=adv, d_logp=logp.ptr, d_grad=grad)
+        dev.sync()
+        got = logp.get()
+        # ln S is below 1, |z| below 12: the bounds of loss_util at K = 86.
+        np.testing.assert_allclose(got, want, rtol=0, atol=2 * lu.U * (4 * 12 + 86 + 5 * 12 + 4))
+        g = dev.get(grad, x)
+        at = np.arange(rows) % 2
+        np.testing.assert_allclose(g[np.arange(rows), at], -(1 - np.exp(want)), rtol=0, atol=4e-5)
+        assert np.isfinite(g).all()
+
+
 def _lists(rng, rows, vocab, most=60):
     out = []
     for b in range(rows):

@@ -129,6 +129,35 @@ def test_vocabularies(dev, dtype, vocab):
     check(batch, off, got, ref, weight, beta=0.3)
 
 
+@pytest.mark.parametrize("dtype,vocab", [("f32", 20003), ("bf16", 45001)])
+def test_more_long_rows_than_the_card_runs_at_once(dev, dtype, vocab):
+    rng = np.random.default_rng(vocab)
+    lengths = [40, 50, 0, 3, 100, 120, 130, 57]
+    off = [int(v) for v in np.concatenate([[0], np.cumsum(lengths)]) + 3]
+    rows = off[-1] + 260
+    x = rng.standard_normal((rows, vocab), dtype=np.float32) * 2
+    actions = rng.integers(0, vocab, rows)
+    actions[10:30] = -1
+    x[40, 5:] = -np.inf
+    actions[40] = 2
+    batch = lg.Batch(dev, x, dtype, None, actions)
+    ref = (rng.normal(size=rows) * 0.5 - 10).astype(np.float32)
+    weight = np.array([1.0, 0.0, 0.5, 1.0], np.float32)
+    got = lg.preference(batch, off, ref, weight, beta=0.02)
+    check(batch, off, got, ref, weight, beta=0.02)
+
+
+@pytest.mark.parametrize("pairs,most", [(1, 1), (3, 8), (512, 2), (513, 2), (40, 16), (700, 5)])
+def test_numbers_of_pairs(dev, pairs, most):
+    """Both sides of the rule that takes a few short pairs in one launch."""
+    rng = np.random.default_rng(pairs)
+    lengths = list(rng.integers(0, most + 1, 2 * pairs))
+    batch, off, ref, weight = _batch(dev, rng, lengths, 300, "f32", True, lead=1, tail=2)
+    kw = dict(beta=0.3, label_smoothing=0.1)
+    got = lg.preference(batch, off, ref, weight, **kw)
+    check(batch, off, got, ref, weight, **kw)
+
+
 def test_far_margins_do_not_overflow(dev):
     """h = +-1e4: the loss is |h| or 0, the gradient full or none."""
     x = np.zeros((4, 8))
