@@ -193,7 +193,7 @@ __device__ __forceinline__ float LanesMax(float v) {
 
 // Sums of N values over the W waves of a workgroup.
 template <int W, int N>
-__device__ __forceinline__ void GroupSum(float (&v)[N], float (*red)[4]) {
+__device__ __forceinline__ void GroupSum(float (&v)[N], float (*red)[8]) {
 #pragma unroll
   for (int i = 0; i < N; ++i)
     v[i] = WaveSum(v[i]);
@@ -209,19 +209,6 @@ __device__ __forceinline__ void GroupSum(float (&v)[N], float (*red)[4]) {
     for (int i = 0; i < N; ++i)
       v[i] = LanesSum<W>(red[threadIdx.x & (W - 1)][i]);
   }
-}
-
-template <int W>
-__device__ __forceinline__ float GroupMax(float v, float (*red)[4]) {
-  v = WaveMax(v);
-  if constexpr (W > 1) {
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0)
-      red[threadIdx.x >> 6][0] = v;
-    __syncthreads();
-    v = LanesMax<W>(red[threadIdx.x & (W - 1)][0]);
-  }
-  return v;
 }
 
 // Sums over a row's entries: of e, of e log2(e), of e d with d = x - y; and the
@@ -246,8 +233,14 @@ __device__ __forceinline__ void AddStats(float x, float y, float m, float c, Sum
   }
 }
 
-// Over the W waves of a workgroup, in one exchange.
-template <int W, bool REF> __device__ __forceinline__ void GroupSums(Sums &s, float (*red)[4]) {
+// Over the W waves of a workgroup, each of which has summed relative to its own
+// maximum `top` (0 where that is -inf): one exchange, and the sums relative to
+// the row's maximum, which is returned (0 for -inf).  Relative to a maximum
+// higher by `step` in log2 units every e falls by exp2(step) and every log2(e)
+// by step.  A wave whose entries all vanish that way adds nothing, with the
+// guard; without, it makes the sums NaN, which asks for it.
+template <int W, bool REF, bool GUARD>
+__device__ __forceinline__ float GroupSums(Sums &s, float top, float c, float (*red)[8]) {
   s.e = WaveSum(s.e);
   s.et = WaveSum(s.et);
   if constexpr (REF) {
@@ -256,23 +249,39 @@ template <int W, bool REF> __device__ __forceinline__ void GroupSums(Sums &s, fl
   }
   if constexpr (W > 1) {
     __syncthreads();
-    if ((threadIdx.x & 63) == 0)
-      *reinterpret_cast<f32x4 *>(red[threadIdx.x >> 6]) = f32x4{s.e, s.et, s.ed, s.least};
+    if ((threadIdx.x & 63) == 0) {
+      float *mine = red[threadIdx.x >> 6];
+      *reinterpret_cast<f32x4 *>(mine) = f32x4{s.e, s.et, s.ed, s.least};
+      mine[4] = top;
+    }
     __syncthreads();
-    const f32x4 v = *reinterpret_cast<const f32x4 *>(red[threadIdx.x & (W - 1)]);
-    s.e = LanesSum<W>(v[0]);
-    s.et = LanesSum<W>(v[1]);
+    const float *other = red[threadIdx.x & (W - 1)];
+    const f32x4 v = *reinterpret_cast<const f32x4 *>(other);
+    const float its = other[4];
+    top = LanesMax<W>(its);
+    top = top == -__builtin_inff() ? 0.f : top;
+    const float step = (its - top) * c, f = Exp2(step);
+    const float none = GUARD ? 0.f : __builtin_nanf("");
+    s.e = LanesSum<W>(f * v[0]);
+    s.et = LanesSum<W>(f == 0.f ? none : f * (v[1] + v[0] * step));
     if constexpr (REF) {
-      s.ed = LanesSum<W>(v[2]);
+      s.ed = LanesSum<W>(f == 0.f ? none : f * v[2]);
       s.least = -LanesMax<W>(-v[3]);
     }
+    return top;
   }
+  return top == -__builtin_inff() ? 0.f : top;
 }
 
-// A NaN, or an entry so far below the reference (u < -60) that exp(-u) may
-// overflow.
-template <bool REF> __device__ __forceinline__ bool NeedsGuard(const Sums &s, float inv_temp) {
-  return s.et != s.et || s.ed != s.ed || (REF && !(s.least * inv_temp - s.ed / s.e * inv_temp > -60.f));
+// A NaN; an entry so far below the reference (u < -60) that exp(-u) may
+// overflow; or coefficients (Coefs a, b) above 1, whose product with a logit of
+// the type's lowest value may.
+template <bool REF>
+__device__ __forceinline__ bool NeedsGuard(const RowLossParams &a, float weight, const Sums &s) {
+  return s.et != s.et || s.ed != s.ed || !(fabsf(weight * a.inv_temp) < 0x1p100f) ||
+         !(fabsf(a.entropy_coef) * a.inv_temp <= 1.f) ||
+         (REF && (!(fabsf(a.kl_coef) <= 1.f) ||
+                  !((s.least - s.ed * Rcp(s.e)) * a.inv_temp > -60.f)));
 }
 
 // What a row's scalars come to, from its statistics.
@@ -303,22 +312,29 @@ struct RowGrad {
   float scale, slope, kl, entropy;
 };
 
-// The same for p_k (a (x_k - m) + b u_k + d), with what p and u need.
+// The same as P_k (a (x_k - m) + b u_k + d) with P = 2^power p, with what P and
+// u need: the scale's power of two is in P, so that a and b stay small whatever
+// the row's weight (a loss scale of 2^16, say).
 struct Coefs {
   float m, c, shift, inv_temp, mean_d, kl_shift, a, b, d;
+  int power;
 };
+constexpr int kLeastPower = -30, kMostPower = 100;
 
 __device__ __forceinline__ Coefs CoefsOf(const RowStats &st, const RowGrad &g, float inv_temp) {
   Coefs k;
+  const int power = __builtin_amdgcn_frexp_expf(g.scale);
+  k.power = power < kLeastPower ? kLeastPower : power > kMostPower ? kMostPower : power;
+  const float scale = ldexpf(g.scale, -k.power);
   k.m = st.m;
   k.c = inv_temp * kLog2e;
-  k.shift = -st.log2_sum;
+  k.shift = static_cast<float>(k.power) - st.log2_sum;
   k.inv_temp = inv_temp;
   k.mean_d = st.mean_d;
-  k.kl_shift = st.mean_d * kLog2e - st.log2_sum;
-  k.a = g.scale * g.entropy * inv_temp;
-  k.b = g.scale * g.kl;
-  k.d = -g.scale * (g.slope + g.entropy * st.mean_z);
+  k.kl_shift = st.mean_d * kLog2e + k.shift;
+  k.a = scale * g.entropy * inv_temp;
+  k.b = scale * g.kl;
+  k.d = -scale * (g.slope + g.entropy * st.mean_z);
   return k;
 }
 
@@ -338,7 +354,7 @@ __device__ __forceinline__ float Phi(float u) {
   return fabsf(u) < 0.25f ? near : far;
 }
 
-// p (exp(-u) - 1 + u), the term of KL, for any u; ym: the reference logit less
+// P (exp(-u) - 1 + u), the term of KL, for any u; ym: the reference logit less
 // the policy's maximum.  Far below 0, where exp(-u) may overflow against a
 // tiny p, their product comes from ym; an entry that is masked here adds
 // nothing but its reference probability.
@@ -352,8 +368,8 @@ __device__ __forceinline__ float KlTerm(const Coefs &k, float p, float u, float 
 
 // KL from the sum of its terms; infinite where the reference lacks what the
 // policy plays (E_p d is, and no term then means anything).
-__device__ __forceinline__ float KlOf(float terms, float mean_d) {
-  return mean_d == __builtin_inff() ? mean_d : Log1p(terms);
+__device__ __forceinline__ float KlOf(float terms, const Coefs &k) {
+  return k.mean_d == __builtin_inff() ? k.mean_d : Log1p(ldexpf(terms, -k.power));
 }
 
 // The gradient of N entries without the action's own term, and their part of
@@ -582,7 +598,7 @@ template <int DT, int W, int NV, bool REF, bool PAST>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void DenseRowKernel(RowLossParams a) {
   using E = Elem<DT>;
   constexpr int VE = E::kPerVec;
-  __shared__ __align__(16) float red[W][4];
+  __shared__ __align__(16) float red[W][8];
   const int tid = W == 1 ? threadIdx.x & 63 : threadIdx.x;
   std::int64_t row = blockIdx.x;
   if constexpr (W == 1)
@@ -636,14 +652,14 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void DenseRowKernel(RowLossP
       for (int i = 0; i < VE; ++i)
         m = fmaxf(m, xs[i]);
     }
-  m = GroupMax<W>(m, red);
-  m = m == -__builtin_inff() ? 0.f : m;
+  const float top = WaveMax(m);
 
   const float c = a.inv_temp * kLog2e;
   Sums sums;
   const auto sum = [&](auto guard) MFH_INLINE {
     constexpr bool GUARD = decltype(guard)::value;
     sums = Sums{};
+    m = top == -__builtin_inff() ? 0.f : top;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       Repack(xr[j]);
@@ -654,10 +670,10 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void DenseRowKernel(RowLossP
     }
     if (has_rest)
       AddStats<REF, GUARD>(xt[0], yt[0], m, c, sums);
-    GroupSums<W, REF>(sums, red);
+    m = GroupSums<W, REF, GUARD>(sums, top, c, red);
   };
   sum(std::false_type{});
-  const bool guarded = NeedsGuard<REF>(sums, a.inv_temp);
+  const bool guarded = NeedsGuard<REF>(a, in.weight, sums);
   if (guarded)
     sum(std::true_type{});
   const RowStats st = Stats(m, sums, a.inv_temp);
@@ -696,7 +712,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void DenseRowKernel(RowLossP
       finish(std::false_type{});
     if (want_kl) {
       GroupSum<W>(kl, red);
-      kl[0] = KlOf(kl[0], st.mean_d);
+      kl[0] = KlOf(kl[0], k);
     }
   }
   if (tid == 0)
@@ -709,7 +725,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void DenseRowKernel(RowLossP
 // caches).
 template <int DT, bool REF>
 __device__ __forceinline__ void StreamRow(const RowLossParams &a, std::int64_t row,
-                                          const RowInputs &in, float (*red)[4]) {
+                                          const RowInputs &in, float (*red)[8]) {
   using E = Elem<DT>;
   constexpr int VE = E::kPerVec, W = 16, kThreads = 64 * W;
   const int tid = threadIdx.x;
@@ -756,11 +772,9 @@ __device__ __forceinline__ void StreamRow(const RowLossParams &a, std::int64_t r
     }
     AddVec<DT, REF, true>(xr, yr, m == -__builtin_inff() ? 0.f : m, c, sums);
   }
-  float top = GroupMax<W>(m, red);
-  top = top == -__builtin_inff() ? 0.f : top;
-  rescale(m, top);
-  m = top;
-  GroupSums<W, REF>(sums, red);
+  const float top = WaveMax(m);
+  rescale(m, top == -__builtin_inff() ? 0.f : top);
+  m = GroupSums<W, REF, true>(sums, top, c, red);
   const RowStats st = Stats(m, sums, a.inv_temp);
   if (st.empty) {
     if (tid == 0)
@@ -790,7 +804,7 @@ __device__ __forceinline__ void StreamRow(const RowLossParams &a, std::int64_t r
                               vecs, has_rest, kThreads, tid, kl[0]);
     if (want_kl) {
       GroupSum<W>(kl, red);
-      kl[0] = KlOf(kl[0], st.mean_d);
+      kl[0] = KlOf(kl[0], k);
     }
   }
   if (tid == 0)
@@ -800,7 +814,7 @@ __device__ __forceinline__ void StreamRow(const RowLossParams &a, std::int64_t r
 // Rows longer than the registers hold.
 template <int DT, bool REF>
 __global__ __launch_bounds__(1024) void StreamRowKernel(RowLossParams a) {
-  __shared__ __align__(16) float red[16][4];
+  __shared__ __align__(16) float red[16][8];
   const std::int64_t row = a.row0 + blockIdx.x;
   if (OutsideSequences(a, row))
     return;
@@ -827,7 +841,7 @@ template <int DT, int NV, bool REF>
 __global__ __launch_bounds__(1024) void LoopRowKernel(RowLossParams a) {
   using E = Elem<DT>;
   constexpr int VE = E::kPerVec, W = 16, kThreads = 64 * W;
-  __shared__ __align__(16) float red[W][4];
+  __shared__ __align__(16) float red[W][8];
   const int tid = threadIdx.x;
   const int n = a.vocab, vecs = n / VE, rest = n - vecs * VE;
   const bool has_rest = tid < rest;
@@ -901,8 +915,8 @@ __global__ __launch_bounds__(1024) void LoopRowKernel(RowLossParams a) {
         for (int i = 0; i < VE; ++i)
           m = fmaxf(m, xs[i]);
       }
-    m = GroupMax<W>(fmaxf(m, xt[0]), red);
-    m = m == -__builtin_inff() ? 0.f : m;
+    const float top = WaveMax(fmaxf(m, xt[0]));
+    m = top == -__builtin_inff() ? 0.f : top;
     Sums sums;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -914,10 +928,10 @@ __global__ __launch_bounds__(1024) void LoopRowKernel(RowLossParams a) {
     }
     if (has_rest)
       AddStats<REF, false>(xt[0], yt[0], m, c, sums);
-    GroupSums<W, REF>(sums, red);
+    m = GroupSums<W, REF, false>(sums, top, c, red);
     // A sum of 0 has a NaN beside it (0 times the -inf of its logits), as a
     // row that needs the guards does.
-    const bool stream = live && NeedsGuard<REF>(sums, a.inv_temp), here = live && !stream;
+    const bool stream = live && NeedsGuard<REF>(a, in.weight, sums), here = live && !stream;
     if (stream) {
       StreamRow<DT, REF>(a, row, in, red);
 #pragma unroll
@@ -951,7 +965,7 @@ __global__ __launch_bounds__(1024) void LoopRowKernel(RowLossParams a) {
                                  yt, vecs, has_rest, kThreads, tid, kl[0]);
       if (want_kl) {
         GroupSum<W>(kl, red);
-        kl[0] = KlOf(kl[0], st.mean_d);
+        kl[0] = KlOf(kl[0], k);
       }
       if (tid == 0)
         WriteRow(a, row, in.weight, acted, res, kl[0]);
@@ -1043,14 +1057,14 @@ __device__ __forceinline__ void MovesRow(const RowLossParams &a, std::int64_t ro
       xa = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(xv[r]), __ffsll(hit) - 1));
     }
   }
-  m = WaveMax(m);
-  m = m == -__builtin_inff() ? 0.f : m;
+  const float top = WaveMax(m);
+  m = top == -__builtin_inff() ? 0.f : top;
   const float c = a.inv_temp * kLog2e;
   Sums sums;
 #pragma unroll
   for (int r = 0; r < NE; ++r)
     AddStats<REF, true>(xv[r], yv[r], m, c, sums);
-  GroupSums<1, REF>(sums, nullptr);
+  (void)GroupSums<1, REF, true>(sums, top, c, nullptr);
   const RowStats st = Stats(m, sums, a.inv_temp);
   const RowResult res = Evaluate(a, in, st, acted, xa);
   const bool want_kl = REF && WantsKl(a);
@@ -1065,7 +1079,7 @@ __device__ __forceinline__ void MovesRow(const RowLossParams &a, std::int64_t ro
       f[r] = ft[0];
     }
     if (want_kl)
-      kl = KlOf(WaveSum(kl), st.mean_d);
+      kl = KlOf(WaveSum(kl), k);
   }
   if (lane == 0) {
     if (st.empty)

@@ -280,6 +280,59 @@ def test_masks_and_far_logits(dev, dtype, vocab):
     check(batch, got, ref, 0.5, 0.1, **sc)
 
 
+@pytest.mark.parametrize("vocab", [1858, 4288, 12000, 33000])
+def test_finite_masks_whole_waves_wide_and_large_weights(dev, vocab):
+    """Masks of the lowest value that cover all of a wave's columns, at
+    temperatures and weights where their products overflow."""
+    rng = np.random.default_rng(vocab + 2)
+    lowest = -np.finfo(np.float32).max
+    x = rng.normal(size=(6, vocab)) * 3
+    ref = x + 0.3 * rng.normal(size=x.shape)
+    x[0, 5:] = lowest
+    x[1, :-3] = ref[1, :-3] = lowest
+    x[2, 40:] = ref[2, 40:] = -np.inf
+    x[3, 100:] = lowest
+    ref[3, 100:] = -np.inf
+    ref[4, 700:] = lowest
+    x[4, 700:] = -1e4
+    actions = np.array([1, vocab - 1, 3, 50, 20, 9])
+    for temp, weight in ((1.0, 1.0), (4.0, 1.0), (4.0, 3e3), (0.3, 1e3)):
+        batch = lg.Batch(dev, x, "f32", None, actions, temp)
+        sc = dict(advantage=rng.normal(size=6).astype(np.float32),
+                  weight=np.full(6, weight, np.float32))
+        got = lg.policy(batch, ref=ref, kl_coef=0.2, entropy_coef=0.1, **sc, **CLIP)
+        check(batch, got, ref, 0.2, 0.1, **sc)
+        got = lg.policy(batch, entropy_coef=0.5, **sc, **CLIP)
+        check(batch, got, None, 0.0, 0.5, **sc)
+
+
+@pytest.mark.parametrize("vocab", [1858, 12000, 33000, 140000])
+def test_weights_of_any_size(dev, vocab):
+    """Loss scales, negative weights, and ones near the ends of the range."""
+    rng = np.random.default_rng(vocab + 3)
+    x = rng.normal(size=(6, vocab)) * 2
+    ref = x + 0.3 * rng.normal(size=x.shape)
+    weight = np.array([65536.0, -2.5, 1e-20, 3e30, -1e-9, 1.0], np.float32)
+    lists = [list(range(5, 45))] * 6 if vocab == 1858 else None
+    for moves in (None, lists) if lists else (None,):
+        batch = lg.Batch(dev, x, "f32", moves, np.full(6, 9))
+        sc = dict(advantage=rng.normal(size=6).astype(np.float32), weight=weight)
+        got = lg.policy(batch, ref=ref, kl_coef=0.2, entropy_coef=0.1, **sc, **CLIP)
+        for b in range(6):   # each row on its own scale
+            part = lg.Batch.__new__(lg.Batch)
+            part.dtype, part.moves, part.temp = "f32", None if moves is None else [moves[b]], 1.0
+            part.values, part.actions = batch.values[b:b + 1], batch.actions[b:b + 1]
+            part.rows, part.vocab = 1, vocab
+            scale = 2.0 ** -np.round(np.log2(abs(float(weight[b]))))
+            w = np.array([float(weight[b]) * scale])
+            mine = {k: v[b:b + 1] * (scale if k in ("loss", "grad") else 1.0)
+                    for k, v in got.items()}
+            sign = np.sign(w[0])
+            mine["loss"], mine["grad"] = mine["loss"] * sign, mine["grad"] * sign
+            check(part, mine, ref[b:b + 1], 0.2, 0.1, advantage=sc["advantage"][b:b + 1],
+                  weight=w * sign)
+
+
 def test_masked_entries_of_move_lists(dev):
     rng = np.random.default_rng(8)
     x = rng.normal(size=(4, 1858))
