@@ -344,7 +344,7 @@ typedef struct {
  * q the softmax of the reference logits over the same entries and
  * temperature.  The first term is 0 in rows without an action or with
  * d_advantage NULL; d_old_logp NULL is the row's own l (rho = 1).  A row of
- * weight 0 is not read and gives zeros.  The gradient of the sum of all
+ * weight 0 gives zeros, whatever its logits hold.  The gradient of the sum of all
  * losses (old_logp, advantage, weight and q held fixed) goes to d_grad, every
  * column of every row (0 outside the row's entries); at rho on a bound the
  * unclipped branch counts.  Where q lacks an entry that p has, KL is infinite
@@ -378,7 +378,7 @@ int mfh_policy_loss_device(const mfh_policy_rows *rows, const mfh_policy_loss *l
  * gradient of 0).  margin is h.  logp
  * is ln p_action, 0 without an action.  The gradient of the sum of all losses
  * goes to the sequences' rows of d_grad, every column.  Rows before the first
- * sequence or behind the last are neither read nor written.  Any output may
+ * sequence or behind the last are left as they are, whatever they hold.  Any output may
  * be NULL; d_grad may be d_logits with the same stride.  d_workspace holds
  * mfh_preference_loss_workspace_bytes(rows) bytes, 8-byte aligned. */
 enum { MFH_PREFERENCE_SIGMOID = 0, MFH_PREFERENCE_HINGE = 1, MFH_PREFERENCE_SQUARE = 2 };

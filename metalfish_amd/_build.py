@@ -24,13 +24,13 @@ CSRC = os.path.join(PKG, "csrc")
 
 # The GEMM's tiles are spread over several sources (gemm_tiles.h), listed
 # first: their device code takes longest to generate.
-HIP_SOURCES = ["hip/gemm_tiles_pipe_a.hip", "hip/gemm_tiles_pipe_b.hip",
+HIP_SOURCES = ["hip/gemm_tiles_pipe_a.hip", "hip/policy_loss.hip", "hip/gemm_tiles_pipe_b.hip",
                "hip/gemm_tiles_pipe_c.hip", "hip/gemm_tiles_single_mid.hip",
                "hip/gemm_tiles_single.hip", "hip/gemm_tiles_mid.hip", "hip/gemm_tiles_small.hip",
                "hip/gemm_tiles_w8_a.hip", "hip/gemm_tiles_w8_b.hip", "hip/gemm_tiles_w8_c.hip",
                "hip/gemm_tiles_w8_single.hip", "hip/gemm_tiles_w8_small.hip", "hip/gemm.hip",
                "hip/panel_gemm.hip", "hip/skinny_gemm.hip", "hip/smolgen_bias.hip",
-               "hip/attention.hip", "hip/rowops.hip", "hip/policy.hip", "hip/policy_loss.hip",
+               "hip/attention.hip", "hip/rowops.hip", "hip/policy.hip",
                "hip/grad_clip.hip", "hip/mfh_api.cpp", "hip/learn_api.cpp",
                "host/policy_tables.cpp"]
 # Host-only parts of libmfhip.so (no device code), compiled with g++.

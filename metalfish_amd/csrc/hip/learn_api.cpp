@@ -177,6 +177,9 @@ bool RowsClash(const void *p, std::int64_t p_stride, const void *q, std::int64_t
          static_cast<std::uintptr_t>(p_stride) - apart < static_cast<std::uintptr_t>(row_bytes);
 }
 
+// No tensor on a card of 288 GB has more.
+constexpr uint64_t kMostElements = uint64_t(1) << 38;
+
 bool Finite(float v) { return std::isfinite(v); }
 
 // Rows by themselves; on success `p` holds them.
@@ -417,7 +420,6 @@ int mfh_grad_set_create(const mfh_grad_tensor *tensors, int n_tensors, int devic
       bool written;
     };
     std::vector<Range> ranges;
-    std::vector<mfh::GradChunk> chunks;
     for (int i = 0; i < n_tensors; ++i) {
       const mfh_grad_tensor &t = tensors[i];
       if (t.dtype < MFH_DTYPE_F32 || t.dtype > MFH_DTYPE_F16)
@@ -425,7 +427,7 @@ int mfh_grad_set_create(const mfh_grad_tensor *tensors, int n_tensors, int devic
       if (t.count == 0)
         continue;
       const int es = mfh::DTypeBytes(t.dtype);
-      if (!t.src || t.count > static_cast<uint64_t>(INT64_MAX / 8))
+      if (!t.src || t.count > kMostElements)
         return Invalid(fn, "a tensor without memory, or too large");
       if (!Aligned(t.src, es) || !Aligned(t.dst, es))
         return Invalid(fn, "pointers must be aligned to their elements");
@@ -436,13 +438,6 @@ int mfh_grad_set_create(const mfh_grad_tensor *tensors, int n_tensors, int devic
       add(t.src, false);
       if (t.dst)
         add(t.dst, true);
-      const uint64_t most = mfh::kGradChunkBytes / es;
-      for (uint64_t at = 0; at < t.count; at += most) {
-        const uint64_t n = std::min<uint64_t>(most, t.count - at);
-        chunks.push_back({static_cast<const char *>(t.src) + at * es,
-                          t.dst ? static_cast<char *>(t.dst) + at * es : nullptr,
-                          static_cast<std::int32_t>(n), t.dtype});
-      }
     }
     // In order of their beginning, a range meets an earlier one exactly when
     // it begins before the furthest end so far, of those written or (if it
@@ -487,6 +482,18 @@ int mfh_grad_set_create(const mfh_grad_tensor *tensors, int n_tensors, int devic
     hipError_t e = on.Set(dev);
     if (e != hipSuccess)
       return HipError(fn, "hipSetDevice", e);
+    std::vector<mfh::GradChunk> chunks;
+    for (int i = 0; i < n_tensors; ++i) {
+      const mfh_grad_tensor &t = tensors[i];
+      const int es = mfh::DTypeBytes(t.dtype);
+      const uint64_t most = mfh::kGradChunkBytes / es;
+      for (uint64_t at = 0; at < t.count; at += most) {
+        const uint64_t n = std::min<uint64_t>(most, t.count - at);
+        chunks.push_back({static_cast<const char *>(t.src) + at * es,
+                          t.dst ? static_cast<char *>(t.dst) + at * es : nullptr,
+                          static_cast<std::int32_t>(n), t.dtype});
+      }
+    }
     auto set = std::make_unique<mfh_grad_set>();
     set->device = dev;
     set->n_chunks = static_cast<std::int64_t>(chunks.size());

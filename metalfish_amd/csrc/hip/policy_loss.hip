@@ -834,14 +834,15 @@ __global__ __launch_bounds__(1024) void StreamRowKernel(RowLossParams a) {
 // row after row (every gridDim.x-th), and as the last pass is done with a
 // vector of the present row it loads the next row's into its registers.  All
 // rows take the same way through the loop, so that there is one such place:
-// rows of weight 0 or none compute nothing of use and store nothing, and rows
-// that need the guards are streamed.  NV: the vectors of a lane, the last
-// one filled for some lane.
-template <int DT, int NV, bool REF>
-__global__ __launch_bounds__(1024) void LoopRowKernel(RowLossParams a) {
+// rows of weight 0 compute nothing of use and store nothing.  NV: the vectors
+// of a lane, the last one filled for some lane.  Takes rows from `row` on;
+// returns the row that it leaves undone because it needs the guards (a.end or
+// more: none).
+template <int DT, int NV, bool REF, bool GUARD>
+__device__ __forceinline__ std::int64_t LoopRows(const RowLossParams &a, std::int64_t row,
+                                                 float (*red)[8]) {
   using E = Elem<DT>;
   constexpr int VE = E::kPerVec, W = 16, kThreads = 64 * W;
-  __shared__ __align__(16) float red[W][8];
   const int tid = threadIdx.x;
   const int n = a.vocab, vecs = n / VE, rest = n - vecs * VE;
   const bool has_rest = tid < rest;
@@ -887,7 +888,6 @@ __global__ __launch_bounds__(1024) void LoopRowKernel(RowLossParams a) {
     }
     return f;
   };
-  std::int64_t row = a.row0 + blockIdx.x;
   bool live = alive(row);
   Few few = load_few(row, Inputs(a, row).action);
 #pragma unroll
@@ -924,25 +924,16 @@ __global__ __launch_bounds__(1024) void LoopRowKernel(RowLossParams a) {
       if (REF)
         Repack(yr[REF ? j : 0]);
       if (filled(j))
-        AddVec<DT, REF, false>(xr[j], yr[REF ? j : 0], m, c, sums);
+        AddVec<DT, REF, GUARD>(xr[j], yr[REF ? j : 0], m, c, sums);
     }
     if (has_rest)
-      AddStats<REF, false>(xt[0], yt[0], m, c, sums);
-    m = GroupSums<W, REF, false>(sums, top, c, red);
-    // A sum of 0 has a NaN beside it (0 times the -inf of its logits), as a
-    // row that needs the guards does.
-    const bool stream = live && NeedsGuard<REF>(a, in.weight, sums), here = live && !stream;
-    if (stream) {
-      StreamRow<DT, REF>(a, row, in, red);
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        asm volatile("" : "=v"(xr[j]));  // no longer needed
-        if (REF)
-          asm volatile("" : "=v"(yr[REF ? j : 0]));
-      }
-    }
+      AddStats<REF, GUARD>(xt[0], yt[0], m, c, sums);
+    m = GroupSums<W, REF, GUARD>(sums, top, c, red);
+    // A row without an entry left needs them too (its sums hold 0 times -inf).
+    if (!GUARD && live && NeedsGuard<REF>(a, in.weight, sums))
+      return row;
     const RowStats st = Stats(m, sums, a.inv_temp);
-    const RowResult res = Evaluate(a, in, st, acted, xa);
+    const RowResult res = Evaluate(a, in, st, acted && !st.empty, xa);
     const Coefs k = CoefsOf(st, res.grad, a.inv_temp);
     float kl[1] = {0.f};
 #pragma unroll
@@ -951,8 +942,8 @@ __global__ __launch_bounds__(1024) void LoopRowKernel(RowLossParams a) {
       if (REF)
         Repack(yr[REF ? j : 0]);
       if (filled(j) && (want_grad || want_kl)) {
-        const u32x4 f = FinishVec<DT, REF, false>(k, want_kl, xr[j], yr[REF ? j : 0], kl[0]);
-        if (want_grad && here)
+        const u32x4 f = FinishVec<DT, REF, GUARD>(k, want_kl, xr[j], yr[REF ? j : 0], kl[0]);
+        if (want_grad && live)
           StoreVec<DT, true>(g + j * kThreads * VE + place(j), f);
       }
       // Not earlier: the present row's vector is in the registers.
@@ -960,8 +951,8 @@ __global__ __launch_bounds__(1024) void LoopRowKernel(RowLossParams a) {
       load(next_row, j, next_live);
       __builtin_amdgcn_sched_barrier(0);
     }
-    if (here) {
-      FinishRest<DT, REF, false>(k, want_kl, want_grad, g, res.grad, acted ? act : -1, xa, ya, xt,
+    if (live && !st.empty) {
+      FinishRest<DT, REF, GUARD>(k, want_kl, want_grad, g, res.grad, acted ? act : -1, xa, ya, xt,
                                  yt, vecs, has_rest, kThreads, tid, kl[0]);
       if (want_kl) {
         GroupSum<W>(kl, red);
@@ -969,7 +960,7 @@ __global__ __launch_bounds__(1024) void LoopRowKernel(RowLossParams a) {
       }
       if (tid == 0)
         WriteRow(a, row, in.weight, acted, res, kl[0]);
-    } else if (!live && !OutsideSequences(a, row)) {
+    } else if (live || !OutsideSequences(a, row)) {
       if (tid == 0)
         WriteZeros(a, row);
       if (want_grad)
@@ -979,7 +970,19 @@ __global__ __launch_bounds__(1024) void LoopRowKernel(RowLossParams a) {
     live = next_live;
     few = next_few;
   }
+  return row;
 }
+
+template <int DT, int NV, bool REF>
+__global__ __launch_bounds__(1024) void LoopRowKernel(RowLossParams a) {
+  __shared__ __align__(16) float red[16][8];
+  // From the first row that needs the guards on, all rows take them (columns
+  // that only fill up a vocabulary are masked in every row).
+  const std::int64_t row = LoopRows<DT, NV, REF, false>(a, a.row0 + blockIdx.x, red);
+  if (row < a.end)
+    (void)LoopRows<DT, NV, REF, true>(a, row, red);
+}
+
 
 // The entries of one row, NE a lane: columns (-1 outside the vocabulary, where
 // the logit is 0, and behind the list) and logits.
@@ -1444,7 +1447,7 @@ hipError_t LaunchPreference(const RowLossParams &rows, const PairLossParams &pai
                             hipStream_t stream, std::string *err) {
   if (pairs.pairs < 0 || pairs.pairs > (1 << 23) ||
       (pairs.pairs > 0 && (!pairs.seq_offsets || (pairs.rows > 0 && !pairs.mark))) ||
-      (rows.g && !pairs.coef)) {
+      (pairs.rows > 0 && rows.g && !pairs.coef)) {
     if (err)
       *err = "preference: needs 0 <= pairs <= 2^23, offsets and a workspace";
     return hipErrorInvalidValue;

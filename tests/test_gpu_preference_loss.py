@@ -158,6 +158,27 @@ def test_numbers_of_pairs(dev, pairs, most):
     check(batch, off, got, ref, weight, **kw)
 
 
+@pytest.mark.parametrize("dtype", lu.TYPES)
+@pytest.mark.parametrize("vocab", [2048, 4288, 32768])
+def test_short_pairs_of_wide_lists(dev, dtype, vocab):
+    """The one launch's LDS at its largest."""
+    rng = np.random.default_rng(vocab)
+    batch, off, ref, weight = _batch(dev, rng, [1, 2, 3, 4], vocab, dtype, True)
+    got = lg.preference(batch, off, ref, weight, beta=0.3)
+    check(batch, off, got, ref, weight, beta=0.3)
+
+
+def test_pairs_of_empty_sequences_without_a_row(dev):
+    loss, margin = lg.Column(dev, 2), lg.Column(dev, 2)
+    for lists in ({}, dict(d_move_offsets=dev.put(np.zeros(1, np.int32)))):
+        rows = backend.policy_rows(None, 0, 10, **lists)
+        backend.preference_loss_device(rows, 2, dev.put(np.zeros(5, np.int32)), d_loss=loss.ptr,
+                                       d_margin=margin.ptr, d_grad=dev.alloc(64))
+        dev.sync()
+        np.testing.assert_allclose(loss.get(), np.log(2.0), rtol=2 ** -23)
+        assert np.all(margin.get() == 0)
+
+
 def test_far_margins_do_not_overflow(dev):
     """h = +-1e4: the loss is |h| or 0, the gradient full or none."""
     x = np.zeros((4, 8))
