@@ -548,9 +548,11 @@ hipError_t LaunchPreference(const RowLossParams &rows, const PairLossParams &pai
 // the norm and of the scaling.  dst may be null (norm only).
 constexpr int kGradChunkBytes = 16384;
 // Sets above this many bytes are read and written past the caches
-// (non-temporal); below, each XCD's L2 still holds the chunks that it read for
-// the norm when it scales them (a workgroup takes the same chunks).
-constexpr std::int64_t kGradCachedBytes = std::int64_t(16) << 20;
+// (non-temporal); below, each XCD's L2 still holds chunks that it read for the
+// norm when it scales them (a workgroup takes the same ones).  Norm and scaling
+// through the caches and past them: 10.6 MB 9.8 and 11.1 us, 23 MB 14.6 and
+// 17.9, 38 MB 20.9 and 24.3, 80 MB 49.6 and 44.0, 637 MB 362 and 304.
+constexpr std::int64_t kGradCachedBytes = std::int64_t(48) << 20;
 struct GradChunk {
   const void *src;
   void *dst;
