@@ -16,15 +16,15 @@
 // written from there (rows longer than 8192 vectors of 16 bytes are read a
 // second time).  What bounds it:
 //  * fp32, or no reference: memory.  16384 x 1858 fp32 with a reference 60.4 us
-//    (365 MB, 6.0 TB/s); 3588 x 32000 bf16: statistics 38 us (6.0 TB/s),
-//    gradient 73 (6.3 TB/s).
-//  * 16 bits with a reference and KL: the vector unit, about 45 instructions an
+//    (365 MB, 6.0 TB/s); 3588 x 32000 bf16: statistics 42 us (5.4 TB/s; 38 the
+//    fastest run), gradient 80 (5.8 TB/s; 76).
+//  * 16 bits with a reference and KL: the vector unit, about 44 instructions an
 //    entry, three of them exponentials: 16384 x 1858 bf16 48 us (3.8 TB/s), 1500
 //    x 50021 133 us (3.4 TB/s; the vector unit busy two thirds of it).
 //  * move lists: the zeros around the entries, and lines of 128 bytes for
 //    gathered logits: 20011 rows of 1858 bf16 20.5 us (74 MB written, about 50
 //    MB of lines read).
-//  * few rows: the launch and the loads that wait on one another, 4.3 us for 16
+//  * few rows: the launch and the loads that wait on one another, 4.4 us for 16
 //    rows of moves.
 #include "mfh_device.h"
 #include "mfh_kernels.h"
@@ -45,7 +45,8 @@ constexpr unsigned kFewRows = 1024;
 // Calls whose arrays hold more bytes than this go past the caches.  1858
 // columns of fp32 with a reference: 512 rows (11 MB) 6.8 us through the caches,
 // 7.1 past them; 1024 rows 9.9 and 9.2, 2048 rows 14.1 and 12.8; 20011 rows of
-// moves in bf16 27.5 and 21, 3588 x 32000 bf16 (statistics) 57.7 and 48.7.
+// moves in bf16 27.5 and 21, 3588 x 32000 bf16 (statistics, fastest runs)
+// 57.7 and 48.7.
 constexpr double kPastBytes = 16e6;
 
 // 16 bytes of a row at any element's alignment (global memory takes
@@ -1237,7 +1238,7 @@ void LaunchLoop(const RowLossParams &p, unsigned rows, hipStream_t s) {
 //  * 1072 vectors (4288 of fp32) on eight waves, four vectors a lane 157 us at
 //    16384 rows, eight a lane 185;
 //  * 4000 vectors (32000 of bf16, 3588 rows) on eight waves 38 us, on sixteen
-//    48.6 (statistics alone);
+//    48.6 (statistics alone, fastest runs);
 //  * 6253 vectors (50021 of bf16 with a reference, 1500 rows) in a loop 133 us,
 //    one row a workgroup 145, streamed twice 173.
 template <int DT, bool REF, bool PAST>
