@@ -306,8 +306,9 @@ int mfh_debug_quantize_fp8(int rows, int cols, const float *w, uint8_t *codes,
  * allocates nothing, keeps nothing between calls and copies nothing to the
  * host, so it can be captured into a HIP graph; only mfh_grad_set_create and
  * _destroy cannot.  Calls do not order each other: two that share an output
- * or a workspace are ordered by the caller.  Array arguments are device
- * memory of one device, in one allocation each; a pointer that is not
+ * or a workspace are ordered by the caller.  What a call writes overlaps none
+ * of its other arrays, but for the gradients in place below.  Array arguments
+ * are device memory of one device, in one allocation each; a pointer that is not
  * (host memory, another device's, another device's stream) is rejected with
  * MFH_ERR_INVALID.  Offsets, indices and actions are read on the device:
  * offsets outside their array are clamped to it. */
@@ -344,12 +345,12 @@ typedef struct {
  * q the softmax of the reference logits over the same entries and
  * temperature.  The first term is 0 in rows without an action or with
  * d_advantage NULL; d_old_logp NULL is the row's own l (rho = 1).  A row of
- * weight 0 gives zeros, whatever its logits hold.  The gradient of the sum of all
- * losses (old_logp, advantage, weight and q held fixed) goes to d_grad, every
+ * weight 0 gives zeros, whatever its logits hold.  The gradient of the sum of
+ * all losses (old_logp, advantage, weight and q held fixed) goes to d_grad, every
  * column of every row (0 outside the row's entries); at rho on a bound the
  * unclipped branch counts.  Where q lacks an entry that p has, KL is infinite
- * and the row's gradient not finite.  kl, entropy and logp (l, 0 without an action) are
- * not weighted.  Any output may be NULL.  d_grad may be d_logits or
+ * and the row's gradient not finite.  kl, entropy and logp (l, 0 without an
+ * action) are not weighted.  Any output may be NULL.  d_grad may be d_logits or
  * d_ref_logits with the same stride, and overlaps neither otherwise. */
 typedef struct {
   const float *d_old_logp;  /* [rows] */
@@ -375,11 +376,10 @@ int mfh_policy_loss_device(const mfh_policy_rows *rows, const mfh_policy_loss *l
  *   HINGE:   max(0, 1 - h)
  *   SQUARE:  (D - 1 / (2 beta))^2
  * times the pair's weight (a pair of weight 0 gives a loss, margin and
- * gradient of 0).  margin is h.  logp
- * is ln p_action, 0 without an action.  The gradient of the sum of all losses
+ * gradient of 0).  margin is h.  logp is ln p_action, 0 without an action.  The gradient of the sum of all losses
  * goes to the sequences' rows of d_grad, every column.  Rows before the first
- * sequence or behind the last are left as they are, whatever they hold.  Any output may
- * be NULL; d_grad may be d_logits with the same stride.  d_workspace holds
+ * sequence or behind the last are left as they are, whatever they hold.  Any
+ * output may be NULL; d_grad may be d_logits with the same stride.  d_workspace holds
  * mfh_preference_loss_workspace_bytes(rows) bytes, 8-byte aligned. */
 enum { MFH_PREFERENCE_SIGMOID = 0, MFH_PREFERENCE_HINGE = 1, MFH_PREFERENCE_SQUARE = 2 };
 typedef struct {
@@ -407,8 +407,9 @@ int mfh_preference_loss_device(const mfh_policy_rows *rows, const mfh_preference
  * after creation, so calls on one set may run at once.  dst receives the
  * scaled gradients: src itself, memory of its own, or NULL for a tensor that
  * counts in the norm only.  No dst may overlap another tensor's src or dst,
- * nor its own src in part.  device -1 is the device of the first tensor (the current one without
- * any).  Waits for the device only in _destroy. */
+ * nor its own src in part.  device -1 is the device of the first tensor (the
+ * current one without any).  Only _destroy waits for the device; the set
+ * outlives every graph that has captured a call on it. */
 typedef struct {
   const void *src;
   void *dst;

@@ -2,8 +2,8 @@
 //
 //   N = sqrt(sum over all tensors of g^2),  out = g min(1, max_norm / N).
 //
-// The tensors are cut into chunks of at most kGradChunk elements, listed once
-// per set; a workgroup of 256 takes whole chunks.  Squares are summed in 64
+// The tensors are cut into chunks of at most kGradChunkBytes, listed once per
+// set; a workgroup of 256 takes whole chunks.  Squares are summed in 64
 // bits: a 32-bit sum would lose small gradients beside large ones and
 // overflow from |g| = 2^64, and the card's 64-bit rate is far above what the
 // memory delivers.  The norm has to be known before anything is written, so
@@ -285,8 +285,8 @@ hipError_t LaunchGradSum(const double *partials, int n, double *sumsq, hipStream
 }
 
 hipError_t LaunchGradScale(const GradChunk *chunks, std::int64_t n_chunks,
-                           bool past, const double *partials, int n, float max_norm, float *norm, hipStream_t stream,
-                           std::string *err) {
+                           bool past, const double *partials, int n, float max_norm,
+                           float *norm, hipStream_t stream, std::string *err) {
   if (n_chunks < 0 || (n_chunks > 0 && !chunks) || n < 1 || !partials) {
     if (err)
       *err = "grad_scale: needs a chunk list and partial sums";

@@ -116,7 +116,8 @@ int PointerDevice(const char *fn, const char *name, const void *p, int want, int
 }
 
 int StreamDevice(const char *fn, hipStream_t stream, int device) {
-  if (!stream)
+  // The standing streams belong to the device that is current at the launch.
+  if (!stream || stream == hipStreamPerThread || stream == hipStreamLegacy)
     return MFH_OK;
   hipDevice_t dev = 0;
   const hipError_t e = hipStreamGetDevice(stream, &dev);
@@ -605,6 +606,11 @@ int mfh_grad_clip_device(const mfh_grad_set *set, float max_norm, float *d_norm,
     return Invalid(fn, "the workspace is too small");
   if (!Aligned(d_norm, 4) || !Aligned(d_workspace, 8))
     return Invalid(fn, "pointers must be aligned to their elements");
+  // One workgroup writes the norm while others still sum the workspace.
+  const auto norm = reinterpret_cast<std::uintptr_t>(d_norm),
+             work = reinterpret_cast<std::uintptr_t>(d_workspace);
+  if (d_norm && norm < work + sizeof(double) * groups && work < norm + sizeof(float))
+    return Invalid(fn, "d_norm lies in the workspace");
   try {
     OnDevice on;
     const Named ptrs[] = {{"d_workspace", d_workspace}, {"d_norm", d_norm}};

@@ -248,3 +248,28 @@ def test_refusals_with_a_device(dev):
     g.set.close()
     with pytest.raises(RuntimeError, match="null argument"):
         g.set.clip_device(1.0, g.norm, g.ws, 1 << 12)
+
+
+def test_a_norm_in_the_workspace_is_refused(dev):
+    """Refused on the host; right behind the workspace it is taken."""
+    g = Grads(dev, [(np.full(9000, 2.0), "f32")])
+    n = g.set.workspace_bytes
+    for at in (0, 4, n - 4):
+        with pytest.raises(RuntimeError, match="d_norm lies in the workspace"):
+            g.set.clip_device(1.0, g.ws + at, g.ws, n)
+    g.set.clip_device(1.0, g.ws + n, g.ws, n)
+    dev.sync()
+    got = dev.get(g.ws + n, np.zeros(1, np.float32))[0]
+    assert got == np.float32(2.0 * np.sqrt(9000.0))
+
+
+def test_the_standing_streams(dev):
+    """hipStreamLegacy and hipStreamPerThread, by their handles."""
+    rng = np.random.default_rng(12)
+    tensors = [(rng.normal(size=n), "f32") for n in (5000, 77)]
+    want = Grads(dev, tensors).clip(0.1)
+    for stream in (1, 2):
+        g = Grads(dev, tensors)
+        g.set.clip_device(0.1, g.norm, g.ws, g.set.workspace_bytes, stream=stream)
+        dev.sync()
+        assert dev.get(g.norm, np.zeros(1, np.float32))[0] == want[0]
