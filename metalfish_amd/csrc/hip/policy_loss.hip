@@ -295,15 +295,19 @@ __device__ __forceinline__ float GroupSums(Sums &s, float top, float c, float (*
   return top == -__builtin_inff() ? 0.f : top;
 }
 
-// A NaN; an entry so far below the reference (u < -60) that exp(-u) may
-// overflow; or coefficients (Coefs a, b) above 1, whose product with a logit of
-// the type's lowest value may.
+// u below which a term of KL comes from the reference instead: there exp(-u)
+// (up to 2^58 above it) may bring back a p that is below 2^-126 and 0.
+constexpr float kFarBelow = -40.f;
+
+// A NaN; an entry far below the reference (u < kFarBelow); or coefficients
+// (Coefs a, b) above 1, whose product with a logit of the type's lowest value
+// may overflow.
 template <bool REF>
 __device__ __forceinline__ bool NeedsGuard(const RowLossParams &a, float weight, const Sums &s) {
   return s.et != s.et || s.ed != s.ed || !(fabsf(weight * a.inv_temp) < 0x1p100f) ||
          !(fabsf(a.entropy_coef) * a.inv_temp <= 1.f) ||
          (REF && (!(fabsf(a.kl_coef) <= 1.f) ||
-                  !((s.least - s.ed * Rcp(s.e)) * a.inv_temp > -60.f)));
+                  !((s.least - s.ed * Rcp(s.e)) * a.inv_temp > kFarBelow)));
 }
 
 // What a row's scalars come to, from its statistics.
@@ -335,18 +339,20 @@ struct RowGrad {
 };
 
 // The same as P_k (a (x_k - m) + b u_k + d) with P = 2^power p, with what P and
-// u need: the scale's power of two is in P, so that a and b stay small whatever
-// the row's weight (a loss scale of 2^16, say).
+// u need: a large scale's power of two is in P, so that a and b stay small
+// whatever the row's weight (a loss scale of 2^16, say).  A small one's is not:
+// the terms of KL, which no weight may change, are sums of P exp(-u), and a P
+// smaller than p vanishes earlier.
 struct Coefs {
   float m, c, shift, inv_temp, mean_d, kl_shift, a, b, d;
   int power;
 };
-constexpr int kLeastPower = -30, kMostPower = 100;
+constexpr int kMostPower = 100;
 
 __device__ __forceinline__ Coefs CoefsOf(const RowStats &st, const RowGrad &g, float inv_temp) {
   Coefs k;
   const int power = __builtin_amdgcn_frexp_expf(g.scale);
-  k.power = power < kLeastPower ? kLeastPower : power > kMostPower ? kMostPower : power;
+  k.power = power < 0 ? 0 : power > kMostPower ? kMostPower : power;
   const float scale = ldexpf(g.scale, -k.power);
   k.m = st.m;
   k.c = inv_temp * kLog2e;
@@ -360,7 +366,7 @@ __device__ __forceinline__ Coefs CoefsOf(const RowStats &st, const RowGrad &g, f
   return k;
 }
 
-// exp(-u) - 1 + u for u > -60: its series for |u| < 1/4 (the first term left out
+// exp(-u) - 1 + u for u > kFarBelow: its series for |u| < 1/4 (the first term left out
 // is 1.2e-8 of the sum), where the difference would cancel.
 __device__ __forceinline__ float Phi(float u) {
   const float e = Exp2(-u * kLog2e);
@@ -377,11 +383,11 @@ __device__ __forceinline__ float Phi(float u) {
 }
 
 // P (exp(-u) - 1 + u), the term of KL, for any u; ym: the reference logit less
-// the policy's maximum.  Far below 0, where exp(-u) may overflow against a
-// tiny p, their product comes from ym; an entry that is masked here adds
+// the policy's maximum.  Far below 0, where exp(-u) is large against a tiny
+// p, their product comes from ym; an entry that is masked here adds
 // nothing but its reference probability.
 __device__ __forceinline__ float KlTerm(const Coefs &k, float p, float u, float ym) {
-  if (!(u > -60.f)) {
+  if (!(u > kFarBelow)) {
     const float q = Exp2(ym * k.c + k.kl_shift);
     return p == 0.f ? q : q - p * (1.f - u);
   }

@@ -1,0 +1,146 @@
+"""KL of the policy loss where the policy and its reference are far apart:
+divergences beyond 88 nats, finite masks in the reference, weights of any
+size, references a constant away, and KL watched without a coefficient.  On
+whole rows of one wave, of several, in the loop and streamed, and on lists.
+
+Bounds: ``loss_util``'s, with u = d - E_p d off by 3 roundings of what d is
+formed from, and for KL of 1 and more as an error of the logarithm: the
+relative errors of the terms p exp(-u), weighted by their shares q."""
+
+import numpy as np
+import pytest
+
+import gpu_util
+import learn_gpu as lg
+import loss_util as lu
+from metalfish_amd import backend
+from oracle import losses
+
+pytestmark = pytest.mark.gpu
+
+LOWEST = {"f32": -float(np.finfo(np.float32).max), "f16": -65504.0,
+          "bf16": -float(lu.from_bits(np.uint16(0x7F7F), "bf16"))}
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _need_gpu():
+    if backend.device_count() < 1:
+        pytest.fail("GPU tests need an MI355X; none visible")
+
+
+@pytest.fixture
+def dev():
+    d = gpu_util.DeviceBuffers()
+    yield d
+    d.free()
+
+
+class Bounds(lu.Bounds):
+    def kl(self):
+        row, p, temp = self.row, self.row.p, self.row.temp
+        on = p > 0
+        with np.errstate(all="ignore"):
+            raw = row.v - row.r
+            zx, zy = (row.v - np.max(row.v)) / temp, (row.r - np.max(row.r)) / temp
+            mean_raw = float(np.sum(np.where(on, p * raw, 0.0)))
+            # Far references are taken relative to both maxima.
+            apart = abs(mean_raw) > 64
+            d = np.where(on, zx - zy if apart else raw / temp, 0.0)
+            size = np.abs(d) + (np.where(on, np.abs(zx) + np.abs(zy), 0.0) if apart else 0.0)
+            mean = float(np.sum(p * d))
+            u = np.where(on, d - mean, 0.0)
+            off_mean = float(np.sum(p * (np.abs(d) * (self.rel_p + (self.k + 7) * lu.U) +
+                                         3 * lu.U * size)))
+            off_u = 3 * lu.U * size + lu.U * np.abs(u) + off_mean
+            q = np.exp(row.lq)
+            offset = 0.0 if apart else abs(np.max(row.v) - np.max(row.r)) / temp
+            rel = np.where(on, self.rel_p + off_u + lu.U * (self.k + 14 + 4 * np.abs(u)),
+                           off_mean + lu.U * (self.k + 14 + 8 * np.abs(zy)
+                                              + 8 * (offset + abs(mean))))
+            rel = np.where(q > 0, rel, 0.0)
+            if row.kl >= 1:
+                bound = float(np.sum(q * rel)) + 3 * lu.U * offset
+            else:
+                grow = np.exp(np.minimum(-u, 700.0))
+                phi = np.maximum(grow - 1 + u, 0.0)
+                terms = p * (phi * (self.rel_p + (self.k + 10) * lu.U) + np.abs(1 - grow) * off_u +
+                             grow * off_u ** 2 +
+                             np.where(np.abs(u) < 0.2, 0.0,
+                                      4 * lu.U * (grow * (1 + np.abs(u)) + 1 + np.abs(u))))
+                bound = float(np.sum(np.where(on, terms, 3 * q * rel)))
+        return 2 * (self.p_mass(bound) + 4 * lu.U * abs(row.kl)), off_u, np.abs(u)
+
+    def p_mass(self, bound):
+        # p below 2^-126 is 0 on the device, at u > -40 with exp(-u) < 2^58; the
+        # oracle's logarithms of sums near 1 are off by 2^-53 a step.
+        return bound + self.row.p.size * 2.0 ** -68 + 2.0 ** -50
+
+    def grad(self, scale, slope, slope_rel, kl_coef=0.0, entropy_coef=0.0):
+        """The same, with what such p miss in the means, and the oracle's own
+        rounding (2^-53 a step) of ln p - ln q - KL."""
+        row, p = self.row, self.row.p
+        on = p > 0
+        with np.errstate(all="ignore"):
+            known = super().grad(scale, slope, slope_rel, kl_coef, entropy_coef)
+            far = abs(kl_coef) * np.max(np.where(on, np.abs(row.v - row.r), 0.0)) / row.temp + \
+                abs(entropy_coef) * np.max(np.where(on, np.abs(self.z), 0.0))
+            own = p * np.where(on, np.abs(row.lp) + np.abs(row.lq) + abs(row.kl), 0.0)
+        return known + abs(scale) * (row.spread(p * far * p.size * 2.0 ** -125) +
+                                     row.spread(own * 2.0 ** -50))
+
+
+def check(batch, got, ref, kl_coef, entropy_coef=0.0, weight=None):
+    """KL, loss and gradient of every row, without a surrogate."""
+    refv = lu.from_bits(lu.to_bits(ref, batch.dtype), batch.dtype)
+    k = lu.additions(batch.vocab, batch.moves is not None)
+    for b in range(batch.rows):
+        w = 1.0 if weight is None else float(weight[b])
+        row = losses.Row(batch.values[b], None if batch.moves is None else batch.moves[b], None,
+                         batch.temp, refv[b])
+        bd = Bounds(row, k)
+        kl = bd.kl()[0]
+        lu.close(got["kl"][b], row.kl, kl)
+        want = kl_coef * row.kl - entropy_coef * row.entropy
+        total = kl_coef * kl + entropy_coef * bd.entropy
+        sizes = kl_coef * abs(row.kl) + entropy_coef * abs(row.entropy) + abs(want)
+        lu.close(got["loss"][b], w * want, 2 * abs(w) * (total + 4 * lu.U * sizes))
+        grad = kl_coef * row.grad_kl() - entropy_coef * row.grad_entropy()
+        lu.close(got["grad"][b], w * grad,
+                 bd.grad(w / batch.temp, 0.0, 0.0, kl_coef, entropy_coef), batch.dtype)
+
+
+# A vocabulary for each kernel: one wave, four, eight, the loop, streamed, and
+# lists of a few and of more than 64 moves (vocabulary, moves).
+SHAPES = {"wave": (256, 0), "waves": (1858, 0), "eight": (12000, 0), "loop": (20003, 0),
+          "streamed": (33001, 0), "list": (1858, 12), "long-list": (1858, 150)}
+
+
+def _rows(rng, shape, dtype, n, far=-50.0):
+    """n rows of entries `far` below 0 in policy and reference alike, and five
+    columns among the entries, the first and the last of the row with them."""
+    vocab, moves = SHAPES[shape]
+    if dtype != "f32" and vocab > 4096:
+        vocab *= 2
+    x = np.full((n, vocab), far)
+    at = np.concatenate([[0, vocab - 1], 1 + rng.choice(vocab - 2, 3, replace=False)])
+    lists = None
+    if moves:
+        more = np.setdiff1d(np.arange(1, vocab - 1), at)
+        lists = [list(at) + list(rng.choice(more, moves - 5, replace=False)) for _ in range(n)]
+    return x, x.copy(), at, lists
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_small_weights_leave_kl_alone(dev, shape):
+    """Entries far below the maximum whose reference is not so far: their
+    terms are of p exp(-u) with p near 2^-100 and exp(-u) near 2^85."""
+    rng = np.random.default_rng(1)
+    weight = np.array([1.0, 1e-3, -1e-6, 1e-9, 1e-20, 2.0], np.float32)
+    for below, ref_below in ((70.0, 11.0), (75.0, 16.0), (95.0, 30.0)):
+        x, ref, at, lists = _rows(rng, shape, "f32", len(weight), -below)
+        ref[:] = -ref_below
+        x[:, at[2]] = ref[:, at[2]] = 0.0
+        batch = lg.Batch(dev, x, "f32", lists, None)
+        got = lg.policy(batch, ref=ref, weight=weight, kl_coef=0.3, entropy_coef=0.1)
+        assert np.all(got["kl"] > 0)
+        check(batch, got, ref, 0.3, 0.1, weight)
