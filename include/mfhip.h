@@ -349,9 +349,10 @@ typedef struct {
  * all losses (old_logp, advantage, weight and q held fixed) goes to d_grad, every
  * column of every row (0 outside the row's entries); at rho on a bound the
  * unclipped branch counts.  Where q lacks an entry that p has, KL is infinite
- * and the row's gradient not finite.  kl, entropy and logp (l, 0 without an
- * action) are not weighted.  Any output may be NULL.  d_grad may be d_logits or
- * d_ref_logits with the same stride, and overlaps neither otherwise. */
+ * and, unless kl_coef is 0, the row's gradient not finite.  kl, entropy and
+ * logp (l, 0 without an action) are not weighted.  Any output may be NULL.
+ * d_grad may be d_logits or d_ref_logits with the same stride, and overlaps
+ * neither otherwise. */
 typedef struct {
   const float *d_old_logp;  /* [rows] */
   const float *d_advantage; /* [rows] */

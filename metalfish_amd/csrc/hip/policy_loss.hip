@@ -299,12 +299,13 @@ __device__ __forceinline__ float GroupSums(Sums &s, float top, float c, float (*
 // (up to 2^58 above it) may bring back a p that is below 2^-126 and 0.
 constexpr float kFarBelow = -40.f;
 
-// A NaN; an entry far below the reference (u < kFarBelow); or coefficients
-// (Coefs a, b) above 1, whose product with a logit of the type's lowest value
-// may overflow.
+// A NaN; an infinite E_p d; an entry far below the reference (u < kFarBelow); or
+// coefficients (Coefs a, b) above 1, whose product with a logit of the type's
+// lowest value may overflow.
 template <bool REF>
 __device__ __forceinline__ bool NeedsGuard(const RowLossParams &a, float weight, const Sums &s) {
-  return s.et != s.et || s.ed != s.ed || !(fabsf(weight * a.inv_temp) < 0x1p100f) ||
+  return s.et != s.et || !(fabsf(s.ed) < __builtin_inff()) ||
+         !(fabsf(weight * a.inv_temp) < 0x1p100f) ||
          !(fabsf(a.entropy_coef) * a.inv_temp <= 1.f) ||
          (REF && (!(fabsf(a.kl_coef) <= 1.f) ||
                   !((s.least - s.ed * Rcp(s.e)) * a.inv_temp > kFarBelow)));
@@ -413,7 +414,9 @@ __device__ __forceinline__ void FinishEntries(const Coefs &k, bool want_kl, cons
     float v = k.a * xm + k.d;
     if constexpr (REF) {
       u[i] = (x[i] - y[i]) * k.inv_temp - k.mean_d;
-      v = k.b * u[i] + v;
+      // Without a coefficient KL is only watched: u may be infinite.
+      if (!GUARD || k.b != 0.f)
+        v = k.b * u[i] + v;
     }
     f[i] = GUARD && p[i] == 0.f ? 0.f : p[i] * v;
   }

@@ -144,3 +144,26 @@ def test_small_weights_leave_kl_alone(dev, shape):
         got = lg.policy(batch, ref=ref, weight=weight, kl_coef=0.3, entropy_coef=0.1)
         assert np.all(got["kl"] > 0)
         check(batch, got, ref, 0.3, 0.1, weight)
+
+
+@pytest.mark.parametrize("dtype", lu.TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_kl_without_a_coefficient_leaves_the_gradient_alone(dev, shape, dtype):
+    """The reference lacks entries that the policy has: KL is infinite, and
+    neither loss nor gradient holds it."""
+    rng = np.random.default_rng(2)
+    x, ref, at, lists = _rows(rng, shape, dtype, 4)
+    x[:] = rng.normal(size=x.shape)
+    ref[:] = x + 0.3 * rng.normal(size=x.shape)
+    ref[0, at[0]] = -np.inf
+    ref[1, at[1:3]] = -np.inf
+    ref[2] = -np.inf
+    action = int(at[3])
+    batch = lg.Batch(dev, x, dtype, lists, [action] * 4)
+    kw = dict(advantage=np.ones(4), entropy_coef=0.1)
+    got, want = lg.policy(batch, ref=ref, **kw), lg.policy(batch, **kw)
+    assert np.all(got["kl"][:3] == np.inf) and np.isfinite(got["kl"][3])
+    for k in ("loss", "logp", "entropy"):
+        lu.close(got[k], want[k], 4 * lu.U * np.abs(want[k]))
+    # The same sums in another order, and one rounding more.
+    lu.close(got["grad"], want["grad"], 16 * lu.U * np.abs(want["grad"]).max(), dtype)
