@@ -234,9 +234,9 @@ __device__ __forceinline__ void GroupSum(float (&v)[N], float (*red)[8]) {
 }
 
 // Sums over a row's entries: of e, of e log2(e), of e d with d = x - y; and the
-// least d.
+// greatest |d|.
 struct Sums {
-  float e = 0.f, et = 0.f, ed = 0.f, least = __builtin_inff();
+  float e = 0.f, et = 0.f, ed = 0.f, far = 0.f;
 };
 
 // One entry's part, t = log2(e).  GUARD: an entry whose e is 0 adds nothing,
@@ -251,7 +251,7 @@ __device__ __forceinline__ void AddStats(float x, float y, float m, float c, Sum
   if constexpr (REF) {
     const float d = x - y;
     s.ed += GUARD && e == 0.f ? 0.f : e * d;
-    s.least = fminf(s.least, d);
+    s.far = fmaxf(s.far, fabsf(d));
   }
 }
 
@@ -267,13 +267,13 @@ __device__ __forceinline__ float GroupSums(Sums &s, float top, float c, float (*
   s.et = WaveSum(s.et);
   if constexpr (REF) {
     s.ed = WaveSum(s.ed);
-    s.least = -WaveMax(-s.least);
+    s.far = WaveMax(s.far);
   }
   if constexpr (W > 1) {
     __syncthreads();
     if ((threadIdx.x & 63) == 0) {
       float *mine = red[threadIdx.x >> 6];
-      *reinterpret_cast<f32x4 *>(mine) = f32x4{s.e, s.et, s.ed, s.least};
+      *reinterpret_cast<f32x4 *>(mine) = f32x4{s.e, s.et, s.ed, s.far};
       mine[4] = top;
     }
     __syncthreads();
@@ -288,7 +288,7 @@ __device__ __forceinline__ float GroupSums(Sums &s, float top, float c, float (*
     s.et = LanesSum<W>(f == 0.f ? none : f * (v[1] + v[0] * step));
     if constexpr (REF) {
       s.ed = LanesSum<W>(f == 0.f ? none : f * v[2]);
-      s.least = -LanesMax<W>(-v[3]);
+      s.far = LanesMax<W>(v[3]);
     }
     return top;
   }
@@ -299,16 +299,16 @@ __device__ __forceinline__ float GroupSums(Sums &s, float top, float c, float (*
 // (up to 2^58 above it) may bring back a p that is below 2^-126 and 0.
 constexpr float kFarBelow = -40.f;
 
-// A NaN; an infinite E_p d; an entry far below the reference (u < kFarBelow); or
-// coefficients (Coefs a, b) above 1, whose product with a logit of the type's
-// lowest value may overflow.
+// A NaN; an entry far from the reference on either side (-kFarBelow bounds |u|:
+// below, KL's terms overflow, and above, u itself may: the lowest value in the
+// reference against 1 / T above 1); or coefficients (Coefs a, b) above 1, whose
+// product with a logit of the type's lowest value may overflow.
 template <bool REF>
 __device__ __forceinline__ bool NeedsGuard(const RowLossParams &a, float weight, const Sums &s) {
-  return s.et != s.et || !(fabsf(s.ed) < __builtin_inff()) ||
-         !(fabsf(weight * a.inv_temp) < 0x1p100f) ||
+  return s.et != s.et || !(fabsf(weight * a.inv_temp) < 0x1p100f) ||
          !(fabsf(a.entropy_coef) * a.inv_temp <= 1.f) ||
          (REF && (!(fabsf(a.kl_coef) <= 1.f) ||
-                  !((s.least - s.ed * Rcp(s.e)) * a.inv_temp > kFarBelow)));
+                  !((s.far + fabsf(s.ed * Rcp(s.e))) * a.inv_temp < -kFarBelow)));
 }
 
 // What a row's scalars come to, from its statistics.
@@ -317,11 +317,11 @@ struct RowStats {
   float log_sum;   // ln S
   float log2_sum;  // log2 S
   float mean_z;    // E_p z
-  float mean_d;    // E_p d
+  float mean_d;    // E_p (x - y), without 1 / T
   bool empty;      // no entry left
 };
 
-__device__ __forceinline__ RowStats Stats(float m, const Sums &sums, float inv_temp) {
+__device__ __forceinline__ RowStats Stats(float m, const Sums &sums) {
   RowStats r;
   r.m = m;
   r.empty = sums.e == 0.f;
@@ -329,7 +329,7 @@ __device__ __forceinline__ RowStats Stats(float m, const Sums &sums, float inv_t
   r.log2_sum = Log2(sum);
   r.log_sum = r.log2_sum * kLn2;
   r.mean_z = sums.et * kLn2 * inv;
-  r.mean_d = sums.ed * inv_temp * inv;
+  r.mean_d = sums.ed * inv;
   return r;
 }
 
@@ -345,7 +345,7 @@ struct RowGrad {
 // the terms of KL, which no weight may change, are sums of P exp(-u), and a P
 // smaller than p vanishes earlier.
 struct Coefs {
-  float m, c, shift, inv_temp, mean_d, kl_shift, a, b, d;
+  float m, c, shift, inv_temp, mean_d, mean_u, kl_shift, a, b, d;
   int power;
 };
 constexpr int kMostPower = 100;
@@ -360,7 +360,8 @@ __device__ __forceinline__ Coefs CoefsOf(const RowStats &st, const RowGrad &g, f
   k.shift = static_cast<float>(k.power) - st.log2_sum;
   k.inv_temp = inv_temp;
   k.mean_d = st.mean_d;
-  k.kl_shift = st.mean_d * kLog2e + k.shift;
+  k.mean_u = st.mean_d * inv_temp;
+  k.kl_shift = k.mean_u * kLog2e + k.shift;
   k.a = scale * g.entropy * inv_temp;
   k.b = scale * g.kl;
   k.d = -scale * (g.slope + g.entropy * st.mean_z);
@@ -383,16 +384,16 @@ __device__ __forceinline__ float Phi(float u) {
   return fabsf(u) < 0.25f ? near : far;
 }
 
-// P (exp(-u) - 1 + u), the term of KL, for any u; ym: the reference logit less
-// the policy's maximum.  Far below 0, where exp(-u) is large against a tiny
-// p, their product comes from ym; an entry that is masked here adds
-// nothing but its reference probability.
-__device__ __forceinline__ float KlTerm(const Coefs &k, float p, float u, float ym) {
+// P (exp(-u) - 1 + u), the term of KL, for any u; pu: P u, finite also where u
+// is not; ym: the reference logit less the policy's maximum.  Far below 0, where
+// exp(-u) is large against a tiny p, their product comes from ym; an entry that
+// is masked here adds nothing but its reference probability.
+__device__ __forceinline__ float KlTerm(const Coefs &k, float p, float u, float pu, float ym) {
   if (!(u > kFarBelow)) {
     const float q = Exp2(ym * k.c + k.kl_shift);
-    return p == 0.f ? q : q - p * (1.f - u);
+    return p == 0.f ? q : q - p + pu;
   }
-  return p == 0.f ? 0.f : p * Phi(u);
+  return p == 0.f ? 0.f : u > -kFarBelow ? pu - p : p * Phi(u);
 }
 
 // KL from the sum of its terms; infinite where the reference lacks what the
@@ -406,24 +407,34 @@ __device__ __forceinline__ float KlOf(float terms, const Coefs &k) {
 template <int N, bool REF, bool GUARD>
 __device__ __forceinline__ void FinishEntries(const Coefs &k, bool want_kl, const float (&x)[N],
                                               const float (&y)[N], float &kl, float (&f)[N]) {
-  float p[N], u[N];
+  float p[N], u[N], pu[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const float xm = x[i] - k.m;
     p[i] = Exp2(xm * k.c + k.shift);
     float v = k.a * xm + k.d;
-    if constexpr (REF) {
-      u[i] = (x[i] - y[i]) * k.inv_temp - k.mean_d;
-      // Without a coefficient KL is only watched: u may be infinite.
-      if (!GUARD || k.b != 0.f)
-        v = k.b * u[i] + v;
+    if constexpr (REF && GUARD) {
+      // p before 1 / T: u may be beyond the 32-bit range where p u is not.
+      const float apart = (x[i] - y[i]) - k.mean_d;
+      u[i] = apart * k.inv_temp;
+      pu[i] = p[i] * k.inv_temp * apart;
+      f[i] = p[i] * v;
+      // Without a coefficient KL is only watched: it may be infinite.
+      if (k.b != 0.f)
+        f[i] += k.b * pu[i];
+    } else if constexpr (REF) {
+      u[i] = (x[i] - y[i]) * k.inv_temp - k.mean_u;
+      f[i] = p[i] * (k.b * u[i] + v);
+    } else {
+      f[i] = p[i] * v;
     }
-    f[i] = GUARD && p[i] == 0.f ? 0.f : p[i] * v;
+    if (GUARD && p[i] == 0.f)
+      f[i] = 0.f;
   }
   if (REF && want_kl) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      kl += GUARD ? KlTerm(k, p[i], u[i], y[i] - k.m) : p[i] * Phi(u[i]);
+      kl += GUARD ? KlTerm(k, p[i], u[i], pu[i], y[i] - k.m) : p[i] * Phi(u[i]);
   }
 }
 
@@ -707,7 +718,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void DenseRowKernel(RowLossP
   const bool guarded = NeedsGuard<REF>(a, in.weight, sums);
   if (guarded)
     sum(std::true_type{});
-  const RowStats st = Stats(m, sums, a.inv_temp);
+  const RowStats st = Stats(m, sums);
   if (st.empty) {
     if (tid == 0)
       WriteZeros(a, row);
@@ -806,7 +817,7 @@ __device__ __forceinline__ void StreamRow(const RowLossParams &a, std::int64_t r
   const float top = WaveMax(m);
   rescale(m, top == -__builtin_inff() ? 0.f : top);
   m = GroupSums<W, REF, true>(sums, top, c, red);
-  const RowStats st = Stats(m, sums, a.inv_temp);
+  const RowStats st = Stats(m, sums);
   if (st.empty) {
     if (tid == 0)
       WriteZeros(a, row);
@@ -963,7 +974,7 @@ __device__ __forceinline__ std::int64_t LoopRows(const RowLossParams &a, std::in
     // A row without an entry left needs them too (its sums hold 0 times -inf).
     if (!GUARD && live && NeedsGuard<REF>(a, in.weight, sums))
       return row;
-    const RowStats st = Stats(m, sums, a.inv_temp);
+    const RowStats st = Stats(m, sums);
     const RowResult res = Evaluate(a, in, st, acted && !st.empty, xa);
     const Coefs k = CoefsOf(st, res.grad, a.inv_temp);
     float kl[1] = {0.f};
@@ -1099,7 +1110,7 @@ __device__ __forceinline__ void MovesRow(const RowLossParams &a, std::int64_t ro
   for (int r = 0; r < NE; ++r)
     AddStats<REF, true>(xv[r], yv[r], m, c, sums);
   (void)GroupSums<1, REF, true>(sums, top, c, nullptr);
-  const RowStats st = Stats(m, sums, a.inv_temp);
+  const RowStats st = Stats(m, sums);
   const RowResult res = Evaluate(a, in, st, acted, xa);
   const bool want_kl = REF && WantsKl(a);
   float kl = 0.f, f[NE] = {};

@@ -167,3 +167,21 @@ def test_kl_without_a_coefficient_leaves_the_gradient_alone(dev, shape, dtype):
         lu.close(got[k], want[k], 4 * lu.U * np.abs(want[k]))
     # The same sums in another order, and one rounding more.
     lu.close(got["grad"], want["grad"], 16 * lu.U * np.abs(want["grad"]).max(), dtype)
+
+
+@pytest.mark.parametrize("dtype", lu.TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("temp", [0.3, 0.7, 1.0])
+def test_entries_masked_in_the_reference_alone(dev, shape, dtype, temp):
+    """The reference masked by the type's lowest value at every other column,
+    where the policy is far below its maximum, but finite."""
+    rng = np.random.default_rng(3)
+    x, ref, at, lists = _rows(rng, shape, dtype, 3)
+    x[:] = rng.normal(size=x.shape)
+    ref[:] = x + 0.3 * rng.normal(size=x.shape)
+    for b, below in enumerate((-1e4, -300.0, -6e4)):
+        x[b, 1::2], ref[b, 1::2] = below, LOWEST[dtype]
+    batch = lg.Batch(dev, x, dtype, lists, None, temp)
+    got = lg.policy(batch, ref=ref, kl_coef=0.3, entropy_coef=0.1)
+    assert all(np.isfinite(v).all() for v in got.values())
+    check(batch, got, ref, 0.3, 0.1)
