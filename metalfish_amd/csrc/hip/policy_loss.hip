@@ -234,10 +234,13 @@ __device__ __forceinline__ void GroupSum(float (&v)[N], float (*red)[8]) {
 }
 
 // Sums over a row's entries: of e, of e log2(e), of e d with d = x - y; and the
-// greatest |d|.
+// greatest |d|, or with the guards the greatest y.
 struct Sums {
-  float e = 0.f, et = 0.f, ed = 0.f, far = 0.f;
+  float e, et, ed, far;
 };
+template <bool GUARD> __device__ __forceinline__ Sums NoSums() {
+  return {0.f, 0.f, 0.f, GUARD ? -__builtin_inff() : 0.f};
+}
 
 // One entry's part, t = log2(e).  GUARD: an entry whose e is 0 adds nothing,
 // also where its logits are infinite.  Rows without such entries are summed
@@ -251,7 +254,7 @@ __device__ __forceinline__ void AddStats(float x, float y, float m, float c, Sum
   if constexpr (REF) {
     const float d = x - y;
     s.ed += GUARD && e == 0.f ? 0.f : e * d;
-    s.far = fmaxf(s.far, fabsf(d));
+    s.far = fmaxf(s.far, GUARD ? y : fabsf(d));
   }
 }
 
@@ -305,7 +308,7 @@ constexpr float kFarBelow = -40.f;
 // product with a logit of the type's lowest value may overflow.
 template <bool REF>
 __device__ __forceinline__ bool NeedsGuard(const RowLossParams &a, float weight, const Sums &s) {
-  return s.et != s.et || !(fabsf(weight * a.inv_temp) < 0x1p100f) ||
+  return s.et != s.et || !(fabsf(weight * a.inv_temp) < 0x1p40f) ||
          !(fabsf(a.entropy_coef) * a.inv_temp <= 1.f) ||
          (REF && (!(fabsf(a.kl_coef) <= 1.f) ||
                   !((s.far + fabsf(s.ed * Rcp(s.e))) * a.inv_temp < -kFarBelow)));
@@ -318,6 +321,7 @@ struct RowStats {
   float log2_sum;  // log2 S
   float mean_z;    // E_p z
   float mean_d;    // E_p (x - y), without 1 / T
+  float far;       // as in Sums
   bool empty;      // no entry left
 };
 
@@ -330,6 +334,7 @@ __device__ __forceinline__ RowStats Stats(float m, const Sums &sums) {
   r.log_sum = r.log2_sum * kLn2;
   r.mean_z = sums.et * kLn2 * inv;
   r.mean_d = sums.ed * inv;
+  r.far = sums.far;
   return r;
 }
 
@@ -343,12 +348,22 @@ struct RowGrad {
 // u need: a large scale's power of two is in P, so that a and b stay small
 // whatever the row's weight (a loss scale of 2^16, say).  A small one's is not:
 // the terms of KL, which no weight may change, are sums of P exp(-u), and a P
-// smaller than p vanishes earlier.
+// smaller than p vanishes earlier.  Without the guards they are below 2^40
+// times exp(40) = 2^58.
+//
+// For the guards: y_m the greatest reference logit and peak the greatest of
+// ln(p_k exp(-u_k)) = (y_k - m) / T + E_p d - ln S.  KL lies between peak and
+// peak + ln(entries).  Above kWide it is taken as peak + ln sum exp((y_k - y_m)
+// / T), which has no overflow; below, its terms in P are at most 2^40 exp(30)
+// = 2^84 each.
 struct Coefs {
-  float m, c, shift, inv_temp, mean_d, mean_u, kl_shift, a, b, d;
+  float m, c, shift, inv_temp, mean_d, mean_u, a, b, d;
+  float y_m, peak, y_shift;
+  bool wide;
   int power;
 };
-constexpr int kMostPower = 100;
+constexpr int kMostPower = 40;
+constexpr float kWide = 30.f;
 
 __device__ __forceinline__ Coefs CoefsOf(const RowStats &st, const RowGrad &g, float inv_temp) {
   Coefs k;
@@ -361,7 +376,10 @@ __device__ __forceinline__ Coefs CoefsOf(const RowStats &st, const RowGrad &g, f
   k.inv_temp = inv_temp;
   k.mean_d = st.mean_d;
   k.mean_u = st.mean_d * inv_temp;
-  k.kl_shift = k.mean_u * kLog2e + k.shift;
+  k.y_m = st.far;
+  k.peak = k.mean_u + (st.far - st.m) * inv_temp - st.log_sum;
+  k.wide = k.peak > kWide;
+  k.y_shift = k.wide ? 0.f : k.peak * kLog2e + static_cast<float>(k.power);
   k.a = scale * g.entropy * inv_temp;
   k.b = scale * g.kl;
   k.d = -scale * (g.slope + g.entropy * st.mean_z);
@@ -385,21 +403,23 @@ __device__ __forceinline__ float Phi(float u) {
 }
 
 // P (exp(-u) - 1 + u), the term of KL, for any u; pu: P u, finite also where u
-// is not; ym: the reference logit less the policy's maximum.  Far below 0, where
-// exp(-u) is large against a tiny p, their product comes from ym; an entry that
-// is masked here adds nothing but its reference probability.
-__device__ __forceinline__ float KlTerm(const Coefs &k, float p, float u, float pu, float ym) {
-  if (!(u > kFarBelow)) {
-    const float q = Exp2(ym * k.c + k.kl_shift);
-    return p == 0.f ? q : q - p + pu;
+// is not.  Far below 0, where exp(-u) is large against a tiny p, their product
+// comes from the reference; an entry that is masked here adds nothing but its
+// reference probability.  With k.wide, exp((y - y_m) / T) instead.
+__device__ __forceinline__ float KlTerm(const Coefs &k, float p, float u, float pu, float y) {
+  if (k.wide || !(u > kFarBelow)) {
+    const float q = Exp2((y - k.y_m) * k.c + k.y_shift);
+    return k.wide || p == 0.f ? q : q - p + pu;
   }
   return p == 0.f ? 0.f : u > -kFarBelow ? pu - p : p * Phi(u);
 }
 
 // KL from the sum of its terms; infinite where the reference lacks what the
 // policy plays (E_p d is, and no term then means anything).
-__device__ __forceinline__ float KlOf(float terms, const Coefs &k) {
-  return k.mean_d == __builtin_inff() ? k.mean_d : Log1p(ldexpf(terms, -k.power));
+__device__ __forceinline__ float KlOf(float terms, const Coefs &k, bool guarded) {
+  if (guarded && k.mean_d == __builtin_inff())
+    return k.mean_d;
+  return guarded && k.wide ? k.peak + Log2(terms) * kLn2 : Log1p(ldexpf(terms, -k.power));
 }
 
 // The gradient of N entries without the action's own term, and their part of
@@ -434,7 +454,7 @@ __device__ __forceinline__ void FinishEntries(const Coefs &k, bool want_kl, cons
   if (REF && want_kl) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      kl += GUARD ? KlTerm(k, p[i], u[i], pu[i], y[i] - k.m) : p[i] * Phi(u[i]);
+      kl += GUARD ? KlTerm(k, p[i], u[i], pu[i], y[i]) : p[i] * Phi(u[i]);
   }
 }
 
@@ -700,7 +720,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void DenseRowKernel(RowLossP
   Sums sums;
   const auto sum = [&](auto guard) MFH_INLINE {
     constexpr bool GUARD = decltype(guard)::value;
-    sums = Sums{};
+    sums = NoSums<GUARD>();
     m = top == -__builtin_inff() ? 0.f : top;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -754,7 +774,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void DenseRowKernel(RowLossP
       finish(std::false_type{});
     if (want_kl) {
       GroupSum<W>(kl, red);
-      kl[0] = KlOf(kl[0], k);
+      kl[0] = KlOf(kl[0], k, guarded);
     }
   }
   if (tid == 0)
@@ -786,7 +806,7 @@ __device__ __forceinline__ void StreamRow(const RowLossParams &a, std::int64_t r
 
   const float c = a.inv_temp * kLog2e;
   float m = xt[0];
-  Sums sums;
+  Sums sums = NoSums<true>();
   // Sums over the old maximum as sums over the new: e and t of each term fall
   // by the same step.
   const auto rescale = [&](float from, float to) MFH_INLINE {
@@ -846,7 +866,7 @@ __device__ __forceinline__ void StreamRow(const RowLossParams &a, std::int64_t r
                               vecs, has_rest, kThreads, tid, kl[0]);
     if (want_kl) {
       GroupSum<W>(kl, red);
-      kl[0] = KlOf(kl[0], k);
+      kl[0] = KlOf(kl[0], k, true);
     }
   }
   if (tid == 0)
@@ -959,7 +979,7 @@ __device__ __forceinline__ std::int64_t LoopRows(const RowLossParams &a, std::in
       }
     const float top = WaveMax(fmaxf(m, xt[0]));
     m = top == -__builtin_inff() ? 0.f : top;
-    Sums sums;
+    Sums sums = NoSums<GUARD>();
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       Repack(xr[j]);
@@ -998,7 +1018,7 @@ __device__ __forceinline__ std::int64_t LoopRows(const RowLossParams &a, std::in
                                  yt, vecs, has_rest, kThreads, tid, kl[0]);
       if (want_kl) {
         GroupSum<W>(kl, red);
-        kl[0] = KlOf(kl[0], k);
+        kl[0] = KlOf(kl[0], k, GUARD);
       }
       if (tid == 0)
         WriteRow(a, row, in.weight, acted, res, kl[0]);
@@ -1105,7 +1125,7 @@ __device__ __forceinline__ void MovesRow(const RowLossParams &a, std::int64_t ro
   const float top = WaveMax(m);
   m = top == -__builtin_inff() ? 0.f : top;
   const float c = a.inv_temp * kLog2e;
-  Sums sums;
+  Sums sums = NoSums<true>();
 #pragma unroll
   for (int r = 0; r < NE; ++r)
     AddStats<REF, true>(xv[r], yv[r], m, c, sums);
@@ -1124,7 +1144,7 @@ __device__ __forceinline__ void MovesRow(const RowLossParams &a, std::int64_t ro
       f[r] = ft[0];
     }
     if (want_kl)
-      kl = KlOf(WaveSum(kl), k);
+      kl = KlOf(WaveSum(kl), k, true);
   }
   if (lane == 0) {
     if (st.empty)

@@ -185,3 +185,40 @@ def test_entries_masked_in_the_reference_alone(dev, shape, dtype, temp):
     got = lg.policy(batch, ref=ref, kl_coef=0.3, entropy_coef=0.1)
     assert all(np.isfinite(v).all() for v in got.values())
     check(batch, got, ref, 0.3, 0.1)
+
+
+@pytest.mark.parametrize("dtype", lu.TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("temp", [0.7, 1.0, 3.0])
+def test_divergences_of_any_size(dev, shape, dtype, temp):
+    """Masks of the reference where p is of order 1, and references that
+    prefer by far what the policy does not."""
+    rng = np.random.default_rng(4)
+    x, ref, at, lists = _rows(rng, shape, dtype, 9)
+    x[:, at[:3]] = ref[:, at[:3]] = 0.0
+    ref[0, at[0]] = -1e4
+    ref[1, at[2]] = LOWEST[dtype]
+    ref[2, at[1]] = 200.0
+    ref[3, at[1]] = 90.0
+    ref[4, at[1]] = 50.0
+    ref[5, at[0]] = -300.0
+    ref[6, at[4]] = 130.0            # where the policy has about nothing
+    ref[7, at[:2]] = -1e4
+    x[8, at[:3]], ref[8, at[:3]] = (30.0, 0.0, -30.0), (-30.0, 1.0, 31.0)
+    batch = lg.Batch(dev, x, dtype, lists, None, temp)
+    got = lg.policy(batch, ref=ref, kl_coef=0.3, entropy_coef=0.1)
+    assert all(np.isfinite(v).all() for v in got.values())
+    check(batch, got, ref, 0.3, 0.1)
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_large_weights_leave_kl_alone(dev, shape):
+    rng = np.random.default_rng(5)
+    weight = np.array([1.0, 65536.0, 2.0 ** 39, 2.0 ** 60, -2.0 ** 90, 2.0 ** 41], np.float32)
+    for far in (130.0, 45.0, 28.0, 1e4):
+        x, ref, at, lists = _rows(rng, shape, "f32", len(weight))
+        x[:, at[:2]] = ref[:, at[:2]] = 0.0
+        ref[:, at[1]] = far
+        batch = lg.Batch(dev, x, "f32", lists, None)
+        got = lg.policy(batch, ref=ref, weight=weight, kl_coef=0.3, entropy_coef=0.1)
+        check(batch, got, ref, 0.3, 0.1, weight)
