@@ -159,6 +159,11 @@ __device__ __forceinline__ float Log1p(float z) {
   return 2.f * s * (1.f + q * (1.f / 3 + q * (1.f / 5 + q * (1.f / 7 + q * (1.f / 9 + q / 11)))));
 }
 
+// A value that is the same in the whole wave, in a scalar register.
+__device__ __forceinline__ float Scalar(float v) {
+  return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v)));
+}
+
 // Reductions over a wave on the data-parallel paths of the vector unit (six
 // dependent instructions; a shuffle through LDS is several times that), the
 // result in every lane.
@@ -234,10 +239,12 @@ __device__ __forceinline__ void GroupSum(float (&v)[N], float (*red)[8]) {
 }
 
 // Sums over a row's entries: of e, of e log2(e), of e d with d = x - y; and the
-// greatest |d|, or with the guards the greatest y.
+// greatest |d|.  With the guards, of e d kDown (several d of the lowest value
+// would add up to infinity where their mean is finite), and the greatest y.
 struct Sums {
   float e, et, ed, far;
 };
+constexpr float kDown = 0x1p-32f, kUp = 0x1p32f;
 template <bool GUARD> __device__ __forceinline__ Sums NoSums() {
   return {0.f, 0.f, 0.f, GUARD ? -__builtin_inff() : 0.f};
 }
@@ -253,7 +260,7 @@ __device__ __forceinline__ void AddStats(float x, float y, float m, float c, Sum
   s.et += GUARD && e == 0.f ? 0.f : e * t;
   if constexpr (REF) {
     const float d = x - y;
-    s.ed += GUARD && e == 0.f ? 0.f : e * d;
+    s.ed += GUARD && e == 0.f ? 0.f : e * (GUARD ? d * kDown : d);
     s.far = fmaxf(s.far, GUARD ? y : fabsf(d));
   }
 }
@@ -314,18 +321,23 @@ __device__ __forceinline__ bool NeedsGuard(const RowLossParams &a, float weight,
                   !((s.far + fabsf(s.ed * Rcp(s.e))) * a.inv_temp < -kFarBelow)));
 }
 
+// A mean of d from the sum of e d kDown: infinite only if that is.
+__device__ __forceinline__ float MeanOf(float down, float inv) {
+  const float mean = down * inv * kUp;
+  return mean == __builtin_inff() && down < mean ? 0x1.fffffep127f : mean;
+}
+
 // What a row's scalars come to, from its statistics.
 struct RowStats {
   float m;         // maximum (0 where every entry is masked)
   float log_sum;   // ln S
   float log2_sum;  // log2 S
   float mean_z;    // E_p z
-  float mean_d;    // E_p (x - y), without 1 / T
-  float far;       // as in Sums
+  float mean_d;    // E_p d, without 1 / T
   bool empty;      // no entry left
 };
 
-__device__ __forceinline__ RowStats Stats(float m, const Sums &sums) {
+__device__ __forceinline__ RowStats Stats(float m, const Sums &sums, bool guarded) {
   RowStats r;
   r.m = m;
   r.empty = sums.e == 0.f;
@@ -333,9 +345,33 @@ __device__ __forceinline__ RowStats Stats(float m, const Sums &sums) {
   r.log2_sum = Log2(sum);
   r.log_sum = r.log2_sum * kLn2;
   r.mean_z = sums.et * kLn2 * inv;
-  r.mean_d = sums.ed * inv;
-  r.far = sums.far;
+  r.mean_d = guarded ? MeanOf(sums.ed, inv) : sums.ed * inv;
   return r;
+}
+
+// What a row with the guards needs besides: y_m, the greatest reference logit,
+// and origins of x and y in d = (x - x_off) - (y - y_off).  They are 0 for a
+// reference nearby, whose small x - y is exact, and the two maxima where E_p (x -
+// y) is beyond kApart: a constant between policy and reference (3.4e38 in a row
+// whose reference is masked everywhere by the lowest value) is none of theirs,
+// and would round the logits away.
+struct Origins {
+  float y_m = 0.f, x_off = 0.f, y_off = 0.f;
+};
+constexpr float kApart = 64.f;
+__device__ __forceinline__ bool FarApart(const RowStats &st, float y_m) {
+  return fabsf(st.mean_d) > kApart && st.mean_d < __builtin_inff() &&
+         fabsf(y_m) < __builtin_inff();
+}
+// One entry's part of the sum of e d kDown from the origins m and y_m.
+__device__ __forceinline__ float ApartPart(float x, float y, float m, float y_m, float c) {
+  const float xm = x - m, e = Exp2(xm * c);
+  return e == 0.f ? 0.f : e * ((xm - (y - y_m)) * kDown);
+}
+// E_p d from there, and the origins.
+__device__ __forceinline__ Origins MoveApart(RowStats &st, const Sums &sums, float down) {
+  st.mean_d = MeanOf(down, Rcp(sums.e));
+  return {sums.far, st.m, sums.far};
 }
 
 // Coefficients of one row's gradient
@@ -350,20 +386,11 @@ struct RowGrad {
 // the terms of KL, which no weight may change, are sums of P exp(-u), and a P
 // smaller than p vanishes earlier.  Without the guards they are below 2^40
 // times exp(40) = 2^58.
-//
-// For the guards: y_m the greatest reference logit and peak the greatest of
-// ln(p_k exp(-u_k)) = (y_k - m) / T + E_p d - ln S.  KL lies between peak and
-// peak + ln(entries).  Above kWide it is taken as peak + ln sum exp((y_k - y_m)
-// / T), which has no overflow; below, its terms in P are at most 2^40 exp(30)
-// = 2^84 each.
 struct Coefs {
-  float m, c, shift, inv_temp, mean_d, mean_u, a, b, d;
-  float y_m, peak, y_shift;
-  bool wide;
+  float m, c, shift, inv_temp, mean_u, a, b, d;
   int power;
 };
 constexpr int kMostPower = 40;
-constexpr float kWide = 30.f;
 
 __device__ __forceinline__ Coefs CoefsOf(const RowStats &st, const RowGrad &g, float inv_temp) {
   Coefs k;
@@ -374,16 +401,35 @@ __device__ __forceinline__ Coefs CoefsOf(const RowStats &st, const RowGrad &g, f
   k.c = inv_temp * kLog2e;
   k.shift = static_cast<float>(k.power) - st.log2_sum;
   k.inv_temp = inv_temp;
-  k.mean_d = st.mean_d;
   k.mean_u = st.mean_d * inv_temp;
-  k.y_m = st.far;
-  k.peak = k.mean_u + (st.far - st.m) * inv_temp - st.log_sum;
-  k.wide = k.peak > kWide;
-  k.y_shift = k.wide ? 0.f : k.peak * kLog2e + static_cast<float>(k.power);
   k.a = scale * g.entropy * inv_temp;
   k.b = scale * g.kl;
   k.d = -scale * (g.slope + g.entropy * st.mean_z);
   return k;
+}
+
+// And with the guards, in scalar registers.  peak is the greatest of
+// ln(p_k exp(-u_k)) = E_p d / T + (y_k - y_off - m + x_off) / T - ln S; KL lies
+// between peak and peak + ln(entries).  Above kWide it is taken as peak +
+// ln sum exp((y_k - y_m) / T), which has no overflow; below, its terms in P are
+// at most 2^40 exp(30) = 2^84 each.
+struct FarCoefs {
+  float mean_d, x_off, y_off, y_m, y_shift, peak;
+  bool wide;
+};
+constexpr float kWide = 30.f;
+__device__ __forceinline__ FarCoefs FarCoefsOf(const RowStats &st, const Coefs &k,
+                                               const Origins &from) {
+  const float apart = (from.y_m - from.y_off) - (st.m - from.x_off);
+  FarCoefs f;
+  f.peak = Scalar(k.mean_u + apart * k.inv_temp - st.log_sum);
+  f.wide = f.peak > kWide;
+  f.y_shift = Scalar(f.wide ? 0.f : f.peak * kLog2e + static_cast<float>(k.power));
+  f.mean_d = Scalar(st.mean_d);
+  f.x_off = Scalar(from.x_off);
+  f.y_off = Scalar(from.y_off);
+  f.y_m = Scalar(from.y_m);
+  return f;
 }
 
 // exp(-u) - 1 + u for u > kFarBelow: its series for |u| < 1/4 (the first term left out
@@ -405,43 +451,51 @@ __device__ __forceinline__ float Phi(float u) {
 // P (exp(-u) - 1 + u), the term of KL, for any u; pu: P u, finite also where u
 // is not.  Far below 0, where exp(-u) is large against a tiny p, their product
 // comes from the reference; an entry that is masked here adds nothing but its
-// reference probability.  With k.wide, exp((y - y_m) / T) instead.
-__device__ __forceinline__ float KlTerm(const Coefs &k, float p, float u, float pu, float y) {
-  if (k.wide || !(u > kFarBelow)) {
-    const float q = Exp2((y - k.y_m) * k.c + k.y_shift);
-    return k.wide || p == 0.f ? q : q - p + pu;
+// reference probability.  With f.wide, exp((y - y_m) / T) instead.
+__device__ __forceinline__ float KlTerm(const Coefs &k, const FarCoefs &f, float p, float u,
+                                        float pu, float y) {
+  if (f.wide || !(u > kFarBelow)) {
+    const float q = Exp2((y - f.y_m) * k.c + f.y_shift);
+    return f.wide || p == 0.f ? q : q - p + pu;
   }
   return p == 0.f ? 0.f : u > -kFarBelow ? pu - p : p * Phi(u);
 }
 
 // KL from the sum of its terms; infinite where the reference lacks what the
 // policy plays (E_p d is, and no term then means anything).
-__device__ __forceinline__ float KlOf(float terms, const Coefs &k, bool guarded) {
-  if (guarded && k.mean_d == __builtin_inff())
-    return k.mean_d;
-  return guarded && k.wide ? k.peak + Log2(terms) * kLn2 : Log1p(ldexpf(terms, -k.power));
+template <bool GUARD>
+__device__ __forceinline__ float KlOf(float terms, const Coefs &k, const FarCoefs &f) {
+  if constexpr (GUARD) {
+    if (f.mean_d == __builtin_inff())
+      return f.mean_d;
+    if (f.wide)
+      return f.peak + Log2(terms) * kLn2;
+  }
+  return Log1p(ldexpf(terms, -k.power));
 }
 
 // The gradient of N entries without the action's own term, and their part of
 // KL.  GUARD: as for the sums, and any u.
 template <int N, bool REF, bool GUARD>
-__device__ __forceinline__ void FinishEntries(const Coefs &k, bool want_kl, const float (&x)[N],
-                                              const float (&y)[N], float &kl, float (&f)[N]) {
-  float p[N], u[N], pu[N];
+__device__ __forceinline__ void FinishEntries(const Coefs &k, const FarCoefs &far, bool want_kl,
+                                              const float (&x)[N], const float (&y)[N], float &kl,
+                                              float (&f)[N]) {
+  float p[N], u[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const float xm = x[i] - k.m;
     p[i] = Exp2(xm * k.c + k.shift);
-    float v = k.a * xm + k.d;
+    const float v = k.a * xm + k.d;
     if constexpr (REF && GUARD) {
       // p before 1 / T: u may be beyond the 32-bit range where p u is not.
-      const float apart = (x[i] - y[i]) - k.mean_d;
-      u[i] = apart * k.inv_temp;
-      pu[i] = p[i] * k.inv_temp * apart;
+      const float apart = ((x[i] - far.x_off) - (y[i] - far.y_off)) - far.mean_d;
+      const float pu = p[i] * k.inv_temp * apart;
       f[i] = p[i] * v;
       // Without a coefficient KL is only watched: it may be infinite.
       if (k.b != 0.f)
-        f[i] += k.b * pu[i];
+        f[i] += k.b * pu;
+      if (want_kl)
+        kl += KlTerm(k, far, p[i], apart * k.inv_temp, pu, y[i]);
     } else if constexpr (REF) {
       u[i] = (x[i] - y[i]) * k.inv_temp - k.mean_u;
       f[i] = p[i] * (k.b * u[i] + v);
@@ -451,10 +505,10 @@ __device__ __forceinline__ void FinishEntries(const Coefs &k, bool want_kl, cons
     if (GUARD && p[i] == 0.f)
       f[i] = 0.f;
   }
-  if (REF && want_kl) {
+  if (REF && !GUARD && want_kl) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      kl += GUARD ? KlTerm(k, p[i], u[i], pu[i], y[i]) : p[i] * Phi(u[i]);
+      kl += p[i] * Phi(u[i]);
   }
 }
 
@@ -520,6 +574,10 @@ __device__ __forceinline__ RowResult Evaluate(const RowLossParams &a, const RowI
     r.grad.slope = s.slope;
   }
   r.entropy = st.log_sum - st.mean_z;
+  // These wait for the end of the row: no vector registers for them.
+  r.logp = Scalar(r.logp);
+  r.surrogate = Scalar(r.surrogate);
+  r.entropy = Scalar(r.entropy);
   r.grad.kl = a.kl_coef;
   r.grad.entropy = a.entropy_coef;
   return r;
@@ -602,10 +660,22 @@ __device__ __forceinline__ void AddVec(u32x4 xr, u32x4 yr, float m, float c, Sum
     AddStats<REF, GUARD>(xs[i], ys[i], m, c, sums);
 }
 
+template <int DT>
+__device__ __forceinline__ void AddApart(u32x4 xr, u32x4 yr, float m, float y_m, float c,
+                                         float &sum) {
+  constexpr int VE = Elem<DT>::kPerVec;
+  float xs[VE], ys[VE];
+  Unpack<DT>(xr, xs);
+  Unpack<DT>(yr, ys);
+#pragma unroll
+  for (int i = 0; i < VE; ++i)
+    sum += ApartPart(xs[i], ys[i], m, y_m, c);
+}
+
 // Four entries at a time: eight would hold more registers.
 template <int DT, bool REF, bool GUARD>
-__device__ __forceinline__ u32x4 FinishVec(const Coefs &k, bool want_kl, u32x4 xr, u32x4 yr,
-                                           float &kl) {
+__device__ __forceinline__ u32x4 FinishVec(const Coefs &k, const FarCoefs &far, bool want_kl,
+                                           u32x4 xr, u32x4 yr, float &kl) {
   using E = Elem<DT>;
   constexpr int VE = E::kPerVec;
   float f[VE];
@@ -618,7 +688,7 @@ __device__ __forceinline__ u32x4 FinishVec(const Coefs &k, bool want_kl, u32x4 x
       if constexpr (REF)
         ys[i] = E::Get(yr, h + i);
     }
-    FinishEntries<4, REF, GUARD>(k, want_kl, xs, ys, kl, part);
+    FinishEntries<4, REF, GUARD>(k, far, want_kl, xs, ys, kl, part);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       f[h + i] = part[i];
@@ -629,15 +699,16 @@ __device__ __forceinline__ u32x4 FinishVec(const Coefs &k, bool want_kl, u32x4 x
 // The elements behind the last whole vector, and the action's own term, by the
 // thread that wrote its column.
 template <int DT, bool REF, bool GUARD>
-__device__ __forceinline__ void FinishRest(const Coefs &k, bool want_kl, bool want_grad, Row<DT> g,
-                                           const RowGrad &grad, int act, float xa, float ya,
-                                           const float (&xt)[1], const float (&yt)[1], int vecs,
-                                           bool has_rest, int threads, int tid, float &kl) {
+__device__ __forceinline__ void FinishRest(const Coefs &k, const FarCoefs &far, bool want_kl,
+                                           bool want_grad, Row<DT> g, const RowGrad &grad, int act,
+                                           float xa, float ya, const float (&xt)[1],
+                                           const float (&yt)[1], int vecs, bool has_rest,
+                                           int threads, int tid, float &kl) {
   using E = Elem<DT>;
   constexpr int VE = E::kPerVec;
   float ft[1];
   if (has_rest) {
-    FinishEntries<1, REF, GUARD>(k, want_kl, xt, yt, kl, ft);
+    FinishEntries<1, REF, GUARD>(k, far, want_kl, xt, yt, kl, ft);
     if (want_grad)
       g[vecs * VE + tid] = E::Round(ft[0]);
   }
@@ -645,7 +716,7 @@ __device__ __forceinline__ void FinishRest(const Coefs &k, bool want_kl, bool wa
   if (want_grad && act >= 0 && tid == (v < vecs ? v % threads : act - vecs * VE)) {
     float none = 0.f;
     const float xs[1] = {xa}, ys[1] = {ya};
-    FinishEntries<1, REF, GUARD>(k, false, xs, ys, none, ft);
+    FinishEntries<1, REF, GUARD>(k, far, false, xs, ys, none, ft);
     g[act] = E::Round(ft[0] + grad.scale * grad.slope);
   }
 }
@@ -738,13 +809,26 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void DenseRowKernel(RowLossP
   const bool guarded = NeedsGuard<REF>(a, in.weight, sums);
   if (guarded)
     sum(std::true_type{});
-  const RowStats st = Stats(m, sums);
+  RowStats st = Stats(m, sums, guarded);
   if (st.empty) {
     if (tid == 0)
       WriteZeros(a, row);
     if (want_grad)
       ZeroRow<DT>(g, n, tid, 64 * W);
     return;
+  }
+  Origins from{sums.far};
+  if (REF && guarded && FarApart(st, sums.far)) {
+    float part[1] = {has_rest ? ApartPart(xt[0], yt[0], m, sums.far, c) : 0.f};
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      Repack(xr[j]);
+      Repack(yr[REF ? j : 0]);
+      if (j * 64 * W + tid < vecs)
+        AddApart<DT>(xr[j], yr[REF ? j : 0], m, sums.far, c, part[0]);
+    }
+    GroupSum<W>(part, red);
+    from = MoveApart(st, sums, part[0]);
   }
   const RowResult res = Evaluate(a, in, st, acted, xa);
   const bool want_kl = REF && WantsKl(a);
@@ -753,6 +837,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void DenseRowKernel(RowLossP
     const Coefs k = CoefsOf(st, res.grad, a.inv_temp);
     const auto finish = [&](auto guard) MFH_INLINE {
       constexpr bool GUARD = decltype(guard)::value;
+      const FarCoefs far = GUARD ? FarCoefsOf(st, k, from) : FarCoefs{};
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         Repack(xr[j]);
@@ -760,22 +845,23 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void DenseRowKernel(RowLossP
           Repack(yr[REF ? j : 0]);
         const int v = j * 64 * W + tid;
         if (v < vecs) {
-          const u32x4 f = FinishVec<DT, REF, GUARD>(k, want_kl, xr[j], yr[REF ? j : 0], kl[0]);
+          const u32x4 f =
+              FinishVec<DT, REF, GUARD>(k, far, want_kl, xr[j], yr[REF ? j : 0], kl[0]);
           if (want_grad)
             StoreVec<DT, PAST>(g + v * VE, f);
         }
       }
-      FinishRest<DT, REF, GUARD>(k, want_kl, want_grad, g, res.grad, acted ? act : -1, xa, ya, xt,
-                                 yt, vecs, has_rest, 64 * W, tid, kl[0]);
+      FinishRest<DT, REF, GUARD>(k, far, want_kl, want_grad, g, res.grad, acted ? act : -1, xa, ya,
+                                 xt, yt, vecs, has_rest, 64 * W, tid, kl[0]);
+      if (want_kl) {
+        GroupSum<W>(kl, red);
+        kl[0] = KlOf<GUARD>(kl[0], k, far);
+      }
     };
     if (guarded)
       finish(std::true_type{});
     else
       finish(std::false_type{});
-    if (want_kl) {
-      GroupSum<W>(kl, red);
-      kl[0] = KlOf(kl[0], k, guarded);
-    }
   }
   if (tid == 0)
     WriteRow(a, row, in.weight, acted, res, kl[0]);
@@ -837,7 +923,7 @@ __device__ __forceinline__ void StreamRow(const RowLossParams &a, std::int64_t r
   const float top = WaveMax(m);
   rescale(m, top == -__builtin_inff() ? 0.f : top);
   m = GroupSums<W, REF, true>(sums, top, c, red);
-  const RowStats st = Stats(m, sums);
+  RowStats st = Stats(m, sums, true);
   if (st.empty) {
     if (tid == 0)
       WriteZeros(a, row);
@@ -845,11 +931,22 @@ __device__ __forceinline__ void StreamRow(const RowLossParams &a, std::int64_t r
       ZeroRow<DT>(g, n, tid, kThreads);
     return;
   }
+  Origins from{sums.far};
+  if (REF && FarApart(st, sums.far)) {
+    float part[1] = {has_rest ? ApartPart(xt[0], yt[0], m, sums.far, c) : 0.f};
+    for (int v = tid; v < vecs; v += kThreads)
+      AddApart<DT>(LoadVec<DT, false>(x + static_cast<std::int64_t>(v) * VE),
+                   LoadVec<DT, false>(y + static_cast<std::int64_t>(v) * VE), m, sums.far, c,
+                   part[0]);
+    GroupSum<W>(part, red);
+    from = MoveApart(st, sums, part[0]);
+  }
   const RowResult res = Evaluate(a, in, st, acted, xa);
   const bool want_kl = REF && WantsKl(a);
   float kl[1] = {0.f};
   if (want_grad || want_kl) {
     const Coefs k = CoefsOf(st, res.grad, a.inv_temp);
+    const FarCoefs far = FarCoefsOf(st, k, from);
     for (int j = (vecs - 1) / kThreads; j >= 0; --j) {
       const std::int64_t v = static_cast<std::int64_t>(j) * kThreads + tid;
       if (v >= vecs)
@@ -858,15 +955,15 @@ __device__ __forceinline__ void StreamRow(const RowLossParams &a, std::int64_t r
       u32x4 yr = {};
       if constexpr (REF)
         yr = LoadVec<DT, false>(y + v * VE);
-      const u32x4 f = FinishVec<DT, REF, true>(k, want_kl, xr, yr, kl[0]);
+      const u32x4 f = FinishVec<DT, REF, true>(k, far, want_kl, xr, yr, kl[0]);
       if (want_grad)
         StoreVec<DT, true>(g + v * VE, f);
     }
-    FinishRest<DT, REF, true>(k, want_kl, want_grad, g, res.grad, acted ? act : -1, xa, ya, xt, yt,
-                              vecs, has_rest, kThreads, tid, kl[0]);
+    FinishRest<DT, REF, true>(k, far, want_kl, want_grad, g, res.grad, acted ? act : -1, xa, ya,
+                              xt, yt, vecs, has_rest, kThreads, tid, kl[0]);
     if (want_kl) {
       GroupSum<W>(kl, red);
-      kl[0] = KlOf(kl[0], k, true);
+      kl[0] = KlOf<true>(kl[0], k, far);
     }
   }
   if (tid == 0)
@@ -994,9 +1091,25 @@ __device__ __forceinline__ std::int64_t LoopRows(const RowLossParams &a, std::in
     // A row without an entry left needs them too (its sums hold 0 times -inf).
     if (!GUARD && live && NeedsGuard<REF>(a, in.weight, sums))
       return row;
-    const RowStats st = Stats(m, sums);
+    RowStats st = Stats(m, sums, GUARD);
+    Origins from{sums.far};
+    if constexpr (REF && GUARD) {
+      if (FarApart(st, sums.far)) {
+        float part[1] = {has_rest ? ApartPart(xt[0], yt[0], m, sums.far, c) : 0.f};
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          Repack(xr[j]);
+          Repack(yr[j]);
+          if (filled(j))
+            AddApart<DT>(xr[j], yr[j], m, sums.far, c, part[0]);
+        }
+        GroupSum<W>(part, red);
+        from = MoveApart(st, sums, part[0]);
+      }
+    }
     const RowResult res = Evaluate(a, in, st, acted && !st.empty, xa);
     const Coefs k = CoefsOf(st, res.grad, a.inv_temp);
+    const FarCoefs far = GUARD ? FarCoefsOf(st, k, from) : FarCoefs{};
     float kl[1] = {0.f};
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -1004,7 +1117,8 @@ __device__ __forceinline__ std::int64_t LoopRows(const RowLossParams &a, std::in
       if (REF)
         Repack(yr[REF ? j : 0]);
       if (filled(j) && (want_grad || want_kl)) {
-        const u32x4 f = FinishVec<DT, REF, GUARD>(k, want_kl, xr[j], yr[REF ? j : 0], kl[0]);
+        const u32x4 f =
+            FinishVec<DT, REF, GUARD>(k, far, want_kl, xr[j], yr[REF ? j : 0], kl[0]);
         if (want_grad && live)
           StoreVec<DT, true>(g + j * kThreads * VE + place(j), f);
       }
@@ -1014,11 +1128,11 @@ __device__ __forceinline__ std::int64_t LoopRows(const RowLossParams &a, std::in
       __builtin_amdgcn_sched_barrier(0);
     }
     if (live && !st.empty) {
-      FinishRest<DT, REF, GUARD>(k, want_kl, want_grad, g, res.grad, acted ? act : -1, xa, ya, xt,
-                                 yt, vecs, has_rest, kThreads, tid, kl[0]);
+      FinishRest<DT, REF, GUARD>(k, far, want_kl, want_grad, g, res.grad, acted ? act : -1, xa, ya,
+                                 xt, yt, vecs, has_rest, kThreads, tid, kl[0]);
       if (want_kl) {
         GroupSum<W>(kl, red);
-        kl[0] = KlOf(kl[0], k, GUARD);
+        kl[0] = KlOf<GUARD>(kl[0], k, far);
       }
       if (tid == 0)
         WriteRow(a, row, in.weight, acted, res, kl[0]);
@@ -1130,21 +1244,30 @@ __device__ __forceinline__ void MovesRow(const RowLossParams &a, std::int64_t ro
   for (int r = 0; r < NE; ++r)
     AddStats<REF, true>(xv[r], yv[r], m, c, sums);
   (void)GroupSums<1, REF, true>(sums, top, c, nullptr);
-  const RowStats st = Stats(m, sums);
+  RowStats st = Stats(m, sums, true);
+  Origins from{sums.far};
+  if (REF && FarApart(st, sums.far)) {
+    float part = 0.f;
+#pragma unroll
+    for (int r = 0; r < NE; ++r)
+      part += ApartPart(xv[r], yv[r], m, sums.far, c);
+    from = MoveApart(st, sums, WaveSum(part));
+  }
   const RowResult res = Evaluate(a, in, st, acted, xa);
   const bool want_kl = REF && WantsKl(a);
   float kl = 0.f, f[NE] = {};
   if (!st.empty && (want_grad || want_kl)) {
     const Coefs k = CoefsOf(st, res.grad, a.inv_temp);
+    const FarCoefs far = FarCoefsOf(st, k, from);
 #pragma unroll
     for (int r = 0; r < NE; ++r) {
       const float xs[1] = {xv[r]}, ys[1] = {yv[r]};
       float ft[1];
-      FinishEntries<1, REF, true>(k, want_kl, xs, ys, kl, ft);
+      FinishEntries<1, REF, true>(k, far, want_kl, xs, ys, kl, ft);
       f[r] = ft[0];
     }
     if (want_kl)
-      kl = KlOf(WaveSum(kl), k, true);
+      kl = KlOf<true>(WaveSum(kl), k, far);
   }
   if (lane == 0) {
     if (st.empty)

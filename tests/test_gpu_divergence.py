@@ -222,3 +222,42 @@ def test_large_weights_leave_kl_alone(dev, shape):
         batch = lg.Batch(dev, x, "f32", lists, None)
         got = lg.policy(batch, ref=ref, weight=weight, kl_coef=0.3, entropy_coef=0.1)
         check(batch, got, ref, 0.3, 0.1, weight)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_several_entries_of_the_lowest_value(dev, shape, dtype):
+    """Their differences add up beyond the 32-bit range; KL, two thirds of one
+    of them, does not."""
+    rng = np.random.default_rng(6)
+    x, ref, at, lists = _rows(rng, shape, dtype, 2)
+    x[:, at[:3]] = ref[:, at[:3]] = 0.0
+    ref[0, at[:2]] = LOWEST[dtype]
+    x[1, at] = ref[1, at] = 0.0
+    ref[1, at[:4]] = LOWEST[dtype]
+    batch = lg.Batch(dev, x, dtype, lists, None)
+    got = lg.policy(batch, ref=ref, kl_coef=0.3, entropy_coef=0.1)
+    assert all(np.isfinite(v).all() for v in got.values())
+    check(batch, got, ref, 0.3, 0.1)
+
+
+@pytest.mark.parametrize("dtype", lu.TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("temp", [0.7, 1.0])
+def test_references_a_constant_away(dev, shape, dtype, temp):
+    """Softmax does not see a constant: a reference of lowest values alone is
+    uniform, one 3e4 lower or higher the same policy as without."""
+    rng = np.random.default_rng(7)
+    x, ref, at, lists = _rows(rng, shape, dtype, 4)
+    x[:] = rng.normal(size=x.shape)
+    ref[:] = x + 0.5 * rng.normal(size=x.shape)
+    ref[0] = LOWEST[dtype]
+    ref[1] -= 3e4
+    ref[2] += 3e4
+    ref[3], x[3] = ref[3] + 100.0, x[3] - 100.0
+    batch = lg.Batch(dev, x, dtype, lists, None, temp)
+    got = lg.policy(batch, ref=ref, kl_coef=0.3, entropy_coef=0.1)
+    check(batch, got, ref, 0.3, 0.1)
+    n = batch.vocab if lists is None else len(lists[0])
+    uniform = np.log(n) - got["entropy"][0]
+    assert abs(got["kl"][0] - uniform) < 1e-4 * np.log(n)
