@@ -239,12 +239,10 @@ __device__ __forceinline__ void GroupSum(float (&v)[N], float (*red)[8]) {
 }
 
 // Sums over a row's entries: of e, of e log2(e), of e d with d = x - y; and the
-// greatest |d|.  With the guards, of e d kDown (several d of the lowest value
-// would add up to infinity where their mean is finite), and the greatest y.
+// greatest |d|, or with the guards the greatest y.
 struct Sums {
   float e, et, ed, far;
 };
-constexpr float kDown = 0x1p-32f, kUp = 0x1p32f;
 template <bool GUARD> __device__ __forceinline__ Sums NoSums() {
   return {0.f, 0.f, 0.f, GUARD ? -__builtin_inff() : 0.f};
 }
@@ -260,7 +258,7 @@ __device__ __forceinline__ void AddStats(float x, float y, float m, float c, Sum
   s.et += GUARD && e == 0.f ? 0.f : e * t;
   if constexpr (REF) {
     const float d = x - y;
-    s.ed += GUARD && e == 0.f ? 0.f : e * (GUARD ? d * kDown : d);
+    s.ed += GUARD && e == 0.f ? 0.f : e * d;
     s.far = fmaxf(s.far, GUARD ? y : fabsf(d));
   }
 }
@@ -321,12 +319,6 @@ __device__ __forceinline__ bool NeedsGuard(const RowLossParams &a, float weight,
                   !((s.far + fabsf(s.ed * Rcp(s.e))) * a.inv_temp < -kFarBelow)));
 }
 
-// A mean of d from the sum of e d kDown: infinite only if that is.
-__device__ __forceinline__ float MeanOf(float down, float inv) {
-  const float mean = down * inv * kUp;
-  return mean == __builtin_inff() && down < mean ? 0x1.fffffep127f : mean;
-}
-
 // What a row's scalars come to, from its statistics.
 struct RowStats {
   float m;         // maximum (0 where every entry is masked)
@@ -337,7 +329,7 @@ struct RowStats {
   bool empty;      // no entry left
 };
 
-__device__ __forceinline__ RowStats Stats(float m, const Sums &sums, bool guarded) {
+__device__ __forceinline__ RowStats Stats(float m, const Sums &sums) {
   RowStats r;
   r.m = m;
   r.empty = sums.e == 0.f;
@@ -345,33 +337,29 @@ __device__ __forceinline__ RowStats Stats(float m, const Sums &sums, bool guarde
   r.log2_sum = Log2(sum);
   r.log_sum = r.log2_sum * kLn2;
   r.mean_z = sums.et * kLn2 * inv;
-  r.mean_d = guarded ? MeanOf(sums.ed, inv) : sums.ed * inv;
+  r.mean_d = sums.ed * inv;
   return r;
 }
 
-// What a row with the guards needs besides: y_m, the greatest reference logit,
-// and origins of x and y in d = (x - x_off) - (y - y_off).  They are 0 for a
-// reference nearby, whose small x - y is exact, and the two maxima where E_p (x -
-// y) is beyond kApart: a constant between policy and reference (3.4e38 in a row
-// whose reference is masked everywhere by the lowest value) is none of theirs,
-// and would round the logits away.
-struct Origins {
-  float y_m = 0.f, x_off = 0.f, y_off = 0.f;
-};
-constexpr float kApart = 64.f;
+// A row with the guards whose E_p d is beyond kApart takes d from the two maxima,
+// as (x - m) - (y - y_m): a constant between policy and reference (3.4e38 in a
+// row whose reference is masked everywhere by the lowest value) would round the
+// logits away.  Nearer, x - y is exact where it is small.  Sums of e d there are
+// of e d kDown: several d of the lowest value would add up to infinity where
+// their mean is finite.
+constexpr float kApart = 64.f, kDown = 0x1p-32f, kUp = 0x1p32f;
 __device__ __forceinline__ bool FarApart(const RowStats &st, float y_m) {
-  return fabsf(st.mean_d) > kApart && st.mean_d < __builtin_inff() &&
-         fabsf(y_m) < __builtin_inff();
+  return !(fabsf(st.mean_d) <= kApart) && fabsf(y_m) < __builtin_inff();
 }
-// One entry's part of the sum of e d kDown from the origins m and y_m.
+// One entry's part of that sum.
 __device__ __forceinline__ float ApartPart(float x, float y, float m, float y_m, float c) {
   const float xm = x - m, e = Exp2(xm * c);
   return e == 0.f ? 0.f : e * ((xm - (y - y_m)) * kDown);
 }
-// E_p d from there, and the origins.
-__device__ __forceinline__ Origins MoveApart(RowStats &st, const Sums &sums, float down) {
-  st.mean_d = MeanOf(down, Rcp(sums.e));
-  return {sums.far, st.m, sums.far};
+// E_p d from it: infinite only if the sum is.
+__device__ __forceinline__ float ApartMean(float down, float e) {
+  const float mean = down * Rcp(e) * kUp;
+  return mean == __builtin_inff() && down < mean ? 0x1.fffffep127f : mean;
 }
 
 // Coefficients of one row's gradient
@@ -408,32 +396,33 @@ __device__ __forceinline__ Coefs CoefsOf(const RowStats &st, const RowGrad &g, f
   return k;
 }
 
-// And with the guards, in scalar registers.  peak is the greatest of
-// ln(p_k exp(-u_k)) = E_p d / T + (y_k - y_off - m + x_off) / T - ln S; KL lies
-// between peak and peak + ln(entries).  Above kWide it is taken as peak +
-// ln sum exp((y_k - y_m) / T), which has no overflow; below, its terms in P are
-// at most 2^40 exp(30) = 2^84 each.
+// And with the guards, in scalar registers: y_m the greatest reference logit,
+// peak the greatest of ln(p_k exp(-u_k)) = (y_k - m) / T + E_p (x - y) / T - ln S.
+// KL lies between peak and peak + ln(entries).  Above kWide it is taken as
+// peak + ln sum exp((y_k - y_m) / T), which has no overflow; below, its terms
+// in P are at most 2^40 exp(30) = 2^84 each.
 struct FarCoefs {
-  float mean_d, x_off, y_off, y_m, y_shift, peak;
-  bool wide;
+  float mean_d, y_m, y_shift, peak;
+  float above;           // u of more is infinite, or may be where p u is not (1 / T > 1)
+  bool apart, wide, kl;  // d from the maxima; peak above kWide; KL in the gradient
 };
 constexpr float kWide = 30.f;
-__device__ __forceinline__ FarCoefs FarCoefsOf(const RowStats &st, const Coefs &k,
-                                               const Origins &from) {
-  const float apart = (from.y_m - from.y_off) - (st.m - from.x_off);
+__device__ __forceinline__ FarCoefs FarCoefsOf(const RowStats &st, const Coefs &k, float y_m,
+                                               bool apart) {
   FarCoefs f;
-  f.peak = Scalar(k.mean_u + apart * k.inv_temp - st.log_sum);
-  f.wide = f.peak > kWide;
+  f.peak = Scalar(k.mean_u + (apart ? 0.f : (y_m - st.m) * k.inv_temp) - st.log_sum);
+  f.above = k.inv_temp > 1.f ? -kFarBelow : 0x1.fffffep127f;
+  f.apart = __builtin_amdgcn_readfirstlane(apart);
+  f.wide = __builtin_amdgcn_readfirstlane(f.peak > kWide);
+  f.kl = __builtin_amdgcn_readfirstlane(k.b != 0.f);
   f.y_shift = Scalar(f.wide ? 0.f : f.peak * kLog2e + static_cast<float>(k.power));
   f.mean_d = Scalar(st.mean_d);
-  f.x_off = Scalar(from.x_off);
-  f.y_off = Scalar(from.y_off);
-  f.y_m = Scalar(from.y_m);
+  f.y_m = Scalar(y_m);
   return f;
 }
 
-// exp(-u) - 1 + u for u > kFarBelow: its series for |u| < 1/4 (the first term left out
-// is 1.2e-8 of the sum), where the difference would cancel.
+// exp(-u) - 1 + u for u > kFarBelow: its series for |u| < 1/4 (the first term
+// left out is 1.2e-8 of the sum), where the difference would cancel.
 __device__ __forceinline__ float Phi(float u) {
   const float e = Exp2(-u * kLog2e);
   float r = -1.f / 5040;
@@ -448,17 +437,22 @@ __device__ __forceinline__ float Phi(float u) {
   return fabsf(u) < 0.25f ? near : far;
 }
 
-// P (exp(-u) - 1 + u), the term of KL, for any u; pu: P u, finite also where u
-// is not.  Far below 0, where exp(-u) is large against a tiny p, their product
-// comes from the reference; an entry that is masked here adds nothing but its
-// reference probability.  With f.wide, exp((y - y_m) / T) instead.
-__device__ __forceinline__ float KlTerm(const Coefs &k, const FarCoefs &f, float p, float u,
-                                        float pu, float y) {
-  if (f.wide || !(u > kFarBelow)) {
-    const float q = Exp2((y - f.y_m) * k.c + f.y_shift);
-    return f.wide || p == 0.f ? q : q - p + pu;
-  }
-  return p == 0.f ? 0.f : u > -kFarBelow ? pu - p : p * Phi(u);
+// P u from P and d less its mean, finite also where u is not.
+__device__ __forceinline__ float TimesU(const Coefs &k, float p, float apart) {
+  return p * k.inv_temp * apart;
+}
+
+// P (exp(-u) - 1 + u), the term of KL, for any u.  Far below 0, where exp(-u) is
+// large against a tiny p, their product comes from the reference; an entry that
+// is masked here adds nothing but its reference probability.  With f.wide,
+// exp((y - y_m) / T) instead.
+__device__ __forceinline__ float KlTerm(const Coefs &k, const FarCoefs &f, float p, float apart,
+                                        float y) {
+  const float u = apart * k.inv_temp;
+  if (!f.wide && u > kFarBelow && u <= f.above)
+    return p * Phi(u);
+  const float q = u > 0.f && !f.wide ? 0.f : Exp2((y - f.y_m) * k.c + f.y_shift);
+  return f.wide || p == 0.f ? q : q - p + TimesU(k, p, apart);
 }
 
 // KL from the sum of its terms; infinite where the reference lacks what the
@@ -485,25 +479,52 @@ __device__ __forceinline__ void FinishEntries(const Coefs &k, const FarCoefs &fa
   for (int i = 0; i < N; ++i) {
     const float xm = x[i] - k.m;
     p[i] = Exp2(xm * k.c + k.shift);
-    const float v = k.a * xm + k.d;
-    if constexpr (REF && GUARD) {
-      // p before 1 / T: u may be beyond the 32-bit range where p u is not.
-      const float apart = ((x[i] - far.x_off) - (y[i] - far.y_off)) - far.mean_d;
-      const float pu = p[i] * k.inv_temp * apart;
-      f[i] = p[i] * v;
-      // Without a coefficient KL is only watched: it may be infinite.
-      if (k.b != 0.f)
-        f[i] += k.b * pu;
-      if (want_kl)
-        kl += KlTerm(k, far, p[i], apart * k.inv_temp, pu, y[i]);
-    } else if constexpr (REF) {
+    float v = k.a * xm + k.d;
+    if constexpr (REF && !GUARD) {
       u[i] = (x[i] - y[i]) * k.inv_temp - k.mean_u;
-      f[i] = p[i] * (k.b * u[i] + v);
-    } else {
-      f[i] = p[i] * v;
+      v = k.b * u[i] + v;
     }
-    if (GUARD && p[i] == 0.f)
-      f[i] = 0.f;
+    f[i] = p[i] * v;
+  }
+  if constexpr (REF && GUARD) {
+    float apart[N];
+    if (far.apart) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        apart[i] = ((x[i] - k.m) - (y[i] - far.y_m)) - far.mean_d;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        apart[i] = (x[i] - y[i]) - far.mean_d;
+    }
+    // Without a coefficient KL is only watched: it may be infinite.
+    if (far.kl) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        f[i] += k.b * TimesU(k, p[i], apart[i]);
+    }
+    if (want_kl) {
+      bool usual = !far.wide;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        u[i] = apart[i] * k.inv_temp;
+        usual = usual && u[i] > kFarBelow && u[i] <= far.above;
+      }
+      if (__all(usual)) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          kl += p[i] * Phi(u[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          kl += KlTerm(k, far, p[i], apart[i], y[i]);
+      }
+    }
+  }
+  if constexpr (GUARD) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      f[i] = p[i] == 0.f ? 0.f : f[i];
   }
   if (REF && !GUARD && want_kl) {
 #pragma unroll
@@ -574,13 +595,20 @@ __device__ __forceinline__ RowResult Evaluate(const RowLossParams &a, const RowI
     r.grad.slope = s.slope;
   }
   r.entropy = st.log_sum - st.mean_z;
-  // These wait for the end of the row: no vector registers for them.
-  r.logp = Scalar(r.logp);
-  r.surrogate = Scalar(r.surrogate);
-  r.entropy = Scalar(r.entropy);
   r.grad.kl = a.kl_coef;
   r.grad.entropy = a.entropy_coef;
   return r;
+}
+
+// What waits for the end of the row, out of the vector registers: with a
+// reference three more decide the waves a SIMD holds (the shortest rows of bf16
+// take 61 registers for eight waves, 65 with these).
+template <bool REF> __device__ __forceinline__ void Park(RowResult &r) {
+  if constexpr (REF) {
+    r.logp = Scalar(r.logp);
+    r.surrogate = Scalar(r.surrogate);
+    r.entropy = Scalar(r.entropy);
+  }
 }
 
 __device__ __forceinline__ void WriteRow(const RowLossParams &a, std::int64_t row, float w,
@@ -809,7 +837,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void DenseRowKernel(RowLossP
   const bool guarded = NeedsGuard<REF>(a, in.weight, sums);
   if (guarded)
     sum(std::true_type{});
-  RowStats st = Stats(m, sums, guarded);
+  RowStats st = Stats(m, sums);
   if (st.empty) {
     if (tid == 0)
       WriteZeros(a, row);
@@ -817,8 +845,8 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void DenseRowKernel(RowLossP
       ZeroRow<DT>(g, n, tid, 64 * W);
     return;
   }
-  Origins from{sums.far};
-  if (REF && guarded && FarApart(st, sums.far)) {
+  const bool apart = REF && guarded && FarApart(st, sums.far);
+  if (apart) {
     float part[1] = {has_rest ? ApartPart(xt[0], yt[0], m, sums.far, c) : 0.f};
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -828,16 +856,17 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void DenseRowKernel(RowLossP
         AddApart<DT>(xr[j], yr[REF ? j : 0], m, sums.far, c, part[0]);
     }
     GroupSum<W>(part, red);
-    from = MoveApart(st, sums, part[0]);
+    st.mean_d = ApartMean(part[0], sums.e);
   }
-  const RowResult res = Evaluate(a, in, st, acted, xa);
+  RowResult res = Evaluate(a, in, st, acted, xa);
+  Park<REF>(res);
   const bool want_kl = REF && WantsKl(a);
   float kl[1] = {0.f};
   if (want_grad || want_kl) {
     const Coefs k = CoefsOf(st, res.grad, a.inv_temp);
     const auto finish = [&](auto guard) MFH_INLINE {
       constexpr bool GUARD = decltype(guard)::value;
-      const FarCoefs far = GUARD ? FarCoefsOf(st, k, from) : FarCoefs{};
+      const FarCoefs far = GUARD ? FarCoefsOf(st, k, sums.far, apart) : FarCoefs{};
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         Repack(xr[j]);
@@ -923,7 +952,7 @@ __device__ __forceinline__ void StreamRow(const RowLossParams &a, std::int64_t r
   const float top = WaveMax(m);
   rescale(m, top == -__builtin_inff() ? 0.f : top);
   m = GroupSums<W, REF, true>(sums, top, c, red);
-  RowStats st = Stats(m, sums, true);
+  RowStats st = Stats(m, sums);
   if (st.empty) {
     if (tid == 0)
       WriteZeros(a, row);
@@ -931,22 +960,22 @@ __device__ __forceinline__ void StreamRow(const RowLossParams &a, std::int64_t r
       ZeroRow<DT>(g, n, tid, kThreads);
     return;
   }
-  Origins from{sums.far};
-  if (REF && FarApart(st, sums.far)) {
+  const bool apart = REF && FarApart(st, sums.far);
+  if (apart) {
     float part[1] = {has_rest ? ApartPart(xt[0], yt[0], m, sums.far, c) : 0.f};
     for (int v = tid; v < vecs; v += kThreads)
       AddApart<DT>(LoadVec<DT, false>(x + static_cast<std::int64_t>(v) * VE),
                    LoadVec<DT, false>(y + static_cast<std::int64_t>(v) * VE), m, sums.far, c,
                    part[0]);
     GroupSum<W>(part, red);
-    from = MoveApart(st, sums, part[0]);
+    st.mean_d = ApartMean(part[0], sums.e);
   }
   const RowResult res = Evaluate(a, in, st, acted, xa);
   const bool want_kl = REF && WantsKl(a);
   float kl[1] = {0.f};
   if (want_grad || want_kl) {
     const Coefs k = CoefsOf(st, res.grad, a.inv_temp);
-    const FarCoefs far = FarCoefsOf(st, k, from);
+    const FarCoefs far = FarCoefsOf(st, k, sums.far, apart);
     for (int j = (vecs - 1) / kThreads; j >= 0; --j) {
       const std::int64_t v = static_cast<std::int64_t>(j) * kThreads + tid;
       if (v >= vecs)
@@ -1091,10 +1120,10 @@ __device__ __forceinline__ std::int64_t LoopRows(const RowLossParams &a, std::in
     // A row without an entry left needs them too (its sums hold 0 times -inf).
     if (!GUARD && live && NeedsGuard<REF>(a, in.weight, sums))
       return row;
-    RowStats st = Stats(m, sums, GUARD);
-    Origins from{sums.far};
+    RowStats st = Stats(m, sums);
+    const bool apart = REF && GUARD && FarApart(st, sums.far);
     if constexpr (REF && GUARD) {
-      if (FarApart(st, sums.far)) {
+      if (apart) {
         float part[1] = {has_rest ? ApartPart(xt[0], yt[0], m, sums.far, c) : 0.f};
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
@@ -1104,12 +1133,13 @@ __device__ __forceinline__ std::int64_t LoopRows(const RowLossParams &a, std::in
             AddApart<DT>(xr[j], yr[j], m, sums.far, c, part[0]);
         }
         GroupSum<W>(part, red);
-        from = MoveApart(st, sums, part[0]);
+        st.mean_d = ApartMean(part[0], sums.e);
       }
     }
-    const RowResult res = Evaluate(a, in, st, acted && !st.empty, xa);
+    RowResult res = Evaluate(a, in, st, acted && !st.empty, xa);
+    Park<REF>(res);
     const Coefs k = CoefsOf(st, res.grad, a.inv_temp);
-    const FarCoefs far = GUARD ? FarCoefsOf(st, k, from) : FarCoefs{};
+    const FarCoefs far = GUARD ? FarCoefsOf(st, k, sums.far, apart) : FarCoefs{};
     float kl[1] = {0.f};
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -1244,21 +1274,21 @@ __device__ __forceinline__ void MovesRow(const RowLossParams &a, std::int64_t ro
   for (int r = 0; r < NE; ++r)
     AddStats<REF, true>(xv[r], yv[r], m, c, sums);
   (void)GroupSums<1, REF, true>(sums, top, c, nullptr);
-  RowStats st = Stats(m, sums, true);
-  Origins from{sums.far};
-  if (REF && FarApart(st, sums.far)) {
+  RowStats st = Stats(m, sums);
+  const bool apart = REF && FarApart(st, sums.far);
+  if (apart) {
     float part = 0.f;
 #pragma unroll
     for (int r = 0; r < NE; ++r)
       part += ApartPart(xv[r], yv[r], m, sums.far, c);
-    from = MoveApart(st, sums, WaveSum(part));
+    st.mean_d = ApartMean(WaveSum(part), sums.e);
   }
   const RowResult res = Evaluate(a, in, st, acted, xa);
   const bool want_kl = REF && WantsKl(a);
   float kl = 0.f, f[NE] = {};
   if (!st.empty && (want_grad || want_kl)) {
     const Coefs k = CoefsOf(st, res.grad, a.inv_temp);
-    const FarCoefs far = FarCoefsOf(st, k, from);
+    const FarCoefs far = FarCoefsOf(st, k, sums.far, apart);
 #pragma unroll
     for (int r = 0; r < NE; ++r) {
       const float xs[1] = {xv[r]}, ys[1] = {yv[r]};
