@@ -323,7 +323,7 @@ enum { MFH_DTYPE_F32 = 0, MFH_DTYPE_BF16 = 1, MFH_DTYPE_F16 = 2 };
  * listed twice counts twice), or all columns when d_move_offsets is NULL.  A
  * logit of -inf takes its entry out; a row with no entry left gives zeros
  * everywhere.  The row's action is the move played (or the token written):
- * a column among its entries, anything else (-1) for none. */
+ * a column among its entries, anything else (-1, a masked one) for none. */
 typedef struct {
   const void *d_logits;
   int64_t stride; /* elements from one row to the next, >= vocab */

@@ -781,9 +781,10 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void DenseRowKernel(RowLossP
     return;
   }
   const int act = in.action;
-  const bool acted = act >= 0 && act < n;
-  const float xa = acted ? E::One(x[act]) : 0.f;
-  const float ya = REF && acted ? E::One(y[act]) : 0.f;
+  const bool listed = act >= 0 && act < n;
+  const float xa = listed ? E::One(x[act]) : 0.f;
+  const float ya = REF && listed ? E::One(y[act]) : 0.f;
+  const bool acted = listed && xa != -__builtin_inff();
   u32x4 xr[NV], yr[REF ? NV : 1];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
@@ -912,9 +913,10 @@ __device__ __forceinline__ void StreamRow(const RowLossParams &a, std::int64_t r
   const Row<DT> g = RowOf<DT>(a.g, row, a.ldg);
   const bool want_grad = a.g != nullptr;
   const int act = in.action;
-  const bool acted = act >= 0 && act < n;
-  const float xa = acted ? E::One(x[act]) : 0.f;
-  const float ya = REF && acted ? E::One(y[act]) : 0.f;
+  const bool listed = act >= 0 && act < n;
+  const float xa = listed ? E::One(x[act]) : 0.f;
+  const float ya = REF && listed ? E::One(y[act]) : 0.f;
+  const bool acted = listed && xa != -__builtin_inff();
   const bool has_rest = tid < rest;
   const float xt[1] = {has_rest ? E::One(x[vecs * VE + tid]) : -__builtin_inff()};
   const float yt[1] = {REF && has_rest ? E::One(y[vecs * VE + tid]) : 0.f};
@@ -1088,9 +1090,9 @@ __device__ __forceinline__ std::int64_t LoopRows(const RowLossParams &a, std::in
     const Row<DT> g = RowOf<DT>(a.g, row, a.ldg);
     const RowInputs in = Inputs(a, row);
     const int act = in.action;
-    const bool acted = act >= 0 && act < n;
     const Few next_few = load_few(next_row, Inputs(a, next_row).action);
     const float xa = E::One(few.xa), ya = REF ? E::One(few.ya) : 0.f;
+    const bool acted = act >= 0 && act < n && xa != -__builtin_inff();
     const float xt[1] = {has_rest ? E::One(few.xt) : -__builtin_inff()};
     const float yt[1] = {REF && has_rest ? E::One(few.yt) : 0.f};
     float m = -__builtin_inff();
@@ -1254,13 +1256,14 @@ __device__ __forceinline__ void MovesRow(const RowLossParams &a, std::int64_t ro
   const float(&yv)[NE] = entries.y;
   if (want_grad)
     clear(n < part_cols ? n : part_cols);
-  // The entry of the action (the first of equal ones).
+  // The entry of the action (the first of equal ones), if no mask took it out.
   bool acted = false;
   float xa = 0.f, m = xv[0];
 #pragma unroll
   for (int r = 0; r < NE; ++r) {
     m = fmaxf(m, xv[r]);
-    const unsigned long long hit = __ballot(act >= 0 && col[r] == act);
+    const unsigned long long hit =
+        __ballot(act >= 0 && col[r] == act && xv[r] != -__builtin_inff());
     if (hit && !acted) {
       acted = true;
       xa = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(xv[r]), __ffsll(hit) - 1));
@@ -1345,7 +1348,7 @@ __device__ __forceinline__ void MovesRow(const RowLossParams &a, std::int64_t ro
         }
         if (writes)
           buf[col[r] - p0] =
-              E::Round(col[r] == act ? value + res.grad.scale * res.grad.slope : value);
+              E::Round(acted && col[r] == act ? value + res.grad.scale * res.grad.slope : value);
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");

@@ -41,8 +41,9 @@ class Row:
         self.v, self.temp = v, temp
         self.lp = log_softmax(v / temp)
         self.empty = self.lp is None
+        # An action that is masked is none of the row's entries.
         self.acted = (not self.empty and action is not None and 0 <= action < x.size
-                      and bool(np.any(self.k == action)))
+                      and bool(np.any((self.k == action) & (v != -np.inf))))
         self.logp = 0.0
         self.delta = np.zeros(self.k.size)
         if self.acted:
