@@ -1544,10 +1544,10 @@ __device__ __forceinline__ PairResult PairLoss(const PairLossParams &a, std::int
   double loss, slope;  // slope: by the difference of the two sums
   if (a.kind == 0) {
     // ln(1 + e^-h) and ln(1 + e^h) = ln(1 + e^-|h|) + max(0, -+h); sig(h)
-    // from the same exponential.
+    // from the same exponential.  Without smoothing h may be +inf.
     const double eps = a.smoothing, tail = exp(-fabs(h)), base = log1p(tail);
     const double small = tail / (1.0 + tail), sig = h >= 0.0 ? 1.0 - small : small;
-    loss = base + (1.0 - eps) * fmax(-h, 0.0) + eps * fmax(h, 0.0);
+    loss = base + (1.0 - eps) * fmax(-h, 0.0) + (eps > 0.0 ? eps * fmax(h, 0.0) : 0.0);
     if (h != h)
       loss = h;
     slope = beta * (eps * sig - (1.0 - eps) * (h >= 0.0 ? small : 1.0 - small));

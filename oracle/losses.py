@@ -150,7 +150,7 @@ def preference_loss(logits, moves, actions, seq_offsets, *, temp=1.0, kind="sigm
         h = beta * diff
         if kind == "sigmoid":
             e = label_smoothing
-            loss = (1 - e) * np.logaddexp(0.0, -h) + e * np.logaddexp(0.0, h)
+            loss = (1 - e) * np.logaddexp(0.0, -h) + (e * np.logaddexp(0.0, h) if e else 0.0)
             sig = np.exp(-np.logaddexp(0.0, -h))
             slope = beta * (e * sig - (1 - e) * np.exp(-np.logaddexp(0.0, h)))
         elif kind == "hinge":

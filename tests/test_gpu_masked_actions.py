@@ -1,5 +1,5 @@
 """Actions that a mask has taken out count as none, in the policy loss and in
-both lines of a pair."""
+both lines of a pair; and infinite margins leave no NaN."""
 
 import numpy as np
 import pytest
@@ -80,3 +80,23 @@ def test_preference_loss(dev, shape, dtype, kind, average):
         assert np.isfinite(v).all(), k
         assert np.array_equal(v, want[k]), k
     assert np.all(got["logp"][hidden] == 0) and np.all(got["grad"][hidden] == 0)
+
+
+@pytest.mark.parametrize("listed", [True, False])
+@pytest.mark.parametrize("kind", ["sigmoid", "hinge", "square"])
+def test_infinite_margins(dev, kind, listed):
+    """A reference that would never have played a move: +inf where that is the
+    preferred line's, with nothing left to learn; -inf in the other."""
+    rng = np.random.default_rng(3)
+    x = rng.normal(size=(4, 60))
+    lists = [list(range(2, 20))] * 4 if listed else None
+    ref = np.array([-np.inf, -2, -2, -np.inf], np.float32)
+    got = lg.preference(lg.Batch(dev, x, "f32", lists, [5, 6, 7, 8]), [0, 1, 2, 3, 4], ref,
+                        kind=kind, beta=0.5)
+    assert list(got["margin"]) == [np.inf, -np.inf]
+    assert got["loss"][1] == np.inf
+    if kind != "square":
+        assert got["loss"][0] == 0 and np.all(got["grad"][:2] == 0)
+        assert np.isfinite(got["grad"][2:]).all() and np.any(got["grad"][2:] != 0)
+    else:
+        assert got["loss"][0] == np.inf

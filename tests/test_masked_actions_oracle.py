@@ -28,3 +28,9 @@ def test_in_either_line_of_a_pair(kind):
     want = losses.preference_loss(x, None, [1, -1, -1, 2], [0, 2, 4], kind=kind, average=True)
     for k in got:
         assert np.array_equal(got[k], want[k]) and np.isfinite(got[k]).all()
+
+
+def test_an_infinite_margin_without_smoothing():
+    out = losses.preference_loss(np.zeros((2, 4)), None, [1, 1], [0, 1, 2],
+                                 ref_logp=[-np.inf, -1.0])
+    assert out["margin"][0] == np.inf and out["loss"][0] == 0 and np.all(out["grad"] == 0)
