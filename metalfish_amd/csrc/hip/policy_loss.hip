@@ -568,6 +568,9 @@ struct Surrogate {
 __device__ __forceinline__ Surrogate Clipped(const RowLossParams &a, const RowInputs &in,
                                              float logp) {
   const float ratio = a.old_logp ? Exp(logp - in.old_logp) : 1.f;
+  // The ratio may overflow: 0 times it is 0 (a NaN stays).
+  if (in.advantage == 0.f && ratio == ratio)
+    return {0.f, 0.f};
   const float plain = ratio * in.advantage;
   const float bounded = fminf(fmaxf(ratio, a.ratio_low), a.ratio_high) * in.advantage;
   // The unclipped branch on ties and for NaN.

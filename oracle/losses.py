@@ -109,9 +109,10 @@ def policy_loss(logits, moves, actions, *, temp=1.0, old_logp=None, advantage=No
         if r.acted and advantage is not None:
             a = float(advantage[b])
             rho = 1.0 if old_logp is None else np.exp(r.logp - float(old_logp[b]))
-            plain = rho * a
-            bounded = min(max(rho, 1.0 - clip_low), 1.0 + clip_high) * a
-            loss, slope = (-bounded, 0.0) if bounded < plain else (-plain, -plain)
+            if a != 0.0:  # without an advantage no ratio counts, however large
+                plain = rho * a
+                bounded = min(max(rho, 1.0 - clip_low), 1.0 + clip_high) * a
+                loss, slope = (-bounded, 0.0) if bounded < plain else (-plain, -plain)
         g = slope * r.grad_logp()
         if kl_coef:
             loss += kl_coef * r.kl

@@ -1,5 +1,5 @@
 """Actions that a mask has taken out count as none, in the policy loss and in
-both lines of a pair; and infinite margins leave no NaN."""
+both lines of a pair; and infinite margins and zero advantages leave no NaN."""
 
 import numpy as np
 import pytest
@@ -100,3 +100,17 @@ def test_infinite_margins(dev, kind, listed):
         assert np.isfinite(got["grad"][2:]).all() and np.any(got["grad"][2:] != 0)
     else:
         assert got["loss"][0] == np.inf
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_a_zero_advantage_is_no_surrogate(dev, shape):
+    """Whatever the ratio: its overflow times 0 is 0."""
+    rng = np.random.default_rng(4)
+    x, lists, actions = _rows(rng, shape, 5)
+    old = np.array([-200.0, -np.inf, -5.0, 3e38, -1e30], np.float32)
+    for low, high in ((0.2, 0.2), (np.inf, np.inf)):
+        batch = lg.Batch(dev, x, "f32", lists, actions)
+        got = lg.policy(batch, old_logp=old, advantage=np.array([0.0, 0.0, 0.0, 0.0, -0.0]),
+                        clip_low=low, clip_high=high)
+        assert np.all(got["loss"] == 0) and np.all(got["grad"] == 0)
+        assert np.all(got["logp"] < 0)

@@ -34,3 +34,9 @@ def test_an_infinite_margin_without_smoothing():
     out = losses.preference_loss(np.zeros((2, 4)), None, [1, 1], [0, 1, 2],
                                  ref_logp=[-np.inf, -1.0])
     assert out["margin"][0] == np.inf and out["loss"][0] == 0 and np.all(out["grad"] == 0)
+
+
+def test_a_zero_advantage_takes_any_ratio():
+    out = losses.policy_loss(np.zeros((2, 4)), None, [1, 1], old_logp=[-np.inf, -2000.0],
+                             advantage=[0.0, -0.0])
+    assert np.all(out["loss"] == 0) and np.all(out["grad"] == 0)
