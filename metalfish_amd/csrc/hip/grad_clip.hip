@@ -174,8 +174,22 @@ __global__ __launch_bounds__(256) void GradSumKernel(const double *partials, int
     *sumsq = sum;
 }
 
+// A factor in 24 bits, as a product where it is below 2^-126 (gradients that
+// have all but overflowed against a small norm): by itself it would keep only
+// the bits of a denormal number.
+struct Factor {
+  float high, low;
+};
+__device__ __forceinline__ Factor FactorOf(double f) {
+  const bool tiny = f < 0x1p-126;
+  return {static_cast<float>(tiny ? f * 0x1p64 : f), tiny ? 0x1p-64f : 1.f};
+}
+__device__ __forceinline__ float operator*(float g, const Factor &f) {
+  return (g * f.high) * f.low;
+}
+
 template <int DT, bool PAST>
-__device__ __forceinline__ void ScaleVec(MFH_GLOBAL Bits<DT> *dst, u32x4 v, float scale) {
+__device__ __forceinline__ void ScaleVec(MFH_GLOBAL Bits<DT> *dst, u32x4 v, const Factor &scale) {
   u32x4 o;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -193,7 +207,7 @@ __device__ __forceinline__ void ScaleVec(MFH_GLOBAL Bits<DT> *dst, u32x4 v, floa
 }
 
 template <int DT, bool PAST>
-__device__ __forceinline__ void ScaleChunk(const GradChunk &c, float scale) {
+__device__ __forceinline__ void ScaleChunk(const GradChunk &c, const Factor &scale) {
   constexpr int VE = kPerVec<DT>;
   const auto *src = (const MFH_GLOBAL Bits<DT> *)c.src;
   auto *dst = (MFH_GLOBAL Bits<DT> *)c.dst;
@@ -216,7 +230,7 @@ __device__ __forceinline__ void ScaleChunk(const GradChunk &c, float scale) {
 }
 
 template <bool PAST>
-__device__ __forceinline__ void ScaleChunk(const GradChunk &c, float scale) {
+__device__ __forceinline__ void ScaleChunk(const GradChunk &c, const Factor &scale) {
   if (c.dtype == DT_F32)
     ScaleChunk<DT_F32, PAST>(c, scale);
   else if (c.dtype == DT_BF16)
@@ -238,7 +252,7 @@ __global__ __launch_bounds__(256) void GradScaleKernel(const GradChunk *list, st
     *norm = static_cast<float>(total);
   // NaN is not <= anything, and goes into every gradient.
   const bool keep = total <= max_norm;
-  const float scale = keep ? 1.f : static_cast<float>(max_norm / total);
+  const Factor scale = FactorOf(keep ? 1.0 : max_norm / total);
   while (k < n) {
     const std::int64_t next = k + gridDim.x;
     const GradChunk ahead = Entry(chunks, next < n ? next : k, n);
