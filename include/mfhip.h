@@ -432,8 +432,8 @@ int mfh_grad_norm_device(const mfh_grad_set *set, double *d_sumsq, void *d_works
 
 /* dst = src * min(1, max_norm / sqrt(*d_sumsq)), the factor rounded to 24 bits
  * at any size, the product to 32 bits and to the type; a sum that is NaN makes
- * every dst NaN.  For gradients spread over several processes, whose
- * sums the caller adds up in between. */
+ * every dst NaN.  For gradients spread over several processes, whose sums the
+ * caller adds up in between. */
 int mfh_grad_scale_device(const mfh_grad_set *set, const double *d_sumsq, float max_norm,
                           void *stream);
 
