@@ -308,9 +308,9 @@ int mfh_debug_quantize_fp8(int rows, int cols, const float *w, uint8_t *codes,
  * _destroy cannot.  Calls do not order each other: two that share an output
  * or a workspace are ordered by the caller.  What a call writes overlaps none
  * of its other arrays, but for the gradients in place below.  Array arguments
- * are device memory of one device, in one allocation each; a pointer that is not
- * (host memory, another device's, another device's stream) is rejected with
- * MFH_ERR_INVALID.  Offsets, indices and actions are read on the device:
+ * are device memory of one device, in one allocation each.  An overlap, or a
+ * pointer to host memory or to another device's, or another device's stream, is
+ * rejected with MFH_ERR_INVALID.  Offsets, indices and actions are read on the device:
  * offsets outside their array are clamped to it. */
 
 enum { MFH_DTYPE_F32 = 0, MFH_DTYPE_BF16 = 1, MFH_DTYPE_F16 = 2 };

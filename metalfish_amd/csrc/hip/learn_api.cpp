@@ -11,9 +11,11 @@
 #include <memory>
 #include <new>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "../../../include/mfhip.h"
+#include "learn_ranges.h"
 #include "mfh_kernels.h"
 #include "mfh_status.h"
 
@@ -22,6 +24,7 @@ struct mfh_grad_set {
   std::int64_t n_chunks = 0;
   bool past = false;                 // too large for the caches
   mfh::GradChunk *chunks = nullptr;  // device memory, read only
+  std::vector<mfh::ByteRange> memory;  // of every src and dst
 };
 
 namespace {
@@ -159,23 +162,24 @@ int Enter(const char *fn, int want, const Named (&ptrs)[N], hipStream_t stream, 
   return e == hipSuccess ? MFH_OK : HipError(fn, "hipSetDevice", e);
 }
 
-// Whether two sets of `rows` rows of `row_bytes`, strides in bytes, share a
-// byte in any other way than being the same rows.
-bool RowsClash(const void *p, std::int64_t p_stride, const void *q, std::int64_t q_stride,
-               std::int64_t rows, std::int64_t row_bytes) {
-  const auto a = reinterpret_cast<std::uintptr_t>(p), b = reinterpret_cast<std::uintptr_t>(q);
-  if (a == b && (p_stride == q_stride || rows <= 1))
-    return false;
-  const std::uintptr_t a_end = a + (rows - 1) * p_stride + row_bytes,
-                       b_end = b + (rows - 1) * q_stride + row_bytes;
-  if (a_end <= b || b_end <= a)
-    return false;
-  if (p_stride != q_stride || rows <= 1)
-    return true;
-  // Equal strides: interleaved rows are apart if they are within one stride.
-  const std::uintptr_t apart = (a > b ? a - b : b - a) % static_cast<std::uintptr_t>(p_stride);
-  return apart < static_cast<std::uintptr_t>(row_bytes) ||
-         static_cast<std::uintptr_t>(p_stride) - apart < static_cast<std::uintptr_t>(row_bytes);
+// An array without gaps.
+mfh::Span Flat(const char *name, const void *p, std::int64_t bytes, bool written) {
+  return {name, p, 1, bytes, bytes, written, false};
+}
+
+// Rows of the logits' shape.
+mfh::Span Rows(const char *name, const void *p, const mfh_policy_rows *r, std::int64_t stride,
+               bool written) {
+  const std::int64_t es = mfh::DTypeBytes(r->dtype);
+  return {name, p, r->rows, r->vocab * es, stride * es, written, true};
+}
+
+// Refuses a call that writes into another of its arrays.
+template <size_t N> int CheckApart(const char *fn, const mfh::Span (&spans)[N]) {
+  size_t a = 0, b = 0;
+  if (!mfh::FindOverlap(spans, &a, &b))
+    return MFH_OK;
+  return Invalid(fn, (std::string(spans[a].name) + " overlaps " + spans[b].name).c_str());
 }
 
 // No tensor on a card of 288 GB has more.
@@ -232,7 +236,7 @@ int CheckGrad(const char *fn, const mfh_policy_rows *r, void *grad, std::int64_t
     return Invalid(fn, "grad_stride must be at least vocab, and rows * stride addressable");
   if (!Aligned(grad, es))
     return Invalid(fn, "pointers must be aligned to their elements");
-  if (r->rows > 0 && RowsClash(r->d_logits, r->stride * es, grad, stride * es, r->rows,
+  if (r->rows > 0 && mfh::RowsClash(r->d_logits, r->stride * es, grad, stride * es, r->rows,
                                static_cast<std::int64_t>(r->vocab) * es))
     return Invalid(fn, "d_grad overlaps d_logits without being it");
   return MFH_OK;
@@ -272,7 +276,7 @@ int mfh_policy_loss_device(const mfh_policy_rows *rows, const mfh_policy_loss *l
     if (rc != MFH_OK)
       return rc;
     if (rows->rows > 0 && loss->d_grad && loss->d_ref_logits &&
-        RowsClash(loss->d_ref_logits, loss->ref_stride * es, loss->d_grad, loss->grad_stride * es,
+        mfh::RowsClash(loss->d_ref_logits, loss->ref_stride * es, loss->d_grad, loss->grad_stride * es,
                   rows->rows, static_cast<std::int64_t>(rows->vocab) * es))
       return Invalid(fn, "d_grad overlaps d_ref_logits without being it");
     if (rows->rows == 0)
@@ -293,6 +297,24 @@ int mfh_policy_loss_device(const mfh_policy_rows *rows, const mfh_policy_loss *l
                           {"d_grad", loss->d_grad}};
     const hipStream_t st = static_cast<hipStream_t>(stream);
     rc = Enter(fn, rows->device, ptrs, st, &on);
+    if (rc != MFH_OK)
+      return rc;
+    const std::int64_t column = rows->rows * 4;
+    const mfh::Span spans[] = {
+        Rows("d_logits", rows->d_logits, rows, rows->stride, false),
+        Flat("d_move_offsets", rows->d_move_offsets, column + 4, false),
+        Flat("d_move_indices", rows->d_move_indices, rows->n_moves * 2, false),
+        Flat("d_actions", rows->d_actions, column, false),
+        Flat("d_old_logp", loss->d_old_logp, column, false),
+        Flat("d_advantage", loss->d_advantage, column, false),
+        Flat("d_weight", loss->d_weight, column, false),
+        Rows("d_ref_logits", loss->d_ref_logits, rows, loss->ref_stride, false),
+        Flat("d_loss", loss->d_loss, column, true),
+        Flat("d_logp", loss->d_logp, column, true),
+        Flat("d_kl", loss->d_kl, column, true),
+        Flat("d_entropy", loss->d_entropy, column, true),
+        Rows("d_grad", loss->d_grad, rows, loss->grad_stride, true)};
+    rc = CheckApart(fn, spans);
     if (rc != MFH_OK)
       return rc;
     p.old_logp = loss->d_old_logp;
@@ -380,6 +402,24 @@ int mfh_preference_loss_device(const mfh_policy_rows *rows, const mfh_preference
                           {"d_workspace", need > 0 ? loss->d_workspace : nullptr}};
     const hipStream_t st = static_cast<hipStream_t>(stream);
     rc = Enter(fn, rows->device, ptrs, st, &on);
+    if (rc != MFH_OK)
+      return rc;
+    const std::int64_t column = rows->rows * 4, pairs = loss->pairs * 4;
+    const mfh::Span spans[] = {
+        Rows("d_logits", rows->d_logits, rows, rows->stride, false),
+        Flat("d_seq_offsets", loss->d_seq_offsets, 2 * pairs + 4, false),
+        Flat("d_move_offsets", rows->d_move_offsets, column + 4, false),
+        Flat("d_move_indices", rows->d_move_indices, rows->n_moves * 2, false),
+        Flat("d_actions", rows->d_actions, column, false),
+        Flat("d_ref_logp", loss->d_ref_logp, column, false),
+        Flat("d_weight", loss->d_weight, pairs, false),
+        Flat("d_loss", loss->d_loss, pairs, true),
+        Flat("d_margin", loss->d_margin, pairs, true),
+        Flat("d_logp", loss->d_logp, column, true),
+        Flat("d_workspace", need > 0 ? loss->d_workspace : nullptr,
+             static_cast<std::int64_t>(need), true),
+        Rows("d_grad", loss->d_grad, rows, loss->grad_stride, true)};
+    rc = CheckApart(fn, spans);
     if (rc != MFH_OK)
       return rc;
     p.g = loss->d_grad;
@@ -483,6 +523,9 @@ int mfh_grad_set_create(const mfh_grad_tensor *tensors, int n_tensors, int devic
     hipError_t e = on.Set(dev);
     if (e != hipSuccess)
       return HipError(fn, "hipSetDevice", e);
+    std::vector<mfh::ByteRange> memory;
+    for (const Range &r : ranges)
+      memory.push_back({r.begin, r.end});
     std::vector<mfh::GradChunk> chunks;
     for (int i = 0; i < n_tensors; ++i) {
       const mfh_grad_tensor &t = tensors[i];
@@ -497,6 +540,7 @@ int mfh_grad_set_create(const mfh_grad_tensor *tensors, int n_tensors, int devic
     }
     auto set = std::make_unique<mfh_grad_set>();
     set->device = dev;
+    set->memory = mfh::Joined(std::move(memory));
     set->n_chunks = static_cast<std::int64_t>(chunks.size());
     std::int64_t total = 0;
     for (const mfh::GradChunk &c : chunks)
@@ -551,6 +595,9 @@ int mfh_grad_norm_device(const mfh_grad_set *set, double *d_sumsq, void *d_works
     return Invalid(fn, "the workspace is too small");
   if (!Aligned(d_sumsq, 8) || !Aligned(d_workspace, 8))
     return Invalid(fn, "pointers must be aligned to their elements");
+  if (mfh::Meets(set->memory, d_sumsq, sizeof(double)) ||
+      mfh::Meets(set->memory, d_workspace, sizeof(double) * static_cast<uint64_t>(groups)))
+    return Invalid(fn, "d_sumsq or the workspace lies in a gradient");
   try {
     OnDevice on;
     const Named ptrs[] = {{"d_sumsq", d_sumsq}, {"d_workspace", d_workspace}};
@@ -578,6 +625,8 @@ int mfh_grad_scale_device(const mfh_grad_set *set, const double *d_sumsq, float 
     return Invalid(fn, "max_norm must be >= 0");
   if (!Aligned(d_sumsq, 8))
     return Invalid(fn, "pointers must be aligned to their elements");
+  if (mfh::Meets(set->memory, d_sumsq, sizeof(double)))
+    return Invalid(fn, "d_sumsq lies in a gradient");
   try {
     OnDevice on;
     const Named ptrs[] = {{"d_sumsq", d_sumsq}};
@@ -611,6 +660,9 @@ int mfh_grad_clip_device(const mfh_grad_set *set, float max_norm, float *d_norm,
              work = reinterpret_cast<std::uintptr_t>(d_workspace);
   if (d_norm && norm < work + sizeof(double) * groups && work < norm + sizeof(float))
     return Invalid(fn, "d_norm lies in the workspace");
+  if ((d_norm && mfh::Meets(set->memory, d_norm, sizeof(float))) ||
+      mfh::Meets(set->memory, d_workspace, sizeof(double) * static_cast<uint64_t>(groups)))
+    return Invalid(fn, "d_norm or the workspace lies in a gradient");
   try {
     OnDevice on;
     const Named ptrs[] = {{"d_workspace", d_workspace}, {"d_norm", d_norm}};

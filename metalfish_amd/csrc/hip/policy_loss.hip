@@ -540,8 +540,8 @@ __device__ __forceinline__ bool WantsKl(const RowLossParams &a) {
 
 // Element i of an input array, i the same in the whole wave, by a scalar load:
 // a vector load would be waited for behind every row load and store that the
-// wave has on its way.  No kernel writes the array while this one runs (an
-// output that is d_old_logp has each row's value read before it is written).
+// wave has on its way.  No kernel writes the array while this one runs: an
+// output that overlaps an input is refused.
 template <class T> __device__ __forceinline__ T Uniform(const T *p, std::int64_t i) {
   return ((const MFH_CONSTANT T *)p)[i];
 }
