@@ -1004,7 +1004,12 @@ __device__ __forceinline__ void StreamRow(const RowLossParams &a, std::int64_t r
     WriteRow(a, row, in.weight, acted, res, kl[0]);
 }
 
-// Rows longer than the registers hold.
+// Rows longer than the registers hold, one workgroup a CU (each asks for half of
+// the LDS, beside `red`): more rows at once push each other's first reading out
+// of the last-level cache.  fp32 with a reference, one and two a CU: 2000 x
+// 100003 605 and 684 us, 700 x 50021 101 and 110, 1818 x 33001 190 and 180;
+// 1000 x 60000 without 91 and 97.
+constexpr unsigned kHalfLds = 80 * 1024;
 template <int DT, bool REF>
 __global__ __launch_bounds__(1024) void StreamRowKernel(RowLossParams a) {
   __shared__ __align__(16) float red[16][8];
@@ -1475,7 +1480,7 @@ void LaunchRows(const RowLossParams &p, unsigned rows, hipStream_t s) {
   else if (vecs <= 8192)
     LaunchLoop<DT, REF, 8>(p, rows, s);
   else
-    hipLaunchKernelGGL((StreamRowKernel<DT, REF>), dim3(rows), dim3(1024), 0, s, p);
+    hipLaunchKernelGGL((StreamRowKernel<DT, REF>), dim3(rows), dim3(1024), kHalfLds, s, p);
 }
 
 template <int DT>
