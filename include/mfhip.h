@@ -343,7 +343,8 @@ typedef struct {
  *   loss = weight (-min(rho A, clip(rho, 1 - clip_low, 1 + clip_high) A)
  *                  + kl_coef KL(p || q) - entropy_coef H(p)),
  * q the softmax of the reference logits over the same entries and
- * temperature.  The first term is 0 in rows without an action or with
+ * temperature (an entry that only the policy's logits mask has its share of q).
+ * The first term is 0 in rows without an action or with
  * d_advantage NULL; d_old_logp NULL is the row's own l (rho = 1).  A row of
  * weight 0 gives zeros, whatever its logits hold.  The gradient of the sum of
  * all losses (old_logp, advantage, weight and q held fixed) goes to d_grad, every
@@ -377,8 +378,9 @@ int mfh_policy_loss_device(const mfh_policy_rows *rows, const mfh_policy_loss *l
  *   HINGE:   max(0, 1 - h)
  *   SQUARE:  (D - 1 / (2 beta))^2
  * times the pair's weight (a pair of weight 0 gives a loss, margin and
- * gradient of 0).  margin is h.  logp is ln p_action, 0 without an action.  The gradient of the sum of all losses
- * goes to the sequences' rows of d_grad, every column.  Rows before the first
+ * gradient of 0).  margin is h.  logp is ln p_action, 0 without an action.
+ * The gradient of the sum of all losses goes to the sequences' rows of d_grad,
+ * every column.  Rows before the first
  * sequence or behind the last are left as they are, whatever they hold.  Any
  * output may be NULL; d_grad may be d_logits with the same stride.  d_workspace holds
  * mfh_preference_loss_workspace_bytes(rows) bytes, 8-byte aligned. */
@@ -409,8 +411,11 @@ int mfh_preference_loss_device(const mfh_policy_rows *rows, const mfh_preference
  * scaled gradients: src itself, memory of its own, or NULL for a tensor that
  * counts in the norm only.  No dst may overlap another tensor's src or dst,
  * nor its own src in part.  device -1 is the device of the first tensor (the
- * current one without any).  Only _destroy waits for the device; the set
- * outlives every graph that has captured a call on it. */
+ * current one without any).  _create copies the list with a blocking copy on
+ * the default stream, and _destroy frees it: both wait for the device's work
+ * (and take about 0.35 ms for 400 tensors on an idle one), so a set is kept for
+ * as long as its gradients keep their addresses.  It outlives every graph that
+ * has captured a call on it. */
 typedef struct {
   const void *src;
   void *dst;

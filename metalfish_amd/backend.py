@@ -653,7 +653,9 @@ class GradSet:
     """The gradients of a net, laid out once: ``tensors`` is a list of (src,
     dst, count, dtype) with device addresses; dst is src (in place), memory
     of its own, or None for a tensor that counts in the norm only.  Norm and
-    clipping run over all of them in two launches."""
+    clipping run over all of them in two launches.  Making and closing a set
+    wait for the device: it is kept for as long as the gradients keep their
+    addresses."""
 
     def __init__(self, tensors, device=-1):
         self._h = None

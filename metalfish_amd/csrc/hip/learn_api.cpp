@@ -237,7 +237,7 @@ int CheckGrad(const char *fn, const mfh_policy_rows *r, void *grad, std::int64_t
   if (!Aligned(grad, es))
     return Invalid(fn, "pointers must be aligned to their elements");
   if (r->rows > 0 && mfh::RowsClash(r->d_logits, r->stride * es, grad, stride * es, r->rows,
-                               static_cast<std::int64_t>(r->vocab) * es))
+                                    static_cast<std::int64_t>(r->vocab) * es))
     return Invalid(fn, "d_grad overlaps d_logits without being it");
   return MFH_OK;
 }
@@ -276,8 +276,9 @@ int mfh_policy_loss_device(const mfh_policy_rows *rows, const mfh_policy_loss *l
     if (rc != MFH_OK)
       return rc;
     if (rows->rows > 0 && loss->d_grad && loss->d_ref_logits &&
-        mfh::RowsClash(loss->d_ref_logits, loss->ref_stride * es, loss->d_grad, loss->grad_stride * es,
-                  rows->rows, static_cast<std::int64_t>(rows->vocab) * es))
+        mfh::RowsClash(loss->d_ref_logits, loss->ref_stride * es, loss->d_grad,
+                       loss->grad_stride * es, rows->rows,
+                       static_cast<std::int64_t>(rows->vocab) * es))
       return Invalid(fn, "d_grad overlaps d_ref_logits without being it");
     if (rows->rows == 0)
       return MFH_OK;

@@ -16,15 +16,15 @@
 // written from there (rows longer than 8192 vectors of 16 bytes are read a
 // second time).  What bounds it:
 //  * fp32, or no reference: memory.  16384 x 1858 fp32 with a reference 60.4 us
-//    (365 MB, 6.0 TB/s); 3588 x 32000 bf16: statistics 42 us (5.4 TB/s; 38 the
-//    fastest run), gradient 80 (5.8 TB/s; 76).
+//    (365 MB, 6.0 TB/s); 3588 x 32000 bf16: statistics 39.5 us (5.8 TB/s),
+//    gradient 78 (5.9 TB/s).
 //  * 16 bits with a reference and KL: the vector unit, about 44 instructions an
 //    entry, three of them exponentials: 16384 x 1858 bf16 48 us (3.8 TB/s), 1500
-//    x 50021 133 us (3.4 TB/s; the vector unit busy two thirds of it).
+//    x 50021 131 us (3.4 TB/s; the vector unit busy two thirds of it).
 //  * move lists: the zeros around the entries, and lines of 128 bytes for
-//    gathered logits: 20011 rows of 1858 bf16 20.5 us (74 MB written, about 50
+//    gathered logits: 20011 rows of 1858 bf16 20.8 us (74 MB written, about 50
 //    MB of lines read).
-//  * few rows: the launch and the loads that wait on one another, 4.4 us for 16
+//  * few rows: the launch and the loads that wait on one another, 5.0 us for 16
 //    rows of moves.
 #include "mfh_device.h"
 #include "mfh_kernels.h"
@@ -1598,7 +1598,10 @@ template <int W> __global__ __launch_bounds__(64 * W) void PairLossKernel(PairLo
 // the pair's rows in turn; marks through the workspace as in the three
 // launches.  Up to 8 rows a pair on average (one a wave) and 512 pairs: 16
 // pairs of 2 rows 6.4 us (9.4 in three launches), 256 pairs of about 5 rows 8.1
-// (11.3); 1024 pairs of 2 rows 15.1 (12.8), 128 pairs of 60 rows 50 (25).
+// (11.3); 1024 pairs of 2 rows 15.1 (12.8), 128 pairs of 60 rows 50 (25).  The
+// host does not know the lengths, and the longest pair is one workgroup's: 100
+// pairs of 3 rows 7.0 (10.0), with one of 120 rows among them 44.5 (10.3), 512
+// pairs of 4 with one of 2000 789 (27).
 constexpr int kPairWaves = 8, kFewPairs = 512;
 template <int DT>
 __global__ __launch_bounds__(64 * kPairWaves) void PairMovesKernel(RowLossParams a,
