@@ -322,7 +322,8 @@ enum { MFH_DTYPE_F32 = 0, MFH_DTYPE_BF16 = 1, MFH_DTYPE_F16 = 2 };
  * vocab <= 32768; an index outside the vocabulary reads logit 0; an index
  * listed twice counts twice), or all columns when d_move_offsets is NULL.  A
  * logit of -inf takes its entry out; a row with no entry left gives zeros
- * everywhere.  The row's action is the move played (or the token written):
+ * everywhere.  Arithmetic is in 32 bits, and a p_k below 2^-126 counts as 0.
+ * The row's action is the move played (or the token written):
  * a column among its entries, anything else (-1, a masked one) for none. */
 typedef struct {
   const void *d_logits;

@@ -403,6 +403,8 @@ __device__ __forceinline__ Coefs CoefsOf(const RowStats &st, const RowGrad &g, f
 // in P are at most 2^40 exp(30) = 2^84 each.
 struct FarCoefs {
   float mean_d, y_m, y_shift, peak;
+  float steep, flat;     // b / T, as a factor of p from 1 on and of d - E_p d below: no
+                         // step of a gradient leaves the range that it is in itself
   float above;           // u of more is infinite, or may be where p u is not (1 / T > 1)
   bool apart, wide, kl;  // d from the maxima; peak above kWide; KL in the gradient
 };
@@ -414,6 +416,9 @@ __device__ __forceinline__ FarCoefs FarCoefsOf(const RowStats &st, const Coefs &
   f.above = k.inv_temp > 1.f ? -kFarBelow : 0x1.fffffep127f;
   f.apart = __builtin_amdgcn_readfirstlane(apart);
   f.wide = __builtin_amdgcn_readfirstlane(f.peak > kWide);
+  const float slope = k.b * k.inv_temp;
+  f.steep = Scalar(fabsf(slope) < 1.f ? 1.f : slope);
+  f.flat = Scalar(fabsf(slope) < 1.f ? slope : 1.f);
   f.kl = __builtin_amdgcn_readfirstlane(k.b != 0.f);
   f.y_shift = Scalar(f.wide ? 0.f : f.peak * kLog2e + static_cast<float>(k.power));
   f.mean_d = Scalar(st.mean_d);
@@ -501,7 +506,7 @@ __device__ __forceinline__ void FinishEntries(const Coefs &k, const FarCoefs &fa
     if (far.kl) {
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        f[i] += k.b * TimesU(k, p[i], apart[i]);
+        f[i] += (p[i] * far.steep) * (apart[i] * far.flat);
     }
     if (want_kl) {
       bool usual = !far.wide;
@@ -627,8 +632,12 @@ __device__ __forceinline__ void WriteRow(const RowLossParams &a, std::int64_t ro
     loss += a.kl_coef * kl;
   if (a.entropy_coef != 0.f)
     loss -= a.entropy_coef * r.entropy;
+  // A coefficient may carry KL (up to 3e38 against masks of the lowest value) out
+  // of the range that the weight brings it back to.
+  const bool over = fabsf(loss) == __builtin_inff() && fabsf(w) < 1.f;
   if (a.loss)
-    a.loss[row] = w * loss;
+    a.loss[row] = over ? w * (r.surrogate - a.entropy_coef * r.entropy) + w * a.kl_coef * kl
+                       : w * loss;
   if (a.logp)
     a.logp[row] = r.logp;
   if (a.kl)

@@ -261,3 +261,21 @@ def test_references_a_constant_away(dev, shape, dtype, temp):
     n = batch.vocab if lists is None else len(lists[0])
     uniform = np.log(n) - got["entropy"][0]
     assert abs(got["kl"][0] - uniform) < 1e-4 * np.log(n)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_products_that_leave_the_range_on_the_way(dev, shape, dtype):
+    """Masks of the lowest value where p is 1/3, with weights and coefficients
+    whose product with KL or u is within the range only in the end."""
+    rng = np.random.default_rng(8)
+    weight = np.array([1e-4, 1e-12, 0.5, 1e-30], np.float32)
+    for temp, kl_coef, w in ((1.0, 3.0, weight), (1.0, 0.05, weight * np.float32(32))):
+        x, ref, at, lists = _rows(rng, shape, dtype, 4)
+        x[:, at[:3]] = ref[:, at[:3]] = 0.0
+        ref[:, at[0]] = LOWEST[dtype]
+        ref[:2, at[1]] = LOWEST[dtype]
+        batch = lg.Batch(dev, x, dtype, lists, None, temp)
+        got = lg.policy(batch, ref=ref, weight=w, kl_coef=kl_coef, entropy_coef=0.1)
+        assert np.isfinite(got["kl"]).all() and np.isfinite(got["grad"]).all()
+        check(batch, got, ref, kl_coef, 0.1, w)
