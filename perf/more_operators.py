@@ -535,6 +535,10 @@ def _own_set(backend, s):
     for f in s["flat"].values():
         gdt = {v: k for k, v in DTYPES.items()}[f["grad"].dtype]
         for b, n in f["tensors"]:
+            # The update runs over the whole flat buffers, padding included, as
+            # the plain form's does (its encoding gives a padding's states codes
+            # above 0, and those change with every step).
+            n = -(-n // BLOCK) * BLOCK
             t = {"param": f["param"][b:].data_ptr(), "grad": f["grad"][b:].data_ptr(),
                  "m": f["m"][b:].data_ptr(), "v": f["v"][b:].data_ptr(), "count": n,
                  "grad_dtype": gdt, "weight_decay": f["decay"]}
