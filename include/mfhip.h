@@ -448,6 +448,182 @@ int mfh_grad_scale_device(const mfh_grad_set *set, const double *d_sumsq, float 
 int mfh_grad_clip_device(const mfh_grad_set *set, float max_norm, float *d_norm,
                          void *d_workspace, uint64_t workspace_bytes, void *stream);
 
+/* ---- Layers of a training step -----------------------------------------
+ *
+ * What lies between the losses above and the next weights: layer norm and
+ * attention with their gradients, and the AdamW update.  The rules of the
+ * calls above hold here too (streams, workspaces, captures, overlaps, pointers);
+ * lengths are read on the device and clamped to their arrays. */
+
+/* Rows of h = residual + alpha x (alpha x where d_residual is NULL), normalised
+ * over their width: the nets' LayerNorm of a layer's input plus its output. */
+typedef struct {
+  const void *d_x;
+  int64_t x_stride; /* elements from one row to the next, >= width */
+  const void *d_residual;
+  int64_t residual_stride;
+  int64_t rows;         /* >= 0 */
+  int32_t width;        /* 1 .. 2^20 */
+  int32_t dtype;        /* MFH_DTYPE_*: of x, residual, y and their gradients */
+  float alpha;          /* finite */
+  float eps;            /* >= 0, added to the variance */
+  const float *d_gamma; /* [width], NULL: 1 */
+  const float *d_beta;  /* [width], NULL: 0 */
+  int32_t device;       /* HIP device ordinal, -1 = the rows' device */
+} mfh_norm_rows;
+
+/* y = (h - mean) rstd gamma + beta with the row's mean and rstd =
+ * 1 / sqrt(variance + eps), in 32 bits and rounded once.  d_mean and d_rstd
+ * [rows] may be NULL.  y may be x or the residual at the same stride. */
+int mfh_layer_norm_device(const mfh_norm_rows *rows, void *d_y, int64_t y_stride, float *d_mean,
+                          float *d_rstd, void *stream);
+
+/* The gradients of layer norm from dy and the forward pass's mean and rstd:
+ * with n = (h - mean) rstd and w = dy gamma,
+ *   dh = rstd (w - mean(w) - n mean(w n)), dresidual = dh, dx = alpha dh,
+ *   dgamma = sum over the rows of dy n, dbeta = that of dy,
+ * sums in 32 bits and in an order that depends on the shape alone; rows = 0
+ * gives sums of 0.  Any output may be NULL.  dx and dresidual may each be dy, x
+ * or the residual at the same stride.  d_workspace (4-byte aligned; NULL if
+ * neither dgamma nor dbeta is wanted) holds mfh_layer_norm_workspace_bytes(rows,
+ * width) bytes. */
+typedef struct {
+  const void *d_dy;
+  int64_t dy_stride;
+  const float *d_mean, *d_rstd; /* [rows] */
+  void *d_dx;
+  int64_t dx_stride;
+  void *d_dresidual;
+  int64_t dresidual_stride;
+  float *d_dgamma, *d_dbeta; /* [width] */
+  void *d_workspace;
+  uint64_t workspace_bytes;
+} mfh_norm_grads;
+int mfh_layer_norm_workspace_bytes(int64_t rows, int32_t width, uint64_t *bytes);
+int mfh_layer_norm_backward_device(const mfh_norm_rows *rows, const mfh_norm_grads *grads,
+                                   void *stream);
+
+/* Heads of tokens in device memory: element d of head h of token t of line b
+ * is p[b * batch + t * token + h * head + d]; strides in elements, >= 0.  An
+ * array that is written has no two elements in one place. */
+typedef struct {
+  void *p;
+  int64_t batch, token, head;
+} mfh_heads;
+
+/* Attention of `heads` query heads over `kv_heads` key heads (each shared by
+ * heads / kv_heads consecutive query heads):
+ *   s_ij = scale q_i . k_j + bias_ij,  lse_i = ln sum_j exp(s_ij),
+ *   out_i = sum_j exp(s_ij - lse_i) v_j
+ * over the keys j that query i sees: with m = d_q_lengths[b] and n =
+ * d_k_lengths[b] (NULL: q_len, k_len; clamped to 0 .. those) j < n, and with
+ * `causal` j <= i + n - m, so the last query sees the last key.  What lies
+ * behind a length is not read.  A query that sees nothing (i >= m among them), or
+ * only keys of bias -inf, has out 0, lse -inf, and gradients of 0.  The bias is
+ * p[b * bias_batch + h * bias_head + i * bias_query + j]; a stride of 0 shares
+ * it.  Scores, statistics and sums are in 32 bits; with bf16 or fp16 inputs the
+ * probabilities and dS are rounded to that type before they are multiplied (in
+ * fp16 |dS| above 65504 becomes infinite). */
+typedef struct {
+  int32_t batch, heads, kv_heads; /* >= 1; batch >= 0 */
+  int32_t q_len, k_len;           /* >= 0; q_len heads / kv_heads, k_len <= 2^30 */
+  int32_t dim;                    /* 1 .. 128 */
+  int32_t dtype;                  /* MFH_DTYPE_*: of q, k, v, out and their gradients */
+  int32_t causal;                 /* 0 or 1 */
+  float scale;                    /* finite */
+  mfh_heads q, k, v;              /* read; k and v have kv_heads heads */
+  const void *d_bias;             /* NULL: none */
+  int32_t bias_dtype;             /* MFH_DTYPE_* */
+  int64_t bias_batch, bias_head, bias_query;
+  const int32_t *d_q_lengths, *d_k_lengths; /* [batch] */
+  int32_t device;                           /* HIP device ordinal, -1 = q's device */
+} mfh_attention;
+
+/* out, and lse [batch][heads][q_len] (NULL to skip).  The workspace (16-byte
+ * aligned) is used where few queries meet many keys; its size may be 0. */
+int mfh_attention_forward_workspace_bytes(const mfh_attention *a, uint64_t *bytes);
+int mfh_attention_forward_device(const mfh_attention *a, const mfh_heads *out, float *d_lse,
+                                 void *d_workspace, uint64_t workspace_bytes, void *stream);
+
+/* The gradients from dout and the forward pass's out and lse; with p_ij =
+ * exp(s_ij - lse_i) formed again and dS_ij = p_ij (dout_i . v_j - dout_i . out_i):
+ *   dq_i = scale sum_j dS_ij k_j,  dk_j = scale sum_i dS_ij q_i,
+ *   dv_j = sum_i p_ij dout_i,      dbias_ij = dS_ij,
+ * dk and dv summed over the heads that share them, dbias over what shares the
+ * bias.  dbias is laid out as the bias (its query stride at least k_len if
+ * q_len > 1); every element is written, 0 where a query sees nothing.  Any output may
+ * be NULL (p of a mfh_heads).  No sum depends on the order in which the device
+ * runs. */
+typedef struct {
+  mfh_heads out, dout; /* read */
+  const float *d_lse;
+  mfh_heads dq, dk, dv;
+  void *d_dbias;
+  void *d_workspace;
+  uint64_t workspace_bytes;
+} mfh_attention_grads;
+int mfh_attention_backward_workspace_bytes(const mfh_attention *a, uint64_t *bytes);
+int mfh_attention_backward_device(const mfh_attention *a, const mfh_attention_grads *grads,
+                                  void *stream);
+
+/* The weights of a net with their AdamW states, laid out once, as a
+ * mfh_grad_set is (the same rules for its memory, creation and end).  state_bits
+ * 32: m and v are float[count].  8: m and v are uint8_t[count], and each block
+ * of 256 consecutive values (the last may be shorter) has a float in m_scale and
+ * v_scale: m = scale * the OCP e4m3 value of its code, v = scale * the value of
+ * its code of five bits of exponent (bias 15) and three of mantissa, no sign.
+ * Codes and scales of 0 are the states before the first step.  copy (NULL:
+ * none) receives the weights rounded to copy_dtype.  Nothing of a tensor
+ * overlaps anything of another, or of its own.  lr_scale multiplies the step's
+ * learning rate. */
+typedef struct {
+  void *param;
+  const void *grad;
+  void *m, *v;
+  float *m_scale, *v_scale; /* [ceil(count / 256)], NULL with 32 bits */
+  void *copy;
+  uint64_t count; /* elements, 0 allowed */
+  int32_t param_dtype, grad_dtype, copy_dtype; /* MFH_DTYPE_* */
+  float lr_scale;                              /* finite, >= 0 */
+  float weight_decay;                          /* finite, >= 0 */
+} mfh_adamw_tensor;
+typedef struct mfh_adamw_set mfh_adamw_set;
+int mfh_adamw_set_create(const mfh_adamw_tensor *tensors, int n_tensors, int state_bits,
+                         int device, mfh_adamw_set **out);
+void mfh_adamw_set_destroy(mfh_adamw_set *set);
+
+/* One step t over every tensor, in one launch:
+ *   g = grad f,  m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
+ *   param = param (1 - lr weight_decay)
+ *           - lr m / (1 - beta1^t) / (sqrt(v / (1 - beta2^t)) + eps)
+ * in 32 bits, param rounded once to its type; the update uses m and v before
+ * they are rounded to 8 bits.  f = grad_scale (1 over a loss scale), and with
+ * d_sumsq (mfh_grad_norm_device of the gradients as they are) times min(1,
+ * max_norm / (grad_scale sqrt(*d_sumsq))): the clipping without writing
+ * gradients.  With skip_nonfinite a *d_sumsq that is not finite leaves
+ * everything as it is.  d_lr and d_step (device, NULL: lr and step) are read
+ * when the step runs, for captured steps.
+ * 8 bits: a block's scale is its largest |m| / 448 (at least 2^-100) and v /
+ * 122880 (at least 2^-120).  Codes are rounded to nearest, or with
+ * `stochastic` up with the probability of the part cut off (to 16 bits), by
+ * bits that are a function of seed, t and the value's place in the set: with beta2
+ * near 1 rounding to nearest would hold v where it is.  A v above 0 keeps a
+ * code above 0.  A state that is not finite makes its block's scale so. */
+typedef struct {
+  double lr;           /* finite, >= 0 */
+  double beta1, beta2; /* 0 <= beta < 1 */
+  double eps;          /* finite, >= 0 */
+  double grad_scale;   /* finite, > 0 */
+  int64_t step;        /* >= 1 */
+  const float *d_lr;
+  const int64_t *d_step;
+  const double *d_sumsq;
+  float max_norm; /* >= 0, infinity does not clip; without d_sumsq unused */
+  int32_t skip_nonfinite, stochastic; /* 0 or 1; skip_nonfinite needs d_sumsq */
+  uint64_t seed;
+} mfh_adamw_step;
+int mfh_adamw_step_device(const mfh_adamw_set *set, const mfh_adamw_step *step, void *stream);
+
 /* ---- Network files (no device needed) ----------------------------------
  *
  * A reader for the reference's `.pb` / `.pb.gz` network files

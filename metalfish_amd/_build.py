@@ -31,7 +31,9 @@ HIP_SOURCES = ["hip/gemm_tiles_pipe_a.hip", "hip/policy_loss.hip", "hip/gemm_til
                "hip/gemm_tiles_w8_single.hip", "hip/gemm_tiles_w8_small.hip", "hip/gemm.hip",
                "hip/panel_gemm.hip", "hip/skinny_gemm.hip", "hip/smolgen_bias.hip",
                "hip/attention.hip", "hip/rowops.hip", "hip/policy.hip",
-               "hip/grad_clip.hip", "hip/mfh_api.cpp", "hip/learn_api.cpp",
+               "hip/layer_norm.hip", "hip/train_attention_bf16.hip",
+               "hip/train_attention_f16.hip", "hip/train_attention_f32.hip", "hip/adamw.hip",
+               "hip/grad_clip.hip", "hip/mfh_api.cpp", "hip/learn_api.cpp", "hip/train_api.cpp",
                "host/policy_tables.cpp"]
 # Host-only parts of libmfhip.so (no device code), compiled with g++.
 HIP_HOST_SOURCES = ["host/weights_file.cpp", "host/pack_planes.cpp"]

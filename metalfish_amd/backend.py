@@ -43,7 +43,12 @@ EXPORTS = ("mfh_net_create", "mfh_net_destroy", "mfh_net_eval", "mfh_net_eval_pl
            "mfh_policy_loss_device", "mfh_preference_loss_workspace_bytes",
            "mfh_preference_loss_device", "mfh_grad_set_create", "mfh_grad_set_destroy",
            "mfh_grad_workspace_bytes", "mfh_grad_norm_device", "mfh_grad_scale_device",
-           "mfh_grad_clip_device")
+           "mfh_grad_clip_device",
+           "mfh_layer_norm_device", "mfh_layer_norm_workspace_bytes",
+           "mfh_layer_norm_backward_device", "mfh_attention_forward_workspace_bytes",
+           "mfh_attention_forward_device", "mfh_attention_backward_workspace_bytes",
+           "mfh_attention_backward_device", "mfh_adamw_set_create", "mfh_adamw_set_destroy",
+           "mfh_adamw_step_device")
 FORMAT_FIELDS = ("input", "output", "network", "policy", "value", "moves_left",
                  "default_activation", "smolgen_activation", "ffn_activation", "input_embedding")
 
@@ -110,6 +115,65 @@ class MfhGradTensor(ctypes.Structure):
                 ("dtype", ctypes.c_int32)]
 
 
+class MfhNormRows(ctypes.Structure):
+    _fields_ = [("d_x", ctypes.c_void_p), ("x_stride", ctypes.c_int64),
+                ("d_residual", ctypes.c_void_p), ("residual_stride", ctypes.c_int64),
+                ("rows", ctypes.c_int64), ("width", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("alpha", ctypes.c_float), ("eps", ctypes.c_float), ("d_gamma", ctypes.c_void_p),
+                ("d_beta", ctypes.c_void_p), ("device", ctypes.c_int32)]
+
+
+class MfhNormGrads(ctypes.Structure):
+    _fields_ = [("d_dy", ctypes.c_void_p), ("dy_stride", ctypes.c_int64),
+                ("d_mean", ctypes.c_void_p), ("d_rstd", ctypes.c_void_p),
+                ("d_dx", ctypes.c_void_p), ("dx_stride", ctypes.c_int64),
+                ("d_dresidual", ctypes.c_void_p), ("dresidual_stride", ctypes.c_int64),
+                ("d_dgamma", ctypes.c_void_p), ("d_dbeta", ctypes.c_void_p),
+                ("d_workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
+
+
+class MfhHeads(ctypes.Structure):
+    _fields_ = [("p", ctypes.c_void_p), ("batch", ctypes.c_int64), ("token", ctypes.c_int64),
+                ("head", ctypes.c_int64)]
+
+
+class MfhAttention(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_int32), ("heads", ctypes.c_int32),
+                ("kv_heads", ctypes.c_int32), ("q_len", ctypes.c_int32),
+                ("k_len", ctypes.c_int32), ("dim", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("causal", ctypes.c_int32), ("scale", ctypes.c_float), ("q", MfhHeads),
+                ("k", MfhHeads), ("v", MfhHeads), ("d_bias", ctypes.c_void_p),
+                ("bias_dtype", ctypes.c_int32), ("bias_batch", ctypes.c_int64),
+                ("bias_head", ctypes.c_int64), ("bias_query", ctypes.c_int64),
+                ("d_q_lengths", ctypes.c_void_p), ("d_k_lengths", ctypes.c_void_p),
+                ("device", ctypes.c_int32)]
+
+
+class MfhAttentionGrads(ctypes.Structure):
+    _fields_ = [("out", MfhHeads), ("dout", MfhHeads), ("d_lse", ctypes.c_void_p),
+                ("dq", MfhHeads), ("dk", MfhHeads), ("dv", MfhHeads),
+                ("d_dbias", ctypes.c_void_p), ("d_workspace", ctypes.c_void_p),
+                ("workspace_bytes", ctypes.c_uint64)]
+
+
+class MfhAdamwTensor(ctypes.Structure):
+    _fields_ = [("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("m", ctypes.c_void_p),
+                ("v", ctypes.c_void_p), ("m_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("copy", ctypes.c_void_p),
+                ("count", ctypes.c_uint64), ("param_dtype", ctypes.c_int32),
+                ("grad_dtype", ctypes.c_int32), ("copy_dtype", ctypes.c_int32),
+                ("lr_scale", ctypes.c_float), ("weight_decay", ctypes.c_float)]
+
+
+class MfhAdamwStep(ctypes.Structure):
+    _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double),
+                ("eps", ctypes.c_double), ("grad_scale", ctypes.c_double),
+                ("step", ctypes.c_int64), ("d_lr", ctypes.c_void_p), ("d_step", ctypes.c_void_p),
+                ("d_sumsq", ctypes.c_void_p), ("max_norm", ctypes.c_float),
+                ("skip_nonfinite", ctypes.c_int32), ("stochastic", ctypes.c_int32),
+                ("seed", ctypes.c_uint64)]
+
+
 _lib = None
 
 
@@ -173,6 +237,17 @@ def lib():
             "mfh_grad_norm_device": ([vp, vp, vp, u64, vp], i),
             "mfh_grad_scale_device": ([vp, vp, ctypes.c_float, vp], i),
             "mfh_grad_clip_device": ([vp, ctypes.c_float, vp, vp, u64, vp], i),
+            "mfh_layer_norm_device": ([vp, vp, ctypes.c_int64, vp, vp, vp], i),
+            "mfh_layer_norm_workspace_bytes": ([ctypes.c_int64, ctypes.c_int32,
+                                                ctypes.POINTER(u64)], i),
+            "mfh_layer_norm_backward_device": ([vp, vp, vp], i),
+            "mfh_attention_forward_workspace_bytes": ([vp, ctypes.POINTER(u64)], i),
+            "mfh_attention_forward_device": ([vp, vp, vp, vp, u64, vp], i),
+            "mfh_attention_backward_workspace_bytes": ([vp, ctypes.POINTER(u64)], i),
+            "mfh_attention_backward_device": ([vp, vp, vp], i),
+            "mfh_adamw_set_create": ([vp, i, i, i, ctypes.POINTER(vp)], i),
+            "mfh_adamw_set_destroy": ([vp], None),
+            "mfh_adamw_step_device": ([vp, vp, vp], i),
         }
         for name, (args, res) in sig.items():
             fn = getattr(L, name)
@@ -697,6 +772,173 @@ class GradSet:
         clipping (mfh_grad_clip_device)."""
         _check(lib().mfh_grad_clip_device(self._h, max_norm, d_norm, d_workspace, workspace_bytes,
                                           stream), "mfh_grad_clip_device")
+
+
+def norm_rows(d_x, rows, width, dtype="f32", x_stride=None, d_residual=None,
+              residual_stride=None, alpha=1.0, d_gamma=None, d_beta=None, eps=1e-3, device=-1):
+    """Rows h = residual + alpha x in device memory for the layer norms below:
+    [rows, width] of ``dtype`` "f32", "bf16" or "f16", strides in elements
+    (``width``); ``d_gamma`` and ``d_beta`` float32 [width], None for 1 and 0.
+    Holds addresses only."""
+    return MfhNormRows(d_x, width if x_stride is None else x_stride, d_residual,
+                       width if residual_stride is None else residual_stride, rows, width,
+                       DTYPE[dtype], alpha, eps, d_gamma, d_beta, device)
+
+
+def layer_norm_device(rows, d_y, y_stride=None, d_mean=None, d_rstd=None, stream=None):
+    """y = (h - mean) rstd gamma + beta of each row of ``rows`` (``norm_rows``),
+    and its statistics, float32 [rows] (mfh_layer_norm_device)."""
+    _check(lib().mfh_layer_norm_device(ctypes.addressof(rows), d_y,
+                                       rows.width if y_stride is None else y_stride, d_mean,
+                                       d_rstd, stream), "mfh_layer_norm_device")
+
+
+def layer_norm_workspace_bytes(rows: int, width: int) -> int:
+    """Bytes of device memory a layer norm's backward pass works in."""
+    n = ctypes.c_uint64(0)
+    _check(lib().mfh_layer_norm_workspace_bytes(rows, width, ctypes.byref(n)),
+           "mfh_layer_norm_workspace_bytes")
+    return n.value
+
+
+def layer_norm_backward_device(rows, d_dy, d_mean, d_rstd, d_dx=None, d_dresidual=None,
+                               d_dgamma=None, d_dbeta=None, dy_stride=None, dx_stride=None,
+                               dresidual_stride=None, d_workspace=None, workspace_bytes=0,
+                               stream=None):
+    """The gradients of ``layer_norm_device`` from dy and the statistics that
+    it left (mfh_layer_norm_backward_device).  Strides default to the width;
+    outputs left None are not written."""
+    w = rows.width
+    g = MfhNormGrads(d_dy, w if dy_stride is None else dy_stride, d_mean, d_rstd, d_dx,
+                     w if dx_stride is None else dx_stride, d_dresidual,
+                     w if dresidual_stride is None else dresidual_stride, d_dgamma, d_dbeta,
+                     d_workspace, workspace_bytes)
+    _check(lib().mfh_layer_norm_backward_device(ctypes.addressof(rows), ctypes.addressof(g),
+                                                stream), "mfh_layer_norm_backward_device")
+
+
+def _heads(p, strides, tokens, heads, dim):
+    """An array of heads: strides (batch, token, head) in elements, or None for
+    [batch, tokens, heads, dim] without gaps."""
+    return MfhHeads(p, *((tokens * heads * dim, heads * dim, dim) if strides is None else strides))
+
+
+def attention_problem(d_q, d_k, d_v, batch, heads, q_len, k_len, dim, dtype="f32", kv_heads=None,
+                      scale=None, causal=False, q_strides=None, k_strides=None, v_strides=None,
+                      d_bias=None, bias_dtype="f32", bias_strides=None, d_q_lengths=None,
+                      d_k_lengths=None, device=-1):
+    """Attention of ``heads`` query heads over ``kv_heads`` (all of them) key
+    heads in device memory, for the calls below.  Strides are (batch, token,
+    head) in elements, None for [batch, tokens, heads, dim] without gaps; the
+    bias's (batch, head, query), 0 where it is shared, None for [batch, heads,
+    q_len, k_len].  ``scale`` defaults to 1 / sqrt(dim); ``causal``: the last
+    query sees the last key; lengths int32 [batch].  Holds addresses only."""
+    kv = heads if kv_heads is None else kv_heads
+    bias = (heads * q_len * k_len, q_len * k_len, k_len) if bias_strides is None else bias_strides
+    return MfhAttention(batch, heads, kv, q_len, k_len, dim, DTYPE[dtype], 1 if causal else 0,
+                        dim ** -0.5 if scale is None else scale,
+                        _heads(d_q, q_strides, q_len, heads, dim),
+                        _heads(d_k, k_strides, k_len, kv, dim),
+                        _heads(d_v, v_strides, k_len, kv, dim), d_bias, DTYPE[bias_dtype], *bias,
+                        d_q_lengths, d_k_lengths, device)
+
+
+def attention_forward_workspace_bytes(problem) -> int:
+    """Bytes of device memory ``attention_forward_device`` works in (0: none)."""
+    n = ctypes.c_uint64(0)
+    _check(lib().mfh_attention_forward_workspace_bytes(ctypes.addressof(problem),
+                                                       ctypes.byref(n)),
+           "mfh_attention_forward_workspace_bytes")
+    return n.value
+
+
+def attention_forward_device(problem, d_out, out_strides=None, d_lse=None, d_workspace=None,
+                             workspace_bytes=0, stream=None):
+    """out = softmax(scale q k^T + bias) v and each row's log-sum-exp, float32
+    [batch, heads, q_len] (mfh_attention_forward_device)."""
+    p = problem
+    out = _heads(d_out, out_strides, p.q_len, p.heads, p.dim)
+    _check(lib().mfh_attention_forward_device(ctypes.addressof(p), ctypes.addressof(out), d_lse,
+                                              d_workspace, workspace_bytes, stream),
+           "mfh_attention_forward_device")
+
+
+def attention_backward_workspace_bytes(problem) -> int:
+    """Bytes of device memory ``attention_backward_device`` works in."""
+    n = ctypes.c_uint64(0)
+    _check(lib().mfh_attention_backward_workspace_bytes(ctypes.addressof(problem),
+                                                        ctypes.byref(n)),
+           "mfh_attention_backward_workspace_bytes")
+    return n.value
+
+
+def attention_backward_device(problem, d_out, d_lse, d_dout, d_dq=None, d_dk=None, d_dv=None,
+                              d_dbias=None, out_strides=None, dout_strides=None, dq_strides=None,
+                              dk_strides=None, dv_strides=None, d_workspace=None,
+                              workspace_bytes=0, stream=None):
+    """The gradients of ``attention_forward_device`` from dout and what it left,
+    the probabilities formed again (mfh_attention_backward_device).  dbias is
+    laid out as the bias; outputs left None are not written."""
+    p = problem
+    q = lambda d, s: _heads(d, s, p.q_len, p.heads, p.dim)  # noqa: E731
+    k = lambda d, s: _heads(d, s, p.k_len, p.kv_heads, p.dim)  # noqa: E731
+    g = MfhAttentionGrads(q(d_out, out_strides), q(d_dout, dout_strides), d_lse,
+                          q(d_dq, dq_strides), k(d_dk, dk_strides), k(d_dv, dv_strides), d_dbias,
+                          d_workspace, workspace_bytes)
+    _check(lib().mfh_attention_backward_device(ctypes.addressof(p), ctypes.addressof(g), stream),
+           "mfh_attention_backward_device")
+
+
+class AdamWSet:
+    """The weights of a net with their AdamW states, laid out once: a step runs
+    over all of them in one launch.  ``tensors`` is a list of dicts: device
+    addresses ``param``, ``grad``, ``m``, ``v``, with 8-bit states ``m_scale`` and
+    ``v_scale`` (a float32 for each 256 values), optionally ``copy``; ``count``,
+    ``param_dtype``, ``grad_dtype``, ``copy_dtype`` ("f32"), ``lr_scale`` (1) and
+    ``weight_decay`` (0).  ``state_bits`` 32: float32 states; 8: uint8 codes.
+    Making and closing a set wait for the device."""
+
+    def __init__(self, tensors, state_bits=32, device=-1):
+        self._h = None
+        arr = (MfhAdamwTensor * max(1, len(tensors)))()
+        for j, t in enumerate(tensors):
+            t = dict(t)
+            arr[j] = MfhAdamwTensor(
+                t.pop("param"), t.pop("grad"), t.pop("m"), t.pop("v"), t.pop("m_scale", None),
+                t.pop("v_scale", None), t.pop("copy", None), t.pop("count"),
+                DTYPE[t.pop("param_dtype", "f32")], DTYPE[t.pop("grad_dtype", "f32")],
+                DTYPE[t.pop("copy_dtype", "f32")], t.pop("lr_scale", 1.0),
+                t.pop("weight_decay", 0.0))
+            if t:
+                raise ValueError(f"AdamWSet: unknown keys {sorted(t)}")
+        handle = ctypes.c_void_p()
+        _check(lib().mfh_adamw_set_create(arr, len(tensors), state_bits, device,
+                                          ctypes.byref(handle)), "mfh_adamw_set_create")
+        self._h = handle
+
+    def close(self):
+        if self._h:
+            lib().mfh_adamw_set_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def step_device(self, lr, step, beta1=0.9, beta2=0.999, eps=1e-8, grad_scale=1.0, d_lr=None,
+                    d_step=None, d_sumsq=None, max_norm=float("inf"), skip_nonfinite=False,
+                    stochastic=False, seed=0, stream=None):
+        """AdamW step number ``step`` (1 on) over every tensor
+        (mfh_adamw_step_device).  ``d_sumsq``: the float64 sum of the
+        gradients' squares (``GradSet.norm_device``) to clip to ``max_norm`` by;
+        ``d_lr`` float32 and ``d_step`` int64 on the device take the place of lr
+        and step; ``stochastic`` rounds 8-bit states by bits from ``seed``."""
+        a = MfhAdamwStep(lr, beta1, beta2, eps, grad_scale, step, d_lr, d_step, d_sumsq, max_norm,
+                         1 if skip_nonfinite else 0, 1 if stochastic else 0, seed)
+        _check(lib().mfh_adamw_step_device(self._h, ctypes.addressof(a), stream),
+               "mfh_adamw_step_device")
 
 
 class WeightsFile:

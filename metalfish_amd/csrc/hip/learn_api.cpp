@@ -15,6 +15,7 @@
 #include <vector>
 
 #include "../../../include/mfhip.h"
+#include "learn_checks.h"
 #include "learn_ranges.h"
 #include "mfh_kernels.h"
 #include "mfh_status.h"
@@ -27,140 +28,9 @@ struct mfh_grad_set {
   std::vector<mfh::ByteRange> memory;  // of every src and dst
 };
 
+using namespace mfh::checks;
+
 namespace {
-
-using mfh::SetError;
-
-int HipError(const char *fn, const char *what, hipError_t e) {
-  (void)hipGetLastError();
-  return SetError(MFH_ERR_HIP, std::string(fn) + ": " + what + ": " + hipGetErrorString(e));
-}
-
-int Invalid(const char *fn, const char *what) {
-  return SetError(MFH_ERR_INVALID, std::string(fn) + ": " + what);
-}
-
-bool Aligned(const void *p, std::uintptr_t bytes) {
-  return reinterpret_cast<std::uintptr_t>(p) % bytes == 0;
-}
-
-// Makes `device` current for a call and puts the caller's device back.
-class OnDevice {
- public:
-  ~OnDevice() {
-    if (before_ >= 0)
-      (void)hipSetDevice(before_);
-  }
-  hipError_t Set(int device) {
-    int now = 0;
-    hipError_t e = hipGetDevice(&now);
-    if (e != hipSuccess || now == device)
-      return e;
-    e = hipSetDevice(device);
-    if (e == hipSuccess)
-      before_ = now;
-    return e;
-  }
-
- private:
-  int before_ = -1;
-};
-
-// Whether device `dev` is a gfx950, looked up once per device.
-bool IsGfx950(int dev) {
-  constexpr int kMaxDevices = 64;
-  static std::atomic<int> known[kMaxDevices] = {};  // 0 unknown, 1 yes, 2 no
-  if (dev < 0 || dev >= kMaxDevices)
-    return false;
-  int k = known[dev].load(std::memory_order_relaxed);
-  if (k == 0) {
-    hipDeviceProp_t prop;
-    if (hipGetDeviceProperties(&prop, dev) != hipSuccess) {
-      (void)hipGetLastError();
-      return false;
-    }
-    k = std::strncmp(prop.gcnArchName, "gfx950", 6) == 0 ? 1 : 2;
-    known[dev].store(k, std::memory_order_relaxed);
-  }
-  return k == 1;
-}
-
-int NeedDevice(const char *fn, int dev) {
-  static std::atomic<int> count{-1};
-  int n = count.load(std::memory_order_relaxed);
-  if (n < 0) {
-    if (hipGetDeviceCount(&n) != hipSuccess) {
-      (void)hipGetLastError();
-      n = 0;
-    }
-    count.store(n, std::memory_order_relaxed);
-  }
-  if (n <= 0)
-    return SetError(MFH_ERR_NO_DEVICE, std::string(fn) + ": no HIP device available");
-  if (dev >= n)
-    return SetError(MFH_ERR_NO_DEVICE, std::string(fn) + ": device ordinal out of range");
-  return MFH_OK;
-}
-
-// The device of `p`; an error if it is not device memory, or (want >= 0)
-// another device's.
-int PointerDevice(const char *fn, const char *name, const void *p, int want, int *dev) {
-  hipPointerAttribute_t attr;
-  const hipError_t e = hipPointerGetAttributes(&attr, p);
-  if (e != hipSuccess)
-    (void)hipGetLastError();
-  if (e != hipSuccess || (attr.type != hipMemoryTypeDevice && attr.type != hipMemoryTypeManaged))
-    return Invalid(fn, (std::string(name) + " is not device memory").c_str());
-  if (want >= 0 && attr.device != want)
-    return Invalid(fn, (std::string(name) + " is on another device").c_str());
-  if (dev)
-    *dev = attr.device;
-  return MFH_OK;
-}
-
-int StreamDevice(const char *fn, hipStream_t stream, int device) {
-  // The standing streams belong to the device that is current at the launch.
-  if (!stream || stream == hipStreamPerThread || stream == hipStreamLegacy)
-    return MFH_OK;
-  hipDevice_t dev = 0;
-  const hipError_t e = hipStreamGetDevice(stream, &dev);
-  if (e != hipSuccess)
-    return HipError(fn, "stream", e);
-  if (dev != device)
-    return Invalid(fn, "the stream is another device's");
-  return MFH_OK;
-}
-
-struct Named {
-  const char *name;
-  const void *p;
-};
-
-// Device, stream and pointers of a call: sets `on` to the device of the
-// first pointer (or `want`), and checks the rest against it.
-template <size_t N>
-int Enter(const char *fn, int want, const Named (&ptrs)[N], hipStream_t stream, OnDevice *on) {
-  int rc = NeedDevice(fn, want);
-  if (rc != MFH_OK)
-    return rc;
-  int dev = want >= 0 ? want : -1;
-  for (const Named &n : ptrs) {
-    if (!n.p)
-      continue;
-    int d = dev;
-    rc = PointerDevice(fn, n.name, n.p, dev, &d);
-    if (rc != MFH_OK)
-      return rc;
-    dev = d;
-  }
-  if (!IsGfx950(dev))
-    return SetError(MFH_ERR_NO_DEVICE, std::string(fn) + ": the device is not gfx950 (MI355X)");
-  rc = StreamDevice(fn, stream, dev);
-  if (rc != MFH_OK)
-    return rc;
-  const hipError_t e = on->Set(dev);
-  return e == hipSuccess ? MFH_OK : HipError(fn, "hipSetDevice", e);
-}
 
 // An array without gaps.
 mfh::Span Flat(const char *name, const void *p, std::int64_t bytes, bool written) {
@@ -173,19 +43,6 @@ mfh::Span Rows(const char *name, const void *p, const mfh_policy_rows *r, std::i
   const std::int64_t es = mfh::DTypeBytes(r->dtype);
   return {name, p, r->rows, r->vocab * es, stride * es, written, true};
 }
-
-// Refuses a call that writes into another of its arrays.
-template <size_t N> int CheckApart(const char *fn, const mfh::Span (&spans)[N]) {
-  size_t a = 0, b = 0;
-  if (!mfh::FindOverlap(spans, &a, &b))
-    return MFH_OK;
-  return Invalid(fn, (std::string(spans[a].name) + " overlaps " + spans[b].name).c_str());
-}
-
-// No tensor on a card of 288 GB has more.
-constexpr uint64_t kMostElements = uint64_t(1) << 38;
-
-bool Finite(float v) { return std::isfinite(v); }
 
 // Rows by themselves; on success `p` holds them.
 int CheckRows(const char *fn, const mfh_policy_rows *r, mfh::RowLossParams *p) {
@@ -519,7 +376,7 @@ int mfh_grad_set_create(const mfh_grad_tensor *tensors, int n_tensors, int devic
         return HipError(fn, "hipGetDevice", e);
     }
     if (!IsGfx950(dev))
-      return SetError(MFH_ERR_NO_DEVICE, std::string(fn) + ": the device is not gfx950 (MI355X)");
+      return mfh::SetError(MFH_ERR_NO_DEVICE, std::string(fn) + ": the device is not gfx950 (MI355X)");
     OnDevice on;
     hipError_t e = on.Set(dev);
     if (e != hipSuccess)
@@ -552,7 +409,7 @@ int mfh_grad_set_create(const mfh_grad_tensor *tensors, int n_tensors, int devic
       e = hipMalloc(reinterpret_cast<void **>(&set->chunks), bytes);
       if (e != hipSuccess) {
         (void)hipGetLastError();
-        return SetError(MFH_ERR_OUT_OF_MEMORY, std::string(fn) + ": chunk list allocation failed");
+        return mfh::SetError(MFH_ERR_OUT_OF_MEMORY, std::string(fn) + ": chunk list allocation failed");
       }
       e = hipMemcpy(set->chunks, chunks.data(), bytes, hipMemcpyHostToDevice);
       if (e != hipSuccess) {
@@ -563,7 +420,7 @@ int mfh_grad_set_create(const mfh_grad_tensor *tensors, int n_tensors, int devic
     *out = set.release();
     return MFH_OK;
   } catch (const std::bad_alloc &) {
-    return SetError(MFH_ERR_OUT_OF_MEMORY, std::string(fn) + ": out of host memory");
+    return mfh::SetError(MFH_ERR_OUT_OF_MEMORY, std::string(fn) + ": out of host memory");
   } catch (const std::exception &e) {
     return Invalid(fn, e.what());
   }

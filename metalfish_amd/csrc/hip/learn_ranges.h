@@ -98,4 +98,78 @@ inline bool Meets(const std::vector<ByteRange> &joined, const void *p, std::uint
   return bytes > 0 && it != joined.end() && it->begin < end;
 }
 
+// An array of up to three dimensions of strided runs of `inner` bytes; strides
+// in bytes, not negative.
+struct Region {
+  struct Dim {
+    std::int64_t n, stride;
+  };
+  const char *name;
+  const void *p;
+  std::int64_t inner;
+  bool written;
+  Dim dims[3];
+};
+inline Region RegionOf(const char *name, const void *p, std::int64_t inner, bool written,
+                       const std::vector<Region::Dim> &dims) {
+  Region r{name, p, inner, written, {{1, 0}, {1, 0}, {1, 0}}};
+  for (size_t i = 0; i < dims.size() && i < 3; ++i)
+    r.dims[i] = dims[i];
+  return r;
+}
+inline bool Empty(const Region &r) {
+  return r.inner <= 0 || r.dims[0].n <= 0 || r.dims[1].n <= 0 || r.dims[2].n <= 0;
+}
+// Bytes from the first to behind the last, of the dimensions whose stride is
+// no multiple of `s` (0: of all).
+inline std::int64_t Reach(const Region &r, std::int64_t s) {
+  std::int64_t n = r.inner;
+  for (const Region::Dim &d : r.dims)
+    if (d.n > 1 && (s == 0 || d.stride % s != 0))
+      n += (d.n - 1) * d.stride;
+  return n;
+}
+
+// Whether each dimension steps over all that the narrower ones reach: then no
+// two runs share a byte.
+inline bool Nested(const Region &r) {
+  Region::Dim d[3] = {r.dims[0], r.dims[1], r.dims[2]};
+  std::sort(d, d + 3, [](const Region::Dim &x, const Region::Dim &y) { return x.stride < y.stride; });
+  std::int64_t reach = r.inner;
+  for (const Region::Dim &x : d)
+    if (x.n > 1) {
+      if (x.stride < reach)
+        return false;
+      reach += (x.n - 1) * x.stride;
+    }
+  return true;
+}
+
+// Whether two arrays share no byte, as far as this can tell: they lie behind
+// one another, or, with respect to one of their strides s, every other stride
+// is a multiple of s or stays inside a part of s that the other array leaves
+// free (columns of one array, say, or heads between heads).
+inline bool Apart(const Region &x, const Region &y) {
+  if (Empty(x) || Empty(y))
+    return true;
+  const std::uintptr_t a = Address(x.p), b = Address(y.p);
+  if (a + static_cast<std::uintptr_t>(Reach(x, 0)) <= b ||
+      b + static_cast<std::uintptr_t>(Reach(y, 0)) <= a)
+    return true;
+  for (const Region *r : {&x, &y})
+    for (const Region::Dim &d : r->dims) {
+      if (d.n <= 1 || d.stride <= 0)
+        continue;
+      const std::int64_t s = d.stride, wide = Reach(x, s), other = Reach(y, s);
+      if (wide > s || other > s)
+        continue;
+      const auto us = static_cast<std::uintptr_t>(s);
+      // From x's run on to y's, round the period.
+      const auto gap = static_cast<std::int64_t>((b % us + us - a % us) % us);
+      if (gap >= wide && gap + other <= s)
+        return true;
+    }
+  return false;
+}
+
 }  // namespace mfh

@@ -574,4 +574,94 @@ hipError_t LaunchGradScale(const GradChunk *chunks, std::int64_t n_chunks,
                            bool past, const double *partials, int n, float max_norm,
                            float *norm, hipStream_t stream, std::string *err);
 
+// ---- Layers of a training step ------------------------------------------
+
+// Layer norm of rows h = residual + alpha x (h = alpha x without a residual):
+// y = (h - mean) rstd gamma + beta.  Strides are in elements.
+struct NormParams {
+  const void *x = nullptr, *residual = nullptr;
+  std::int64_t ldx = 0, ldr = 0;
+  std::int64_t rows = 0;
+  int width = 0, dtype = DT_F32;
+  float alpha = 1.f, eps = 0.f;
+  const float *gamma = nullptr, *beta = nullptr;  // null: 1, 0
+  // Forward: y, mean and rstd (each optional).  Backward: mean and rstd read.
+  void *y = nullptr;
+  std::int64_t ldy = 0;
+  float *mean = nullptr, *rstd = nullptr;
+  // Backward.
+  const void *dy = nullptr;
+  std::int64_t lddy = 0;
+  void *dx = nullptr, *dresidual = nullptr;
+  std::int64_t lddx = 0, lddr = 0;
+  float *dgamma = nullptr, *dbeta = nullptr;
+  float *partials = nullptr;  // NormPartials(rows, width) x 2 x width
+};
+// Workgroups of the backward pass: one row of partial sums of the weights'
+// gradients each.  A function of the shape alone, so the order of the sums is.
+int NormPartials(std::int64_t rows, int width);
+hipError_t LaunchNorm(const NormParams &p, hipStream_t stream, std::string *err);
+hipError_t LaunchNormBackward(const NormParams &p, hipStream_t stream, std::string *err);
+
+// Heads of tokens: element d of head h of token t of line b is at
+// p + b batch + t token + h head + d, in elements.
+struct HeadsView {
+  const void *p = nullptr;
+  std::int64_t batch = 0, token = 0, head = 0;
+};
+
+// Attention with gradients.  The queries of all heads that share a key head
+// are its rows: row r is query r % q_len of head kv_head group + r / q_len.
+struct TrainAttention {
+  int batch = 0, heads = 0, kv_heads = 0, group = 1;
+  int q_len = 0, k_len = 0, dim = 0, dtype = DT_F32;
+  float scale = 1.f;
+  bool causal = false;
+  HeadsView q, k, v, out, dout, dq, dk, dv;
+  const void *bias = nullptr;
+  void *dbias = nullptr;  // laid out as the bias
+  int bias_dtype = DT_F32;
+  std::int64_t bias_batch = 0, bias_head = 0, bias_query = 0;
+  const std::int32_t *q_lengths = nullptr, *k_lengths = nullptr;
+  float *lse = nullptr;  // [batch][heads][q_len]
+  void *workspace = nullptr;
+};
+// Bytes of workspace (0: none).
+std::uint64_t AttentionForwardWorkspace(const TrainAttention &a);
+std::uint64_t AttentionBackwardWorkspace(const TrainAttention &a);
+hipError_t LaunchAttentionForward(const TrainAttention &a, hipStream_t stream, std::string *err);
+hipError_t LaunchAttentionBackward(const TrainAttention &a, hipStream_t stream, std::string *err);
+
+// A part of one weight tensor of an AdamW set, at most kAdamChunk values: a
+// unit of work.  States in 8 bits: a chunk begins on a whole block of
+// kAdamBlock values, with a scale each; first_block is its first block's
+// number in the set.
+constexpr int kAdamBlock = 256;
+constexpr int kAdamChunk = 4096;
+struct AdamChunk {
+  void *param;
+  const void *grad;
+  void *m, *v, *copy;
+  float *m_scale, *v_scale;
+  std::int64_t first_block;
+  std::int32_t count;
+  std::uint8_t param_dtype, grad_dtype, copy_dtype, pad;
+  float lr_scale, weight_decay;
+};
+struct AdamParams {
+  double lr = 0, beta1 = 0, beta2 = 0, eps = 0;
+  double grad_scale = 1;
+  std::int64_t step = 1;
+  const float *d_lr = nullptr;
+  const std::int64_t *d_step = nullptr;
+  const double *sumsq = nullptr;
+  float max_norm = 0.f;
+  bool skip_nonfinite = false, stochastic = false;
+  std::uint64_t seed = 0;
+};
+// Sets above this many bytes are read and written past the caches.
+constexpr std::int64_t kAdamCachedBytes = std::int64_t(64) << 20;
+hipError_t LaunchAdamW(const AdamChunk *chunks, std::int64_t n_chunks, bool eight, bool past,
+                       const AdamParams &p, hipStream_t stream, std::string *err);
+
 }  // namespace mfh
