@@ -1,14 +1,18 @@
-// Attention with gradients: the pieces that its kernels share.
+// Attention with gradients: the kernels, and the pieces that they share.
 //
 // The matrix instruction computes D[16 x 16] = A[16 x 32] B[32 x 16] from eight
 // values a lane of A and of B: lane l holds row (column) l % 16 and eight of the
 // 32 places summed over, and D leaves it with column l % 16, rows 4 (l / 16) ..
 // + 3.  The sum does not care which places a lane holds as long as A and B
-// agree, so two 16 x 16 results, eight values a lane, are one operand of the
-// next product as they lie in registers: scores become probabilities and feed
-// the product with V (or dout, Q, K) without passing through memory.  The other
-// operand then takes its rows 4 (l / 16) .. + 3 of both tiles, column l % 16,
-// from a row-major tile in LDS: two transposing reads of four values.
+// agree, and rows may be taken in any order.  Results of four instructions over
+// the rows RowOf(t, i) of a tile of 64 leave lane l, for one column, with rows
+// 8 (l / 16) .. + 7 and the same 32 further: two operands of eight values for the
+// next product as they lie in registers.  Scores become probabilities and feed
+// the products with V (or dout, Q, K) without passing through memory, and a bias
+// comes in vectors of eight.  The other operand takes those eight rows of one
+// column from a row-major tile in LDS: two transposing reads of four values.
+// Columns are taken in such an order too that a lane ends with consecutive
+// elements of a head.
 //
 // fp32 runs the same code on the 16 x 16 x 4 instruction, eight times.
 #pragma once
@@ -106,24 +110,36 @@ __device__ __forceinline__ void ToRow(typename Mat<DT>::T *p, typename Mat<DT>::
     *reinterpret_cast<typename Mat<DT>::Frag *>(p) = f;
   }
 }
-// Column col0 + lane % 16 of rows row .. row + 3 and row + 16 .. row + 19 of a
-// tile, row = row0 + 4 (lane / 16).
+// The row of a 64-row tile that row i of result t stands for, and the element
+// of a head that row i of result t of a transposed product does.
+__device__ __forceinline__ constexpr int RowOf64(int t, int i) {
+  return 32 * (t >> 1) + 8 * (i >> 2) + 4 * (t & 1) + (i & 3);
+}
+// Eight rows from row0 + 8 (lane / 16) on of a tile, at the element of a head of
+// DP that row lane % 16 of result t of a transposed product stands for, or
+// (DP = 64, t = 0 .. 3, keys) plainly column col0 + lane % 16.
 template <int DT, int LD>
-__device__ __forceinline__ typename Mat<DT>::Frag FromColumns(const typename Mat<DT>::T *tile,
-                                                              int row0, int col0, int lane) {
-  const int fr = lane & 15, row = row0 + 4 * (lane >> 4);
+__device__ __forceinline__ typename Mat<DT>::Frag Columns(const typename Mat<DT>::T *tile, int row0,
+                                                          int quad_step, int col0, int lane) {
+  const int fr = lane & 15, row = row0 + 8 * (lane >> 4);
   if constexpr (DT == DT_F32) {
+    const float *p = tile + row * LD + col0 + quad_step * (fr >> 2) + (fr & 3);
     f32x8 f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      f[j] = tile[(row + j) * LD + col0 + fr];
-      f[4 + j] = tile[(row + 16 + j) * LD + col0 + fr];
-    }
+    for (int j = 0; j < 8; ++j)
+      f[j] = p[j * LD];
     return f;
   } else {
-    const std::uint16_t *p = tile + (row + (fr >> 2)) * LD + col0 + 4 * (fr & 3);
-    return TwoReads<typename Mat<DT>::Frag>(p, p + 16 * LD);
+    const std::uint16_t *p = tile + (row + (fr >> 2)) * LD + col0 + quad_step * (fr & 3);
+    return TwoReads<typename Mat<DT>::Frag>(p, p + 4 * LD);
   }
+}
+// Element (DP / 4) (i / 4) + 4 t + i % 4 of a head: a lane of the result then has
+// the DP / 4 elements from (DP / 4) (lane / 16) on.
+template <int DT, int DP, int LD>
+__device__ __forceinline__ typename Mat<DT>::Frag HeadColumns(const typename Mat<DT>::T *tile,
+                                                              int row0, int t, int lane) {
+  return Columns<DT, LD>(tile, row0, DP / 4, 4 * t, lane);
 }
 
 // Eight values from element d0 of a head's row in memory, zeros behind `dim`.
@@ -173,6 +189,42 @@ __device__ __forceinline__ void ToMemory(Row<DT> row, int d0, int dim, f32x4 v) 
   for (int e = 0; e < 4; ++e)
     if (d0 + e < dim)
       row[d0 + e] = Elem<DT>::Round(v[e]);
+}
+
+// A lane's elements of a head, DP / 4 of them from (DP / 4) (lane / 16) on.
+template <int DT, int DP>
+__device__ __forceinline__ void StoreHead(Row<DT> row, int lane, int dim, const f32x4 *v,
+                                          float scale) {
+  const int d0 = DP / 4 * (lane >> 4);
+  if constexpr (DT == DT_F32) {
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i)
+      ToMemory<DT>(row, d0 + 4 * i, dim, v[i] * scale);
+  } else {
+#pragma unroll
+    for (int i = 0; i < DP / 16; i += 2) {
+      if (d0 + 4 * i + 8 <= dim) {
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          f[e] = v[i + (e >> 2)][e & 3] * scale;
+        StoreVec<DT, false>(row + d0 + 4 * i, Elem<DT>::Pack(f));
+      } else {
+        ToMemory<DT>(row, d0 + 4 * i, dim, v[i] * scale);
+        ToMemory<DT>(row, d0 + 4 * i + 4, dim, v[i + 1] * scale);
+      }
+    }
+  }
+}
+// The same to a row of partial sums.
+template <int DP>
+__device__ __forceinline__ void StorePartial(float *row, int lane, int dim4, const f32x4 *v) {
+#pragma unroll
+  for (int i = 0; i < DP / 16; ++i) {
+    const int d = DP / 4 * (lane >> 4) + 4 * i;
+    if (d < dim4)
+      *reinterpret_cast<f32x4 *>(row + d) = v[i];
+  }
 }
 
 // Sum and maximum over the four lanes that hold one column of a result.
@@ -283,52 +335,71 @@ __device__ __forceinline__ float Bias1(const void *p, int dtype, std::int64_t at
   const std::uint16_t v = ((const MFH_GLOBAL std::uint16_t *)p)[at];
   return dtype == DT_BF16 ? Elem<DT_BF16>::One(v) : Elem<DT_F16>::One(v);
 }
-// Four consecutive values, of which n are in the array.
-__device__ __forceinline__ f32x4 Bias4(const void *p, int dtype, std::int64_t at, int n) {
-  f32x4 f{0.f, 0.f, 0.f, 0.f};
-  if (n >= 4) {
-    if (dtype == DT_F32)
-      return __builtin_bit_cast(f32x4, *(const MFH_GLOBAL u32x4_a4 *)((const MFH_GLOBAL float *)p + at));
-    const u32x2 v = *(const MFH_GLOBAL u32x2_a2 *)((const MFH_GLOBAL std::uint16_t *)p + at);
+// Eight consecutive values, of which n are in the array, as two results have them.
+__device__ __forceinline__ void Bias8(const void *p, int dtype, std::int64_t at, int n, f32x4 *f) {
+  if (n >= 8) {
+    if (dtype == DT_F32) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const auto one = static_cast<std::uint16_t>(v[e >> 1] >> (16 * (e & 1)));
-      f[e] = dtype == DT_BF16 ? Elem<DT_BF16>::One(one) : Elem<DT_F16>::One(one);
+      for (int i = 0; i < 2; ++i)
+        f[i] = __builtin_bit_cast(
+            f32x4, *(const MFH_GLOBAL u32x4_a4 *)((const MFH_GLOBAL float *)p + at + 4 * i));
+      return;
     }
-    return f;
+    const u32x4 v = *(const MFH_GLOBAL u32x4_a2 *)((const MFH_GLOBAL std::uint16_t *)p + at);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      f[e >> 2][e & 3] =
+          dtype == DT_BF16 ? Elem<DT_BF16>::Get(v, e) : Elem<DT_F16>::Get(v, e);
+    return;
   }
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (e < n)
-      f[e] = Bias1(p, dtype, at + e);
-  return f;
+  for (int e = 0; e < 8; ++e)
+    f[e >> 2][e & 3] = e < n ? Bias1(p, dtype, at + e) : 0.f;
 }
-__device__ __forceinline__ void StoreBias4(void *p, int dtype, std::int64_t at, int n, f32x4 f) {
+template <int DT>
+__device__ __forceinline__ void Store8(Row<DT> row, int n, const f32x4 *f) {
+  float v[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    v[e] = f[e >> 2][e & 3];
+  if (n >= 8) {
+    StoreVec<DT, false>(row, Elem<DT>::Pack(v));
+    if constexpr (DT == DT_F32)
+      StoreVec<DT, false>(row + 4, Elem<DT>::Pack(v + 4));
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (e < n)
+      row[e] = Elem<DT>::Round(v[e]);
+}
+__device__ __forceinline__ void StoreBias8(void *p, int dtype, std::int64_t at, int n,
+                                           const f32x4 *f) {
   if (dtype == DT_F32)
-    ToMemory<DT_F32>((Row<DT_F32>)p + at, 0, n, f);
+    Store8<DT_F32>((Row<DT_F32>)p + at, n, f);
   else if (dtype == DT_BF16)
-    ToMemory<DT_BF16>((Row<DT_BF16>)p + at, 0, n, f);
+    Store8<DT_BF16>((Row<DT_BF16>)p + at, n, f);
   else
-    ToMemory<DT_F16>((Row<DT_F16>)p + at, 0, n, f);
+    Store8<DT_F16>((Row<DT_F16>)p + at, n, f);
 }
 
 // kTile rows of a view as a row-major tile in LDS, 256 threads: chunk i of a
-// thread is eight values of row RowOfChunk(i).
+// thread is eight values of row RowIn(i).
 template <int DT, int DP> struct Stage {
   static constexpr int kChunks = kTile * DP / 8 / 256, kAcross = DP / 8;
   typename Mat<DT>::Frag f[kChunks];
-  static __device__ __forceinline__ int RowOf(int i) { return (i * 256 + threadIdx.x) / kAcross; }
+  static __device__ __forceinline__ int RowIn(int i) { return (i * 256 + threadIdx.x) / kAcross; }
   static __device__ __forceinline__ int At(int i) { return (i * 256 + threadIdx.x) % kAcross * 8; }
   __device__ __forceinline__ void Store(typename Mat<DT>::T *tile) const {
 #pragma unroll
     for (int i = 0; i < kChunks; ++i)
-      ToRow<DT>(tile + RowOf(i) * kLd<DT, DP> + At(i), f[i]);
+      ToRow<DT>(tile + RowIn(i) * kLd<DT, DP> + At(i), f[i]);
   }
   // Keys first .. of a line: zeros from `end` on.
   __device__ __forceinline__ void Keys(const HeadsView &v, const Line &l, int first, int dim) {
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
-      const int j = first + RowOf(i);
+      const int j = first + RowIn(i);
       f[i] = typename Mat<DT>::Frag{};
       if (j < l.k_len)
         f[i] = FromMemory<DT>(In<DT>(v, l.b, l.kv, j), At(i), dim);
@@ -338,7 +409,7 @@ template <int DT, int DP> struct Stage {
   __device__ __forceinline__ void Rows(const Args &s, const HeadsView &v, const Line &l, int first) {
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
-      const int r = first + RowOf(i);
+      const int r = first + RowIn(i);
       f[i] = typename Mat<DT>::Frag{};
       if (r < s.rows) {
         const int h = r / s.a.q_len, q = r - h * s.a.q_len;
@@ -349,23 +420,90 @@ template <int DT, int DP> struct Stage {
   }
 };
 
-// Scores of a key tile against the 16 rows of a wave, keys down: lane l has
-// row l % 16 and keys 16 t + 4 (l / 16) + e.
+// Products of a tile of 64 rows in LDS with the 16 columns of a wave, from
+// `init` on: lane l has column l % 16, rows RowOf64.
 template <int DT, int DP>
-__device__ __forceinline__ void Scores(const typename Mat<DT>::T *tile,
-                                       const typename Mat<DT>::Frag *rows, int lane, f32x4 *out) {
+__device__ __forceinline__ void Products(const typename Mat<DT>::T *tile,
+                                         const typename Mat<DT>::Frag *cols, int lane,
+                                         const f32x4 *init, f32x4 *out) {
   const int fr = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
-    out[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    out[t] = init[t];
 #pragma unroll
     for (int c = 0; c < DP / 32; ++c)
-      out[t] = Mat<DT>::Mul(FromRow<DT>(tile + (16 * t + fr) * kLd<DT, DP> + 32 * c + 8 * g),
-                            rows[c], out[t]);
+      out[t] = Mat<DT>::Mul(FromRow<DT>(tile + RowOf64(t, fr) * kLd<DT, DP> + 32 * c + 8 * g),
+                            cols[c], out[t]);
+  }
+}
+__device__ __forceinline__ void Fill(f32x4 *v, int n, float f) {
+#pragma unroll
+  for (int i = 0; i < n; ++i)
+    v[i] = f32x4{f, f, f, f};
+}
+
+// A row of a workgroup's tile as a lane has it.
+struct RowOfWave {
+  int r, h, q, head, last;
+  bool live;
+};
+__device__ __forceinline__ RowOfWave RowFor(const Args &s, const Line &l, int r) {
+  RowOfWave w;
+  w.r = r;
+  w.live = r < s.rows;
+  w.h = w.live ? r / s.a.q_len : 0;
+  w.q = w.live ? r - w.h * s.a.q_len : 0;
+  w.head = l.kv * s.a.group + w.h;
+  w.last = w.live ? l.Last(w.q) : -1;
+  return w;
+}
+template <int DT, int DP>
+__device__ __forceinline__ void LoadRow(const Args &s, const HeadsView &v, const Line &l,
+                                        const RowOfWave &w, int lane, typename Mat<DT>::Frag *f) {
+#pragma unroll
+  for (int c = 0; c < DP / 32; ++c) {
+    f[c] = typename Mat<DT>::Frag{};
+    if (w.last >= 0)
+      f[c] = FromMemory<DT>(In<DT>(v, l.b, w.head, w.q), 32 * c + 8 * (lane >> 4), s.a.dim);
   }
 }
 
-template <int DT, int DP>
+// Scores in units of ln 2 with whatever is not seen at -inf: x holds products,
+// and in the end (x scale + bias) log2 e.  A bias of the type's lowest value
+// would overflow in those units, so it keeps natural ones and the differences
+// are multiplied.
+__device__ __forceinline__ float Units(const TrainAttention &a) { return a.bias ? kLog2e : 1.f; }
+__device__ __forceinline__ void ToScores(const TrainAttention &a, std::int64_t bias_at, int j0,
+                                         int last, f32x4 *x) {
+  if (a.bias) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int j = j0 + 32 * u;
+      f32x4 bias[2];
+      Fill(bias, 2, 0.f);
+      if (j <= last)
+        Bias8(a.bias, a.bias_dtype, bias_at + j, a.k_len - j, bias);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        x[2 * u + (e >> 2)][e & 3] = x[2 * u + (e >> 2)][e & 3] * a.scale + bias[e >> 2][e & 3];
+    }
+  } else {
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+      x[t] *= a.scale * kLog2e;
+  }
+  if (j0 + 39 > last) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (j0 + 32 * (t >> 1) + 4 * (t & 1) + e > last)
+          x[t][e] = -__builtin_inff();
+  }
+}
+
+// ONE: all keys in one tile.
+template <int DT, int DP, bool ONE>
 __global__ __launch_bounds__(256) void ForwardKernel(Args s) {
   using M = Mat<DT>;
   constexpr int LD = kLd<DT, DP>;
@@ -376,90 +514,77 @@ __global__ __launch_bounds__(256) void ForwardKernel(Args s) {
   const TrainAttention &a = s.a;
   const Line l = LineOf(s, part.line);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, g = lane >> 4;
-  const int first = part.tile * kTile, r = first + 16 * wave + fr;
-  const bool live = r < s.rows;
-  const int h = live ? r / a.q_len : 0, q = live ? r - h * a.q_len : 0, head = l.kv * a.group + h;
-  const int last = live ? l.Last(q) : -1;
-  typename M::Frag qf[DP / 32];
-#pragma unroll
-  for (int c = 0; c < DP / 32; ++c) {
-    qf[c] = typename M::Frag{};
-    if (last >= 0)
-      qf[c] = FromMemory<DT>(In<DT>(a.q, l.b, head, q), 32 * c + 8 * g, a.dim);
-  }
-  const std::int64_t bias_at = a.bias ? BiasAt(a, l.b, head, q) : 0;
+  const int first = part.tile * kTile;
+  const RowOfWave w = RowFor(s, l, first + 16 * wave + fr);
   const int seen = KeysSeen(s, l, first);
-  const int per = (s.steps + s.splits - 1) / s.splits;
-  const int begin = part.split * per, end = min(begin + per, (seen + kTile - 1) / kTile);
-  f32x4 acc[DP / 16];
-#pragma unroll
-  for (int i = 0; i < DP / 16; ++i)
-    acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float most = -__builtin_inff(), total = 0.f;
+  const int per = ONE ? 1 : (s.steps + s.splits - 1) / s.splits;
+  const int begin = ONE ? 0 : part.split * per, end = min(begin + per, (seen + kTile - 1) / kTile);
   Stage<DT, DP> kt, vt;
   if (begin < end) {
     kt.Keys(a.k, l, begin * kTile, a.dim);
     vt.Keys(a.v, l, begin * kTile, a.dim);
   }
+  typename M::Frag qf[DP / 32];
+  LoadRow<DT, DP>(s, a.q, l, w, lane, qf);
+  const std::int64_t bias_at = a.bias ? BiasAt(a, l.b, w.head, w.q) : 0;
+  const float units = Units(a);
+  f32x4 acc[DP / 16], zero[4];
+  Fill(acc, DP / 16, 0.f);
+  Fill(zero, 4, 0.f);
+  float most = -__builtin_inff(), total = 0.f;
   for (int step = begin; step < end; ++step) {
     kt.Store(ks);
     vt.Store(vs);
     __syncthreads();
-    if (step + 1 < end) {
+    if (!ONE && step + 1 < end) {
       kt.Keys(a.k, l, (step + 1) * kTile, a.dim);
       vt.Keys(a.v, l, (step + 1) * kTile, a.dim);
     }
     f32x4 x[4];
-    Scores<DT, DP>(ks, qf, lane, x);
-    const int j0 = step * kTile + 4 * g;
+    Products<DT, DP>(ks, qf, lane, zero, x);
+    ToScores(a, bias_at, step * kTile + 8 * g, w.last, x);
     float top = most;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int j = j0 + 16 * t;
-      f32x4 bias{0.f, 0.f, 0.f, 0.f};
-      if (a.bias && j <= last)
-        bias = Bias4(a.bias, a.bias_dtype, bias_at + j, a.k_len - j);
+    for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[t][e] = j + e <= last ? x[t][e] * a.scale + bias[e] : -__builtin_inff();
+      for (int e = 0; e < 4; ++e)
         top = fmaxf(top, x[t][e]);
-      }
-    }
     top = OverRows(top, true);
     const float base = top == -__builtin_inff() ? 0.f : top;
-    const float old = Exp2((most - base) * kLog2e);
+    const float old = Exp2((most - base) * units);
     most = top;
     total *= old;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        x[t][e] = Exp2((x[t][e] - base) * kLog2e);
+        x[t][e] = Exp2((x[t][e] - base) * units);
         total += x[t][e];
       }
+    if constexpr (!ONE) {
 #pragma unroll
-    for (int i = 0; i < DP / 16; ++i)
-      acc[i] *= old;
+      for (int i = 0; i < DP / 16; ++i)
+        acc[i] *= old;
+    }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const typename M::Frag p = M::Pack(x[2 * u], x[2 * u + 1]);
 #pragma unroll
       for (int i = 0; i < DP / 16; ++i)
-        acc[i] = M::Mul(FromColumns<DT, LD>(vs, 32 * u, 16 * i, lane), p, acc[i]);
+        acc[i] = M::Mul(HeadColumns<DT, DP, LD>(vs, 32 * u, i, lane), p, acc[i]);
     }
-    __syncthreads();
+    if constexpr (!ONE)
+      __syncthreads();
   }
   total = OverRows(total, false);
-  if (!live)
+  if (!w.live)
     return;
-  const std::int64_t flat = static_cast<std::int64_t>(part.line) * s.rows + r;
-  if (s.splits > 1) {
+  const std::int64_t flat = static_cast<std::int64_t>(part.line) * s.rows + w.r;
+  // Natural units from here on.
+  most *= a.bias ? 1.f : kLn2;
+  if (!ONE && s.splits > 1) {
     const std::int64_t n = static_cast<std::int64_t>(s.lines) * s.rows;
-    float *o = s.partials + (part.split * n + flat) * s.dim4;
-#pragma unroll
-    for (int i = 0; i < DP / 16; ++i)
-      if (16 * i + 4 * g < s.dim4)
-        *reinterpret_cast<f32x4 *>(o + 16 * i + 4 * g) = acc[i];
+    StorePartial<DP>(s.partials + (part.split * n + flat) * s.dim4, lane, s.dim4, acc);
     if (g == 0) {
       float *st = s.partials + s.splits * n * s.dim4 + (part.split * n + flat) * 2;
       st[0] = most;
@@ -467,58 +592,87 @@ __global__ __launch_bounds__(256) void ForwardKernel(Args s) {
     }
     return;
   }
-  const float inv = total == 0.f ? 0.f : 1.f / total;
-  const Row<DT> out = Out<DT>(a.out, l.b, head, q);
-#pragma unroll
-  for (int i = 0; i < DP / 16; ++i)
-    ToMemory<DT>(out, 16 * i + 4 * g, a.dim, acc[i] * inv);
+  StoreHead<DT, DP>(Out<DT>(a.out, l.b, w.head, w.q), lane, a.dim, acc,
+                    total == 0.f ? 0.f : 1.f / total);
   if (a.lse && g == 0)
     a.lse[flat] = total == 0.f ? -__builtin_inff() : most + kLn2 * __builtin_amdgcn_logf(total);
 }
 
-// Joins the splits of a forward pass: one wave a row.
+constexpr int kMostSplits = 256;
+
+// Joins the splits of a forward pass: a workgroup a row.  All lanes form the
+// splits' weights, then groups of lanes that hold a row add every so many splits.
 template <int DT>
 __global__ __launch_bounds__(256) void JoinForwardKernel(Args s) {
-  const std::int64_t n = static_cast<std::int64_t>(s.lines) * s.rows;
-  const std::int64_t flat = static_cast<std::int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (flat >= n)
-    return;
-  const int lane = threadIdx.x & 63;
+  __shared__ float red[2][4], weight[kMostSplits];
+  __shared__ f32x4 sums[256];
+  const std::int64_t n = static_cast<std::int64_t>(s.lines) * s.rows, flat = blockIdx.x;
   const float *st = s.partials + s.splits * n * s.dim4;
-  float most = -__builtin_inff();
-  for (int k = 0; k < s.splits; ++k)
-    most = fmaxf(most, st[(k * n + flat) * 2]);
+  const int k = threadIdx.x;
+  float most = -__builtin_inff(), total = 0.f;
+  if (k < s.splits) {
+    most = st[(k * n + flat) * 2];
+    total = st[(k * n + flat) * 2 + 1];
+  }
+  const float mine = most;
+  most = WaveMax(most);
+  if ((k & 63) == 0)
+    red[0][k >> 6] = most;
+  __syncthreads();
+  most = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
   const float base = most == -__builtin_inff() ? 0.f : most;
-  float total = 0.f;
-  f32x2 o{0.f, 0.f};
-  for (int k = 0; k < s.splits; ++k) {
-    const float w = Exp2((st[(k * n + flat) * 2] - base) * kLog2e);
-    total += w * st[(k * n + flat) * 2 + 1];
-    if (2 * lane < s.dim4) {
-      const f32x2 v = *reinterpret_cast<const f32x2 *>(s.partials + (k * n + flat) * s.dim4 + 2 * lane);
-      // An empty split of a row holds zeros.
-      o[0] += w * v[0];
-      o[1] += w * v[1];
+  const float w = Exp2((mine - base) * kLog2e);
+  weight[k] = w;
+  total = WaveSum(total * w);
+  if ((k & 63) == 0)
+    red[1][k >> 6] = total;
+  __syncthreads();
+  total = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+  const int across = s.dim4 / 4, groups = 256 / across, group = k / across, c = k % across;
+  f32x4 o{0.f, 0.f, 0.f, 0.f};
+  if (group < groups) {
+#pragma unroll 4
+    for (int i = group; i < s.splits; i += groups) {
+      // A split that saw nothing holds zeros.
+      const f32x4 v = *reinterpret_cast<const f32x4 *>(s.partials + (i * n + flat) * s.dim4 + 4 * c);
+      o += v * weight[i];
     }
   }
-  const float inv = total == 0.f ? 0.f : 1.f / total;
+  sums[k] = o;
+  __syncthreads();
+  if (k >= across)
+    return;
+  for (int i = 1; i < groups; ++i)
+    o += sums[i * across + k];
   const int line = static_cast<int>(flat / s.rows), r = static_cast<int>(flat % s.rows);
   const int b = line / s.a.kv_heads, head = line % s.a.kv_heads * s.a.group + r / s.a.q_len;
-  const Row<DT> out = Out<DT>(s.a.out, b, head, r % s.a.q_len);
-#pragma unroll
-  for (int e = 0; e < 2; ++e)
-    if (2 * lane + e < s.a.dim)
-      out[2 * lane + e] = Elem<DT>::Round(o[e] * inv);
-  if (s.a.lse && lane == 0)
+  ToMemory<DT>(Out<DT>(s.a.out, b, head, r % s.a.q_len), 4 * k, s.a.dim,
+               o * (total == 0.f ? 0.f : 1.f / total));
+  if (s.a.lse && k == 0)
     s.a.lse[flat] = total == 0.f ? -__builtin_inff() : most + kLn2 * __builtin_amdgcn_logf(total);
 }
 
-// A row's log-sum-exp as what its scores are taken off: +inf where it sees
-// nothing, so that every probability is 0.
-__device__ __forceinline__ float Lse(float v) { return v == -__builtin_inff() ? __builtin_inff() : v; }
+// A row's log-sum-exp in the units of its scores, as what they are taken off:
+// +inf where it sees nothing, so that every probability is 0.
+__device__ __forceinline__ float Lse(const TrainAttention &a, float v) {
+  if (v == -__builtin_inff())
+    return __builtin_inff();
+  return a.bias ? v : v * kLog2e;
+}
+// delta = dout . out of a row, over the four lanes that share it.
+template <int DT, int DP>
+__device__ __forceinline__ float Delta(const typename Mat<DT>::Frag *out,
+                                       const typename Mat<DT>::Frag *dout) {
+  float delta = 0.f;
+#pragma unroll
+  for (int c = 0; c < DP / 32; ++c)
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      delta += Mat<DT>::Get(out[c], e) * Mat<DT>::Get(dout[c], e);
+  return OverRows(delta, false);
+}
 
-// delta = dout . out of each row, then dq (and dbias) of a tile of rows over the
-// keys.
+// delta of each row, then dq (and dbias) of a tile of rows over the keys.
 template <int DT, int DP>
 __global__ __launch_bounds__(256) void BackwardRowsKernel(Args s) {
   using M = Mat<DT>;
@@ -530,46 +684,38 @@ __global__ __launch_bounds__(256) void BackwardRowsKernel(Args s) {
   const TrainAttention &a = s.a;
   const Line l = LineOf(s, part.line);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, g = lane >> 4;
-  const int first = part.tile * kTile, r = first + 16 * wave + fr;
-  const bool live = r < s.rows;
-  const int h = live ? r / a.q_len : 0, q = live ? r - h * a.q_len : 0, head = l.kv * a.group + h;
-  const int last = live ? l.Last(q) : -1;
-  const std::int64_t flat = static_cast<std::int64_t>(part.line) * s.rows + r;
-  typename M::Frag qf[DP / 32], df[DP / 32];
-  float delta = 0.f;
-#pragma unroll
-  for (int c = 0; c < DP / 32; ++c) {
-    qf[c] = df[c] = typename M::Frag{};
-    if (last >= 0) {
-      const int d0 = 32 * c + 8 * g;
-      qf[c] = FromMemory<DT>(In<DT>(a.q, l.b, head, q), d0, a.dim);
-      df[c] = FromMemory<DT>(In<DT>(a.dout, l.b, head, q), d0, a.dim);
-      const typename M::Frag o = FromMemory<DT>(In<DT>(a.out, l.b, head, q), d0, a.dim);
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        delta += M::Get(o, e) * M::Get(df[c], e);
-    }
-  }
-  delta = OverRows(delta, false);
-  if (live && g == 0 && part.split == 0)
-    s.delta[flat] = delta;
-  if (!a.dq.p && !a.dbias)
-    return;
-  const float lse = last >= 0 ? Lse(a.lse[flat]) : __builtin_inff();
-  const std::int64_t bias_at = a.bias ? BiasAt(a, l.b, head, q) : 0;
+  const int first = part.tile * kTile;
+  const RowOfWave w = RowFor(s, l, first + 16 * wave + fr);
+  const std::int64_t flat = static_cast<std::int64_t>(part.line) * s.rows + w.r;
   // Every element of the bias's gradient is written, so no key is left out.
   const int seen = a.dbias ? a.k_len : KeysSeen(s, l, first);
   const int per = (s.steps + s.splits - 1) / s.splits;
   const int begin = part.split * per, end = min(begin + per, (seen + kTile - 1) / kTile);
-  f32x4 acc[DP / 16];
-#pragma unroll
-  for (int i = 0; i < DP / 16; ++i)
-    acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const bool any = begin < end && (a.dq.p || a.dbias);
   Stage<DT, DP> kt, vt;
-  if (begin < end) {
+  if (any) {
     kt.Keys(a.k, l, begin * kTile, a.dim);
     vt.Keys(a.v, l, begin * kTile, a.dim);
   }
+  typename M::Frag qf[DP / 32], df[DP / 32];
+  LoadRow<DT, DP>(s, a.q, l, w, lane, qf);
+  LoadRow<DT, DP>(s, a.dout, l, w, lane, df);
+  float delta;
+  {
+    typename M::Frag of[DP / 32];
+    LoadRow<DT, DP>(s, a.out, l, w, lane, of);
+    delta = Delta<DT, DP>(of, df);
+  }
+  if (w.live && g == 0 && part.split == 0)
+    s.delta[flat] = delta;
+  if (!a.dq.p && !a.dbias)
+    return;
+  const float lse = w.last >= 0 ? Lse(a, a.lse[flat]) : __builtin_inff(), units = Units(a);
+  const std::int64_t bias_at = a.bias ? BiasAt(a, l.b, w.head, w.q) : 0;
+  f32x4 acc[DP / 16], zero[4], minus[4];
+  Fill(acc, DP / 16, 0.f);
+  Fill(zero, 4, 0.f);
+  Fill(minus, 4, -delta);
   for (int step = begin; step < end; ++step) {
     kt.Store(ks);
     vt.Store(vs);
@@ -579,47 +725,48 @@ __global__ __launch_bounds__(256) void BackwardRowsKernel(Args s) {
       vt.Keys(a.v, l, (step + 1) * kTile, a.dim);
     }
     f32x4 x[4], dp[4];
-    Scores<DT, DP>(ks, qf, lane, x);
-    Scores<DT, DP>(vs, df, lane, dp);
+    Products<DT, DP>(ks, qf, lane, zero, x);
+    Products<DT, DP>(vs, df, lane, minus, dp);
+    const int j0 = step * kTile + 8 * g;
+    ToScores(a, bias_at, j0, w.last, x);
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int j = step * kTile + 4 * g + 16 * t;
-      f32x4 bias{0.f, 0.f, 0.f, 0.f};
-      if (a.bias && j <= last)
-        bias = Bias4(a.bias, a.bias_dtype, bias_at + j, a.k_len - j);
+    for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float p = Exp2((x[t][e] * a.scale + bias[e] - lse) * kLog2e);
-        x[t][e] = j + e <= last ? p * (dp[t][e] - delta) : 0.f;
+        const float p = Exp2((x[t][e] - lse) * units);
+        x[t][e] = p * dp[t][e];
       }
-      if (a.dbias && live && j < a.k_len)
-        StoreBias4(a.dbias, a.bias_dtype, bias_at + j, a.k_len - j, x[t]);
+    if (a.dbias && w.live) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if (j0 + 32 * u < a.k_len)
+          StoreBias8(a.dbias, a.bias_dtype, bias_at + j0 + 32 * u, a.k_len - j0 - 32 * u, x + 2 * u);
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const typename M::Frag ds = M::Pack(x[2 * u], x[2 * u + 1]);
 #pragma unroll
       for (int i = 0; i < DP / 16; ++i)
-        acc[i] = M::Mul(FromColumns<DT, LD>(ks, 32 * u, 16 * i, lane), ds, acc[i]);
+        acc[i] = M::Mul(HeadColumns<DT, DP, LD>(ks, 32 * u, i, lane), ds, acc[i]);
     }
     __syncthreads();
   }
-  if (!live || !a.dq.p)
+  if (!w.live || !a.dq.p)
     return;
   if (s.splits > 1) {
     const std::int64_t n = static_cast<std::int64_t>(s.lines) * s.rows;
-    float *o = s.partials + (part.split * n + flat) * s.dim4;
-#pragma unroll
-    for (int i = 0; i < DP / 16; ++i)
-      if (16 * i + 4 * g < s.dim4)
-        *reinterpret_cast<f32x4 *>(o + 16 * i + 4 * g) = acc[i];
+    StorePartial<DP>(s.partials + (part.split * n + flat) * s.dim4, lane, s.dim4, acc);
     return;
   }
-  const Row<DT> out = Out<DT>(a.dq, l.b, head, q);
-#pragma unroll
-  for (int i = 0; i < DP / 16; ++i)
-    ToMemory<DT>(out, 16 * i + 4 * g, a.dim, acc[i] * a.scale);
+  StoreHead<DT, DP>(Out<DT>(a.dq, l.b, w.head, w.q), lane, a.dim, acc, a.scale);
 }
+
+// What a workgroup of the keys' kernel holds of its 64 rows, next to the tiles.
+struct RowInfo {
+  __attribute__((aligned(16))) int last[kTile];
+  __attribute__((aligned(16))) float lse[kTile], delta[kTile];
+  std::int64_t bias[kTile];
+};
 
 // dk and dv of a tile of keys over the rows that share them; each wave has 16
 // keys and holds them, and rows go through LDS.
@@ -628,9 +775,7 @@ __global__ __launch_bounds__(256) void BackwardKeysKernel(Args s) {
   using M = Mat<DT>;
   constexpr int LD = kLd<DT, DP>;
   __shared__ __attribute__((aligned(16))) typename M::T qs[kTile * LD], dos[kTile * LD];
-  __shared__ __attribute__((aligned(16))) int lasts[kTile];
-  __shared__ __attribute__((aligned(16))) float lses[kTile], deltas[kTile];
-  __shared__ std::int64_t biases[kTile];
+  __shared__ RowInfo info;
   Part part;
   if (!PartOf(s, &part))
     return;
@@ -647,55 +792,72 @@ __global__ __launch_bounds__(256) void BackwardKeysKernel(Args s) {
       vf[c] = FromMemory<DT>(In<DT>(a.v, l.b, l.kv, j), 32 * c + 8 * g, a.dim);
     }
   }
-  f32x4 dk[DP / 16], dv[DP / 16];
-#pragma unroll
-  for (int i = 0; i < DP / 16; ++i)
-    dk[i] = dv[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const float units = Units(a), scale = a.bias ? a.scale : a.scale * kLog2e;
+  f32x4 dk[DP / 16], dv[DP / 16], zero[4];
+  Fill(dk, DP / 16, 0.f);
+  Fill(dv, DP / 16, 0.f);
+  Fill(zero, 4, 0.f);
   const int per = (s.steps + s.splits - 1) / s.splits;
-  const int begin = part.split * per, end = min(begin + per, s.steps);
-  for (int step = begin; step < end; ++step) {
-    const int first = step * kTile;
-    if (KeysSeen(s, l, first) <= key0)
-      continue;  // the same in the whole workgroup
-    Stage<DT, DP> qt, dt;
-    qt.Rows(s, a.q, l, first);
-    dt.Rows(s, a.dout, l, first);
+  const int end = min((part.split + 1) * per, s.steps);
+  // The next tile from `step` on of which a row sees one of these keys.
+  const auto next = [&](int step) {
+    while (step < end && KeysSeen(s, l, step * kTile) <= key0)
+      ++step;
+    return step;
+  };
+  Stage<DT, DP> qt, dt;
+  int my_last = -1;
+  float my_lse = 0.f, my_delta = 0.f;
+  std::int64_t my_bias = 0;
+  const auto load = [&](int step) {
+    qt.Rows(s, a.q, l, step * kTile);
+    dt.Rows(s, a.dout, l, step * kTile);
+    if (threadIdx.x < kTile) {
+      const RowOfWave w = RowFor(s, l, step * kTile + threadIdx.x);
+      const std::int64_t flat = static_cast<std::int64_t>(part.line) * s.rows + w.r;
+      my_last = w.last;
+      my_lse = __builtin_inff();
+      my_delta = 0.f;
+      if (w.last >= 0) {
+        my_lse = Lse(a, a.lse[flat]);
+        my_delta = s.delta[flat];
+      }
+      my_bias = a.bias ? BiasAt(a, l.b, w.head, w.q) : 0;
+    }
+  };
+  int step = next(part.split * per);
+  if (step < end)
+    load(step);
+  while (step < end) {
     qt.Store(qs);
     dt.Store(dos);
     if (threadIdx.x < kTile) {
-      const int r = first + threadIdx.x;
-      int last = -1;
-      float lse = __builtin_inff(), delta = 0.f;
-      if (r < s.rows) {
-        const int h = r / a.q_len, q = r - h * a.q_len;
-        const std::int64_t flat = static_cast<std::int64_t>(part.line) * s.rows + r;
-        last = l.Last(q);
-        if (last >= 0) {
-          lse = Lse(a.lse[flat]);
-          delta = s.delta[flat];
-        }
-        biases[threadIdx.x] = a.bias ? BiasAt(a, l.b, l.kv * a.group + h, q) : 0;
-      }
-      lasts[threadIdx.x] = last;
-      lses[threadIdx.x] = lse;
-      deltas[threadIdx.x] = delta;
+      info.last[threadIdx.x] = my_last;
+      info.lse[threadIdx.x] = my_lse;
+      info.delta[threadIdx.x] = my_delta;
+      info.bias[threadIdx.x] = my_bias;
     }
     __syncthreads();
-    f32x4 x[4], dp[4];
-    Scores<DT, DP>(qs, kf, lane, x);
-    Scores<DT, DP>(dos, vf, lane, dp);
+    step = next(step + 1);
+    if (step < end)
+      load(step);
+    f32x4 x[4], dp[4], minus[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+      minus[t] = -*reinterpret_cast<const f32x4 *>(info.delta + RowOf64(t, 4 * g));
+    Products<DT, DP>(qs, kf, lane, zero, x);
+    Products<DT, DP>(dos, vf, lane, minus, dp);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      const int at = 16 * t + 4 * g;
-      const f32x4 lse = *reinterpret_cast<const f32x4 *>(lses + at),
-                  delta = *reinterpret_cast<const f32x4 *>(deltas + at);
+      const int at = RowOf64(t, 4 * g);
+      const f32x4 lse = *reinterpret_cast<const f32x4 *>(info.lse + at);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const bool sees = j <= lasts[at + e];
-        const float bias = a.bias && sees ? Bias1(a.bias, a.bias_dtype, biases[at + e] + j) : 0.f;
-        const float p = Exp2((x[t][e] * a.scale + bias - lse[e]) * kLog2e);
+        const bool sees = j <= info.last[at + e];
+        const float bias = a.bias && sees ? Bias1(a.bias, a.bias_dtype, info.bias[at + e] + j) : 0.f;
+        const float p = Exp2((x[t][e] * scale + bias - lse[e]) * units);
         x[t][e] = sees ? p : 0.f;
-        dp[t][e] = sees ? p * (dp[t][e] - delta[e]) : 0.f;
+        dp[t][e] *= x[t][e];
       }
     }
 #pragma unroll
@@ -704,8 +866,8 @@ __global__ __launch_bounds__(256) void BackwardKeysKernel(Args s) {
                              ds = M::Pack(dp[2 * u], dp[2 * u + 1]);
 #pragma unroll
       for (int i = 0; i < DP / 16; ++i) {
-        dv[i] = M::Mul(FromColumns<DT, LD>(dos, 32 * u, 16 * i, lane), p, dv[i]);
-        dk[i] = M::Mul(FromColumns<DT, LD>(qs, 32 * u, 16 * i, lane), ds, dk[i]);
+        dv[i] = M::Mul(HeadColumns<DT, DP, LD>(dos, 32 * u, i, lane), p, dv[i]);
+        dk[i] = M::Mul(HeadColumns<DT, DP, LD>(qs, 32 * u, i, lane), ds, dk[i]);
       }
     }
     __syncthreads();
@@ -716,39 +878,31 @@ __global__ __launch_bounds__(256) void BackwardKeysKernel(Args s) {
     const std::int64_t n = static_cast<std::int64_t>(s.lines) * a.k_len;
     const std::int64_t flat = static_cast<std::int64_t>(part.line) * a.k_len + j;
     float *o = s.partials + (2 * part.split * n + flat) * s.dim4;
-#pragma unroll
-    for (int i = 0; i < DP / 16; ++i)
-      if (16 * i + 4 * g < s.dim4) {
-        *reinterpret_cast<f32x4 *>(o + 16 * i + 4 * g) = dk[i];
-        *reinterpret_cast<f32x4 *>(o + n * s.dim4 + 16 * i + 4 * g) = dv[i];
-      }
+    StorePartial<DP>(o, lane, s.dim4, dk);
+    StorePartial<DP>(o + n * s.dim4, lane, s.dim4, dv);
     return;
   }
-#pragma unroll
-  for (int i = 0; i < DP / 16; ++i) {
-    if (a.dk.p)
-      ToMemory<DT>(Out<DT>(a.dk, l.b, l.kv, j), 16 * i + 4 * g, a.dim, dk[i] * a.scale);
-    if (a.dv.p)
-      ToMemory<DT>(Out<DT>(a.dv, l.b, l.kv, j), 16 * i + 4 * g, a.dim, dv[i]);
-  }
+  if (a.dk.p)
+    StoreHead<DT, DP>(Out<DT>(a.dk, l.b, l.kv, j), lane, a.dim, dk, a.scale);
+  if (a.dv.p)
+    StoreHead<DT, DP>(Out<DT>(a.dv, l.b, l.kv, j), lane, a.dim, dv, 1.f);
 }
 
-// Adds up the splits of dq (KEYS false) or of dk and dv: one wave a row.
+// Adds up the splits of dq (KEYS false) or of dk and dv: four elements a thread.
 template <int DT, bool KEYS>
 __global__ __launch_bounds__(256) void JoinBackwardKernel(Args s) {
-  const int per = KEYS ? s.a.k_len : s.rows;
+  const int per = KEYS ? s.a.k_len : s.rows, across = s.dim4 / 4;
   const std::int64_t n = static_cast<std::int64_t>(s.lines) * per;
   const std::int64_t all = KEYS ? 2 * n : n;
-  const std::int64_t at = static_cast<std::int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (at >= all || 2 * lane >= s.dim4)
+  const std::int64_t id = static_cast<std::int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const std::int64_t at = id / across;
+  const int c = static_cast<int>(id % across);
+  if (at >= all)
     return;
-  f32x2 o{0.f, 0.f};
-  for (int k = 0; k < s.splits; ++k) {
-    const f32x2 v = *reinterpret_cast<const f32x2 *>(s.partials + (k * all + at) * s.dim4 + 2 * lane);
-    o[0] += v[0];
-    o[1] += v[1];
-  }
+  f32x4 o{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int k = 0; k < s.splits; ++k)
+    o += *reinterpret_cast<const f32x4 *>(s.partials + (k * all + at) * s.dim4 + 4 * c);
   const bool second = KEYS && at >= n;
   const std::int64_t flat = second ? at - n : at;
   const int line = static_cast<int>(flat / per), r = static_cast<int>(flat % per);
@@ -762,11 +916,116 @@ __global__ __launch_bounds__(256) void JoinBackwardKernel(Args s) {
   } else {
     out = Out<DT>(s.a.dq, b, kv * s.a.group + r / s.a.q_len, r % s.a.q_len);
   }
-  const float scale = second ? 1.f : s.a.scale;
+  ToMemory<DT>(out, 4 * c, s.a.dim, o * (second ? 1.f : s.a.scale));
+}
+
+// The whole backward pass of a head of up to 64 queries and 64 keys, none of
+// them shared: one workgroup, each input read once.  A wave has 16 queries while
+// scores, probabilities, dS and dq are formed, and 16 keys for dk and dv; P and dS
+// change hands through LDS.
+template <int DT, int DP>
+__global__ __launch_bounds__(256) void SquareBackwardKernel(Args s) {
+  using M = Mat<DT>;
+  constexpr int LD = kLd<DT, DP>, LP = kLd<DT, kTile>;
+  __shared__ __attribute__((aligned(16))) typename M::T ks[kTile * LD], vs[kTile * LD],
+      qs[kTile * LD], dos[kTile * LD];
+  __shared__ __attribute__((aligned(16))) typename M::T ps[kTile * LP], dss[kTile * LP];
+  Part part;
+  if (!PartOf(s, &part))
+    return;
+  const TrainAttention &a = s.a;
+  const Line l = LineOf(s, part.line);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, g = lane >> 4;
+  const int mine = 16 * wave + fr;  // a query, and later a key
+  const RowOfWave w = RowFor(s, l, mine);
+  const std::int64_t flat = static_cast<std::int64_t>(part.line) * s.rows + mine;
+  typename M::Frag qf[DP / 32], df[DP / 32];
+  {
+    typename M::Frag kf[DP / 32], vf[DP / 32];
 #pragma unroll
-  for (int e = 0; e < 2; ++e)
-    if (2 * lane + e < s.a.dim)
-      out[2 * lane + e] = Elem<DT>::Round(o[e] * scale);
+    for (int c = 0; c < DP / 32; ++c) {
+      kf[c] = vf[c] = typename M::Frag{};
+      if (mine < l.k_len) {
+        kf[c] = FromMemory<DT>(In<DT>(a.k, l.b, l.kv, mine), 32 * c + 8 * g, a.dim);
+        vf[c] = FromMemory<DT>(In<DT>(a.v, l.b, l.kv, mine), 32 * c + 8 * g, a.dim);
+      }
+    }
+    LoadRow<DT, DP>(s, a.q, l, w, lane, qf);
+    LoadRow<DT, DP>(s, a.dout, l, w, lane, df);
+#pragma unroll
+    for (int c = 0; c < DP / 32; ++c) {
+      const int at = mine * LD + 32 * c + 8 * g;
+      ToRow<DT>(ks + at, kf[c]);
+      ToRow<DT>(vs + at, vf[c]);
+      ToRow<DT>(qs + at, qf[c]);
+      ToRow<DT>(dos + at, df[c]);
+    }
+  }
+  float delta;
+  {
+    typename M::Frag of[DP / 32];
+    LoadRow<DT, DP>(s, a.out, l, w, lane, of);
+    delta = Delta<DT, DP>(of, df);
+  }
+  if (w.live && g == 0)
+    s.delta[flat] = delta;
+  const float lse = w.last >= 0 ? Lse(a, a.lse[flat]) : __builtin_inff(), units = Units(a);
+  const std::int64_t bias_at = a.bias ? BiasAt(a, l.b, w.head, w.q) : 0;
+  __syncthreads();
+  f32x4 x[4], dp[4], zero[4], minus[4];
+  Fill(zero, 4, 0.f);
+  Fill(minus, 4, -delta);
+  Products<DT, DP>(ks, qf, lane, zero, x);
+  Products<DT, DP>(vs, df, lane, minus, dp);
+  ToScores(a, bias_at, 8 * g, w.last, x);
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      x[t][e] = Exp2((x[t][e] - lse) * units);
+      dp[t][e] *= x[t][e];
+    }
+  if (a.dbias && w.live) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      if (8 * g + 32 * u < a.k_len)
+        StoreBias8(a.dbias, a.bias_dtype, bias_at + 8 * g + 32 * u, a.k_len - 8 * g - 32 * u,
+                   dp + 2 * u);
+  }
+  f32x4 acc[DP / 16], more[DP / 16];
+  Fill(acc, DP / 16, 0.f);
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const typename M::Frag ds = M::Pack(dp[2 * u], dp[2 * u + 1]);
+    ToRow<DT>(ps + mine * LP + 32 * u + 8 * g, M::Pack(x[2 * u], x[2 * u + 1]));
+    ToRow<DT>(dss + mine * LP + 32 * u + 8 * g, ds);
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i)
+      acc[i] = M::Mul(HeadColumns<DT, DP, LD>(ks, 32 * u, i, lane), ds, acc[i]);
+  }
+  if (w.live && a.dq.p)
+    StoreHead<DT, DP>(Out<DT>(a.dq, l.b, w.head, w.q), lane, a.dim, acc, a.scale);
+  if (!a.dk.p && !a.dv.p)
+    return;
+  __syncthreads();
+  Fill(acc, DP / 16, 0.f);
+  Fill(more, DP / 16, 0.f);
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const typename M::Frag p = Columns<DT, LP>(ps, 32 * u, 4, 16 * wave, lane),
+                           ds = Columns<DT, LP>(dss, 32 * u, 4, 16 * wave, lane);
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) {
+      acc[i] = M::Mul(HeadColumns<DT, DP, LD>(qs, 32 * u, i, lane), ds, acc[i]);
+      more[i] = M::Mul(HeadColumns<DT, DP, LD>(dos, 32 * u, i, lane), p, more[i]);
+    }
+  }
+  if (mine >= a.k_len)
+    return;
+  if (a.dk.p)
+    StoreHead<DT, DP>(Out<DT>(a.dk, l.b, l.kv, mine), lane, a.dim, acc, a.scale);
+  if (a.dv.p)
+    StoreHead<DT, DP>(Out<DT>(a.dv, l.b, l.kv, mine), lane, a.dim, more, 1.f);
 }
 
 // The gradient of a bias that lines or heads share: a workgroup has 64 queries
@@ -783,38 +1042,31 @@ __global__ __launch_bounds__(256) void BiasGradKernel(Args s, int plane_heads) {
   const int b0 = a.bias_batch ? b_plane : 0, b1 = a.bias_batch ? b_plane + 1 : a.batch;
   const int h0 = a.bias_head ? h_plane : 0, h1 = a.bias_head ? h_plane + 1 : a.heads;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, g = lane >> 4;
-  const int q = qt * kTile + 16 * wave + fr;
+  const int q = qt * kTile + 16 * wave + fr, j0 = kt * kTile + 8 * g;
   const bool live = q < a.q_len;
   const std::int64_t bias_at = BiasAt(a, b_plane, h_plane, live ? q : 0);
   f32x4 acc[4], bias[4];
+  Fill(acc, 4, 0.f);
+  Fill(bias, 4, 0.f);
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const int j = kt * kTile + 16 * t + 4 * g;
-    acc[t] = bias[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (live && j < a.k_len)
-      bias[t] = Bias4(a.bias, a.bias_dtype, bias_at + j, a.k_len - j);
-  }
+  for (int u = 0; u < 2; ++u)
+    if (live && j0 + 32 * u < a.k_len)
+      Bias8(a.bias, a.bias_dtype, bias_at + j0 + 32 * u, a.k_len - j0 - 32 * u, bias + 2 * u);
   for (int b = b0; b < b1; ++b)
     for (int head = h0; head < h1; ++head) {
       const int kv = head / a.group;
       const Line l = LineOf(s, b * a.kv_heads + kv);
-      const int last = live ? l.Last(q) : -1;
+      RowOfWave w{0, 0, q, head, live ? l.Last(q) : -1, live};
       const std::int64_t flat = (static_cast<std::int64_t>(b) * a.heads + head) * a.q_len + q;
       typename M::Frag qf[DP / 32], df[DP / 32];
-#pragma unroll
-      for (int c = 0; c < DP / 32; ++c) {
-        qf[c] = df[c] = typename M::Frag{};
-        if (last >= 0) {
-          qf[c] = FromMemory<DT>(In<DT>(a.q, b, head, q), 32 * c + 8 * g, a.dim);
-          df[c] = FromMemory<DT>(In<DT>(a.dout, b, head, q), 32 * c + 8 * g, a.dim);
-        }
-      }
-      const float lse = last >= 0 ? Lse(a.lse[flat]) : __builtin_inff();
-      const float delta = last >= 0 ? s.delta[flat] : 0.f;
+      LoadRow<DT, DP>(s, a.q, l, w, lane, qf);
+      LoadRow<DT, DP>(s, a.dout, l, w, lane, df);
+      const float lse = w.last >= 0 ? Lse(a, a.lse[flat]) : __builtin_inff();
+      const float delta = w.last >= 0 ? s.delta[flat] : 0.f;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        f32x4 x{0.f, 0.f, 0.f, 0.f}, dp{0.f, 0.f, 0.f, 0.f};
-        const int key = kt * kTile + 16 * t + fr, j = kt * kTile + 16 * t + 4 * g;
+        f32x4 x{0.f, 0.f, 0.f, 0.f}, dp{-delta, -delta, -delta, -delta};
+        const int key = kt * kTile + RowOf64(t, fr), j = kt * kTile + RowOf64(t, 4 * g);
 #pragma unroll
         for (int c = 0; c < DP / 32; ++c) {
           typename M::Frag kf{}, vf{};
@@ -828,23 +1080,21 @@ __global__ __launch_bounds__(256) void BiasGradKernel(Args s, int plane_heads) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float p = Exp2((x[e] * a.scale + bias[t][e] - lse) * kLog2e);
-          acc[t][e] += j + e <= last ? p * (dp[e] - delta) : 0.f;
+          acc[t][e] += j + e <= w.last ? p * dp[e] : 0.f;
         }
       }
     }
   if (!live)
     return;
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const int j = kt * kTile + 16 * t + 4 * g;
-    if (j < a.k_len)
-      StoreBias4(a.dbias, a.bias_dtype, bias_at + j, a.k_len - j, acc[t]);
-  }
+  for (int u = 0; u < 2; ++u)
+    if (j0 + 32 * u < a.k_len)
+      StoreBias8(a.dbias, a.bias_dtype, bias_at + j0 + 32 * u, a.k_len - j0 - 32 * u, acc + 2 * u);
 }
 
 // Workgroups that fill the card twice; a split loops over two tiles at least.
 inline int SplitsOf(std::int64_t groups, int steps) {
-  const std::int64_t want = 512 / std::max<std::int64_t>(groups, 1);
+  const std::int64_t want = std::min<std::int64_t>(512 / std::max<std::int64_t>(groups, 1), kMostSplits);
   return static_cast<int>(std::max<std::int64_t>(1, std::min<std::int64_t>(want, steps / 2)));
 }
 inline int Tiles(int n) { return (n + kTile - 1) / kTile; }
@@ -894,18 +1144,19 @@ template <class K> hipError_t Run(K kernel, Args s, hipStream_t stream) {
   }
   return e;
 }
-// Four rows a workgroup; splits have few.
-template <class K> hipError_t RunJoin(K kernel, const Args &s, std::int64_t n, hipStream_t stream) {
-  if (n == 0)
+// Splits have few rows.
+template <class K> hipError_t RunJoin(K kernel, const Args &s, std::int64_t groups, hipStream_t stream) {
+  if (groups == 0)
     return hipSuccess;
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((n + 3) / 4)), dim3(256), 0, stream, s);
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(groups)), dim3(256), 0, stream, s);
   return hipGetLastError();
 }
 
 template <int DT, int DP> hipError_t Forward(const TrainAttention &a, hipStream_t stream) {
   Args s = ArgsOf(a, false);
   s.partials = static_cast<float *>(a.workspace);
-  hipError_t e = Run(ForwardKernel<DT, DP>, s, stream);
+  hipError_t e = s.steps <= 1 ? Run(ForwardKernel<DT, DP, true>, s, stream)
+                              : Run(ForwardKernel<DT, DP, false>, s, stream);
   if (e == hipSuccess && s.splits > 1)
     e = RunJoin(JoinForwardKernel<DT>, s, static_cast<std::int64_t>(s.lines) * s.rows, stream);
   return e;
@@ -918,18 +1169,28 @@ template <int DT, int DP> hipError_t Backward(const TrainAttention &a, hipStream
   const bool shared = SharedBias(a);
   if (shared)
     s.a.dbias = nullptr;
-  hipError_t e = Run(BackwardRowsKernel<DT, DP>, s, stream);
+  constexpr bool kSquare = DP == 32 || (DP == 64 && DT != DT_F32);  // tiles fit in 64 KB
+  const bool square = kSquare && a.group == 1 && a.q_len <= kTile && a.k_len <= kTile && a.q_len > 0 &&
+                      a.k_len > 0;
+  const auto joins = [&](std::int64_t rows) { return (rows * (s.dim4 / 4) + 255) / 256; };
+  hipError_t e = hipSuccess;
+  if constexpr (kSquare) {
+    if (square)
+      e = Run(SquareBackwardKernel<DT, DP>, s, stream);
+  }
+  if (!square)
+    e = Run(BackwardRowsKernel<DT, DP>, s, stream);
   if (e == hipSuccess && s.splits > 1 && a.dq.p)
-    e = RunJoin(JoinBackwardKernel<DT, false>, s, static_cast<std::int64_t>(s.lines) * s.rows,
+    e = RunJoin(JoinBackwardKernel<DT, false>, s, joins(static_cast<std::int64_t>(s.lines) * s.rows),
                 stream);
-  if (e == hipSuccess && (a.dk.p || a.dv.p)) {
+  if (e == hipSuccess && (a.dk.p || a.dv.p) && !square) {
     Args k = ArgsOf(a, true);
     k.delta = s.delta;
     k.partials = s.partials;
     e = Run(BackwardKeysKernel<DT, DP>, k, stream);
     if (e == hipSuccess && k.splits > 1)
-      e = RunJoin(JoinBackwardKernel<DT, true>, k, 2 * static_cast<std::int64_t>(k.lines) * a.k_len,
-                  stream);
+      e = RunJoin(JoinBackwardKernel<DT, true>, k,
+                  joins(2 * static_cast<std::int64_t>(k.lines) * a.k_len), stream);
   }
   if (e == hipSuccess && shared) {
     s.a.dbias = a.dbias;
