@@ -504,8 +504,9 @@ int mfh_layer_norm_backward_device(const mfh_norm_rows *rows, const mfh_norm_gra
                                    void *stream);
 
 /* Heads of tokens in device memory: element d of head h of token t of line b
- * is p[b * batch + t * token + h * head + d]; strides in elements, >= 0.  An
- * array that is written has no two elements in one place. */
+ * is p[b * batch + t * token + h * head + d]; strides in elements, >= 0, of
+ * tokens below 2^32.  An array that is written has no two elements in one
+ * place. */
 typedef struct {
   void *p;
   int64_t batch, token, head;
@@ -527,7 +528,7 @@ typedef struct {
 typedef struct {
   int32_t batch, heads, kv_heads; /* >= 1; batch >= 0 */
   int32_t q_len, k_len;           /* >= 0; q_len heads / kv_heads, k_len <= 2^30 */
-  int32_t dim;                    /* 1 .. 128 */
+  int32_t dim;                    /* a multiple of 8, 8 .. 128 */
   int32_t dtype;                  /* MFH_DTYPE_*: of q, k, v, out and their gradients */
   int32_t causal;                 /* 0 or 1 */
   float scale;                    /* finite */

@@ -135,6 +135,8 @@ int CheckHeads(const char *fn, const char *name, const mfh_attention *a, const m
     if (n[i] > 1)
       reach += (n[i] - 1) * stride[i];
   }
+  if (n[1] > 1 && stride[1] > INT64_C(0xFFFFFFFF))
+    return bad("strides of tokens must be below 2^32");
   if (reach > kMostBytes / es)
     return bad("strides must be >= 0 and the array addressable");
   if (n[0] == 0 || n[1] == 0)
@@ -162,8 +164,8 @@ int CheckAttention(const char *fn, const mfh_attention *a, std::vector<mfh::Regi
   const std::int64_t group = a->heads / a->kv_heads;
   if (a->q_len * group > (1 << 30) || static_cast<std::int64_t>(a->batch) * a->heads > (1 << 30))
     return Invalid(fn, "q_len * heads / kv_heads and batch * heads must be at most 2^30");
-  if (a->dim < 1 || a->dim > 128)
-    return Invalid(fn, "dim must be 1 .. 128");
+  if (a->dim < 8 || a->dim > 128 || a->dim % 8 != 0)
+    return Invalid(fn, "dim must be a multiple of 8, 8 .. 128");
   if (!KnownType(a->dtype) || (a->d_bias && !KnownType(a->bias_dtype)))
     return Invalid(fn, "unknown dtype");
   if (a->causal != 0 && a->causal != 1)
@@ -184,6 +186,7 @@ int CheckAttention(const char *fn, const mfh_attention *a, std::vector<mfh::Regi
   t->dtype = a->dtype;
   t->scale = a->scale;
   t->causal = a->causal != 0;
+  t->bias = a->d_bias;
   t->q_lengths = a->d_q_lengths;
   t->k_lengths = a->d_k_lengths;
   int rc = CheckHeads(fn, "q", a, a->q, a->heads, a->q_len, false, regions, &t->q);
@@ -458,7 +461,6 @@ int mfh_attention_forward_device(const mfh_attention *a, const mfh_heads *out, f
     rc = Enter(fn, a->device, ptrs, st, &on);
     if (rc != MFH_OK)
       return rc;
-    t.bias = a->d_bias;
     t.bias_dtype = a->bias_dtype;
     t.bias_batch = a->bias_batch;
     t.bias_head = a->bias_head;
@@ -559,7 +561,6 @@ int mfh_attention_backward_device(const mfh_attention *a, const mfh_attention_gr
     rc = Enter(fn, a->device, ptrs, st, &on);
     if (rc != MFH_OK)
       return rc;
-    t.bias = a->d_bias;
     t.bias_dtype = a->bias_dtype;
     t.bias_batch = a->bias_batch;
     t.bias_head = a->bias_head;

@@ -142,53 +142,38 @@ __device__ __forceinline__ typename Mat<DT>::Frag HeadColumns(const typename Mat
   return Columns<DT, LD>(tile, row0, DP / 4, 4 * t, lane);
 }
 
-// Eight values from element d0 of a head's row in memory, zeros behind `dim`.
+// Eight values of a head's row in memory.
 template <int DT>
-__device__ __forceinline__ typename Mat<DT>::Frag FromMemory(ConstRow<DT> row, int d0, int dim) {
-  using Frag = typename Mat<DT>::Frag;
-  if (d0 + 8 <= dim) {
-    if constexpr (DT == DT_F32) {
-      const u32x4 a = *(const MFH_GLOBAL u32x4_a4 *)(row + d0),
-                  b = *(const MFH_GLOBAL u32x4_a4 *)(row + d0 + 4);
-      return __builtin_bit_cast(Frag, (__attribute__((ext_vector_type(8))) unsigned int){
-                                          a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
-    } else {
-      return __builtin_bit_cast(Frag, LoadVec<DT, false>(row + d0));
-    }
+__device__ __forceinline__ typename Mat<DT>::Frag FromMemory(ConstRow<DT> p) {
+  if constexpr (DT == DT_F32) {
+    const f32x4 a = __builtin_bit_cast(f32x4, LoadVec<DT, false>(p)),
+                b = __builtin_bit_cast(f32x4, LoadVec<DT, false>(p + 4));
+    return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+  } else {
+    return __builtin_bit_cast(typename Mat<DT>::Frag, LoadVec<DT, false>(p));
   }
-  Frag f{};
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (d0 + e < dim) {
-      if constexpr (DT == DT_F32)
-        f[e] = __uint_as_float(row[d0 + e]);
-      else
-        f[e] = __builtin_bit_cast(typename Mat<DT>::E, row[d0 + e]);
-    }
-  return f;
 }
 
-
-// Stores four consecutive values from element d0 of a row.
+// Stores four consecutive values, with eight: the next four too.
 template <int DT>
-__device__ __forceinline__ void ToMemory(Row<DT> row, int d0, int dim, f32x4 v) {
-  if (d0 + 4 <= dim) {
-    if constexpr (DT == DT_F32) {
-      *(MFH_GLOBAL u32x4_a4 *)(row + d0) = __builtin_bit_cast(u32x4, v);
-    } else {
-      u32x2 p;
+__device__ __forceinline__ void ToMemory(Row<DT> p, f32x4 v) {
+  if constexpr (DT == DT_F32) {
+    StoreVec<DT, false>(p, __builtin_bit_cast(u32x4, v));
+  } else {
+    u32x2 o;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        p[i] = Elem<DT>::Round(v[2 * i]) |
-               static_cast<std::uint32_t>(Elem<DT>::Round(v[2 * i + 1])) << 16;
-      *(MFH_GLOBAL u32x2_a2 *)(row + d0) = p;
-    }
-    return;
+    for (int i = 0; i < 2; ++i)
+      o[i] = Elem<DT>::Round(v[2 * i]) |
+             static_cast<std::uint32_t>(Elem<DT>::Round(v[2 * i + 1])) << 16;
+    *(MFH_GLOBAL u32x2_a2 *)p = o;
   }
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (d0 + e < dim)
-      row[d0 + e] = Elem<DT>::Round(v[e]);
+}
+template <int DT>
+__device__ __forceinline__ void ToMemory(Row<DT> p, f32x4 v, f32x4 w) {
+  const float f[8] = {v[0], v[1], v[2], v[3], w[0], w[1], w[2], w[3]};
+  StoreVec<DT, false>(p, Elem<DT>::Pack(f));
+  if constexpr (DT == DT_F32)
+    StoreVec<DT, false>(p + 4, Elem<DT>::Pack(f + 4));
 }
 
 // A lane's elements of a head, DP / 4 of them from (DP / 4) (lane / 16) on.
@@ -196,33 +181,18 @@ template <int DT, int DP>
 __device__ __forceinline__ void StoreHead(Row<DT> row, int lane, int dim, const f32x4 *v,
                                           float scale) {
   const int d0 = DP / 4 * (lane >> 4);
-  if constexpr (DT == DT_F32) {
 #pragma unroll
-    for (int i = 0; i < DP / 16; ++i)
-      ToMemory<DT>(row, d0 + 4 * i, dim, v[i] * scale);
-  } else {
-#pragma unroll
-    for (int i = 0; i < DP / 16; i += 2) {
-      if (d0 + 4 * i + 8 <= dim) {
-        float f[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          f[e] = v[i + (e >> 2)][e & 3] * scale;
-        StoreVec<DT, false>(row + d0 + 4 * i, Elem<DT>::Pack(f));
-      } else {
-        ToMemory<DT>(row, d0 + 4 * i, dim, v[i] * scale);
-        ToMemory<DT>(row, d0 + 4 * i + 4, dim, v[i + 1] * scale);
-      }
-    }
-  }
+  for (int i = 0; i < DP / 16; i += 2)
+    if (d0 + 4 * i < dim)
+      ToMemory<DT>(row + d0 + 4 * i, v[i] * scale, v[i + 1] * scale);
 }
 // The same to a row of partial sums.
 template <int DP>
-__device__ __forceinline__ void StorePartial(float *row, int lane, int dim4, const f32x4 *v) {
+__device__ __forceinline__ void StorePartial(float *row, int lane, int dim, const f32x4 *v) {
 #pragma unroll
   for (int i = 0; i < DP / 16; ++i) {
     const int d = DP / 4 * (lane >> 4) + 4 * i;
-    if (d < dim4)
+    if (d < dim)
       *reinterpret_cast<f32x4 *>(row + d) = v[i];
   }
 }
@@ -247,28 +217,45 @@ struct Args {
   int tiles = 0;   // of the axis that workgroups share
   int steps = 0;   // tiles of the axis that they loop over
   int splits = 1;  // of that axis
-  int dim4 = 0;    // dim rounded up to whole groups of four: a partial row
-  std::int64_t work = 0;            // lines * tiles * splits
-  std::int64_t first = 0, end = 0;  // the parts of one launch
+  int wide = 1;    // 16-column sets of a wave: a tile has 64 times as many
+  int line0 = 0, lines_now = 0, tile0 = 0;  // the part of one launch
+  bool spread = false;
+  int down = 0;    // tiles from the last to the first, in so many interleaved runs
   float *partials = nullptr;
   float *delta = nullptr;  // [lines][rows]
 };
 
+__device__ __forceinline__ int Uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 // Which part a workgroup does.  Workgroups go round the eight dies by their
-// number; parts of one line stay on one, whose cache then holds its keys.
+// number.  Without splits blockIdx.x is the line and y the tile; with many lines
+// (spread) x is a multiple of eight, so that the parts of one line share a die's
+// cache and neighbouring heads, which share memory lines, do too; where the last
+// tiles have most to do (causal rows), they come first.  With splits (few lines)
+// each die takes an eighth of them in the order of memory: 3 queries over 20011 keys,
+// four lines, 10.9 us; one line after another along x, 18.4.
 struct Part {
   int line, tile, split;
 };
-__device__ __forceinline__ bool PartOf(const Args &a, Part *p) {
-  const std::int64_t per = (a.end - a.first + 7) / 8;
-  const std::int64_t w = a.first + (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if (w >= a.end)
-    return false;
-  const std::int64_t t = w / a.splits;
-  p->split = static_cast<int>(w % a.splits);
-  p->line = static_cast<int>(t / a.tiles);
-  p->tile = static_cast<int>(t % a.tiles);
-  return true;
+__device__ __forceinline__ bool PartOf(const Args &s, Part *p) {
+  const int x = blockIdx.x, per = static_cast<int>(gridDim.x >> 3);
+  const int at = s.spread ? (x & 7) * per + (x >> 3) : x;
+  if (s.splits > 1) {
+    const int t = at / s.splits;
+    p->split = at - t * s.splits;
+    p->line = t / s.tiles;
+    p->tile = t - p->line * s.tiles;
+    return p->line < s.lines;
+  }
+  int tile = s.tile0 + static_cast<int>(blockIdx.y);
+  if (s.down) {
+    const int each = (s.tiles + s.down - 1) / s.down;
+    tile = tile % s.down * each + (each - 1 - tile / s.down);
+  }
+  p->line = s.line0 + at;
+  p->tile = tile;
+  p->split = 0;
+  return at < s.lines_now && tile < s.tiles;
 }
 
 __device__ __forceinline__ int LengthOf(const std::int32_t *lengths, int b, int most) {
@@ -290,31 +277,46 @@ struct Line {
 };
 __device__ __forceinline__ Line LineOf(const Args &s, int line) {
   Line l;
-  l.b = line / s.a.kv_heads;
-  l.kv = line % s.a.kv_heads;
-  l.q_len = LengthOf(s.a.q_lengths, l.b, s.a.q_len);
-  l.k_len = LengthOf(s.a.k_lengths, l.b, s.a.k_len);
+  l.b = s.a.kv_heads == 1 ? line : line / s.a.kv_heads;
+  l.kv = line - l.b * s.a.kv_heads;
+  l.q_len = Uniform(LengthOf(s.a.q_lengths, l.b, s.a.q_len));
+  l.k_len = Uniform(LengthOf(s.a.k_lengths, l.b, s.a.k_len));
   l.causal = s.a.causal;
   return l;
 }
-// One more than the last key that any of rows first .. first + kTile - 1 sees.
-__device__ __forceinline__ int KeysSeen(const Args &s, const Line &l, int first) {
-  const int last = min(first + kTile, s.rows) - 1;
-  const int h0 = first / s.a.q_len, h1 = last / s.a.q_len;
+// `count` rows of a line from `first` on: the head and query of the first, and
+// whether all are that head's.
+struct Span64 {
+  int h, q;
+  bool same;
+};
+__device__ __forceinline__ Span64 SpanOf(const Args &s, int first, int count) {
+  if (s.a.group == 1)
+    return {0, first, true};
+  const int h = first / s.a.q_len, q = first - h * s.a.q_len;
+  return {h, q, q + count <= s.a.q_len};
+}
+// One more than the last key that any of them sees.
+__device__ __forceinline__ int KeysSeen(const Line &l, const Span64 &t, int count) {
   int q = l.q_len - 1;
-  if (h0 == h1) {
-    if (first - h0 * s.a.q_len >= l.q_len)
+  if (t.same) {
+    if (t.q >= l.q_len)
       return 0;
-    q = min(q, last - h0 * s.a.q_len);
+    q = min(q, t.q + count - 1);
   }
   return q < 0 ? 0 : max(0, l.Last(q) + 1);
 }
 
-// Address of a row of a view: row r of a line.
+// A token's offset: strides of tokens are below 2^32.
+__device__ __forceinline__ std::uint64_t Tokens(const HeadsView &v, int token) {
+  return static_cast<std::uint64_t>(static_cast<std::uint32_t>(token)) *
+         static_cast<std::uint32_t>(v.token);
+}
 template <int DT, class P>
 __device__ __forceinline__ P RowAt(const HeadsView &v, int b, int head, int token) {
-  return (P)v.p + (static_cast<std::int64_t>(b) * v.batch + static_cast<std::int64_t>(token) * v.token +
-                   static_cast<std::int64_t>(head) * v.head);
+  return (P)v.p +
+         (static_cast<std::int64_t>(b) * v.batch + static_cast<std::int64_t>(head) * v.head) +
+         Tokens(v, token);
 }
 template <int DT>
 __device__ __forceinline__ ConstRow<DT> In(const HeadsView &v, int b, int head, int token) {
@@ -329,58 +331,62 @@ __device__ __forceinline__ std::int64_t BiasAt(const TrainAttention &a, int b, i
   return static_cast<std::int64_t>(b) * a.bias_batch + static_cast<std::int64_t>(head) * a.bias_head +
          static_cast<std::int64_t>(q) * a.bias_query;
 }
-__device__ __forceinline__ float Bias1(const void *p, int dtype, std::int64_t at) {
-  if (dtype == DT_F32)
-    return ((const MFH_GLOBAL float *)p)[at];
-  const std::uint16_t v = ((const MFH_GLOBAL std::uint16_t *)p)[at];
+__device__ __forceinline__ float OfHalf(int dtype, std::uint16_t v) {
   return dtype == DT_BF16 ? Elem<DT_BF16>::One(v) : Elem<DT_F16>::One(v);
 }
-// Eight consecutive values, of which n are in the array, as two results have them.
-__device__ __forceinline__ void Bias8(const void *p, int dtype, std::int64_t at, int n, f32x4 *f) {
-  if (n >= 8) {
-    if (dtype == DT_F32) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        f[i] = __builtin_bit_cast(
-            f32x4, *(const MFH_GLOBAL u32x4_a4 *)((const MFH_GLOBAL float *)p + at + 4 * i));
+// How a bias is read: not at all, in vectors of eight (rows of a multiple of
+// eight keys), or value by value.
+enum : int { kNoBias, kVectors, kValues };
+// Eight consecutive values from key j on (any of the row's where there are less).
+template <int BIAS>
+__device__ __forceinline__ void Bias8(const TrainAttention &a, std::int64_t row, int j, f32x4 *f) {
+  if constexpr (BIAS == kVectors) {
+    row += min(j, a.k_len - 8);
+    if (a.bias_dtype == DT_F32) {
+      const auto *p = (ConstRow<DT_F32>)a.bias + row;
+      f[0] = __builtin_bit_cast(f32x4, LoadVec<DT_F32, false>(p));
+      f[1] = __builtin_bit_cast(f32x4, LoadVec<DT_F32, false>(p + 4));
       return;
     }
-    const u32x4 v = *(const MFH_GLOBAL u32x4_a2 *)((const MFH_GLOBAL std::uint16_t *)p + at);
+    const u32x4 v = LoadVec<DT_BF16, false>((ConstRow<DT_BF16>)a.bias + row);
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       f[e >> 2][e & 3] =
-          dtype == DT_BF16 ? Elem<DT_BF16>::Get(v, e) : Elem<DT_F16>::Get(v, e);
-    return;
+          a.bias_dtype == DT_BF16 ? Elem<DT_BF16>::Get(v, e) : Elem<DT_F16>::Get(v, e);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const std::int64_t at = row + min(j + e, a.k_len - 1);
+      f[e >> 2][e & 3] = a.bias_dtype == DT_F32
+                             ? ((const MFH_GLOBAL float *)a.bias)[at]
+                             : OfHalf(a.bias_dtype, ((const MFH_GLOBAL std::uint16_t *)a.bias)[at]);
+    }
   }
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    f[e >> 2][e & 3] = e < n ? Bias1(p, dtype, at + e) : 0.f;
 }
-template <int DT>
-__device__ __forceinline__ void Store8(Row<DT> row, int n, const f32x4 *f) {
-  float v[8];
+template <int BIAS, int DT>
+__device__ __forceinline__ void Store8(Row<DT> p, int n, const f32x4 *f) {
+  if constexpr (BIAS == kVectors) {
+    ToMemory<DT>(p, f[0], f[1]);
+  } else {
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    v[e] = f[e >> 2][e & 3];
-  if (n >= 8) {
-    StoreVec<DT, false>(row, Elem<DT>::Pack(v));
-    if constexpr (DT == DT_F32)
-      StoreVec<DT, false>(row + 4, Elem<DT>::Pack(v + 4));
-    return;
+    for (int e = 0; e < 8; ++e)
+      if (e < n)
+        p[e] = Elem<DT>::Round(f[e >> 2][e & 3]);
   }
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (e < n)
-      row[e] = Elem<DT>::Round(v[e]);
 }
-__device__ __forceinline__ void StoreBias8(void *p, int dtype, std::int64_t at, int n,
+// The gradient of as many as there are.
+template <int BIAS>
+__device__ __forceinline__ void StoreBias8(const TrainAttention &a, std::int64_t row, int j,
                                            const f32x4 *f) {
-  if (dtype == DT_F32)
-    Store8<DT_F32>((Row<DT_F32>)p + at, n, f);
-  else if (dtype == DT_BF16)
-    Store8<DT_BF16>((Row<DT_BF16>)p + at, n, f);
+  const int n = a.k_len - j;
+  if (n <= 0)
+    return;
+  if (a.bias_dtype == DT_F32)
+    Store8<BIAS, DT_F32>((Row<DT_F32>)a.dbias + row + j, n, f);
+  else if (a.bias_dtype == DT_BF16)
+    Store8<BIAS, DT_BF16>((Row<DT_BF16>)a.dbias + row + j, n, f);
   else
-    Store8<DT_F16>((Row<DT_F16>)p + at, n, f);
+    Store8<BIAS, DT_F16>((Row<DT_F16>)a.dbias + row + j, n, f);
 }
 
 // kTile rows of a view as a row-major tile in LDS, 256 threads: chunk i of a
@@ -395,46 +401,52 @@ template <int DT, int DP> struct Stage {
     for (int i = 0; i < kChunks; ++i)
       ToRow<DT>(tile + RowIn(i) * kLd<DT, DP> + At(i), f[i]);
   }
-  // Keys first .. of a line: zeros from `end` on.
+  // Keys first .. of a line: zeros from its end on.
   __device__ __forceinline__ void Keys(const HeadsView &v, const Line &l, int first, int dim) {
+    const ConstRow<DT> base = In<DT>(v, l.b, l.kv, 0);
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
       const int j = first + RowIn(i);
       f[i] = typename Mat<DT>::Frag{};
-      if (j < l.k_len)
-        f[i] = FromMemory<DT>(In<DT>(v, l.b, l.kv, j), At(i), dim);
+      if (j < l.k_len && At(i) < dim)
+        f[i] = FromMemory<DT>(base + Tokens(v, j) + At(i));
     }
   }
   // Rows first .. of a line: zeros where a row sees nothing.
-  __device__ __forceinline__ void Rows(const Args &s, const HeadsView &v, const Line &l, int first) {
+  __device__ __forceinline__ void Rows(const Args &s, const HeadsView &v, const Line &l,
+                                       const Span64 &t, int first) {
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
-      const int r = first + RowIn(i);
+      int h = t.h, q = t.q + RowIn(i);
       f[i] = typename Mat<DT>::Frag{};
-      if (r < s.rows) {
-        const int h = r / s.a.q_len, q = r - h * s.a.q_len;
-        if (l.Last(q) >= 0)
-          f[i] = FromMemory<DT>(In<DT>(v, l.b, l.kv * s.a.group + h, q), At(i), s.a.dim);
+      if (!t.same) {
+        const int r = first + RowIn(i);
+        h = r / s.a.q_len;
+        q = h < s.a.group ? r - h * s.a.q_len : s.a.q_len;
       }
+      if (l.Last(q) >= 0 && At(i) < s.a.dim)
+        f[i] = FromMemory<DT>(In<DT>(v, l.b, l.kv * s.a.group + h, q) + At(i));
     }
   }
 };
 
-// Products of a tile of 64 rows in LDS with the 16 columns of a wave, from
-// `init` on: lane l has column l % 16, rows RowOf64.
-template <int DT, int DP>
+// Products of a tile of 64 rows in LDS with N times 16 columns of a wave, added
+// to `out`: lane l has column l % 16 of each, rows RowOf64.
+template <int DT, int DP, int N>
 __device__ __forceinline__ void Products(const typename Mat<DT>::T *tile,
-                                         const typename Mat<DT>::Frag *cols, int lane,
-                                         const f32x4 *init, f32x4 *out) {
+                                         const typename Mat<DT>::Frag (*cols)[DP / 32], int lane,
+                                         f32x4 (*out)[4]) {
   const int fr = lane & 15, g = lane >> 4;
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    out[t] = init[t];
+  for (int t = 0; t < 4; ++t)
 #pragma unroll
-    for (int c = 0; c < DP / 32; ++c)
-      out[t] = Mat<DT>::Mul(FromRow<DT>(tile + RowOf64(t, fr) * kLd<DT, DP> + 32 * c + 8 * g),
-                            cols[c], out[t]);
-  }
+    for (int c = 0; c < DP / 32; ++c) {
+      const typename Mat<DT>::Frag f =
+          FromRow<DT>(tile + RowOf64(t, fr) * kLd<DT, DP> + 32 * c + 8 * g);
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        out[n][t] = Mat<DT>::Mul(f, cols[n][c], out[n][t]);
+    }
 }
 __device__ __forceinline__ void Fill(f32x4 *v, int n, float f) {
 #pragma unroll
@@ -444,16 +456,20 @@ __device__ __forceinline__ void Fill(f32x4 *v, int n, float f) {
 
 // A row of a workgroup's tile as a lane has it.
 struct RowOfWave {
-  int r, h, q, head, last;
+  int r, q, head, last;
   bool live;
 };
 __device__ __forceinline__ RowOfWave RowFor(const Args &s, const Line &l, int r) {
   RowOfWave w;
   w.r = r;
   w.live = r < s.rows;
-  w.h = w.live ? r / s.a.q_len : 0;
-  w.q = w.live ? r - w.h * s.a.q_len : 0;
-  w.head = l.kv * s.a.group + w.h;
+  int h = 0;
+  w.q = w.live ? r : 0;
+  if (s.a.group > 1) {
+    h = w.live ? r / s.a.q_len : 0;
+    w.q = w.live ? r - h * s.a.q_len : 0;
+  }
+  w.head = l.kv * s.a.group + h;
   w.last = w.live ? l.Last(w.q) : -1;
   return w;
 }
@@ -461,36 +477,56 @@ template <int DT, int DP>
 __device__ __forceinline__ void LoadRow(const Args &s, const HeadsView &v, const Line &l,
                                         const RowOfWave &w, int lane, typename Mat<DT>::Frag *f) {
 #pragma unroll
-  for (int c = 0; c < DP / 32; ++c) {
+  for (int c = 0; c < DP / 32; ++c)
     f[c] = typename Mat<DT>::Frag{};
-    if (w.last >= 0)
-      f[c] = FromMemory<DT>(In<DT>(v, l.b, w.head, w.q), 32 * c + 8 * (lane >> 4), s.a.dim);
-  }
+  if (w.last < 0)
+    return;
+  const int d0 = 8 * (lane >> 4);
+  const ConstRow<DT> row = In<DT>(v, l.b, s.a.group == 1 ? l.kv : w.head, w.q) + d0;
+#pragma unroll
+  for (int c = 0; c < DP / 32; ++c)
+    if (32 * c + d0 < s.a.dim)
+      f[c] = FromMemory<DT>(row + 32 * c);
+}
+// The same of a key.
+template <int DT, int DP>
+__device__ __forceinline__ void LoadKey(const Args &s, const HeadsView &v, const Line &l, int j,
+                                        int lane, typename Mat<DT>::Frag *f) {
+#pragma unroll
+  for (int c = 0; c < DP / 32; ++c)
+    f[c] = typename Mat<DT>::Frag{};
+  if (j >= l.k_len)
+    return;
+  const int d0 = 8 * (lane >> 4);
+  const ConstRow<DT> row = In<DT>(v, l.b, l.kv, j) + d0;
+#pragma unroll
+  for (int c = 0; c < DP / 32; ++c)
+    if (32 * c + d0 < s.a.dim)
+      f[c] = FromMemory<DT>(row + 32 * c);
 }
 
 // Scores in units of ln 2 with whatever is not seen at -inf: x holds products,
 // and in the end (x scale + bias) log2 e.  A bias of the type's lowest value
 // would overflow in those units, so it keeps natural ones and the differences
 // are multiplied.
-__device__ __forceinline__ float Units(const TrainAttention &a) { return a.bias ? kLog2e : 1.f; }
+template <int BIAS> constexpr float kUnits = BIAS ? kLog2e : 1.f;
+template <int BIAS>
 __device__ __forceinline__ void ToScores(const TrainAttention &a, std::int64_t bias_at, int j0,
                                          int last, f32x4 *x) {
-  if (a.bias) {
+  if constexpr (BIAS != kNoBias) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int j = j0 + 32 * u;
       f32x4 bias[2];
-      Fill(bias, 2, 0.f);
-      if (j <= last)
-        Bias8(a.bias, a.bias_dtype, bias_at + j, a.k_len - j, bias);
+      Bias8<BIAS>(a, bias_at, j0 + 32 * u, bias);
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         x[2 * u + (e >> 2)][e & 3] = x[2 * u + (e >> 2)][e & 3] * a.scale + bias[e >> 2][e & 3];
     }
   } else {
+    const float scale = a.scale * kLog2e;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
-      x[t] *= a.scale * kLog2e;
+      x[t] *= scale;
   }
   if (j0 + 39 > last) {
 #pragma unroll
@@ -502,9 +538,9 @@ __device__ __forceinline__ void ToScores(const TrainAttention &a, std::int64_t b
   }
 }
 
-// ONE: all keys in one tile.
-template <int DT, int DP, bool ONE>
-__global__ __launch_bounds__(256) void ForwardKernel(Args s) {
+// N sets of 16 rows a wave.  ONE: all keys in one tile.
+template <int DT, int DP, int N, int BIAS, bool ONE>
+__global__ __launch_bounds__(256, N) void ForwardKernel(Args s) {
   using M = Mat<DT>;
   constexpr int LD = kLd<DT, DP>;
   __shared__ __attribute__((aligned(16))) typename M::T ks[kTile * LD], vs[kTile * LD];
@@ -514,9 +550,8 @@ __global__ __launch_bounds__(256) void ForwardKernel(Args s) {
   const TrainAttention &a = s.a;
   const Line l = LineOf(s, part.line);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, g = lane >> 4;
-  const int first = part.tile * kTile;
-  const RowOfWave w = RowFor(s, l, first + 16 * wave + fr);
-  const int seen = KeysSeen(s, l, first);
+  const int first = part.tile * kTile * N;
+  const int seen = KeysSeen(l, SpanOf(s, first, kTile * N), kTile * N);
   const int per = ONE ? 1 : (s.steps + s.splits - 1) / s.splits;
   const int begin = ONE ? 0 : part.split * per, end = min(begin + per, (seen + kTile - 1) / kTile);
   Stage<DT, DP> kt, vt;
@@ -524,14 +559,21 @@ __global__ __launch_bounds__(256) void ForwardKernel(Args s) {
     kt.Keys(a.k, l, begin * kTile, a.dim);
     vt.Keys(a.v, l, begin * kTile, a.dim);
   }
-  typename M::Frag qf[DP / 32];
-  LoadRow<DT, DP>(s, a.q, l, w, lane, qf);
-  const std::int64_t bias_at = a.bias ? BiasAt(a, l.b, w.head, w.q) : 0;
-  const float units = Units(a);
-  f32x4 acc[DP / 16], zero[4];
-  Fill(acc, DP / 16, 0.f);
-  Fill(zero, 4, 0.f);
-  float most = -__builtin_inff(), total = 0.f;
+  RowOfWave w[N];
+  typename M::Frag qf[N][DP / 32];
+  std::int64_t bias_at[N];
+  f32x4 acc[N][DP / 16];
+  float most[N], total[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    w[n] = RowFor(s, l, first + 16 * (N * wave + n) + fr);
+    LoadRow<DT, DP>(s, a.q, l, w[n], lane, qf[n]);
+    bias_at[n] = BIAS ? BiasAt(a, l.b, w[n].head, w[n].q) : 0;
+    Fill(acc[n], DP / 16, 0.f);
+    most[n] = -__builtin_inff();
+    total[n] = 0.f;
+  }
+  constexpr float units = kUnits<BIAS>;
   for (int step = begin; step < end; ++step) {
     kt.Store(ks);
     vt.Store(vs);
@@ -540,62 +582,77 @@ __global__ __launch_bounds__(256) void ForwardKernel(Args s) {
       kt.Keys(a.k, l, (step + 1) * kTile, a.dim);
       vt.Keys(a.v, l, (step + 1) * kTile, a.dim);
     }
-    f32x4 x[4];
-    Products<DT, DP>(ks, qf, lane, zero, x);
-    ToScores(a, bias_at, step * kTile + 8 * g, w.last, x);
-    float top = most;
+    f32x4 x[N][4];
+    Fill(x[0], 4 * N, 0.f);
+    Products<DT, DP, N>(ks, qf, lane, x);
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int n = 0; n < N; ++n) {
+      ToScores<BIAS>(a, bias_at[n], step * kTile + 8 * g, w[n].last, x[n]);
+      float top = most[n];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        top = fmaxf(top, x[t][e]);
-    top = OverRows(top, true);
-    const float base = top == -__builtin_inff() ? 0.f : top;
-    const float old = Exp2((most - base) * units);
-    most = top;
-    total *= old;
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+        for (int e = 0; e < 4; ++e)
+          top = fmaxf(top, x[n][t][e]);
+      top = OverRows(top, true);
+      const float base = top == -__builtin_inff() ? 0.f : top;
+      const float old = Exp2((most[n] - base) * units);
+      most[n] = top;
+      total[n] *= old;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[t][e] = Exp2((x[t][e] - base) * units);
-        total += x[t][e];
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[n][t][e] = Exp2((x[n][t][e] - base) * units);
+          total[n] += x[n][t][e];
+        }
+      if constexpr (!ONE) {
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i)
+          acc[n][i] *= old;
       }
-    if constexpr (!ONE) {
-#pragma unroll
-      for (int i = 0; i < DP / 16; ++i)
-        acc[i] *= old;
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const typename M::Frag p = M::Pack(x[2 * u], x[2 * u + 1]);
+      typename M::Frag p[N];
 #pragma unroll
-      for (int i = 0; i < DP / 16; ++i)
-        acc[i] = M::Mul(HeadColumns<DT, DP, LD>(vs, 32 * u, i, lane), p, acc[i]);
+      for (int n = 0; n < N; ++n)
+        p[n] = M::Pack(x[n][2 * u], x[n][2 * u + 1]);
+#pragma unroll
+      for (int i = 0; i < DP / 16; ++i) {
+        const typename M::Frag v = HeadColumns<DT, DP, LD>(vs, 32 * u, i, lane);
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+          acc[n][i] = M::Mul(v, p[n], acc[n][i]);
+      }
     }
     if constexpr (!ONE)
       __syncthreads();
   }
-  total = OverRows(total, false);
-  if (!w.live)
-    return;
-  const std::int64_t flat = static_cast<std::int64_t>(part.line) * s.rows + w.r;
-  // Natural units from here on.
-  most *= a.bias ? 1.f : kLn2;
-  if (!ONE && s.splits > 1) {
-    const std::int64_t n = static_cast<std::int64_t>(s.lines) * s.rows;
-    StorePartial<DP>(s.partials + (part.split * n + flat) * s.dim4, lane, s.dim4, acc);
-    if (g == 0) {
-      float *st = s.partials + s.splits * n * s.dim4 + (part.split * n + flat) * 2;
-      st[0] = most;
-      st[1] = total;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    total[n] = OverRows(total[n], false);
+    if (!w[n].live)
+      continue;
+    const std::int64_t flat = static_cast<std::int64_t>(part.line) * s.rows + w[n].r;
+    // Natural units from here on.
+    most[n] *= BIAS ? 1.f : kLn2;
+    if (!ONE && s.splits > 1) {
+      const std::int64_t all = static_cast<std::int64_t>(s.lines) * s.rows;
+      StorePartial<DP>(s.partials + (part.split * all + flat) * s.a.dim, lane, s.a.dim, acc[n]);
+      if (g == 0) {
+        float *st = s.partials + s.splits * all * s.a.dim + (part.split * all + flat) * 2;
+        st[0] = most[n];
+        st[1] = total[n];
+      }
+      continue;
     }
-    return;
+    StoreHead<DT, DP>(Out<DT>(a.out, l.b, w[n].head, w[n].q), lane, a.dim, acc[n],
+                      total[n] == 0.f ? 0.f : 1.f / total[n]);
+    if (a.lse && g == 0)
+      a.lse[flat] = total[n] == 0.f ? -__builtin_inff()
+                                    : most[n] + kLn2 * __builtin_amdgcn_logf(total[n]);
   }
-  StoreHead<DT, DP>(Out<DT>(a.out, l.b, w.head, w.q), lane, a.dim, acc,
-                    total == 0.f ? 0.f : 1.f / total);
-  if (a.lse && g == 0)
-    a.lse[flat] = total == 0.f ? -__builtin_inff() : most + kLn2 * __builtin_amdgcn_logf(total);
 }
 
 constexpr int kMostSplits = 256;
@@ -607,7 +664,7 @@ __global__ __launch_bounds__(256) void JoinForwardKernel(Args s) {
   __shared__ float red[2][4], weight[kMostSplits];
   __shared__ f32x4 sums[256];
   const std::int64_t n = static_cast<std::int64_t>(s.lines) * s.rows, flat = blockIdx.x;
-  const float *st = s.partials + s.splits * n * s.dim4;
+  const float *st = s.partials + s.splits * n * s.a.dim;
   const int k = threadIdx.x;
   float most = -__builtin_inff(), total = 0.f;
   if (k < s.splits) {
@@ -628,13 +685,13 @@ __global__ __launch_bounds__(256) void JoinForwardKernel(Args s) {
     red[1][k >> 6] = total;
   __syncthreads();
   total = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
-  const int across = s.dim4 / 4, groups = 256 / across, group = k / across, c = k % across;
+  const int across = s.a.dim / 4, groups = 256 / across, group = k / across, c = k % across;
   f32x4 o{0.f, 0.f, 0.f, 0.f};
   if (group < groups) {
 #pragma unroll 4
     for (int i = group; i < s.splits; i += groups) {
       // A split that saw nothing holds zeros.
-      const f32x4 v = *reinterpret_cast<const f32x4 *>(s.partials + (i * n + flat) * s.dim4 + 4 * c);
+      const f32x4 v = *reinterpret_cast<const f32x4 *>(s.partials + (i * n + flat) * s.a.dim + 4 * c);
       o += v * weight[i];
     }
   }
@@ -646,7 +703,7 @@ __global__ __launch_bounds__(256) void JoinForwardKernel(Args s) {
     o += sums[i * across + k];
   const int line = static_cast<int>(flat / s.rows), r = static_cast<int>(flat % s.rows);
   const int b = line / s.a.kv_heads, head = line % s.a.kv_heads * s.a.group + r / s.a.q_len;
-  ToMemory<DT>(Out<DT>(s.a.out, b, head, r % s.a.q_len), 4 * k, s.a.dim,
+  ToMemory<DT>(Out<DT>(s.a.out, b, head, r % s.a.q_len) + 4 * k,
                o * (total == 0.f ? 0.f : 1.f / total));
   if (s.a.lse && k == 0)
     s.a.lse[flat] = total == 0.f ? -__builtin_inff() : most + kLn2 * __builtin_amdgcn_logf(total);
@@ -654,10 +711,10 @@ __global__ __launch_bounds__(256) void JoinForwardKernel(Args s) {
 
 // A row's log-sum-exp in the units of its scores, as what they are taken off:
 // +inf where it sees nothing, so that every probability is 0.
-__device__ __forceinline__ float Lse(const TrainAttention &a, float v) {
+template <int BIAS> __device__ __forceinline__ float Lse(float v) {
   if (v == -__builtin_inff())
     return __builtin_inff();
-  return a.bias ? v : v * kLog2e;
+  return BIAS ? v : v * kLog2e;
 }
 // delta = dout . out of a row, over the four lanes that share it.
 template <int DT, int DP>
@@ -673,8 +730,8 @@ __device__ __forceinline__ float Delta(const typename Mat<DT>::Frag *out,
 }
 
 // delta of each row, then dq (and dbias) of a tile of rows over the keys.
-template <int DT, int DP>
-__global__ __launch_bounds__(256) void BackwardRowsKernel(Args s) {
+template <int DT, int DP, int N, int BIAS>
+__global__ __launch_bounds__(256, N) void BackwardRowsKernel(Args s) {
   using M = Mat<DT>;
   constexpr int LD = kLd<DT, DP>;
   __shared__ __attribute__((aligned(16))) typename M::T ks[kTile * LD], vs[kTile * LD];
@@ -684,38 +741,39 @@ __global__ __launch_bounds__(256) void BackwardRowsKernel(Args s) {
   const TrainAttention &a = s.a;
   const Line l = LineOf(s, part.line);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, g = lane >> 4;
-  const int first = part.tile * kTile;
-  const RowOfWave w = RowFor(s, l, first + 16 * wave + fr);
-  const std::int64_t flat = static_cast<std::int64_t>(part.line) * s.rows + w.r;
+  const int first = part.tile * kTile * N;
   // Every element of the bias's gradient is written, so no key is left out.
-  const int seen = a.dbias ? a.k_len : KeysSeen(s, l, first);
+  const int seen = a.dbias ? a.k_len : KeysSeen(l, SpanOf(s, first, kTile * N), kTile * N);
   const int per = (s.steps + s.splits - 1) / s.splits;
   const int begin = part.split * per, end = min(begin + per, (seen + kTile - 1) / kTile);
-  const bool any = begin < end && (a.dq.p || a.dbias);
   Stage<DT, DP> kt, vt;
-  if (any) {
+  if (begin < end && (a.dq.p || a.dbias)) {
     kt.Keys(a.k, l, begin * kTile, a.dim);
     vt.Keys(a.v, l, begin * kTile, a.dim);
   }
-  typename M::Frag qf[DP / 32], df[DP / 32];
-  LoadRow<DT, DP>(s, a.q, l, w, lane, qf);
-  LoadRow<DT, DP>(s, a.dout, l, w, lane, df);
-  float delta;
-  {
+  RowOfWave w[N];
+  typename M::Frag qf[N][DP / 32], df[N][DP / 32];
+  float delta[N], lse[N];
+  std::int64_t bias_at[N];
+  f32x4 acc[N][DP / 16];
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    w[n] = RowFor(s, l, first + 16 * (N * wave + n) + fr);
+    const std::int64_t flat = static_cast<std::int64_t>(part.line) * s.rows + w[n].r;
+    LoadRow<DT, DP>(s, a.q, l, w[n], lane, qf[n]);
+    LoadRow<DT, DP>(s, a.dout, l, w[n], lane, df[n]);
     typename M::Frag of[DP / 32];
-    LoadRow<DT, DP>(s, a.out, l, w, lane, of);
-    delta = Delta<DT, DP>(of, df);
+    LoadRow<DT, DP>(s, a.out, l, w[n], lane, of);
+    delta[n] = Delta<DT, DP>(of, df[n]);
+    if (w[n].live && g == 0 && part.split == 0)
+      s.delta[flat] = delta[n];
+    lse[n] = w[n].last >= 0 ? Lse<BIAS>(a.lse[flat]) : __builtin_inff();
+    bias_at[n] = BIAS ? BiasAt(a, l.b, w[n].head, w[n].q) : 0;
+    Fill(acc[n], DP / 16, 0.f);
   }
-  if (w.live && g == 0 && part.split == 0)
-    s.delta[flat] = delta;
   if (!a.dq.p && !a.dbias)
     return;
-  const float lse = w.last >= 0 ? Lse(a, a.lse[flat]) : __builtin_inff(), units = Units(a);
-  const std::int64_t bias_at = a.bias ? BiasAt(a, l.b, w.head, w.q) : 0;
-  f32x4 acc[DP / 16], zero[4], minus[4];
-  Fill(acc, DP / 16, 0.f);
-  Fill(zero, 4, 0.f);
-  Fill(minus, 4, -delta);
+  constexpr float units = kUnits<BIAS>;
   for (int step = begin; step < end; ++step) {
     kt.Store(ks);
     vt.Store(vs);
@@ -724,41 +782,56 @@ __global__ __launch_bounds__(256) void BackwardRowsKernel(Args s) {
       kt.Keys(a.k, l, (step + 1) * kTile, a.dim);
       vt.Keys(a.v, l, (step + 1) * kTile, a.dim);
     }
-    f32x4 x[4], dp[4];
-    Products<DT, DP>(ks, qf, lane, zero, x);
-    Products<DT, DP>(vs, df, lane, minus, dp);
+    f32x4 x[N][4], dp[N][4];
+    Fill(x[0], 4 * N, 0.f);
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      Fill(dp[n], 4, -delta[n]);
+    Products<DT, DP, N>(ks, qf, lane, x);
+    Products<DT, DP, N>(vs, df, lane, dp);
     const int j0 = step * kTile + 8 * g;
-    ToScores(a, bias_at, j0, w.last, x);
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int n = 0; n < N; ++n) {
+      ToScores<BIAS>(a, bias_at[n], j0, w[n].last, x[n]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float p = Exp2((x[t][e] - lse) * units);
-        x[t][e] = p * dp[t][e];
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          x[n][t][e] = Exp2((x[n][t][e] - lse[n]) * units) * dp[n][t][e];
+      if (BIAS && a.dbias && w[n].live) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          StoreBias8<BIAS>(a, bias_at[n], j0 + 32 * u, x[n] + 2 * u);
       }
-    if (a.dbias && w.live) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        if (j0 + 32 * u < a.k_len)
-          StoreBias8(a.dbias, a.bias_dtype, bias_at + j0 + 32 * u, a.k_len - j0 - 32 * u, x + 2 * u);
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const typename M::Frag ds = M::Pack(x[2 * u], x[2 * u + 1]);
+      typename M::Frag ds[N];
 #pragma unroll
-      for (int i = 0; i < DP / 16; ++i)
-        acc[i] = M::Mul(HeadColumns<DT, DP, LD>(ks, 32 * u, i, lane), ds, acc[i]);
+      for (int n = 0; n < N; ++n)
+        ds[n] = M::Pack(x[n][2 * u], x[n][2 * u + 1]);
+#pragma unroll
+      for (int i = 0; i < DP / 16; ++i) {
+        const typename M::Frag k = HeadColumns<DT, DP, LD>(ks, 32 * u, i, lane);
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+          acc[n][i] = M::Mul(k, ds[n], acc[n][i]);
+      }
     }
     __syncthreads();
   }
-  if (!w.live || !a.dq.p)
-    return;
-  if (s.splits > 1) {
-    const std::int64_t n = static_cast<std::int64_t>(s.lines) * s.rows;
-    StorePartial<DP>(s.partials + (part.split * n + flat) * s.dim4, lane, s.dim4, acc);
-    return;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    if (!w[n].live || !a.dq.p)
+      continue;
+    if (s.splits > 1) {
+      const std::int64_t all = static_cast<std::int64_t>(s.lines) * s.rows,
+                         flat = static_cast<std::int64_t>(part.line) * s.rows + w[n].r;
+      StorePartial<DP>(s.partials + (part.split * all + flat) * s.a.dim, lane, s.a.dim, acc[n]);
+    } else {
+      StoreHead<DT, DP>(Out<DT>(a.dq, l.b, w[n].head, w[n].q), lane, a.dim, acc[n], a.scale);
+    }
   }
-  StoreHead<DT, DP>(Out<DT>(a.dq, l.b, w.head, w.q), lane, a.dim, acc, a.scale);
 }
 
 // What a workgroup of the keys' kernel holds of its 64 rows, next to the tiles.
@@ -768,10 +841,10 @@ struct RowInfo {
   std::int64_t bias[kTile];
 };
 
-// dk and dv of a tile of keys over the rows that share them; each wave has 16
-// keys and holds them, and rows go through LDS.
-template <int DT, int DP>
-__global__ __launch_bounds__(256) void BackwardKeysKernel(Args s) {
+// dk and dv of a tile of keys over the rows that share them; each wave has N
+// times 16 keys and holds them, and rows go through LDS.
+template <int DT, int DP, int N, int BIAS>
+__global__ __launch_bounds__(256, N) void BackwardKeysKernel(Args s) {
   using M = Mat<DT>;
   constexpr int LD = kLd<DT, DP>;
   __shared__ __attribute__((aligned(16))) typename M::T qs[kTile * LD], dos[kTile * LD];
@@ -782,36 +855,40 @@ __global__ __launch_bounds__(256) void BackwardKeysKernel(Args s) {
   const TrainAttention &a = s.a;
   const Line l = LineOf(s, part.line);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, g = lane >> 4;
-  const int key0 = part.tile * kTile, j = key0 + 16 * wave + fr;
-  typename M::Frag kf[DP / 32], vf[DP / 32];
+  const int key0 = part.tile * kTile * N;
+  int j[N];
+  typename M::Frag kf[N][DP / 32], vf[N][DP / 32];
+  f32x4 dk[N][DP / 16], dv[N][DP / 16];
 #pragma unroll
-  for (int c = 0; c < DP / 32; ++c) {
-    kf[c] = vf[c] = typename M::Frag{};
-    if (j < l.k_len) {
-      kf[c] = FromMemory<DT>(In<DT>(a.k, l.b, l.kv, j), 32 * c + 8 * g, a.dim);
-      vf[c] = FromMemory<DT>(In<DT>(a.v, l.b, l.kv, j), 32 * c + 8 * g, a.dim);
-    }
+  for (int n = 0; n < N; ++n) {
+    j[n] = key0 + 16 * (N * wave + n) + fr;
+    LoadKey<DT, DP>(s, a.k, l, j[n], lane, kf[n]);
+    LoadKey<DT, DP>(s, a.v, l, j[n], lane, vf[n]);
+    Fill(dk[n], DP / 16, 0.f);
+    Fill(dv[n], DP / 16, 0.f);
   }
-  const float units = Units(a), scale = a.bias ? a.scale : a.scale * kLog2e;
-  f32x4 dk[DP / 16], dv[DP / 16], zero[4];
-  Fill(dk, DP / 16, 0.f);
-  Fill(dv, DP / 16, 0.f);
-  Fill(zero, 4, 0.f);
+  const float scale = BIAS ? a.scale : a.scale * kLog2e;
   const int per = (s.steps + s.splits - 1) / s.splits;
   const int end = min((part.split + 1) * per, s.steps);
   // The next tile from `step` on of which a row sees one of these keys.
+  Span64 span{};
   const auto next = [&](int step) {
-    while (step < end && KeysSeen(s, l, step * kTile) <= key0)
-      ++step;
+    for (; step < end; ++step) {
+      span = SpanOf(s, step * kTile, kTile);
+      if (KeysSeen(l, span, kTile) > key0)
+        break;
+    }
     return step;
   };
   Stage<DT, DP> qt, dt;
   int my_last = -1;
   float my_lse = 0.f, my_delta = 0.f;
   std::int64_t my_bias = 0;
+  bool all_see = false;
   const auto load = [&](int step) {
-    qt.Rows(s, a.q, l, step * kTile);
-    dt.Rows(s, a.dout, l, step * kTile);
+    qt.Rows(s, a.q, l, span, step * kTile);
+    dt.Rows(s, a.dout, l, span, step * kTile);
+    all_see = span.same && span.q + kTile <= l.q_len && l.Last(span.q) >= key0 + kTile * N - 1;
     if (threadIdx.x < kTile) {
       const RowOfWave w = RowFor(s, l, step * kTile + threadIdx.x);
       const std::int64_t flat = static_cast<std::int64_t>(part.line) * s.rows + w.r;
@@ -819,10 +896,10 @@ __global__ __launch_bounds__(256) void BackwardKeysKernel(Args s) {
       my_lse = __builtin_inff();
       my_delta = 0.f;
       if (w.last >= 0) {
-        my_lse = Lse(a, a.lse[flat]);
+        my_lse = Lse<BIAS>(a.lse[flat]);
         my_delta = s.delta[flat];
       }
-      my_bias = a.bias ? BiasAt(a, l.b, w.head, w.q) : 0;
+      my_bias = BIAS ? BiasAt(a, l.b, w.head, w.q) : 0;
     }
   };
   int step = next(part.split * per);
@@ -838,60 +915,105 @@ __global__ __launch_bounds__(256) void BackwardKeysKernel(Args s) {
       info.bias[threadIdx.x] = my_bias;
     }
     __syncthreads();
+    const bool plain = all_see;
     step = next(step + 1);
     if (step < end)
       load(step);
-    f32x4 x[4], dp[4], minus[4];
+    f32x4 x[N][4], dp[N][4];
+    Fill(x[0], 4 * N, 0.f);
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-      minus[t] = -*reinterpret_cast<const f32x4 *>(info.delta + RowOf64(t, 4 * g));
-    Products<DT, DP>(qs, kf, lane, zero, x);
-    Products<DT, DP>(dos, vf, lane, minus, dp);
+    for (int t = 0; t < 4; ++t) {
+      dp[0][t] = -*reinterpret_cast<const f32x4 *>(info.delta + RowOf64(t, 4 * g));
+#pragma unroll
+      for (int n = 1; n < N; ++n)
+        dp[n][t] = dp[0][t];
+    }
+    // All of the step's biases at once: rows apart, keys side by side in lanes.
+    f32x4 bias[BIAS ? N : 1][4];
+    if constexpr (BIAS != kNoBias) {
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const std::int64_t at = info.bias[RowOf64(t, 4 * g + e)] + min(j[n], a.k_len - 1);
+            bias[n][t][e] =
+                a.bias_dtype == DT_F32
+                    ? ((const MFH_GLOBAL float *)a.bias)[at]
+                    : OfHalf(a.bias_dtype, ((const MFH_GLOBAL std::uint16_t *)a.bias)[at]);
+          }
+    }
+    Products<DT, DP, N>(qs, kf, lane, x);
+    Products<DT, DP, N>(dos, vf, lane, dp);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const int at = RowOf64(t, 4 * g);
       const f32x4 lse = *reinterpret_cast<const f32x4 *>(info.lse + at);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const bool sees = j <= info.last[at + e];
-        const float bias = a.bias && sees ? Bias1(a.bias, a.bias_dtype, info.bias[at + e] + j) : 0.f;
-        const float p = Exp2((x[t][e] * scale + bias - lse[e]) * units);
-        x[t][e] = sees ? p : 0.f;
-        dp[t][e] *= x[t][e];
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (BIAS != kNoBias)
+            x[n][t][e] = Exp2((x[n][t][e] * scale + bias[n][t][e] - lse[e]) * kLog2e);
+          else
+            x[n][t][e] = Exp2(x[n][t][e] * scale - lse[e]);
+        }
+      if (!plain) {
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            x[n][t][e] = j[n] <= info.last[at + e] ? x[n][t][e] : 0.f;
       }
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        dp[n][t] *= x[n][t];
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const typename M::Frag p = M::Pack(x[2 * u], x[2 * u + 1]),
-                             ds = M::Pack(dp[2 * u], dp[2 * u + 1]);
+      typename M::Frag p[N], ds[N];
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        p[n] = M::Pack(x[n][2 * u], x[n][2 * u + 1]);
+        ds[n] = M::Pack(dp[n][2 * u], dp[n][2 * u + 1]);
+      }
 #pragma unroll
       for (int i = 0; i < DP / 16; ++i) {
-        dv[i] = M::Mul(HeadColumns<DT, DP, LD>(dos, 32 * u, i, lane), p, dv[i]);
-        dk[i] = M::Mul(HeadColumns<DT, DP, LD>(qs, 32 * u, i, lane), ds, dk[i]);
+        const typename M::Frag d = HeadColumns<DT, DP, LD>(dos, 32 * u, i, lane),
+                               q = HeadColumns<DT, DP, LD>(qs, 32 * u, i, lane);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          dv[n][i] = M::Mul(d, p[n], dv[n][i]);
+          dk[n][i] = M::Mul(q, ds[n], dk[n][i]);
+        }
       }
     }
     __syncthreads();
   }
-  if (j >= a.k_len)
-    return;
-  if (s.splits > 1) {
-    const std::int64_t n = static_cast<std::int64_t>(s.lines) * a.k_len;
-    const std::int64_t flat = static_cast<std::int64_t>(part.line) * a.k_len + j;
-    float *o = s.partials + (2 * part.split * n + flat) * s.dim4;
-    StorePartial<DP>(o, lane, s.dim4, dk);
-    StorePartial<DP>(o + n * s.dim4, lane, s.dim4, dv);
-    return;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    if (j[n] >= a.k_len)
+      continue;
+    if (s.splits > 1) {
+      const std::int64_t all = static_cast<std::int64_t>(s.lines) * a.k_len,
+                         flat = static_cast<std::int64_t>(part.line) * a.k_len + j[n];
+      float *o = s.partials + (2 * part.split * all + flat) * s.a.dim;
+      StorePartial<DP>(o, lane, s.a.dim, dk[n]);
+      StorePartial<DP>(o + all * s.a.dim, lane, s.a.dim, dv[n]);
+      continue;
+    }
+    if (a.dk.p)
+      StoreHead<DT, DP>(Out<DT>(a.dk, l.b, l.kv, j[n]), lane, a.dim, dk[n], a.scale);
+    if (a.dv.p)
+      StoreHead<DT, DP>(Out<DT>(a.dv, l.b, l.kv, j[n]), lane, a.dim, dv[n], 1.f);
   }
-  if (a.dk.p)
-    StoreHead<DT, DP>(Out<DT>(a.dk, l.b, l.kv, j), lane, a.dim, dk, a.scale);
-  if (a.dv.p)
-    StoreHead<DT, DP>(Out<DT>(a.dv, l.b, l.kv, j), lane, a.dim, dv, 1.f);
 }
 
 // Adds up the splits of dq (KEYS false) or of dk and dv: four elements a thread.
 template <int DT, bool KEYS>
 __global__ __launch_bounds__(256) void JoinBackwardKernel(Args s) {
-  const int per = KEYS ? s.a.k_len : s.rows, across = s.dim4 / 4;
+  const int per = KEYS ? s.a.k_len : s.rows, across = s.a.dim / 4;
   const std::int64_t n = static_cast<std::int64_t>(s.lines) * per;
   const std::int64_t all = KEYS ? 2 * n : n;
   const std::int64_t id = static_cast<std::int64_t>(blockIdx.x) * 256 + threadIdx.x;
@@ -902,7 +1024,7 @@ __global__ __launch_bounds__(256) void JoinBackwardKernel(Args s) {
   f32x4 o{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
   for (int k = 0; k < s.splits; ++k)
-    o += *reinterpret_cast<const f32x4 *>(s.partials + (k * all + at) * s.dim4 + 4 * c);
+    o += *reinterpret_cast<const f32x4 *>(s.partials + (k * all + at) * s.a.dim + 4 * c);
   const bool second = KEYS && at >= n;
   const std::int64_t flat = second ? at - n : at;
   const int line = static_cast<int>(flat / per), r = static_cast<int>(flat % per);
@@ -916,14 +1038,14 @@ __global__ __launch_bounds__(256) void JoinBackwardKernel(Args s) {
   } else {
     out = Out<DT>(s.a.dq, b, kv * s.a.group + r / s.a.q_len, r % s.a.q_len);
   }
-  ToMemory<DT>(out, 4 * c, s.a.dim, o * (second ? 1.f : s.a.scale));
+  ToMemory<DT>(out + 4 * c, o * (second ? 1.f : s.a.scale));
 }
 
 // The whole backward pass of a head of up to 64 queries and 64 keys, none of
 // them shared: one workgroup, each input read once.  A wave has 16 queries while
 // scores, probabilities, dS and dq are formed, and 16 keys for dk and dv; P and dS
 // change hands through LDS.
-template <int DT, int DP>
+template <int DT, int DP, int BIAS>
 __global__ __launch_bounds__(256) void SquareBackwardKernel(Args s) {
   using M = Mat<DT>;
   constexpr int LD = kLd<DT, DP>, LP = kLd<DT, kTile>;
@@ -939,45 +1061,36 @@ __global__ __launch_bounds__(256) void SquareBackwardKernel(Args s) {
   const int mine = 16 * wave + fr;  // a query, and later a key
   const RowOfWave w = RowFor(s, l, mine);
   const std::int64_t flat = static_cast<std::int64_t>(part.line) * s.rows + mine;
-  typename M::Frag qf[DP / 32], df[DP / 32];
+  typename M::Frag qf[1][DP / 32], df[1][DP / 32], of[DP / 32];
   {
     typename M::Frag kf[DP / 32], vf[DP / 32];
-#pragma unroll
-    for (int c = 0; c < DP / 32; ++c) {
-      kf[c] = vf[c] = typename M::Frag{};
-      if (mine < l.k_len) {
-        kf[c] = FromMemory<DT>(In<DT>(a.k, l.b, l.kv, mine), 32 * c + 8 * g, a.dim);
-        vf[c] = FromMemory<DT>(In<DT>(a.v, l.b, l.kv, mine), 32 * c + 8 * g, a.dim);
-      }
-    }
-    LoadRow<DT, DP>(s, a.q, l, w, lane, qf);
-    LoadRow<DT, DP>(s, a.dout, l, w, lane, df);
+    LoadKey<DT, DP>(s, a.k, l, mine, lane, kf);
+    LoadRow<DT, DP>(s, a.q, l, w, lane, qf[0]);
+    LoadKey<DT, DP>(s, a.v, l, mine, lane, vf);
+    LoadRow<DT, DP>(s, a.dout, l, w, lane, df[0]);
+    LoadRow<DT, DP>(s, a.out, l, w, lane, of);
 #pragma unroll
     for (int c = 0; c < DP / 32; ++c) {
       const int at = mine * LD + 32 * c + 8 * g;
       ToRow<DT>(ks + at, kf[c]);
+      ToRow<DT>(qs + at, qf[0][c]);
       ToRow<DT>(vs + at, vf[c]);
-      ToRow<DT>(qs + at, qf[c]);
-      ToRow<DT>(dos + at, df[c]);
+      ToRow<DT>(dos + at, df[0][c]);
     }
   }
-  float delta;
-  {
-    typename M::Frag of[DP / 32];
-    LoadRow<DT, DP>(s, a.out, l, w, lane, of);
-    delta = Delta<DT, DP>(of, df);
-  }
+  const float delta = Delta<DT, DP>(of, df[0]);
   if (w.live && g == 0)
     s.delta[flat] = delta;
-  const float lse = w.last >= 0 ? Lse(a, a.lse[flat]) : __builtin_inff(), units = Units(a);
-  const std::int64_t bias_at = a.bias ? BiasAt(a, l.b, w.head, w.q) : 0;
+  const float lse = w.last >= 0 ? Lse<BIAS>(a.lse[flat]) : __builtin_inff();
+  constexpr float units = kUnits<BIAS>;
+  const std::int64_t bias_at = BIAS ? BiasAt(a, l.b, w.head, w.q) : 0;
   __syncthreads();
-  f32x4 x[4], dp[4], zero[4], minus[4];
-  Fill(zero, 4, 0.f);
-  Fill(minus, 4, -delta);
-  Products<DT, DP>(ks, qf, lane, zero, x);
-  Products<DT, DP>(vs, df, lane, minus, dp);
-  ToScores(a, bias_at, 8 * g, w.last, x);
+  f32x4 xs[1][4], dps[1][4], *x = xs[0], *dp = dps[0];
+  Fill(x, 4, 0.f);
+  Fill(dp, 4, -delta);
+  Products<DT, DP, 1>(ks, qf, lane, xs);
+  Products<DT, DP, 1>(vs, df, lane, dps);
+  ToScores<BIAS>(a, bias_at, 8 * g, w.last, x);
 #pragma unroll
   for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -985,12 +1098,10 @@ __global__ __launch_bounds__(256) void SquareBackwardKernel(Args s) {
       x[t][e] = Exp2((x[t][e] - lse) * units);
       dp[t][e] *= x[t][e];
     }
-  if (a.dbias && w.live) {
+  if (BIAS && a.dbias && w.live) {
 #pragma unroll
     for (int u = 0; u < 2; ++u)
-      if (8 * g + 32 * u < a.k_len)
-        StoreBias8(a.dbias, a.bias_dtype, bias_at + 8 * g + 32 * u, a.k_len - 8 * g - 32 * u,
-                   dp + 2 * u);
+      StoreBias8<BIAS>(a, bias_at, 8 * g + 32 * u, dp + 2 * u);
   }
   f32x4 acc[DP / 16], more[DP / 16];
   Fill(acc, DP / 16, 0.f);
@@ -1030,12 +1141,12 @@ __global__ __launch_bounds__(256) void SquareBackwardKernel(Args s) {
 
 // The gradient of a bias that lines or heads share: a workgroup has 64 queries
 // and 64 keys of one of its planes and loops over what shares it.
-template <int DT, int DP>
-__global__ __launch_bounds__(256) void BiasGradKernel(Args s, int plane_heads) {
+template <int DT, int DP, int BIAS>
+__global__ __launch_bounds__(256) void BiasGradKernel(Args s, int plane_heads, std::int64_t first) {
   using M = Mat<DT>;
   const TrainAttention &a = s.a;
   const int k_tiles = (a.k_len + kTile - 1) / kTile, q_tiles = (a.q_len + kTile - 1) / kTile;
-  const std::int64_t id = s.first + blockIdx.x;
+  const std::int64_t id = first + blockIdx.x;
   const int kt = static_cast<int>(id % k_tiles), qt = static_cast<int>(id / k_tiles % q_tiles);
   const int plane = static_cast<int>(id / k_tiles / q_tiles);
   const int b_plane = plane / plane_heads, h_plane = plane % plane_heads;
@@ -1050,32 +1161,29 @@ __global__ __launch_bounds__(256) void BiasGradKernel(Args s, int plane_heads) {
   Fill(bias, 4, 0.f);
 #pragma unroll
   for (int u = 0; u < 2; ++u)
-    if (live && j0 + 32 * u < a.k_len)
-      Bias8(a.bias, a.bias_dtype, bias_at + j0 + 32 * u, a.k_len - j0 - 32 * u, bias + 2 * u);
+    Bias8<BIAS>(a, bias_at, j0 + 32 * u, bias + 2 * u);
   for (int b = b0; b < b1; ++b)
     for (int head = h0; head < h1; ++head) {
       const int kv = head / a.group;
       const Line l = LineOf(s, b * a.kv_heads + kv);
-      RowOfWave w{0, 0, q, head, live ? l.Last(q) : -1, live};
+      RowOfWave w{q, q, head, live ? l.Last(q) : -1, live};
       const std::int64_t flat = (static_cast<std::int64_t>(b) * a.heads + head) * a.q_len + q;
       typename M::Frag qf[DP / 32], df[DP / 32];
       LoadRow<DT, DP>(s, a.q, l, w, lane, qf);
       LoadRow<DT, DP>(s, a.dout, l, w, lane, df);
-      const float lse = w.last >= 0 ? Lse(a, a.lse[flat]) : __builtin_inff();
+      const float lse = w.last >= 0 ? Lse<BIAS>(a.lse[flat]) : __builtin_inff();
       const float delta = w.last >= 0 ? s.delta[flat] : 0.f;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         f32x4 x{0.f, 0.f, 0.f, 0.f}, dp{-delta, -delta, -delta, -delta};
         const int key = kt * kTile + RowOf64(t, fr), j = kt * kTile + RowOf64(t, 4 * g);
+        typename M::Frag kf[DP / 32], vf[DP / 32];
+        LoadKey<DT, DP>(s, a.k, l, key, lane, kf);
+        LoadKey<DT, DP>(s, a.v, l, key, lane, vf);
 #pragma unroll
         for (int c = 0; c < DP / 32; ++c) {
-          typename M::Frag kf{}, vf{};
-          if (key < l.k_len) {
-            kf = FromMemory<DT>(In<DT>(a.k, b, kv, key), 32 * c + 8 * g, a.dim);
-            vf = FromMemory<DT>(In<DT>(a.v, b, kv, key), 32 * c + 8 * g, a.dim);
-          }
-          x = M::Mul(kf, qf[c], x);
-          dp = M::Mul(vf, df[c], dp);
+          x = M::Mul(kf[c], qf[c], x);
+          dp = M::Mul(vf[c], df[c], dp);
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -1088,28 +1196,42 @@ __global__ __launch_bounds__(256) void BiasGradKernel(Args s, int plane_heads) {
     return;
 #pragma unroll
   for (int u = 0; u < 2; ++u)
-    if (j0 + 32 * u < a.k_len)
-      StoreBias8(a.dbias, a.bias_dtype, bias_at + j0 + 32 * u, a.k_len - j0 - 32 * u, acc + 2 * u);
+    StoreBias8<BIAS>(a, bias_at, j0 + 32 * u, acc + 2 * u);
 }
 
 // Workgroups that fill the card twice; a split loops over two tiles at least.
 inline int SplitsOf(std::int64_t groups, int steps) {
-  const std::int64_t want = std::min<std::int64_t>(512 / std::max<std::int64_t>(groups, 1), kMostSplits);
+  const std::int64_t want =
+      std::min<std::int64_t>(512 / std::max<std::int64_t>(groups, 1), kMostSplits);
   return static_cast<int>(std::max<std::int64_t>(1, std::min<std::int64_t>(want, steps / 2)));
 }
-inline int Tiles(int n) { return (n + kTile - 1) / kTile; }
+inline int Tiles(int n, int wide = 1) {
+  return static_cast<int>((static_cast<std::int64_t>(n) + kTile * wide - 1) / (kTile * wide));
+}
 
-// Shapes of the three launches, and the workspace that they share.
+inline int HowBias(const TrainAttention &a) {
+  if (!a.bias || a.k_len == 0)
+    return kNoBias;
+  return a.k_len % 8 == 0 ? kVectors : kValues;
+}
+
+// Shapes of the launches, and the workspace that they share.
 inline Args ArgsOf(const TrainAttention &a, bool keys) {
   Args s;
   s.a = a;
   s.lines = a.batch * a.kv_heads;
   s.rows = a.group * a.q_len;
-  s.dim4 = (a.dim + 3) & ~3;
-  s.tiles = keys ? Tiles(a.k_len) : Tiles(s.rows);
+  const int across = keys ? a.k_len : s.rows;
+  // Two sets of columns a wave halve the reads of LDS per product, where that
+  // leaves work for half of the card and registers hold them.
+  const bool fits =
+      (a.dim <= 32 || (a.dim <= 64 && a.dtype != DT_F32)) && HowBias(a) != kValues;
+  s.wide = fits && static_cast<std::int64_t>(s.lines) * Tiles(across, 2) >= 128 ? 2 : 1;
+  s.tiles = Tiles(across, s.wide);
   s.steps = keys ? Tiles(s.rows) : Tiles(a.k_len);
   s.splits = SplitsOf(static_cast<std::int64_t>(s.lines) * s.tiles, s.steps);
-  s.work = static_cast<std::int64_t>(s.lines) * s.tiles * s.splits;
+  if (!keys && a.causal)
+    s.down = a.group;
   return s;
 }
 // Whether the bias is shared by lines or heads.
@@ -1121,27 +1243,46 @@ inline std::uint64_t DeltaBytes(const Args &s) {
 }
 inline std::uint64_t ForwardBytes(const Args &s) {
   return s.splits == 1 ? 0
-                       : static_cast<std::uint64_t>(s.splits) * s.lines * s.rows * (s.dim4 + 2) * 4;
+                       : static_cast<std::uint64_t>(s.splits) * s.lines * s.rows * (s.a.dim + 2) * 4;
 }
 inline std::uint64_t RowsBytes(const Args &s) {
-  return s.splits == 1 ? 0 : static_cast<std::uint64_t>(s.splits) * s.lines * s.rows * s.dim4 * 4;
+  return s.splits == 1 ? 0 : static_cast<std::uint64_t>(s.splits) * s.lines * s.rows * s.a.dim * 4;
 }
 inline std::uint64_t KeysBytes(const Args &s) {
   return s.splits == 1
              ? 0
-             : static_cast<std::uint64_t>(s.splits) * 2 * s.lines * s.a.k_len * s.dim4 * 4;
+             : static_cast<std::uint64_t>(s.splits) * 2 * s.lines * s.a.k_len * s.a.dim * 4;
 }
 
-// A launch has less than 2^32 threads; more work takes several.
+// A launch has less than 2^32 threads, and less than 2^16 workgroups along y;
+// more work takes several.
 constexpr std::int64_t kMostGroups = std::int64_t(1) << 23;
 template <class K> hipError_t Run(K kernel, Args s, hipStream_t stream) {
-  hipError_t e = hipSuccess;
-  for (s.first = 0; e == hipSuccess && s.first < s.work; s.first = s.end) {
-    s.end = std::min(s.work, s.first + kMostGroups);
-    const auto groups = static_cast<unsigned>((s.end - s.first + 7) / 8 * 8);
-    hipLaunchKernelGGL(kernel, dim3(groups), dim3(256), 0, stream, s);
-    e = hipGetLastError();
+  if (s.lines == 0 || s.tiles == 0)
+    return hipSuccess;
+  if (s.splits > 1) {
+    const std::int64_t parts = static_cast<std::int64_t>(s.lines) * s.tiles * s.splits;
+    s.spread = true;
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((parts + 7) / 8 * 8)), dim3(256), 0, stream,
+                       s);
+    return hipGetLastError();
   }
+  const std::int64_t tiles =
+      s.down ? static_cast<std::int64_t>((s.tiles + s.down - 1) / s.down) * s.down : s.tiles;
+  const std::int64_t most_tiles = std::min<std::int64_t>(tiles, 65535);
+  const std::int64_t most_lines = std::max<std::int64_t>(8, kMostGroups / most_tiles / 8 * 8);
+  hipError_t e = hipSuccess;
+  for (std::int64_t line = 0; e == hipSuccess && line < s.lines; line += most_lines)
+    for (std::int64_t tile = 0; e == hipSuccess && tile < tiles; tile += most_tiles) {
+      s.line0 = static_cast<int>(line);
+      s.lines_now = static_cast<int>(std::min<std::int64_t>(most_lines, s.lines - line));
+      s.tile0 = static_cast<int>(tile);
+      s.spread = s.lines_now >= 64;
+      const dim3 grid(s.spread ? (s.lines_now + 7) / 8 * 8 : s.lines_now,
+                      static_cast<unsigned>(std::min<std::int64_t>(most_tiles, tiles - tile)));
+      hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, s);
+      e = hipGetLastError();
+    }
   return e;
 }
 // Splits have few rows.
@@ -1152,34 +1293,52 @@ template <class K> hipError_t RunJoin(K kernel, const Args &s, std::int64_t grou
   return hipGetLastError();
 }
 
-template <int DT, int DP> hipError_t Forward(const TrainAttention &a, hipStream_t stream) {
+// Where ArgsOf may ask for two sets of columns.
+template <int DT, int DP> constexpr bool kTwo = DP == 32 || (DP == 64 && DT != DT_F32);
+
+template <int DT, int DP, int BIAS>
+hipError_t Forward(const TrainAttention &a, hipStream_t stream) {
+  constexpr int kWide = kTwo<DT, DP> && BIAS != kValues ? 2 : 1;
   Args s = ArgsOf(a, false);
   s.partials = static_cast<float *>(a.workspace);
-  hipError_t e = s.steps <= 1 ? Run(ForwardKernel<DT, DP, true>, s, stream)
-                              : Run(ForwardKernel<DT, DP, false>, s, stream);
+  hipError_t e;
+  if (s.steps <= 1) {
+    s.wide = 1;
+    s.tiles = Tiles(s.rows);
+    e = Run(ForwardKernel<DT, DP, 1, BIAS, true>, s, stream);
+  } else if (s.wide == 2) {
+    e = Run(ForwardKernel<DT, DP, kWide, BIAS, false>, s, stream);
+  } else {
+    e = Run(ForwardKernel<DT, DP, 1, BIAS, false>, s, stream);
+  }
   if (e == hipSuccess && s.splits > 1)
     e = RunJoin(JoinForwardKernel<DT>, s, static_cast<std::int64_t>(s.lines) * s.rows, stream);
   return e;
 }
 
-template <int DT, int DP> hipError_t Backward(const TrainAttention &a, hipStream_t stream) {
+template <int DT, int DP, int BIAS>
+hipError_t Backward(const TrainAttention &a, hipStream_t stream) {
+  constexpr int kWide = kTwo<DT, DP> && BIAS != kValues ? 2 : 1;
+  constexpr bool kSquare = kTwo<DT, DP>;  // six tiles in LDS, two workgroups a CU
   Args s = ArgsOf(a, false);
   s.delta = static_cast<float *>(a.workspace);
   s.partials = reinterpret_cast<float *>(static_cast<char *>(a.workspace) + DeltaBytes(s));
   const bool shared = SharedBias(a);
   if (shared)
     s.a.dbias = nullptr;
-  constexpr bool kSquare = DP == 32 || (DP == 64 && DT != DT_F32);  // tiles fit in 64 KB
   const bool square = kSquare && a.group == 1 && a.q_len <= kTile && a.k_len <= kTile && a.q_len > 0 &&
                       a.k_len > 0;
-  const auto joins = [&](std::int64_t rows) { return (rows * (s.dim4 / 4) + 255) / 256; };
+  const auto joins = [&](std::int64_t rows) { return (rows * (a.dim / 4) + 255) / 256; };
   hipError_t e = hipSuccess;
   if constexpr (kSquare) {
-    if (square)
-      e = Run(SquareBackwardKernel<DT, DP>, s, stream);
+    if (square) {
+      s.tiles = 1;
+      e = Run(SquareBackwardKernel<DT, DP, BIAS>, s, stream);
+    }
   }
   if (!square)
-    e = Run(BackwardRowsKernel<DT, DP>, s, stream);
+    e = s.wide == 2 ? Run(BackwardRowsKernel<DT, DP, kWide, BIAS>, s, stream)
+                    : Run(BackwardRowsKernel<DT, DP, 1, BIAS>, s, stream);
   if (e == hipSuccess && s.splits > 1 && a.dq.p)
     e = RunJoin(JoinBackwardKernel<DT, false>, s, joins(static_cast<std::int64_t>(s.lines) * s.rows),
                 stream);
@@ -1187,32 +1346,45 @@ template <int DT, int DP> hipError_t Backward(const TrainAttention &a, hipStream
     Args k = ArgsOf(a, true);
     k.delta = s.delta;
     k.partials = s.partials;
-    e = Run(BackwardKeysKernel<DT, DP>, k, stream);
+    e = k.wide == 2 ? Run(BackwardKeysKernel<DT, DP, kWide, BIAS>, k, stream)
+                    : Run(BackwardKeysKernel<DT, DP, 1, BIAS>, k, stream);
     if (e == hipSuccess && k.splits > 1)
       e = RunJoin(JoinBackwardKernel<DT, true>, k,
                   joins(2 * static_cast<std::int64_t>(k.lines) * a.k_len), stream);
   }
-  if (e == hipSuccess && shared) {
-    s.a.dbias = a.dbias;
-    const int planes_b = a.bias_batch ? a.batch : 1, planes_h = a.bias_head ? a.heads : 1;
-    s.work = static_cast<std::int64_t>(Tiles(a.q_len)) * Tiles(a.k_len) * planes_b * planes_h;
-    for (s.first = 0; e == hipSuccess && s.first < s.work; s.first += kMostGroups) {
-      const auto groups = static_cast<unsigned>(std::min(s.work - s.first, kMostGroups));
-      hipLaunchKernelGGL((BiasGradKernel<DT, DP>), dim3(groups), dim3(256), 0, stream, s, planes_h);
-      e = hipGetLastError();
+  if constexpr (BIAS != kNoBias) {
+    if (e == hipSuccess && shared) {
+      s.a.dbias = a.dbias;
+      const int planes_b = a.bias_batch ? a.batch : 1, planes_h = a.bias_head ? a.heads : 1;
+      const std::int64_t work =
+          static_cast<std::int64_t>(Tiles(a.q_len)) * Tiles(a.k_len) * planes_b * planes_h;
+      for (std::int64_t first = 0; e == hipSuccess && first < work; first += kMostGroups) {
+        const auto groups = static_cast<unsigned>(std::min(work - first, kMostGroups));
+        hipLaunchKernelGGL((BiasGradKernel<DT, DP, BIAS>), dim3(groups), dim3(256), 0, stream, s,
+                           planes_h, first);
+        e = hipGetLastError();
+      }
     }
   }
   return e;
+}
+
+template <int DT, int DP>
+hipError_t ByBias(const TrainAttention &a, bool backward, hipStream_t stream) {
+  const int how = HowBias(a);
+  if (how == kNoBias)
+    return backward ? Backward<DT, DP, kNoBias>(a, stream) : Forward<DT, DP, kNoBias>(a, stream);
+  if (how == kVectors)
+    return backward ? Backward<DT, DP, kVectors>(a, stream) : Forward<DT, DP, kVectors>(a, stream);
+  return backward ? Backward<DT, DP, kValues>(a, stream) : Forward<DT, DP, kValues>(a, stream);
 }
 
 // By head size: a tile's columns are padded to 32, 64 or 128.
 template <int DT>
 hipError_t ByDim(const TrainAttention &a, bool backward, hipStream_t stream) {
   if (a.dim <= 32)
-    return backward ? Backward<DT, 32>(a, stream) : Forward<DT, 32>(a, stream);
-  if (a.dim <= 64)
-    return backward ? Backward<DT, 64>(a, stream) : Forward<DT, 64>(a, stream);
-  return backward ? Backward<DT, 128>(a, stream) : Forward<DT, 128>(a, stream);
+    return ByBias<DT, 32>(a, backward, stream);
+  return a.dim <= 64 ? ByBias<DT, 64>(a, backward, stream) : ByBias<DT, 128>(a, backward, stream);
 }
 
 // One source a type.

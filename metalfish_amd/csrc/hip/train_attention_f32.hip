@@ -14,13 +14,13 @@ namespace {
 
 bool Sound(const TrainAttention &a) {
   return a.batch >= 0 && a.heads >= 1 && a.kv_heads >= 1 && a.heads == a.kv_heads * a.group &&
-         a.q_len >= 0 && a.k_len >= 0 && a.dim >= 1 && a.dim <= 128;
+         a.q_len >= 0 && a.k_len >= 0 && a.dim >= 8 && a.dim <= 128 && a.dim % 8 == 0;
 }
 
 hipError_t Launch(const TrainAttention &a, bool backward, hipStream_t stream, std::string *err) {
   if (!Sound(a)) {
     if (err)
-      *err = "attention: needs heads of 1 to 128 elements, whole groups of them a key head";
+      *err = "attention: needs heads of 8 to 128 elements, a multiple of 8, whole groups of them a key head";
     return hipErrorInvalidValue;
   }
   if (a.dtype == DT_F32)

@@ -142,12 +142,12 @@ BAD_ATTENTION = {
     "batch": dict(batch=-1), "heads": dict(heads=0, kv_heads=1), "kv": dict(set_kv_heads=0),
     "group": dict(kv_heads=3), "q-len": dict(q_len=-1), "k-len": dict(k_len=-1),
     "k-long": dict(k_len=(1 << 30) + 1), "q-long": dict(q_len=(1 << 28) + 1, kv_heads=1),
-    "many": dict(batch=1 << 29), "dim": dict(dim=0, scale=1.0), "dim-large": dict(dim=129),
+    "many": dict(batch=1 << 29), "dim": dict(dim=0, scale=1.0), "dim-large": dict(dim=136), "dim-odd": dict(dim=12),
     "dtype": dict(set_dtype=3), "causal": dict(set_causal=2), "scale": dict(scale=NAN),
     "scale-infinite": dict(scale=INF), "device": dict(device=-2), "q": dict(d_q=None),
     "k": dict(d_k=None), "v": dict(d_v=None), "q-alignment": dict(d_q=A + 2),
     "k-alignment": dict(d_k=A + 1, dtype="bf16"), "stride": dict(q_strides=(-1, 32, 8)),
-    "stride-far": dict(k_strides=(1 << 60, 32, 8)), "lengths-alignment": dict(d_q_lengths=A + 2),
+    "stride-far": dict(k_strides=(1 << 60, 32, 8)), "token-far": dict(v_strides=(0, 1 << 32, 8)), "lengths-alignment": dict(d_q_lengths=A + 2),
     "k-lengths-alignment": dict(d_k_lengths=A + 3),
 }
 BAD_BIAS = {
