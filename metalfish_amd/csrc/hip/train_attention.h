@@ -430,9 +430,9 @@ template <int DT, int DP> struct Stage {
   }
 };
 
-// Products of a tile of 64 rows in LDS with N times 16 columns of a wave, added
-// to `out`: lane l has column l % 16 of each, rows RowOf64.
-template <int DT, int DP, int N>
+// Products of a tile of 64 rows in LDS with N times 16 columns of a wave (ADD:
+// added to `out`): lane l has column l % 16 of each, rows RowOf64.
+template <int DT, int DP, int N, bool ADD>
 __device__ __forceinline__ void Products(const typename Mat<DT>::T *tile,
                                          const typename Mat<DT>::Frag (*cols)[DP / 32], int lane,
                                          f32x4 (*out)[4]) {
@@ -445,7 +445,8 @@ __device__ __forceinline__ void Products(const typename Mat<DT>::T *tile,
           FromRow<DT>(tile + RowOf64(t, fr) * kLd<DT, DP> + 32 * c + 8 * g);
 #pragma unroll
       for (int n = 0; n < N; ++n)
-        out[n][t] = Mat<DT>::Mul(f, cols[n][c], out[n][t]);
+        out[n][t] =
+            Mat<DT>::Mul(f, cols[n][c], ADD || c > 0 ? out[n][t] : f32x4{0.f, 0.f, 0.f, 0.f});
     }
 }
 __device__ __forceinline__ void Fill(f32x4 *v, int n, float f) {
@@ -505,14 +506,16 @@ __device__ __forceinline__ void LoadKey(const Args &s, const HeadsView &v, const
       f[c] = FromMemory<DT>(row + 32 * c);
 }
 
-// Scores in units of ln 2 with whatever is not seen at -inf: x holds products,
-// and in the end (x scale + bias) log2 e.  A bias of the type's lowest value
-// would overflow in those units, so it keeps natural ones and the differences
-// are multiplied.
-template <int BIAS> constexpr float kUnits = BIAS ? kLog2e : 1.f;
+// Scores less `off`, whatever is not seen at -inf, from products.  Without a
+// bias in units of ln 2, ready for the exponential; a bias of the type's lowest value
+// would overflow in those, so with one they are natural and the differences are
+// multiplied (Exp).
+template <int BIAS> __device__ __forceinline__ float Exp(float x) {
+  return Exp2(BIAS ? x * kLog2e : x);
+}
 template <int BIAS>
 __device__ __forceinline__ void ToScores(const TrainAttention &a, std::int64_t bias_at, int j0,
-                                         int last, f32x4 *x) {
+                                         int last, float off, f32x4 *x) {
   if constexpr (BIAS != kNoBias) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -520,13 +523,16 @@ __device__ __forceinline__ void ToScores(const TrainAttention &a, std::int64_t b
       Bias8<BIAS>(a, bias_at, j0 + 32 * u, bias);
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        x[2 * u + (e >> 2)][e & 3] = x[2 * u + (e >> 2)][e & 3] * a.scale + bias[e >> 2][e & 3];
+        x[2 * u + (e >> 2)][e & 3] =
+            (x[2 * u + (e >> 2)][e & 3] * a.scale + bias[e >> 2][e & 3]) - off;
     }
   } else {
     const float scale = a.scale * kLog2e;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
-      x[t] *= scale;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        x[t][e] = x[t][e] * scale - off;
   }
   if (j0 + 39 > last) {
 #pragma unroll
@@ -538,9 +544,12 @@ __device__ __forceinline__ void ToScores(const TrainAttention &a, std::int64_t b
   }
 }
 
+// Waves a SIMD that registers have to allow.
+template <int DT, int DP> constexpr int kWaves = DT == DT_F32 && DP == 128 ? 1 : 2;
+
 // N sets of 16 rows a wave.  ONE: all keys in one tile.
 template <int DT, int DP, int N, int BIAS, bool ONE>
-__global__ __launch_bounds__(256, N) void ForwardKernel(Args s) {
+__global__ __launch_bounds__(256, (kWaves<DT, DP>)) void ForwardKernel(Args s) {
   using M = Mat<DT>;
   constexpr int LD = kLd<DT, DP>;
   __shared__ __attribute__((aligned(16))) typename M::T ks[kTile * LD], vs[kTile * LD];
@@ -573,7 +582,6 @@ __global__ __launch_bounds__(256, N) void ForwardKernel(Args s) {
     most[n] = -__builtin_inff();
     total[n] = 0.f;
   }
-  constexpr float units = kUnits<BIAS>;
   for (int step = begin; step < end; ++step) {
     kt.Store(ks);
     vt.Store(vs);
@@ -583,11 +591,10 @@ __global__ __launch_bounds__(256, N) void ForwardKernel(Args s) {
       vt.Keys(a.v, l, (step + 1) * kTile, a.dim);
     }
     f32x4 x[N][4];
-    Fill(x[0], 4 * N, 0.f);
-    Products<DT, DP, N>(ks, qf, lane, x);
+    Products<DT, DP, N, false>(ks, qf, lane, x);
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      ToScores<BIAS>(a, bias_at[n], step * kTile + 8 * g, w[n].last, x[n]);
+      ToScores<BIAS>(a, bias_at[n], step * kTile + 8 * g, w[n].last, 0.f, x[n]);
       float top = most[n];
 #pragma unroll
       for (int t = 0; t < 4; ++t)
@@ -596,14 +603,14 @@ __global__ __launch_bounds__(256, N) void ForwardKernel(Args s) {
           top = fmaxf(top, x[n][t][e]);
       top = OverRows(top, true);
       const float base = top == -__builtin_inff() ? 0.f : top;
-      const float old = Exp2((most[n] - base) * units);
+      const float old = Exp<BIAS>(most[n] - base);
       most[n] = top;
       total[n] *= old;
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          x[n][t][e] = Exp2((x[n][t][e] - base) * units);
+          x[n][t][e] = Exp<BIAS>(x[n][t][e] - base);
           total[n] += x[n][t][e];
         }
       if constexpr (!ONE) {
@@ -656,6 +663,46 @@ __global__ __launch_bounds__(256, N) void ForwardKernel(Args s) {
 }
 
 constexpr int kMostSplits = 256;
+constexpr int kFewSplits = 8;
+
+// Joins up to kFewSplits splits of a forward pass: four elements a thread, each
+// of which forms its row's weights.
+template <int DT>
+__global__ __launch_bounds__(256) void JoinFewKernel(Args s) {
+  const std::int64_t n = static_cast<std::int64_t>(s.lines) * s.rows;
+  const std::int64_t id = static_cast<std::int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int across = s.a.dim / 4;
+  const std::int64_t flat = id / across;
+  const int c = static_cast<int>(id % across);
+  if (flat >= n)
+    return;
+  const float *st = s.partials + s.splits * n * s.a.dim;
+  f32x4 v[kFewSplits];
+  float most[kFewSplits], total[kFewSplits], top = -__builtin_inff();
+#pragma unroll
+  for (int k = 0; k < kFewSplits; ++k) {
+    const int i = min(k, s.splits - 1);
+    most[k] = st[(i * n + flat) * 2];
+    total[k] = st[(i * n + flat) * 2 + 1];
+    v[k] = *reinterpret_cast<const f32x4 *>(s.partials + (i * n + flat) * s.a.dim + 4 * c);
+    top = fmaxf(top, most[k]);
+  }
+  const float base = top == -__builtin_inff() ? 0.f : top;
+  f32x4 o{0.f, 0.f, 0.f, 0.f};
+  float sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < kFewSplits; ++k)
+    if (k < s.splits) {
+      const float w = Exp2((most[k] - base) * kLog2e);
+      sum += total[k] * w;
+      o += v[k] * w;
+    }
+  const int line = static_cast<int>(flat / s.rows), r = static_cast<int>(flat % s.rows);
+  const int b = line / s.a.kv_heads, head = line % s.a.kv_heads * s.a.group + r / s.a.q_len;
+  ToMemory<DT>(Out<DT>(s.a.out, b, head, r % s.a.q_len) + 4 * c, o * (sum == 0.f ? 0.f : 1.f / sum));
+  if (s.a.lse && c == 0)
+    s.a.lse[flat] = sum == 0.f ? -__builtin_inff() : top + kLn2 * __builtin_amdgcn_logf(sum);
+}
 
 // Joins the splits of a forward pass: a workgroup a row.  All lanes form the
 // splits' weights, then groups of lanes that hold a row add every so many splits.
@@ -731,7 +778,7 @@ __device__ __forceinline__ float Delta(const typename Mat<DT>::Frag *out,
 
 // delta of each row, then dq (and dbias) of a tile of rows over the keys.
 template <int DT, int DP, int N, int BIAS>
-__global__ __launch_bounds__(256, N) void BackwardRowsKernel(Args s) {
+__global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardRowsKernel(Args s) {
   using M = Mat<DT>;
   constexpr int LD = kLd<DT, DP>;
   __shared__ __attribute__((aligned(16))) typename M::T ks[kTile * LD], vs[kTile * LD];
@@ -773,7 +820,6 @@ __global__ __launch_bounds__(256, N) void BackwardRowsKernel(Args s) {
   }
   if (!a.dq.p && !a.dbias)
     return;
-  constexpr float units = kUnits<BIAS>;
   for (int step = begin; step < end; ++step) {
     kt.Store(ks);
     vt.Store(vs);
@@ -783,21 +829,20 @@ __global__ __launch_bounds__(256, N) void BackwardRowsKernel(Args s) {
       vt.Keys(a.v, l, (step + 1) * kTile, a.dim);
     }
     f32x4 x[N][4], dp[N][4];
-    Fill(x[0], 4 * N, 0.f);
 #pragma unroll
     for (int n = 0; n < N; ++n)
       Fill(dp[n], 4, -delta[n]);
-    Products<DT, DP, N>(ks, qf, lane, x);
-    Products<DT, DP, N>(vs, df, lane, dp);
+    Products<DT, DP, N, false>(ks, qf, lane, x);
+    Products<DT, DP, N, true>(vs, df, lane, dp);
     const int j0 = step * kTile + 8 * g;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      ToScores<BIAS>(a, bias_at[n], j0, w[n].last, x[n]);
+      ToScores<BIAS>(a, bias_at[n], j0, w[n].last, lse[n], x[n]);
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          x[n][t][e] = Exp2((x[n][t][e] - lse[n]) * units) * dp[n][t][e];
+          x[n][t][e] = Exp<BIAS>(x[n][t][e]) * dp[n][t][e];
       if (BIAS && a.dbias && w[n].live) {
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -837,14 +882,14 @@ __global__ __launch_bounds__(256, N) void BackwardRowsKernel(Args s) {
 // What a workgroup of the keys' kernel holds of its 64 rows, next to the tiles.
 struct RowInfo {
   __attribute__((aligned(16))) int last[kTile];
-  __attribute__((aligned(16))) float lse[kTile], delta[kTile];
+  __attribute__((aligned(16))) float lse[kTile], delta[kTile];  // delta negated
   std::int64_t bias[kTile];
 };
 
 // dk and dv of a tile of keys over the rows that share them; each wave has N
 // times 16 keys and holds them, and rows go through LDS.
 template <int DT, int DP, int N, int BIAS>
-__global__ __launch_bounds__(256, N) void BackwardKeysKernel(Args s) {
+__global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardKeysKernel(Args s) {
   using M = Mat<DT>;
   constexpr int LD = kLd<DT, DP>;
   __shared__ __attribute__((aligned(16))) typename M::T qs[kTile * LD], dos[kTile * LD];
@@ -897,7 +942,7 @@ __global__ __launch_bounds__(256, N) void BackwardKeysKernel(Args s) {
       my_delta = 0.f;
       if (w.last >= 0) {
         my_lse = Lse<BIAS>(a.lse[flat]);
-        my_delta = s.delta[flat];
+        my_delta = -s.delta[flat];
       }
       my_bias = BIAS ? BiasAt(a, l.b, w.head, w.q) : 0;
     }
@@ -920,10 +965,9 @@ __global__ __launch_bounds__(256, N) void BackwardKeysKernel(Args s) {
     if (step < end)
       load(step);
     f32x4 x[N][4], dp[N][4];
-    Fill(x[0], 4 * N, 0.f);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      dp[0][t] = -*reinterpret_cast<const f32x4 *>(info.delta + RowOf64(t, 4 * g));
+      dp[0][t] = *reinterpret_cast<const f32x4 *>(info.delta + RowOf64(t, 4 * g));
 #pragma unroll
       for (int n = 1; n < N; ++n)
         dp[n][t] = dp[0][t];
@@ -944,8 +988,8 @@ __global__ __launch_bounds__(256, N) void BackwardKeysKernel(Args s) {
                     : OfHalf(a.bias_dtype, ((const MFH_GLOBAL std::uint16_t *)a.bias)[at]);
           }
     }
-    Products<DT, DP, N>(qs, kf, lane, x);
-    Products<DT, DP, N>(dos, vf, lane, dp);
+    Products<DT, DP, N, false>(qs, kf, lane, x);
+    Products<DT, DP, N, true>(dos, vf, lane, dp);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const int at = RowOf64(t, 4 * g);
@@ -1043,15 +1087,17 @@ __global__ __launch_bounds__(256) void JoinBackwardKernel(Args s) {
 
 // The whole backward pass of a head of up to 64 queries and 64 keys, none of
 // them shared: one workgroup, each input read once.  A wave has 16 queries while
-// scores, probabilities, dS and dq are formed, and 16 keys for dk and dv; P and dS
-// change hands through LDS.
+// scores, probabilities, dS and dq are formed, and 16 keys for dk and dv; P and
+// then dS change hands through a tile of LDS that held V before (256 x 16 heads of
+// 64 elements, bf16 with a bias: 79 us; with tiles of their own, and so two
+// workgroups a CU instead of four, 84).
 template <int DT, int DP, int BIAS>
-__global__ __launch_bounds__(256) void SquareBackwardKernel(Args s) {
+__global__ __launch_bounds__(256, 2) void SquareBackwardKernel(Args s) {
   using M = Mat<DT>;
   constexpr int LD = kLd<DT, DP>, LP = kLd<DT, kTile>;
-  __shared__ __attribute__((aligned(16))) typename M::T ks[kTile * LD], vs[kTile * LD],
-      qs[kTile * LD], dos[kTile * LD];
-  __shared__ __attribute__((aligned(16))) typename M::T ps[kTile * LP], dss[kTile * LP];
+  __shared__ __attribute__((aligned(16))) typename M::T ks[kTile * LD], qs[kTile * LD],
+      dos[kTile * LD], ps[kTile * (LP > LD ? LP : LD)];
+  typename M::T *vs = ps;  // until the products with V are done
   Part part;
   if (!PartOf(s, &part))
     return;
@@ -1082,20 +1128,18 @@ __global__ __launch_bounds__(256) void SquareBackwardKernel(Args s) {
   if (w.live && g == 0)
     s.delta[flat] = delta;
   const float lse = w.last >= 0 ? Lse<BIAS>(a.lse[flat]) : __builtin_inff();
-  constexpr float units = kUnits<BIAS>;
   const std::int64_t bias_at = BIAS ? BiasAt(a, l.b, w.head, w.q) : 0;
   __syncthreads();
   f32x4 xs[1][4], dps[1][4], *x = xs[0], *dp = dps[0];
-  Fill(x, 4, 0.f);
   Fill(dp, 4, -delta);
-  Products<DT, DP, 1>(ks, qf, lane, xs);
-  Products<DT, DP, 1>(vs, df, lane, dps);
-  ToScores<BIAS>(a, bias_at, 8 * g, w.last, x);
+  Products<DT, DP, 1, false>(ks, qf, lane, xs);
+  Products<DT, DP, 1, true>(vs, df, lane, dps);
+  ToScores<BIAS>(a, bias_at, 8 * g, w.last, lse, x);
 #pragma unroll
   for (int t = 0; t < 4; ++t)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      x[t][e] = Exp2((x[t][e] - lse) * units);
+      x[t][e] = Exp<BIAS>(x[t][e]);
       dp[t][e] *= x[t][e];
     }
   if (BIAS && a.dbias && w.live) {
@@ -1103,40 +1147,42 @@ __global__ __launch_bounds__(256) void SquareBackwardKernel(Args s) {
     for (int u = 0; u < 2; ++u)
       StoreBias8<BIAS>(a, bias_at, 8 * g + 32 * u, dp + 2 * u);
   }
-  f32x4 acc[DP / 16], more[DP / 16];
+  f32x4 acc[DP / 16];
   Fill(acc, DP / 16, 0.f);
+  typename M::Frag ds[2];
+  __syncthreads();
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    const typename M::Frag ds = M::Pack(dp[2 * u], dp[2 * u + 1]);
+    ds[u] = M::Pack(dp[2 * u], dp[2 * u + 1]);
     ToRow<DT>(ps + mine * LP + 32 * u + 8 * g, M::Pack(x[2 * u], x[2 * u + 1]));
-    ToRow<DT>(dss + mine * LP + 32 * u + 8 * g, ds);
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i)
-      acc[i] = M::Mul(HeadColumns<DT, DP, LD>(ks, 32 * u, i, lane), ds, acc[i]);
+      acc[i] = M::Mul(HeadColumns<DT, DP, LD>(ks, 32 * u, i, lane), ds[u], acc[i]);
   }
   if (w.live && a.dq.p)
     StoreHead<DT, DP>(Out<DT>(a.dq, l.b, w.head, w.q), lane, a.dim, acc, a.scale);
   if (!a.dk.p && !a.dv.p)
     return;
-  __syncthreads();
-  Fill(acc, DP / 16, 0.f);
-  Fill(more, DP / 16, 0.f);
+  // The wave's 16 keys' column sums of P and then of dS, each times a tile.
+  const auto over_rows = [&](const typename M::T *tile, const HeadsView &out, float scale) {
+    __syncthreads();
+    Fill(acc, DP / 16, 0.f);
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const typename M::Frag p = Columns<DT, LP>(ps, 32 * u, 4, 16 * wave, lane),
-                           ds = Columns<DT, LP>(dss, 32 * u, 4, 16 * wave, lane);
+    for (int u = 0; u < 2; ++u) {
+      const typename M::Frag p = Columns<DT, LP>(ps, 32 * u, 4, 16 * wave, lane);
 #pragma unroll
-    for (int i = 0; i < DP / 16; ++i) {
-      acc[i] = M::Mul(HeadColumns<DT, DP, LD>(qs, 32 * u, i, lane), ds, acc[i]);
-      more[i] = M::Mul(HeadColumns<DT, DP, LD>(dos, 32 * u, i, lane), p, more[i]);
+      for (int i = 0; i < DP / 16; ++i)
+        acc[i] = M::Mul(HeadColumns<DT, DP, LD>(tile, 32 * u, i, lane), p, acc[i]);
     }
-  }
-  if (mine >= a.k_len)
-    return;
-  if (a.dk.p)
-    StoreHead<DT, DP>(Out<DT>(a.dk, l.b, l.kv, mine), lane, a.dim, acc, a.scale);
-  if (a.dv.p)
-    StoreHead<DT, DP>(Out<DT>(a.dv, l.b, l.kv, mine), lane, a.dim, more, 1.f);
+    if (mine < a.k_len && out.p)
+      StoreHead<DT, DP>(Out<DT>(out, l.b, l.kv, mine), lane, a.dim, acc, scale);
+  };
+  over_rows(dos, a.dv, 1.f);
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+    ToRow<DT>(ps + mine * LP + 32 * u + 8 * g, ds[u]);
+  over_rows(qs, a.dk, a.scale);
 }
 
 // The gradient of a bias that lines or heads share: a workgroup has 64 queries
@@ -1201,8 +1247,9 @@ __global__ __launch_bounds__(256) void BiasGradKernel(Args s, int plane_heads, s
 
 // Workgroups that fill the card twice; a split loops over two tiles at least.
 inline int SplitsOf(std::int64_t groups, int steps) {
-  const std::int64_t want =
-      std::min<std::int64_t>(512 / std::max<std::int64_t>(groups, 1), kMostSplits);
+  const std::int64_t g = std::max<std::int64_t>(groups, 1);
+  const std::int64_t want = std::min<std::int64_t>(
+      std::max<std::int64_t>(512 / g, std::min<std::int64_t>(1024 / g, steps / 16)), kMostSplits);
   return static_cast<int>(std::max<std::int64_t>(1, std::min<std::int64_t>(want, steps / 2)));
 }
 inline int Tiles(int n, int wide = 1) {
@@ -1226,7 +1273,7 @@ inline Args ArgsOf(const TrainAttention &a, bool keys) {
   // leaves work for half of the card and registers hold them.
   const bool fits =
       (a.dim <= 32 || (a.dim <= 64 && a.dtype != DT_F32)) && HowBias(a) != kValues;
-  s.wide = fits && static_cast<std::int64_t>(s.lines) * Tiles(across, 2) >= 128 ? 2 : 1;
+  s.wide = fits && static_cast<std::int64_t>(s.lines) * Tiles(across, 2) >= (keys && a.bias ? 128 : 1024) ? 2 : 1;
   s.tiles = Tiles(across, s.wide);
   s.steps = keys ? Tiles(s.rows) : Tiles(a.k_len);
   s.splits = SplitsOf(static_cast<std::int64_t>(s.lines) * s.tiles, s.steps);
@@ -1311,15 +1358,18 @@ hipError_t Forward(const TrainAttention &a, hipStream_t stream) {
   } else {
     e = Run(ForwardKernel<DT, DP, 1, BIAS, false>, s, stream);
   }
-  if (e == hipSuccess && s.splits > 1)
-    e = RunJoin(JoinForwardKernel<DT>, s, static_cast<std::int64_t>(s.lines) * s.rows, stream);
+  const std::int64_t rows = static_cast<std::int64_t>(s.lines) * s.rows;
+  if (e == hipSuccess && s.splits > kFewSplits)
+    e = RunJoin(JoinForwardKernel<DT>, s, rows, stream);
+  else if (e == hipSuccess && s.splits > 1)
+    e = RunJoin(JoinFewKernel<DT>, s, (rows * (a.dim / 4) + 255) / 256, stream);
   return e;
 }
 
 template <int DT, int DP, int BIAS>
 hipError_t Backward(const TrainAttention &a, hipStream_t stream) {
   constexpr int kWide = kTwo<DT, DP> && BIAS != kValues ? 2 : 1;
-  constexpr bool kSquare = kTwo<DT, DP>;  // six tiles in LDS, two workgroups a CU
+  constexpr bool kSquare = DT != DT_F32 || DP < 128;  // four tiles in LDS, two workgroups a CU
   Args s = ArgsOf(a, false);
   s.delta = static_cast<float *>(a.workspace);
   s.partials = reinterpret_cast<float *>(static_cast<char *>(a.workspace) + DeltaBytes(s));
