@@ -91,7 +91,7 @@ def run(dev, rows, width, dtype, residual=True, alpha=0.43, affine=True, eps=1e-
 
 # Every lane count and its borders: 16, 64, 256, 1024 lanes, rows read again.
 WIDTHS = (1, 3, 8, 63, 64, 65, 127, 129, 256, 500, 511, 513, 1023, 1024, 1025, 2047, 4096, 4099,
-          8191, 16383, 16384, 16385, 20001)
+          8191, 16383, 16384, 16385, 20001, 32768, 40001)
 
 
 @pytest.mark.parametrize("dtype", lu.HALF)
