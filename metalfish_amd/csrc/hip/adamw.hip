@@ -4,9 +4,11 @@
 //   param = param (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
 // Bound by memory: with states and gradients in 32 bits a weight costs 28
-// bytes, with states in 8 bits 16 and less.  The tensors are cut into chunks of
-// kAdamChunk values, listed once per set, and a workgroup takes whole chunks;
-// every value is read and written once, in whole vectors.
+// bytes (159 M of them 753 us, 5.9 TB/s), with states in 8 bits, bf16 gradients
+// and a bf16 copy 16 (427 us, 6.0 TB/s; the vector unit is busy four fifths of that).
+// The tensors are cut into chunks of kAdamChunk values, listed once per set, and a
+// workgroup takes whole chunks; every value is read and written once, in whole
+// vectors.
 //
 // States in 8 bits are codes in blocks of kAdamBlock values with one fp32 scale
 // each.  A block is four values a lane of one wave, so its largest value is one
@@ -25,13 +27,19 @@
 namespace mfh {
 namespace {
 
-constexpr int kMaxGroups = 4096;
+// A workgroup a chunk, up to this many: 159 M weights with a bf16 copy, bf16
+// gradients and states in 8 bits 427 us, on 8192 workgroups that loop 470; all in
+// 32 bits 753 and 801.
+constexpr int kMaxGroups = 1 << 20;
 constexpr int kPer = 4;                          // consecutive values of a lane
 constexpr int kDeep = kAdamChunk / (256 * kPer);  // such runs of a lane in a chunk
 static_assert(kAdamBlock == 64 * kPer, "a block is one run of a wave");
 
 typedef unsigned int u32x2_a2 __attribute__((ext_vector_type(2), aligned(2), may_alias));
 typedef unsigned int u32_a1 __attribute__((aligned(1), may_alias));
+
+// How states are held: in 32 bits, or in 8 rounded to nearest or stochastically.
+enum : int { kFull, kNearest, kStochastic };
 
 // Uniform over the launch.
 struct Step {
@@ -43,7 +51,7 @@ struct Step {
   const double *sumsq;
   double max_norm;
   float b1, c1, b2, c2, eps, rbc2;  // c = 1 - b, rbc2 = 1 / sqrt(1 - b2^t)
-  bool skip, stochastic;
+  bool skip;
   std::uint64_t seed;
 };
 
@@ -167,19 +175,20 @@ __device__ __forceinline__ float WaveMaxBits(unsigned v) {
 // Code of x >= 0 over its scale, already multiplied by the power of two that
 // takes the code's smallest normal number to fp32's: exponent and three bits
 // of mantissa are then the bits above 20, subnormal codes those of a subnormal
-// number.  `up`: what the twenty bits below are rounded with (nearest: half
-// less a unit, plus the code's last bit).
-__device__ __forceinline__ unsigned CodeOf(float y, bool nearest, unsigned up, unsigned most) {
+// number.  The twenty bits below are rounded to nearest, ties to even, or
+// (STOCHASTIC) up by `up`.
+template <bool STOCHASTIC>
+__device__ __forceinline__ unsigned CodeOf(float y, unsigned up, unsigned most) {
   const unsigned bits = __float_as_uint(y);
-  const unsigned code = (bits + (nearest ? 0x7FFFFu + ((bits >> 20) & 1u) : up)) >> 20;
-  return code < most ? code : most;
+  const unsigned add = STOCHASTIC ? up : 0x7FFFFu + ((bits >> 20) & 1u);
+  return min((bits + add) >> 20, most);
 }
 
 // 32 bits that look random, from a value's place and the step's key: odd
 // multipliers (the golden ratio, the square roots of 3 and 2) with shifts in
-// between.
-__device__ __forceinline__ unsigned RandomBits(unsigned at, unsigned key_low, unsigned key_high) {
-  unsigned x = (at ^ key_low) * 0x9E3779B1u;
+// between.  `x`: the place, with the key's low bits, times the first of them.
+constexpr unsigned kGolden = 0x9E3779B1u;
+__device__ __forceinline__ unsigned RandomBits(unsigned x, unsigned key_high) {
   x ^= x >> 15;
   x = x * 0xBB67AE85u + key_high;
   x ^= x >> 13;
@@ -187,17 +196,25 @@ __device__ __forceinline__ unsigned RandomBits(unsigned at, unsigned key_low, un
   return x ^ (x >> 16);
 }
 
+// Square root on the vector unit's own (1 ulp), which takes no subnormal
+// numbers.
+__device__ __forceinline__ float Sqrt(float v) {
+  const bool small = v < 0x1p-96f;
+  const float r = __builtin_amdgcn_sqrtf(small ? v * 0x1p64f : v);
+  return small ? r * 0x1p-32f : r;
+}
+
 struct Uniform {
   Factor f;
   double lr, size;
   float b1, c1, b2, c2, eps, rbc2;
-  bool stochastic;
   unsigned key_low, key_high;
 };
 
-template <int PDT, int GDT, bool EIGHT, bool FULL, bool PAST>
+template <int PDT, int GDT, int STATE, bool FULL, bool PAST>
 __device__ __forceinline__ void DoChunk(const AdamChunk &c, const Uniform &u) {
 #pragma clang fp contract(off)
+  constexpr bool EIGHT = STATE != kFull;
   const float size = static_cast<float>(u.size * c.lr_scale);
   const float keep = static_cast<float>(1.0 - u.lr * c.lr_scale * c.weight_decay);
   const int lane_at = threadIdx.x * kPer;
@@ -242,8 +259,9 @@ __device__ __forceinline__ void DoChunk(const AdamChunk &c, const Uniform &u) {
       const float gr = (g[j][e] * u.f.high) * u.f.low;
       m[j][e] = m[j][e] * u.b1 + gr * u.c1;
       v[j][e] = v[j][e] * u.b2 + (gr * gr) * u.c2;
-      const float denom = sqrtf(v[j][e]) * u.rbc2 + u.eps;
-      p[j][e] = p[j][e] * keep - size * (m[j][e] / denom);
+      const float denom = __builtin_fmaf(Sqrt(v[j][e]), u.rbc2, u.eps);
+      const float update = m[j][e] * __builtin_amdgcn_rcpf(denom);
+      p[j][e] = __builtin_fmaf(-size, update, p[j][e] * keep);
       if constexpr (EIGHT) {
         if (FULL || e < n) {
           m_most = max(m_most, __float_as_uint(m[j][e]) & 0x7FFFFFFFu);
@@ -269,59 +287,84 @@ __device__ __forceinline__ void DoChunk(const AdamChunk &c, const Uniform &u) {
     if constexpr (!EIGHT) {
       Store4<DT_F32, FULL, PAST>(c.m, at, n, m[j]);
       Store4<DT_F32, FULL, PAST>(c.v, at, n, v[j]);
-      continue;
+    } else {
+      const float m_scale = WaveMaxBits(m_most) * (1.f / 448.f);
+      const float v_scale = WaveMaxBits(v_most) * (1.f / 122880.f);
+      ms[j] = m_scale < 0x1p-100f ? 0x1p-100f : m_scale;  // NaN stays
+      vs[j] = v_scale < 0x1p-120f ? 0x1p-120f : v_scale;
     }
-    const int block = at / kAdamBlock;
-    float m_scale = WaveMaxBits(m_most) * (1.f / 448.f);
-    float v_scale = WaveMaxBits(v_most) * (1.f / 122880.f);
-    m_scale = m_scale < 0x1p-100f ? 0x1p-100f : m_scale;  // NaN stays
-    v_scale = v_scale < 0x1p-120f ? 0x1p-120f : v_scale;
-    const float m_inv = 1.f / m_scale, v_inv = 1.f / v_scale;
-    unsigned m_out = 0, v_out = 0;
-    const std::uint64_t place = static_cast<std::uint64_t>(c.first_block) * kAdamBlock + at;
-    const unsigned key_low = u.key_low ^ static_cast<unsigned>(place >> 32) * 0x6A09E667u;
+  }
+  if constexpr (EIGHT) {
+    // The reciprocals of all the wave's scales in one division: lane 2 j has m's of
+    // run j, lane 2 j + 1 v's.
+    const int lane = threadIdx.x & 63;
+    float scale = 1.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      unsigned r = 0;
-      if (u.stochastic)
-        r = RandomBits(static_cast<unsigned>(place) + e, key_low, u.key_high);
-      const float x = m[j][e] * m_inv, y = v[j][e] * v_inv;
-      unsigned a = CodeOf(fabsf(x) * 0x1p-120f, !u.stochastic, (r & 0xFFFFu) << 4, 0x7Eu);
-      if (x < 0.f)
-        a |= 0x80u;
-      unsigned b = CodeOf(y * 0x1p-112f, !u.stochastic, (r >> 16) << 4, 0xFFu);
-      if (b == 0 && v[j][e] > 0.f)
-        b = 1;
-      m_out |= a << (8 * e);
-      v_out |= b << (8 * e);
+    for (int j = 0; j < kDeep; ++j) {
+      scale = lane == 2 * j ? ms[j] : scale;
+      scale = lane == 2 * j + 1 ? vs[j] : scale;
     }
-    StoreCodes<FULL, PAST>(c.m, at, n, m_out);
-    StoreCodes<FULL, PAST>(c.v, at, n, v_out);
-    if ((threadIdx.x & 63) == 0) {
-      ((MFH_GLOBAL float *)c.m_scale)[block] = m_scale;
-      ((MFH_GLOBAL float *)c.v_scale)[block] = v_scale;
+    const int inverse = __float_as_int(1.f / scale);
+    // Places of a run differ in their two last bits, so their products with the
+    // first multiplier differ by what the key's last bits say.
+    unsigned steps[4];
+#pragma unroll
+    for (unsigned e = 0; e < 4; ++e)
+      steps[e] = (((u.key_low ^ e) & 3u) - (u.key_low & 3u)) * kGolden;
+#pragma unroll
+    for (int j = 0; j < kDeep; ++j) {
+      const int at = j * 256 * kPer + lane_at, n = c.count - at;
+      if (!FULL && j * 256 * kPer + (lane_at & ~(kAdamBlock - 1)) >= c.count)
+        break;
+      const float m_inv = __int_as_float(__builtin_amdgcn_readlane(inverse, 2 * j)),
+                  v_inv = __int_as_float(__builtin_amdgcn_readlane(inverse, 2 * j + 1));
+      unsigned m_out = 0, v_out = 0, first = 0;
+      if constexpr (STATE == kStochastic) {
+        const std::uint64_t place = static_cast<std::uint64_t>(c.first_block) * kAdamBlock + at;
+        const unsigned key = u.key_low ^ static_cast<unsigned>(place >> 32) * 0x6A09E664u;
+        first = (static_cast<unsigned>(place) ^ key) * kGolden;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        unsigned r = 0;
+        if constexpr (STATE == kStochastic)
+          r = RandomBits(first + steps[e], u.key_high);
+        const float x = m[j][e] * m_inv, y = v[j][e] * v_inv;
+        unsigned a = CodeOf<STATE == kStochastic>(fabsf(x) * 0x1p-120f, (r & 0xFFFFu) << 4, 0x7Eu);
+        a |= x < 0.f ? 0x80u : 0u;
+        unsigned b = CodeOf<STATE == kStochastic>(y * 0x1p-112f, (r >> 16) << 4, 0xFFu);
+        b = max(b, v[j][e] > 0.f ? 1u : 0u);
+        m_out |= a << (8 * e);
+        v_out |= b << (8 * e);
+      }
+      StoreCodes<FULL, PAST>(c.m, at, n, m_out);
+      StoreCodes<FULL, PAST>(c.v, at, n, v_out);
+      if (lane == 0) {
+        ((MFH_GLOBAL float *)c.m_scale)[at / kAdamBlock] = ms[j];
+        ((MFH_GLOBAL float *)c.v_scale)[at / kAdamBlock] = vs[j];
+      }
     }
   }
 }
 
-template <int PDT, int GDT, bool EIGHT, bool PAST>
+template <int PDT, int GDT, int STATE, bool PAST>
 __device__ __forceinline__ void AnyChunk(const AdamChunk &c, const Uniform &u) {
   if (c.count == kAdamChunk)
-    DoChunk<PDT, GDT, EIGHT, true, PAST>(c, u);
+    DoChunk<PDT, GDT, STATE, true, PAST>(c, u);
   else
-    DoChunk<PDT, GDT, EIGHT, false, PAST>(c, u);
+    DoChunk<PDT, GDT, STATE, false, PAST>(c, u);
 }
-template <int PDT, bool EIGHT, bool PAST>
+template <int PDT, int STATE, bool PAST>
 __device__ __forceinline__ void ByGrad(const AdamChunk &c, const Uniform &u) {
   if (c.grad_dtype == DT_F32)
-    AnyChunk<PDT, DT_F32, EIGHT, PAST>(c, u);
+    AnyChunk<PDT, DT_F32, STATE, PAST>(c, u);
   else if (c.grad_dtype == DT_BF16)
-    AnyChunk<PDT, DT_BF16, EIGHT, PAST>(c, u);
+    AnyChunk<PDT, DT_BF16, STATE, PAST>(c, u);
   else
-    AnyChunk<PDT, DT_F16, EIGHT, PAST>(c, u);
+    AnyChunk<PDT, DT_F16, STATE, PAST>(c, u);
 }
 
-template <bool EIGHT, bool PAST>
+template <int STATE, bool PAST>
 __global__ __launch_bounds__(256) void AdamWKernel(const AdamChunk *list, std::int64_t n, Step s) {
   const auto *chunks = (const MFH_CONSTANT AdamChunk *)list;
   Uniform u;
@@ -354,7 +397,6 @@ __global__ __launch_bounds__(256) void AdamWKernel(const AdamChunk *list, std::i
   u.b2 = s.b2;
   u.c2 = s.c2;
   u.eps = s.eps;
-  u.stochastic = s.stochastic;
   std::uint64_t key = s.seed + static_cast<std::uint64_t>(step) * 0x9E3779B97F4A7C15ull;
   key ^= key >> 29;
   u.key_low = static_cast<unsigned>(key);
@@ -376,11 +418,11 @@ __global__ __launch_bounds__(256) void AdamWKernel(const AdamChunk *list, std::i
     c.lr_scale = chunks[k].lr_scale;
     c.weight_decay = chunks[k].weight_decay;
     if (c.param_dtype == DT_F32)
-      ByGrad<DT_F32, EIGHT, PAST>(c, u);
+      ByGrad<DT_F32, STATE, PAST>(c, u);
     else if (c.param_dtype == DT_BF16)
-      ByGrad<DT_BF16, EIGHT, PAST>(c, u);
+      ByGrad<DT_BF16, STATE, PAST>(c, u);
     else
-      ByGrad<DT_F16, EIGHT, PAST>(c, u);
+      ByGrad<DT_F16, STATE, PAST>(c, u);
   }
 }
 
@@ -414,16 +456,17 @@ hipError_t LaunchAdamW(const AdamChunk *chunks, std::int64_t n_chunks, bool eigh
   s.c2 = static_cast<float>(1.0 - p.beta2);
   s.eps = static_cast<float>(p.eps);
   s.skip = p.skip_nonfinite;
-  s.stochastic = p.stochastic;
   s.seed = p.seed;
   const dim3 grid(static_cast<unsigned>(std::min<std::int64_t>(n_chunks, kMaxGroups)));
   const auto launch = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, chunks, n_chunks, s);
   };
-  if (eight)
-    past ? launch(AdamWKernel<true, true>) : launch(AdamWKernel<true, false>);
+  if (!eight)
+    past ? launch(AdamWKernel<kFull, true>) : launch(AdamWKernel<kFull, false>);
+  else if (p.stochastic)
+    past ? launch(AdamWKernel<kStochastic, true>) : launch(AdamWKernel<kStochastic, false>);
   else
-    past ? launch(AdamWKernel<false, true>) : launch(AdamWKernel<false, false>);
+    past ? launch(AdamWKernel<kNearest, true>) : launch(AdamWKernel<kNearest, false>);
   return hipGetLastError();
 }
 

@@ -64,7 +64,7 @@ class Tensor:
         # the states; bits of m that cancel are u of |beta1 m| + |(1 - beta1) g|.
         up = np.abs(want - self.param * (1 - lr * self.decay))
         raw = beta1 * np.abs(self.m) + (1 - beta1) * np.abs(self.grad) * factor
-        lost = up * np.where(m != 0, raw / np.maximum(np.abs(m), 1e-300), 1.0)
+        lost = up * raw / np.where(m != 0, np.abs(m).astype(np.float64), np.inf)
         tol = 4 * lu.U * np.abs(want) + 12 * lu.U * (up + lost)
         got = self.d["param"].get()
         lu.check(got, want, tol + lu.rounding(want, self.d["param"].dtype), "param")
