@@ -524,7 +524,10 @@ typedef struct {
  * p[b * bias_batch + h * bias_head + i * bias_query + j]; a stride of 0 shares
  * it.  Scores, statistics and sums are in 32 bits; with bf16 or fp16 inputs the
  * probabilities and dS are rounded to that type before they are multiplied (in
- * fp16 |dS| above 65504 becomes infinite). */
+ * fp16 |dS| above 65504 becomes infinite).  A finite bias that masks every key of
+ * a query (the type's lowest value, say) leaves it uniform over them.  A key
+ * that `causal` or a bias of -inf takes out has probability 0, which its values
+ * are still multiplied by: one that is not finite may come out as NaN. */
 typedef struct {
   int32_t batch, heads, kv_heads; /* >= 1; batch >= 0 */
   int32_t q_len, k_len;           /* >= 0; q_len heads / kv_heads, k_len <= 2^30 */

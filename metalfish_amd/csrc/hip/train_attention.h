@@ -223,6 +223,7 @@ struct Args {
   int down = 0;    // tiles from the last to the first, in so many interleaved runs
   float *partials = nullptr;
   float *delta = nullptr;  // [lines][rows]
+  float *rest = nullptr;   // [lines][rows], with a bias (Coarse)
 };
 
 __device__ __forceinline__ int Uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -781,6 +782,17 @@ template <int BIAS> __device__ __forceinline__ float Lse(float v) {
     return __builtin_inff();
   return BIAS ? v : v * kLog2e;
 }
+// A row's probabilities from a bias as large as this are too coarse by its
+// log-sum-exp alone: ln(sum) is below a rounding of it, and where a mask of the
+// type's lowest value takes every key, each would have probability 1.  Such rows
+// are divided by their own sum: the exponent of 2 gets `rest` = -log2 of that
+// added, 0 in all others.
+__device__ __forceinline__ bool Coarse(float lse) {
+  return fabsf(lse) > 256.f && fabsf(lse) < __builtin_inff();
+}
+template <int BIAS> __device__ __forceinline__ float Probability(float x, float rest) {
+  return Exp2(BIAS ? __builtin_fmaf(x, kLog2e, rest) : x);
+}
 // delta = dout . out of a row, over the four lanes that share it.
 template <int DT, int DP>
 __device__ __forceinline__ float Delta(const typename Mat<DT>::Frag *out,
@@ -818,9 +830,10 @@ __global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardRowsKernel(Args
   }
   RowOfWave w[N];
   typename M::Frag qf[N][DP / 32], df[N][DP / 32];
-  float delta[N], lse[N];
+  float delta[N], lse[N], rest[N];
   std::int64_t bias_at[N];
   f32x4 acc[N][DP / 16];
+  bool coarse = false;
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     w[n] = RowFor(s, l, first + 16 * (N * wave + n) + fr);
@@ -833,8 +846,45 @@ __global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardRowsKernel(Args
     if (w[n].live && g == 0 && part.split == 0)
       s.delta[flat] = delta[n];
     lse[n] = w[n].last >= 0 ? Lse<BIAS>(a.lse[flat]) : __builtin_inff();
+    rest[n] = 0.f;
+    coarse = coarse || Coarse(lse[n]);
     bias_at[n] = BIAS ? BiasAt(a, l.b, w[n].head, w[n].q) : 0;
     Fill(acc[n], DP / 16, 0.f);
+  }
+  if constexpr (BIAS != kNoBias) {
+    if (__syncthreads_or(coarse)) {
+      // Rare: all keys once more beforehand, for their sum.
+      float sum[N] = {};
+      for (int step = 0; step < s.steps; ++step) {
+        kt.Keys(a.k, l, step * kTile, a.dim);
+        __syncthreads();
+        kt.Store(ks);
+        __syncthreads();
+        f32x4 x[N][4];
+        Products<DT, DP, N, false>(ks, qf, lane, x);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          ToScores<BIAS>(a, bias_at[n], step * kTile + 8 * g, w[n].last, lse[n], x[n]);
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              sum[n] += Exp<BIAS>(x[n][t][e]);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const float all = OverRows(sum[n], false);
+        rest[n] = Coarse(lse[n]) ? -__builtin_amdgcn_logf(all) : 0.f;
+      }
+      __syncthreads();
+      if (begin < end)
+        kt.Keys(a.k, l, begin * kTile, a.dim);
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      if (w[n].live && g == 0 && part.split == 0)
+        s.rest[static_cast<std::int64_t>(part.line) * s.rows + w[n].r] = rest[n];
   }
   if (!a.dq.p && !a.dbias)
     return;
@@ -860,7 +910,7 @@ __global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardRowsKernel(Args
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          x[n][t][e] = Exp<BIAS>(x[n][t][e]) * dp[n][t][e];
+          x[n][t][e] = Probability<BIAS>(x[n][t][e], rest[n]) * dp[n][t][e];
       if (BIAS && a.dbias && w[n].live) {
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -900,7 +950,7 @@ __global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardRowsKernel(Args
 // What a workgroup of the keys' kernel holds of its 64 rows, next to the tiles.
 struct RowInfo {
   __attribute__((aligned(16))) int last[kTile];
-  __attribute__((aligned(16))) float lse[kTile], delta[kTile];  // delta negated
+  __attribute__((aligned(16))) float lse[kTile], delta[kTile], rest[kTile];  // delta negated
   std::int64_t bias[kTile];
 };
 
@@ -945,7 +995,7 @@ __global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardKeysKernel(Args
   };
   Stage<DT, DP> qt, dt;
   int my_last = -1;
-  float my_lse = 0.f, my_delta = 0.f;
+  float my_lse = 0.f, my_delta = 0.f, my_rest = 0.f;
   std::int64_t my_bias = 0;
   bool all_see = false;
   const auto load = [&](int step) {
@@ -961,6 +1011,8 @@ __global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardKeysKernel(Args
       if (w.last >= 0) {
         my_lse = Lse<BIAS>(a.lse[flat]);
         my_delta = -s.delta[flat];
+        if constexpr (BIAS != kNoBias)
+          my_rest = s.rest[flat];
       }
       my_bias = BIAS ? BiasAt(a, l.b, w.head, w.q) : 0;
     }
@@ -975,6 +1027,7 @@ __global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardKeysKernel(Args
       info.last[threadIdx.x] = my_last;
       info.lse[threadIdx.x] = my_lse;
       info.delta[threadIdx.x] = my_delta;
+      info.rest[threadIdx.x] = my_rest;
       info.bias[threadIdx.x] = my_bias;
     }
     __syncthreads();
@@ -1012,12 +1065,16 @@ __global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardKeysKernel(Args
     for (int t = 0; t < 4; ++t) {
       const int at = RowOf64(t, 4 * g);
       const f32x4 lse = *reinterpret_cast<const f32x4 *>(info.lse + at);
+      f32x4 rest{0.f, 0.f, 0.f, 0.f};
+      if constexpr (BIAS != kNoBias)
+        rest = *reinterpret_cast<const f32x4 *>(info.rest + at);
 #pragma unroll
       for (int n = 0; n < N; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           if constexpr (BIAS != kNoBias)
-            x[n][t][e] = Exp2((x[n][t][e] * scale + bias[n][t][e] - lse[e]) * kLog2e);
+            x[n][t][e] =
+                Probability<BIAS>(x[n][t][e] * scale + bias[n][t][e] - lse[e], rest[e]);
           else
             x[n][t][e] = Exp2(x[n][t][e] * scale - lse[e]);
         }
@@ -1153,11 +1210,26 @@ __global__ __launch_bounds__(256, 2) void SquareBackwardKernel(Args s) {
   Products<DT, DP, 1, false>(ks, qf, lane, xs);
   Products<DT, DP, 1, true>(vs, df, lane, dps);
   ToScores<BIAS>(a, bias_at, 8 * g, w.last, lse, x);
+  float rest = 0.f;
+  if constexpr (BIAS != kNoBias) {
+    if (__any(Coarse(lse))) {
+      float sum = 0.f;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          sum += Exp<BIAS>(x[t][e]);
+      sum = OverRows(sum, false);
+      rest = Coarse(lse) ? -__builtin_amdgcn_logf(sum) : 0.f;
+    }
+    if (w.live && g == 0)
+      s.rest[flat] = rest;
+  }
 #pragma unroll
   for (int t = 0; t < 4; ++t)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      x[t][e] = Exp<BIAS>(x[t][e]);
+      x[t][e] = Probability<BIAS>(x[t][e], rest);
       dp[t][e] *= x[t][e];
     }
   if (BIAS && a.dbias && w.live) {
@@ -1236,7 +1308,7 @@ __global__ __launch_bounds__(256) void BiasGradKernel(Args s, int plane_heads, s
       LoadRow<DT, DP>(s, a.q, l, w, lane, qf);
       LoadRow<DT, DP>(s, a.dout, l, w, lane, df);
       const float lse = w.last >= 0 ? Lse<BIAS>(a.lse[flat]) : __builtin_inff();
-      const float delta = w.last >= 0 ? s.delta[flat] : 0.f;
+      const float delta = w.last >= 0 ? s.delta[flat] : 0.f, rest = w.last >= 0 ? s.rest[flat] : 0.f;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         f32x4 x{0.f, 0.f, 0.f, 0.f}, dp{-delta, -delta, -delta, -delta};
@@ -1251,7 +1323,7 @@ __global__ __launch_bounds__(256) void BiasGradKernel(Args s, int plane_heads, s
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float p = Exp2((x[e] * a.scale + bias[t][e] - lse) * kLog2e);
+          const float p = Probability<BIAS>(x[e] * a.scale + bias[t][e] - lse, rest);
           acc[t][e] += j + e <= w.last ? p * dp[e] : 0.f;
         }
       }
@@ -1306,6 +1378,8 @@ inline bool SharedBias(const TrainAttention &a) {
 inline std::uint64_t DeltaBytes(const Args &s) {
   return (static_cast<std::uint64_t>(s.lines) * s.rows * 4 + 15) & ~std::uint64_t(15);
 }
+// delta, and with a bias `rest`.
+inline std::uint64_t RowValuesBytes(const Args &s) { return DeltaBytes(s) * (s.a.bias ? 2 : 1); }
 inline std::uint64_t ForwardBytes(const Args &s) {
   return s.splits == 1 ? 0
                        : static_cast<std::uint64_t>(s.splits) * s.lines * s.rows * (s.a.dim + 2) * 4;
@@ -1395,7 +1469,8 @@ hipError_t Backward(const TrainAttention &a, hipStream_t stream) {
   constexpr bool kSquare = DT != DT_F32 || DP < 128;  // four tiles in LDS, two workgroups a CU
   Args s = ArgsOf(a, false);
   s.delta = static_cast<float *>(a.workspace);
-  s.partials = reinterpret_cast<float *>(static_cast<char *>(a.workspace) + DeltaBytes(s));
+  s.rest = reinterpret_cast<float *>(static_cast<char *>(a.workspace) + DeltaBytes(s));
+  s.partials = reinterpret_cast<float *>(static_cast<char *>(a.workspace) + RowValuesBytes(s));
   const bool shared = SharedBias(a);
   if (shared)
     s.a.dbias = nullptr;
@@ -1418,6 +1493,7 @@ hipError_t Backward(const TrainAttention &a, hipStream_t stream) {
   if (e == hipSuccess && (a.dk.p || a.dv.p) && !square) {
     Args k = ArgsOf(a, true);
     k.delta = s.delta;
+    k.rest = s.rest;
     k.partials = s.partials;
     e = k.wide == 2 ? Run(BackwardKeysKernel<DT, DP, kWide, BIAS>, k, stream)
                     : Run(BackwardKeysKernel<DT, DP, 1, BIAS>, k, stream);

@@ -37,7 +37,7 @@ std::uint64_t AttentionForwardWorkspace(const TrainAttention &a) {
 
 std::uint64_t AttentionBackwardWorkspace(const TrainAttention &a) {
   const attend::Args rows = attend::ArgsOf(a, false), keys = attend::ArgsOf(a, true);
-  return attend::DeltaBytes(rows) +
+  return attend::RowValuesBytes(rows) +
          std::max(attend::RowsBytes(rows), attend::KeysBytes(keys));
 }
 

@@ -220,6 +220,50 @@ def test_masks_by_the_bias(dev, q_len, k_len, dtype):
     assert np.abs(out[0, 7, 1] - c.v[0, :, 1].mean(0)).max() < 0.05
 
 
+LOWEST = {"f32": float(np.finfo(np.float32).min), "bf16": -(2.0 - 2.0 ** -7) * 2.0 ** 127,
+          "f16": -65504.0}
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bias_dtype,mask", [("f32", LOWEST["f32"]), ("f32", -1e9), ("f32", -1e4),
+                                             ("f32", 1e9), ("bf16", LOWEST["bf16"]),
+                                             ("f16", LOWEST["f16"])])
+@pytest.mark.parametrize("q_len,k_len,shared", [(64, 64, ()), (40, 150, ()), (9, 1200, ()),
+                                                (70, 65, (0,)), (33, 64, (1,))])
+def test_rows_that_a_finite_mask_takes_whole(dev, q_len, k_len, shared, bias_dtype, mask, dtype):
+    """A row with the same large bias on every key is uniform over them, in its
+    gradients too, though ln(keys) is less than a rounding of its log-sum-exp.
+
+    Their queries are 0, so each score is the mask's value itself and p = 1 / keys
+    but for the sum's and the exponential's roundings: the bounds are those of the
+    same rows with a bias of 0."""
+    rng = np.random.default_rng(12)
+    rows = [0, 5, q_len - 1]
+    shape = [1 if i in shared else n for i, n in enumerate((2, 2, q_len, k_len))]
+    bias = rng.normal(size=shape)
+    bias[:, :, rows] = mask
+    c = Case(dev, 2, 2, q_len, k_len, 32, dtype, bias=bias, bias_dtype=bias_dtype, shared=shared)
+    c.q[:, rows] = 0.0
+    c.d["q"] = lu.Heads(dev, c.q.shape, dtype, c.q)
+    c.p.q.p = c.d["q"].p
+    (q, k, v), rest = c.oracle()
+    want = layers.attention_backward(q, k, v, c.dout, *rest)
+    plain = c.bias.copy()
+    plain[:, :, rows] = 0.0
+    flat = layers.attention(q, k, v, c.scale, plain)
+    tol = lu.attention_bounds(q, k, v, c.scale, plain, {**want, "lse": flat["lse"]}, dtype, c.dout)
+    out, _ = c.forward()
+    lu.check(out, want["out"], tol["out"], "out")
+    got = c.backward()
+    n = np.prod([want["dbias"].shape[i] for i in shared]) if shared else 1
+    tol["dbias"] = tol["dbias"].sum(shared, keepdims=True) + n * lu.U * np.abs(
+        want["dbias"]).sum(shared, keepdims=True)
+    want["dbias"] = want["dbias"].sum(shared, keepdims=True)
+    tol["dbias"] += lu.rounding(want["dbias"], bias_dtype)
+    for name in got:
+        lu.check(got[name], want[name], tol[name], name)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_large_scores(dev, dtype):
     # Scores of +-500: one key of each row holds nearly all of it.
