@@ -616,8 +616,8 @@ void mfh_adamw_set_destroy(mfh_adamw_set *set);
 typedef struct {
   double lr;           /* finite, >= 0 */
   double beta1, beta2; /* 0 <= beta < 1 */
-  double eps;          /* finite, >= 0 */
-  double grad_scale;   /* finite, > 0 */
+  double eps;          /* finite, >= 0; above 0 and below 2^-126: 2^-126 */
+  double grad_scale;   /* > 0; it and lr at most the largest float */
   int64_t step;        /* >= 1 */
   const float *d_lr;
   const int64_t *d_step;

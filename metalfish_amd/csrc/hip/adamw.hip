@@ -22,6 +22,7 @@
 #include "mfh_device.h"
 #include "mfh_kernels.h"
 
+#include <algorithm>
 #include <cmath>
 
 namespace mfh {
@@ -454,7 +455,8 @@ hipError_t LaunchAdamW(const AdamChunk *chunks, std::int64_t n_chunks, bool eigh
   s.c1 = static_cast<float>(1.0 - p.beta1);
   s.b2 = static_cast<float>(p.beta2);
   s.c2 = static_cast<float>(1.0 - p.beta2);
-  s.eps = static_cast<float>(p.eps);
+  // The unit's reciprocal of less would be infinite, and 0 times it NaN.
+  s.eps = p.eps > 0 ? std::max(static_cast<float>(p.eps), 0x1p-126f) : 0.f;
   s.skip = p.skip_nonfinite;
   s.seed = p.seed;
   const dim3 grid(static_cast<unsigned>(std::min<std::int64_t>(n_chunks, kMaxGroups)));

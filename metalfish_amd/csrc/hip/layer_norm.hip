@@ -352,48 +352,46 @@ __global__ __launch_bounds__(kBackBlock<T>) void NormBackwardKernel(NormParams p
     else
       load(row + step, &now);
   }
-  if constexpr (!kSums)
-    return;
-  else {
-  if (!p.partials)
-    return;
-  // The workgroup's rows together, in the order of its row groups.
-  float *out = p.partials + static_cast<std::int64_t>(blockIdx.x) * 2 * width;
+  if constexpr (kSums) {
+    if (!p.partials)
+      return;
+    // The workgroup's rows together, in the order of its row groups.
+    float *out = p.partials + static_cast<std::int64_t>(blockIdx.x) * 2 * width;
 #pragma unroll
-  for (int part = 0; part < 2; ++part) {
-    float *v = part ? dbeta : dgamma;
-    if constexpr (T <= 32) {
+    for (int part = 0; part < 2; ++part) {
+      float *v = part ? dbeta : dgamma;
+      if constexpr (T <= 32) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if constexpr (T == 16)
-          v[i] += __shfl_xor(v[i], 16, 64);
-        v[i] += __shfl_xor(v[i], 32, 64);
-      }
-    }
-    {
-      // A wave's rows are one by now; then those of the others, one after another.
-      constexpr int kTeams = kBackBlock<T> / (T < 64 ? 64 : T), kTeam = kBackBlock<T> / kTeams;
-      const int team = threadIdx.x / kTeam;
-      const bool mine = threadIdx.x % kTeam < T;
-      for (int w = 0; w < kTeams; ++w) {
-        __syncthreads();
-        if (team == w && mine) {
-#pragma unroll
-          for (int i = 0; i < N; ++i)
-            sums[i * T + t] = w ? sums[i * T + t] + v[i] : v[i];
+        for (int i = 0; i < N; ++i) {
+          if constexpr (T == 16)
+            v[i] += __shfl_xor(v[i], 16, 64);
+          v[i] += __shfl_xor(v[i], 32, 64);
         }
       }
-      if (team != kTeams - 1 || !mine)
-        continue;
+      {
+        // A wave's rows are one by now; then those of the others, one after another.
+        constexpr int kTeams = kBackBlock<T> / (T < 64 ? 64 : T), kTeam = kBackBlock<T> / kTeams;
+        const int team = threadIdx.x / kTeam;
+        const bool mine = threadIdx.x % kTeam < T;
+        for (int w = 0; w < kTeams; ++w) {
+          __syncthreads();
+          if (team == w && mine) {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+              sums[i * T + t] = w ? sums[i * T + t] + v[i] : v[i];
+          }
+        }
+        if (team != kTeams - 1 || !mine)
+          continue;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          v[i] = sums[i * T + t];
+      }
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        v[i] = sums[i * T + t];
+        if (i % VE >= lane.skip[i / VE])
+          out[part * width + lane.first[i / VE] + i % VE] = v[i];
     }
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (i % VE >= lane.skip[i / VE])
-        out[part * width + lane.first[i / VE] + i % VE] = v[i];
-  }
   }
 }
 
@@ -574,7 +572,6 @@ __global__ __launch_bounds__(1024) void LongNormKernel(NormParams p) {
     }
   }
 }
-
 
 template <int DT>
 __device__ __forceinline__ void StoreGrads(const NormParams &p, std::int64_t row, int c0,

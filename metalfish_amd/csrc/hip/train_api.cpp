@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <cstdint>
 #include <memory>
@@ -146,8 +147,9 @@ int CheckHeads(const char *fn, const char *name, const mfh_attention *a, const m
   if (!Aligned(v.p, es))
     return Invalid(fn, "pointers must be aligned to their elements");
   const mfh::Region r = mfh::RegionOf(name, v.p, a->dim * es, written,
-                                      {{n[0], stride[0] * es}, {n[1], stride[1] * es},
-                                       {n[2], stride[2] * es}});
+                                      {{n[0], n[0] > 1 ? stride[0] * es : 0},
+                                       {n[1], n[1] > 1 ? stride[1] * es : 0},
+                                       {n[2], n[2] > 1 ? stride[2] * es : 0}});
   if (written && !mfh::Nested(r))
     return bad("a written array has no two elements in one place");
   regions->push_back(r);
@@ -216,7 +218,7 @@ int CheckBias(const char *fn, const char *name, const mfh_attention *a, const vo
       return Invalid(fn, "bias strides must be >= 0 and the bias addressable");
     if (n[i] > 1)
       reach += (n[i] - 1) * stride[i];
-    dims.push_back({stride[i] ? n[i] : 1, stride[i] * es});
+    dims.push_back({stride[i] ? n[i] : 1, n[i] > 1 ? stride[i] * es : 0});
   }
   if (reach > kMostBytes / es)
     return Invalid(fn, "bias strides must be >= 0 and the bias addressable");
@@ -748,8 +750,8 @@ int mfh_adamw_step_device(const mfh_adamw_set *set, const mfh_adamw_step *step, 
   if (!(step->lr >= 0.0) || !std::isfinite(step->lr) || !beta(step->beta1) || !beta(step->beta2) ||
       !(step->eps >= 0.0) || !std::isfinite(step->eps))
     return Invalid(fn, "lr and eps must be finite and >= 0, beta1 and beta2 in [0, 1)");
-  if (!(step->grad_scale > 0.0) || !std::isfinite(step->grad_scale))
-    return Invalid(fn, "grad_scale must be positive and finite");
+  if (!(step->grad_scale > 0.0) || step->grad_scale > FLT_MAX || step->lr > FLT_MAX)
+    return Invalid(fn, "grad_scale must be positive, and it and lr finite in 32 bits");
   if (step->step < 1)
     return Invalid(fn, "step must be >= 1");
   if ((step->skip_nonfinite != 0 && step->skip_nonfinite != 1) ||

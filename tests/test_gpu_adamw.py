@@ -269,6 +269,15 @@ def test_stochastic_states_follow_a_falling_gradient(dev):
     assert abs(kept[True] - want) < 0.1 * want and kept[False] > 0.9
 
 
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("eps", [1e-300, 1e-45, 1e-40, 2.0 ** -126])
+def test_weights_without_gradients_stay_under_a_tiny_eps(dev, eps, eight):
+    """0 / eps is 0, however small eps is above 0 (rows that no batch has met)."""
+    rng = np.random.default_rng(15)
+    t = Tensor(dev, rng, 700, eight, fresh=True, grad=np.zeros(700), weight_decay=0.5)
+    steps(dev, [t], eight, n=2, first=1, eps=eps)
+
+
 def test_steps_that_are_refused(dev):
     rng = np.random.default_rng(13)
     t = Tensor(dev, rng, 300, False)
@@ -278,6 +287,7 @@ def test_steps_that_are_refused(dev):
     for kw in (dict(lr=-1.0), dict(lr=nan), dict(lr=float("inf")), dict(step=0), dict(step=-3),
                dict(beta1=1.0), dict(beta1=-0.1), dict(beta2=1.0), dict(beta2=nan), dict(eps=-1e-8),
                dict(eps=nan), dict(grad_scale=0.0), dict(grad_scale=-1.0), dict(grad_scale=nan),
+               dict(grad_scale=1e39), dict(lr=1e39),
                dict(max_norm=-1.0, d_sumsq=ok), dict(max_norm=nan, d_sumsq=ok),
                dict(skip_nonfinite=True), dict(d_sumsq=ok + 4), dict(d_lr=ok + 2), dict(d_step=ok + 4),
                dict(d_sumsq=t.d["grad"].p), dict(d_lr=t.d["param"].p + 4), dict(d_step=t.d["m"].p),

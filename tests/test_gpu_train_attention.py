@@ -373,6 +373,48 @@ def test_a_long_cache_beyond_32_bits(dev):
     lu.check(dk, want["dk"], tol["dk"])
 
 
+@pytest.mark.parametrize("case", [
+    dict(q_len=3, k_len=1500, kv_heads=2, causal=True, q_lengths=[3, 1], k_lengths=[1500, 900]),
+    dict(q_len=700, k_len=9), dict(q_len=200, k_len=300, bias="random", shared=(0,), causal=True),
+    dict(q_len=64, k_len=64, bias="random")])
+def test_captured_calls_give_what_eager_ones_do(dev, case):
+    """Replayed on new inputs each, with eager calls of the same problem between."""
+    c = Case(dev, 2, 4, dim=32, dtype="bf16", **case)
+    p, n = c.p, max(backend.attention_backward_workspace_bytes(c.p),
+                    backend.attention_forward_workspace_bytes(c.p))
+    grads = [lu.Heads(dev, t.shape, "bf16") for t in (c.q, c.k, c.v)]
+    ws = [dict(d_workspace=dev.alloc(n), workspace_bytes=n) for _ in range(2)]
+    if c.bias is not None:
+        for w in ws:
+            w["d_dbias"] = c.dbias.p
+
+    def call(w, stream):
+        f = {k: w[k] for k in ("d_workspace", "workspace_bytes")}
+        backend.attention_forward_device(p, c.out.p, d_lse=c.lse.p, stream=stream, **f)
+        backend.attention_backward_device(p, c.out.p, c.lse.p, c.d["dout"].p, d_dq=grads[0].p,
+                                          d_dk=grads[1].p, d_dv=grads[2].p, stream=stream, **w)
+
+    def outputs():
+        every = [c.out.get(), c.lse.bits()] + [g.get() for g in grads]
+        return every + ([c.dbias.bits()] if c.bias is not None else [])
+
+    stream = dev.stream()
+    launch = dev.capture(stream, lambda: call(ws[0], stream))
+    rng = np.random.default_rng(21)
+    seen = []
+    for _ in range(4):
+        c.d["q"].flat[c.d["q"].at] = lu.to_bits(rng.normal(size=c.q.size), "bf16").reshape(c.q.shape)
+        dev.write(c.d["q"].base, c.d["q"].flat)
+        launch()
+        dev.sync(stream)
+        got = outputs()
+        call(ws[1], None)
+        dev.sync()
+        assert all(np.array_equal(a, b) for a, b in zip(got, outputs()))
+        seen.append(got[0])
+    assert not any(np.array_equal(a, b) for a, b in zip(seen, seen[1:]))
+
+
 def test_host_memory_is_refused(dev):
     c = Case(dev, 1, 1, 4, 4, 8, "f32")
     host = np.zeros(32, np.float32)
