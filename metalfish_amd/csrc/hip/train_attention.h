@@ -354,20 +354,18 @@ __device__ __forceinline__ float OfHalf(int dtype, std::uint16_t v) {
   return dtype == DT_BF16 ? Elem<DT_BF16>::One(v) : Elem<DT_F16>::One(v);
 }
 // How a bias is read: not at all, in vectors of eight (rows of a multiple of
-// eight keys), or value by value.
-enum : int { kNoBias, kVectors, kValues };
+// eight keys) of 16 or of 32 bits a value, or value by value.
+enum : int { kNoBias, kHalves, kVectors, kValues };
 // Eight consecutive values from key j on (any of the row's where there are less).
 template <int BIAS>
 __device__ __forceinline__ void Bias8(const TrainAttention &a, std::int64_t row, int j, f32x4 *f) {
   if constexpr (BIAS == kVectors) {
-    row += min(j, a.k_len - 8);
-    if (a.bias_dtype == DT_F32) {
-      const auto *p = (ConstRow<DT_F32>)a.bias + row;
-      f[0] = __builtin_bit_cast(f32x4, LoadVec<DT_F32, false>(p));
-      f[1] = __builtin_bit_cast(f32x4, LoadVec<DT_F32, false>(p + 4));
-      return;
-    }
-    const u32x4 v = LoadVec<DT_BF16, false>((ConstRow<DT_BF16>)a.bias + row);
+    const auto *p = (ConstRow<DT_F32>)a.bias + row + min(j, a.k_len - 8);
+    f[0] = __builtin_bit_cast(f32x4, LoadVec<DT_F32, false>(p));
+    f[1] = __builtin_bit_cast(f32x4, LoadVec<DT_F32, false>(p + 4));
+  } else if constexpr (BIAS == kHalves) {
+    const u32x4 v =
+        LoadVec<DT_BF16, false>((ConstRow<DT_BF16>)a.bias + row + min(j, a.k_len - 8));
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       f[e >> 2][e & 3] =
@@ -384,7 +382,7 @@ __device__ __forceinline__ void Bias8(const TrainAttention &a, std::int64_t row,
 }
 template <int BIAS, int DT>
 __device__ __forceinline__ void Store8(Row<DT> p, int n, const f32x4 *f) {
-  if constexpr (BIAS == kVectors) {
+  if constexpr (BIAS != kValues) {
     ToMemory<DT>(p, f[0], f[1]);
   } else {
 #pragma unroll
@@ -400,7 +398,7 @@ __device__ __forceinline__ void StoreBias8(const TrainAttention &a, std::int64_t
   const int n = a.k_len - j;
   if (n <= 0)
     return;
-  if (a.bias_dtype == DT_F32)
+  if (BIAS == kVectors || (BIAS == kValues && a.bias_dtype == DT_F32))
     Store8<BIAS, DT_F32>((Row<DT_F32>)a.dbias + row + j, n, f);
   else if (a.bias_dtype == DT_BF16)
     Store8<BIAS, DT_BF16>((Row<DT_BF16>)a.dbias + row + j, n, f);
@@ -446,6 +444,54 @@ template <int DT, int DP> struct Stage {
       if (l.Last(q) >= 0 && At(i) < s.a.dim)
         f[i] = FromMemory<DT>(In<DT>(v, l.b, l.kv * s.a.group + h, q) + At(i));
     }
+  }
+};
+
+// A bias of 16-bit values beside kTile rows and ACROSS keys in LDS, in whole
+// vectors (kHalves); rows that are not the line's and keys behind its end hold
+// anything.
+template <int ACROSS> struct BiasStage {
+  static constexpr int kLd = ACROSS + 8, kChunks = kTile * ACROSS / 8 / 256;
+  u32x4 f[kChunks];
+  static __device__ __forceinline__ int RowIn(int i) {
+    return (i * 256 + static_cast<int>(threadIdx.x)) / (ACROSS / 8);
+  }
+  static __device__ __forceinline__ int At(int i) {
+    return (i * 256 + static_cast<int>(threadIdx.x)) % (ACROSS / 8) * 8;
+  }
+  __device__ __forceinline__ void Load(const Args &s, const Line &l, const Span64 &t, int first,
+                                       int key0) {
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      int h = t.h, q = t.q + RowIn(i);
+      if (!t.same) {
+        const int r = first + RowIn(i);
+        h = r / s.a.q_len;
+        q = h < s.a.group ? r - h * s.a.q_len : s.a.q_len;
+      }
+      f[i] = u32x4{0, 0, 0, 0};
+      if (q < s.a.q_len && key0 + At(i) < s.a.k_len)
+        f[i] = LoadVec<DT_BF16, false>((ConstRow<DT_BF16>)s.a.bias +
+                                       BiasAt(s.a, l.b, l.kv * s.a.group + h, q) + key0 + At(i));
+    }
+  }
+  __device__ __forceinline__ void Store(std::uint16_t *tile) const {
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i)
+      *reinterpret_cast<u32x4 *>(tile + RowIn(i) * kLd + At(i)) = f[i];
+  }
+  // Four rows from `row` on of the key col0 + lane % 16.
+  static __device__ __forceinline__ f32x4 Four(const std::uint16_t *tile, int row, int col0, int lane,
+                                               int dtype) {
+    const int fr = lane & 15;
+    typedef __attribute__((address_space(3))) s16x4 *Lds;
+    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (Lds)(tile + (row + (fr >> 2)) * kLd + col0 + 4 * (fr & 3)));
+    f32x4 f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      f[e] = OfHalf(dtype, static_cast<std::uint16_t>(x[e]));
+    return f;
   }
 };
 
@@ -962,6 +1008,11 @@ __global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardKeysKernel(Args
   constexpr int LD = kLd<DT, DP>;
   __shared__ __attribute__((aligned(16))) typename M::T qs[kTile * LD], dos[kTile * LD];
   __shared__ RowInfo info;
+  // A bias of 16 bits goes through LDS too: read from memory value by value, a key a
+  // lane, the backward pass of 4 x 16 bf16 heads of 64 over 1024 tokens took 295 us,
+  // so 198.
+  using Biases = BiasStage<kTile * N>;
+  __shared__ __attribute__((aligned(16))) std::uint16_t bs[BIAS == kHalves ? kTile * Biases::kLd : 1];
   Part part;
   if (!PartOf(s, &part))
     return;
@@ -994,6 +1045,7 @@ __global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardKeysKernel(Args
     return step;
   };
   Stage<DT, DP> qt, dt;
+  Biases bt;
   int my_last = -1;
   float my_lse = 0.f, my_delta = 0.f, my_rest = 0.f;
   std::int64_t my_bias = 0;
@@ -1001,6 +1053,8 @@ __global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardKeysKernel(Args
   const auto load = [&](int step) {
     qt.Rows(s, a.q, l, span, step * kTile);
     dt.Rows(s, a.dout, l, span, step * kTile);
+    if constexpr (BIAS == kHalves)
+      bt.Load(s, l, span, step * kTile, key0);
     all_see = span.same && span.q + kTile <= l.q_len && l.Last(span.q) >= key0 + kTile * N - 1;
     if (threadIdx.x < kTile) {
       const RowOfWave w = RowFor(s, l, step * kTile + threadIdx.x);
@@ -1023,6 +1077,8 @@ __global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardKeysKernel(Args
   while (step < end) {
     qt.Store(qs);
     dt.Store(dos);
+    if constexpr (BIAS == kHalves)
+      bt.Store(bs);
     if (threadIdx.x < kTile) {
       info.last[threadIdx.x] = my_last;
       info.lse[threadIdx.x] = my_lse;
@@ -1044,8 +1100,9 @@ __global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardKeysKernel(Args
         dp[n][t] = dp[0][t];
     }
     // All of the step's biases at once: rows apart, keys side by side in lanes.
-    f32x4 bias[BIAS ? N : 1][4];
-    if constexpr (BIAS != kNoBias) {
+    constexpr bool kEach = BIAS == kVectors || BIAS == kValues;
+    f32x4 bias[kEach ? N : 1][4];
+    if constexpr (kEach) {
 #pragma unroll
       for (int n = 0; n < N; ++n)
 #pragma unroll
@@ -1054,7 +1111,7 @@ __global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardKeysKernel(Args
           for (int e = 0; e < 4; ++e) {
             const std::int64_t at = info.bias[RowOf64(t, 4 * g + e)] + min(j[n], a.k_len - 1);
             bias[n][t][e] =
-                a.bias_dtype == DT_F32
+                BIAS == kVectors || a.bias_dtype == DT_F32
                     ? ((const MFH_GLOBAL float *)a.bias)[at]
                     : OfHalf(a.bias_dtype, ((const MFH_GLOBAL std::uint16_t *)a.bias)[at]);
           }
@@ -1069,15 +1126,20 @@ __global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardKeysKernel(Args
       if constexpr (BIAS != kNoBias)
         rest = *reinterpret_cast<const f32x4 *>(info.rest + at);
 #pragma unroll
-      for (int n = 0; n < N; ++n)
+      for (int n = 0; n < N; ++n) {
+        f32x4 b{0.f, 0.f, 0.f, 0.f};
+        if constexpr (kEach)
+          b = bias[n][t];
+        else if constexpr (BIAS == kHalves)
+          b = Biases::Four(bs, at, 16 * (N * wave + n), lane, a.bias_dtype);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           if constexpr (BIAS != kNoBias)
-            x[n][t][e] =
-                Probability<BIAS>(x[n][t][e] * scale + bias[n][t][e] - lse[e], rest[e]);
+            x[n][t][e] = Probability<BIAS>(x[n][t][e] * scale + b[e] - lse[e], rest[e]);
           else
             x[n][t][e] = Exp2(x[n][t][e] * scale - lse[e]);
         }
+      }
       if (!plain) {
 #pragma unroll
         for (int n = 0; n < N; ++n)
@@ -1349,7 +1411,9 @@ inline int Tiles(int n, int wide = 1) {
 inline int HowBias(const TrainAttention &a) {
   if (!a.bias || a.k_len == 0)
     return kNoBias;
-  return a.k_len % 8 == 0 ? kVectors : kValues;
+  if (a.k_len % 8 != 0)
+    return kValues;
+  return a.bias_dtype == DT_F32 ? kVectors : kHalves;
 }
 
 // Shapes of the launches, and the workspace that they share.
@@ -1359,11 +1423,14 @@ inline Args ArgsOf(const TrainAttention &a, bool keys) {
   s.lines = a.batch * a.kv_heads;
   s.rows = a.group * a.q_len;
   const int across = keys ? a.k_len : s.rows;
-  // Two sets of columns a wave halve the reads of LDS per product, where that
-  // leaves work for half of the card and registers hold them.
+  // Two sets of columns a wave halve the reads of LDS per product, where enough
+  // workgroups are left and registers hold them.  Keys with a bias gain from
+  // fewer: bf16 heads of 64, 4 x 16 over 1024 tokens (512 workgroups) 198 us, with one
+  // set 220; 2 x 8 (128) 73.9 and 73.1.
   const bool fits =
       (a.dim <= 32 || (a.dim <= 64 && a.dtype != DT_F32)) && HowBias(a) != kValues;
-  s.wide = fits && static_cast<std::int64_t>(s.lines) * Tiles(across, 2) >= (keys && a.bias ? 128 : 1024) ? 2 : 1;
+  const std::int64_t enough = keys && a.bias ? 512 : 1024;
+  s.wide = fits && static_cast<std::int64_t>(s.lines) * Tiles(across, 2) >= enough ? 2 : 1;
   s.tiles = Tiles(across, s.wide);
   s.steps = keys ? Tiles(s.rows) : Tiles(a.k_len);
   s.splits = SplitsOf(static_cast<std::int64_t>(s.lines) * s.tiles, s.steps);
@@ -1523,6 +1590,8 @@ hipError_t ByBias(const TrainAttention &a, bool backward, hipStream_t stream) {
   const int how = HowBias(a);
   if (how == kNoBias)
     return backward ? Backward<DT, DP, kNoBias>(a, stream) : Forward<DT, DP, kNoBias>(a, stream);
+  if (how == kHalves)
+    return backward ? Backward<DT, DP, kHalves>(a, stream) : Forward<DT, DP, kHalves>(a, stream);
   if (how == kVectors)
     return backward ? Backward<DT, DP, kVectors>(a, stream) : Forward<DT, DP, kVectors>(a, stream);
   return backward ? Backward<DT, DP, kValues>(a, stream) : Forward<DT, DP, kValues>(a, stream);
