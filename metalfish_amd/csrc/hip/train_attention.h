@@ -984,6 +984,8 @@ __global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardRowsKernel(Args
     if (!w[n].live || !a.dq.p)
       continue;
     if (s.splits > 1) {
+      if (w[n].last < 0)
+        continue;
       const std::int64_t all = static_cast<std::int64_t>(s.lines) * s.rows,
                          flat = static_cast<std::int64_t>(part.line) * s.rows + w[n].r;
       StorePartial<DP>(s.partials + (part.split * all + flat) * s.a.dim, lane, s.a.dim, acc[n]);
@@ -1177,6 +1179,8 @@ __global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardKeysKernel(Args
     if (j[n] >= a.k_len)
       continue;
     if (s.splits > 1) {
+      if (j[n] >= l.k_len)
+        continue;  // zeros that the join knows of
       const std::int64_t all = static_cast<std::int64_t>(s.lines) * a.k_len,
                          flat = static_cast<std::int64_t>(part.line) * a.k_len + j[n];
       float *o = s.partials + (2 * part.split * all + flat) * s.a.dim;
@@ -1192,6 +1196,7 @@ __global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardKeysKernel(Args
 }
 
 // Adds up the splits of dq (KEYS false) or of dk and dv: four elements a thread.
+// What no split holds is 0: keys behind a line's end, rows that see nothing.
 template <int DT, bool KEYS>
 __global__ __launch_bounds__(256) void JoinBackwardKernel(Args s) {
   const int per = KEYS ? s.a.k_len : s.rows, across = s.a.dim / 4;
@@ -1202,14 +1207,18 @@ __global__ __launch_bounds__(256) void JoinBackwardKernel(Args s) {
   const int c = static_cast<int>(id % across);
   if (at >= all)
     return;
-  f32x4 o{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-  for (int k = 0; k < s.splits; ++k)
-    o += *reinterpret_cast<const f32x4 *>(s.partials + (k * all + at) * s.a.dim + 4 * c);
   const bool second = KEYS && at >= n;
   const std::int64_t flat = second ? at - n : at;
   const int line = static_cast<int>(flat / per), r = static_cast<int>(flat % per);
   const int b = line / s.a.kv_heads, kv = line % s.a.kv_heads;
+  const Line l{b, kv, LengthOf(s.a.q_lengths, b, s.a.q_len), LengthOf(s.a.k_lengths, b, s.a.k_len),
+               s.a.causal};
+  f32x4 o{0.f, 0.f, 0.f, 0.f};
+  if (KEYS ? r < l.k_len : l.Last(r % s.a.q_len) >= 0) {
+#pragma unroll 8
+    for (int k = 0; k < s.splits; ++k)
+      o += *reinterpret_cast<const f32x4 *>(s.partials + (k * all + at) * s.a.dim + 4 * c);
+  }
   Row<DT> out;
   if constexpr (KEYS) {
     const HeadsView &v = second ? s.a.dv : s.a.dk;
