@@ -192,6 +192,24 @@ def test_biases(dev, shared, bias_dtype, dtype):
          shared=shared, causal=True).check()
 
 
+@pytest.mark.parametrize("bias_dtype", DTYPES)
+@pytest.mark.parametrize("k_len", [1, 3, 7, 8, 9, 12, 15, 17, 63, 65, 70, 129, 134, 333])
+def test_rows_of_a_bias_that_end_inside_a_vector(dev, k_len, bias_dtype):
+    """Alone and side by side in memory; the last row's end is the array's."""
+    for n, dtype in enumerate(DTYPES):
+        for shared, q_len in (((), 20), ((), 64), ((0, 1), 33)):
+            Case(dev, 2, 2, q_len, k_len, 32, dtype, bias="random", bias_dtype=bias_dtype,
+                 shared=shared, seed=k_len + n, causal=n == 1).check()
+
+
+@pytest.mark.parametrize("q_len,k_len", [(70, 521), (1021, 139)])
+@pytest.mark.parametrize("bias_dtype", DTYPES)
+def test_two_sets_of_columns_with_an_odd_bias(dev, q_len, k_len, bias_dtype):
+    for dtype in ("bf16", "f16"):
+        Case(dev, 8, 16, q_len, k_len, 32, dtype, kv_heads=16, bias="random", bias_dtype=bias_dtype,
+             k_lengths=[k_len, 1, 77, 0, 64, 138, 130, k_len - 1], seed=k_len).check()
+
+
 def test_a_bias_shared_by_queries(dev):
     c = Case(dev, 2, 2, 20, 70, 16, "f32", bias="random", shared=(2,))
     (q, k, v), rest = c.oracle()
