@@ -26,7 +26,7 @@ constexpr int MaxHeld(int dtype, bool backward) {
 }
 constexpr int kMaxSummed = 8192;  // and of the weights' gradients beside it
 constexpr int kColumnGroups = 64;  // workgroups down the rows of wider ones
-constexpr int kMaxGroups = 256;   // workgroups of the backward pass
+constexpr int kMaxGroups = 256, kMoreGroups = 512;  // of the backward pass, up to 8 values a lane
 
 // Sum over the T lanes of a row, in every one of them.
 template <int T>
@@ -216,9 +216,10 @@ __global__ __launch_bounds__(kBlock<T>) void NormKernel(NormParams p) {
   }
 }
 
-// The backward pass has eight waves a workgroup and one workgroup a CU: each leaves
-// 8 bytes a column of partial sums, which more workgroups of fewer rows would let
-// grow beside 2053 x 5003 fp16 (four waves, two workgroups a CU: 36 us, so 27).
+// The backward pass has eight waves a workgroup and, of wide rows, one workgroup a
+// CU: each leaves 8 bytes a column of partial sums, which more workgroups of fewer
+// rows would let grow beside 2053 x 5003 fp16 (four waves, two workgroups a CU: 36
+// us, so 27).
 template <int T> constexpr int kBackBlock = T > 512 ? T : 512;
 
 template <int DT, int T, int NV, bool PAST>
@@ -712,10 +713,13 @@ Shape ShapeOf(int width, int dtype) {
   return {1024, vectors <= 1024 * most ? most : 2 * most};
 }
 
-int Groups(std::int64_t rows, int lanes) {
+// Workgroups of a backward pass: one a CU, or two where registers hold both (rows of
+// up to 2048 values; 65536 x 256 bf16 27.7 us, with one 31.8; 200000 x 64 fp32 34.7 and
+// 44.0; with 16 values a lane, 16384 x 1024 bf16 with a residual, 45.4 and 39.1).
+int Groups(std::int64_t rows, int lanes, int values) {
   const std::int64_t per = lanes > 512 ? 1 : 512 / lanes;
-  return static_cast<int>(
-      std::min<std::int64_t>((rows + per - 1) / per, lanes > 512 ? 512 : kMaxGroups));
+  const std::int64_t most = lanes > 512 || values <= 8 ? kMoreGroups : kMaxGroups;
+  return static_cast<int>(std::min<std::int64_t>((rows + per - 1) / per, most));
 }
 
 // Calls whose rows hold more bytes than this go past the caches, if every row
@@ -755,7 +759,7 @@ void LaunchForward(const NormParams &p, hipStream_t stream) {
 template <int DT, int T, int NV, bool PAST>
 void LaunchShape(const NormParams &p, bool backward, hipStream_t stream) {
   if (backward)
-    hipLaunchKernelGGL((NormBackwardKernel<DT, T, NV, PAST>), dim3(Groups(p.rows, T)),
+    hipLaunchKernelGGL((NormBackwardKernel<DT, T, NV, PAST>), dim3(Groups(p.rows, T, NV * Elem<DT>::kPerVec)),
                        dim3(kBackBlock<T>), 0, stream, p);
   else
     LaunchForward<DT, T, NV, PAST>(p, stream);
@@ -804,7 +808,7 @@ template <int DT> void LaunchType(const NormParams &p, bool backward, hipStream_
 template <int DT> void LaunchTiny(const NormParams &p, bool backward, hipStream_t stream) {
   const std::int64_t groups = (p.rows + 255) / 256;
   if (backward) {
-    hipLaunchKernelGGL(TinyNormBackwardKernel<DT>, dim3(Groups(groups, 512)), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL(TinyNormBackwardKernel<DT>, dim3(Groups(groups, 512, 8)), dim3(256), 0, stream, p);
     return;
   }
   // Less than 2^32 threads a launch.
@@ -864,8 +868,9 @@ int PartsOf(const NormParams &p) {
   if (p.width > kMaxSummed)
     return NormPartials(p.rows, p.width);
   if (p.width < (p.dtype == DT_F32 ? 4 : 8))
-    return Groups((p.rows + 255) / 256, 512);
-  return Groups(p.rows, ShapeOf(p.width, p.dtype).lanes);
+    return Groups((p.rows + 255) / 256, 512, 8);
+  const Shape s = ShapeOf(p.width, p.dtype);
+  return Groups(p.rows, s.lanes, s.vectors * (p.dtype == DT_F32 ? 4 : 8));
 }
 
 bool Sound(const NormParams &p) {
@@ -875,7 +880,9 @@ bool Sound(const NormParams &p) {
 }  // namespace
 
 int NormPartials(std::int64_t rows, int width) {
-  return static_cast<int>(std::min<std::int64_t>(rows, width > kMaxSummed ? kColumnGroups : kMaxGroups));
+  // At least what Groups says of any type: 256 lanes of 8 values have 2048 columns.
+  const int most = width > kMaxSummed ? kColumnGroups : width > 2048 ? kMaxGroups : kMoreGroups;
+  return static_cast<int>(std::min<std::int64_t>(rows, most));
 }
 
 hipError_t LaunchNorm(const NormParams &p, hipStream_t stream, std::string *err) {

@@ -124,6 +124,14 @@ def test_in_place(dev, width, dtype):
     assert all(np.array_equal(b[k], d[k]) for k in b)
 
 
+@pytest.mark.parametrize("dtype", lu.HALF)
+@pytest.mark.parametrize("rows,width", [(140_001, 3), (70_001, 40), (20_003, 250), (4_500, 513),
+                                        (4_100, 2048), (4_100, 2049)])
+def test_more_rows_than_the_workgroups_have(dev, rows, width, dtype):
+    """Both sides of every number of workgroups; nothing behind the workspace."""
+    run(dev, rows, width, dtype, seed=width)
+
+
 def test_large_means_keep_their_variance(dev):
     # The variance is 1e-6 of the mean's square: a difference of mean squares
     # would hold no digit of it.
