@@ -5,7 +5,7 @@
 //
 // Bound by memory: with states and gradients in 32 bits a weight costs 28
 // bytes (159 M of them 753 us, 5.9 TB/s), with states in 8 bits, bf16 gradients
-// and a bf16 copy 16 (427 us, 6.0 TB/s; the vector unit is busy four fifths of that).
+// and a bf16 copy 16 (427 to 436 us, 5.9 TB/s; the vector unit is busy four fifths of that).
 // The tensors are cut into chunks of kAdamChunk values, listed once per set, and a
 // workgroup takes whole chunks; every value is read and written once, in whole
 // vectors.
