@@ -220,6 +220,7 @@ struct Args {
   int wide = 1;    // 16-column sets of a wave: a tile has 64 times as many
   int line0 = 0, lines_now = 0, tile0 = 0;  // the part of one launch
   bool spread = false, turn = false;        // the order of workgroups
+  int across = 0;                           // of them along x, in a launch of both passes
   int down = 0;    // tiles from the last to the first, in so many interleaved runs
   float *partials = nullptr;
   float *delta = nullptr;  // [lines][rows]
@@ -242,11 +243,10 @@ __device__ __forceinline__ int Uniform(int v) { return __builtin_amdgcn_readfirs
 struct Part {
   int line, tile, split;
 };
-__device__ __forceinline__ bool PartOf(const Args &s, Part *p) {
-  const int x = blockIdx.x, per = static_cast<int>(gridDim.x >> 3);
-  const int at = s.spread ? (x & 7) * per + (x >> 3) : x;
+__device__ __forceinline__ bool PartOf(const Args &s, int x, int across, int down, Part *p) {
+  const int at = s.spread ? (x & 7) * (across >> 3) + (x >> 3) : x;
   // y counts a line's parts.
-  int line = at, y = s.tile0 + static_cast<int>(blockIdx.y), tile = y;
+  int line = at, y = s.tile0 + down, tile = y;
   bool mine = at < s.lines_now;
   p->split = 0;
   if (s.splits > 1) {
@@ -275,6 +275,10 @@ __device__ __forceinline__ bool PartOf(const Args &s, Part *p) {
   p->line = s.line0 + line;
   p->tile = tile;
   return mine && tile < s.tiles;
+}
+
+__device__ __forceinline__ bool PartOf(const Args &s, Part *p) {
+  return PartOf(s, blockIdx.x, gridDim.x, blockIdx.y, p);
 }
 
 __device__ __forceinline__ int LengthOf(const std::int32_t *lengths, int b, int most) {
@@ -458,6 +462,24 @@ template <int DT, int DP> struct Stage {
       f[i] = typename Mat<DT>::Frag{};
       if (j < l.k_len && At(i) < dim)
         f[i] = FromMemory<DT>(base + Tokens(v, j) + At(i));
+    }
+  }
+  // Less the products of each row with another's: lanes beside each other hold a row.
+  __device__ __forceinline__ void StoreDots(const Stage &with, float *dots) const {
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      float v = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        v += Mat<DT>::Get(f[i], e) * Mat<DT>::Get(with.f[i], e);
+      v += Dpp<0xB1, 0xF>(0.f, v);  // its neighbour's, the pair's, the four's, the eight's
+      v += Dpp<0x4E, 0xF>(0.f, v);
+      if constexpr (kAcross >= 8)
+        v += Dpp<0x141, 0xF>(0.f, v);
+      if constexpr (kAcross >= 16)
+        v += Dpp<0x140, 0xF>(0.f, v);
+      if (At(i) == 0)
+        dots[RowIn(i)] = -v;
     }
   }
   // Rows first .. of a line: zeros where a row sees nothing.
@@ -892,13 +914,10 @@ __device__ __forceinline__ float Delta(const typename Mat<DT>::Frag *out,
 // stays in the registers of one wave.  4 x 32 x 2048 x 64 bf16 570 us for both (603
 // TFLOP/s of the five).
 template <int DT, int DP, int N, int BIAS>
-__global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardRowsKernel(Args s) {
+__device__ __forceinline__ void BackwardRows(const Args &s, const Part &part,
+                                             typename Mat<DT>::T *ks, typename Mat<DT>::T *vs) {
   using M = Mat<DT>;
   constexpr int LD = kLd<DT, DP>;
-  __shared__ __attribute__((aligned(16))) typename M::T ks[kTile * LD], vs[kTile * LD];
-  Part part;
-  if (!PartOf(s, &part))
-    return;
   const TrainAttention &a = s.a;
   const Line l = LineOf(s, part.line);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, g = lane >> 4;
@@ -927,7 +946,7 @@ __global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardRowsKernel(Args
     typename M::Frag of[DP / 32];
     LoadRow<DT, DP>(s, a.out, l, w[n], lane, of);
     delta[n] = Delta<DT, DP>(of, df[n]);
-    if (w[n].live && g == 0 && part.split == 0)
+    if (s.delta && w[n].live && g == 0 && part.split == 0)
       s.delta[flat] = delta[n];
     lse[n] = w[n].last >= 0 ? Lse<BIAS>(a.lse[flat]) : __builtin_inff();
     rest[n] = 0.f;
@@ -1033,6 +1052,14 @@ __global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardRowsKernel(Args
   }
 }
 
+template <int DT, int DP, int N, int BIAS>
+__global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardRowsKernel(Args s) {
+  __shared__ __attribute__((aligned(16))) typename Mat<DT>::T tiles[2][kTile * kLd<DT, DP>];
+  Part part;
+  if (PartOf(s, &part))
+    BackwardRows<DT, DP, N, BIAS>(s, part, tiles[0], tiles[1]);
+}
+
 // What a workgroup of the keys' kernel holds of its 64 rows, next to the tiles.
 struct RowInfo {
   __attribute__((aligned(16))) int last[kTile];
@@ -1044,20 +1071,13 @@ struct RowInfo {
 // times 16 keys and holds them, and rows go through LDS.  Bound by LDS: a step of 64
 // rows of 64 elements reads 32 KB a wave, for 32 matrix instructions at N = 1 and 64 at
 // N = 2 (four lines of up to 1021 tokens, 16 heads over 4: 38 us).
-template <int DT, int DP, int N, int BIAS>
-__global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardKeysKernel(Args s) {
+template <int DT, int DP, int N, int BIAS, bool ALONE>
+__device__ __forceinline__ void BackwardKeys(const Args &s, const Part &part,
+                                             typename Mat<DT>::T *qs, typename Mat<DT>::T *dos,
+                                             RowInfo &info, std::uint16_t *bs) {
   using M = Mat<DT>;
   constexpr int LD = kLd<DT, DP>;
-  __shared__ __attribute__((aligned(16))) typename M::T qs[kTile * LD], dos[kTile * LD];
-  __shared__ RowInfo info;
-  // A bias of 16 bits goes through LDS too: read from memory value by value, a key a
-  // lane, the backward pass of 4 x 16 bf16 heads of 64 over 1024 tokens took 295 us,
-  // so 198.
   using Biases = BiasStage<kTile * N>;
-  __shared__ __attribute__((aligned(16))) std::uint16_t bs[BIAS == kHalves ? kTile * Biases::kLd : 1];
-  Part part;
-  if (!PartOf(s, &part))
-    return;
   const TrainAttention &a = s.a;
   const Line l = LineOf(s, part.line);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, g = lane >> 4;
@@ -1086,7 +1106,7 @@ __global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardKeysKernel(Args
     }
     return step;
   };
-  Stage<DT, DP> qt, dt;
+  Stage<DT, DP> qt, dt, ot;
   Biases bt;
   int my_last = -1;
   float my_lse = 0.f, my_delta = 0.f, my_rest = 0.f;
@@ -1095,6 +1115,8 @@ __global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardKeysKernel(Args
   const auto load = [&](int step) {
     qt.Rows(s, a.q, l, span, step * kTile);
     dt.Rows(s, a.dout, l, span, step * kTile);
+    if constexpr (ALONE)
+      ot.Rows(s, a.out, l, span, step * kTile);
     if constexpr (BIAS == kHalves)
       bt.Load(s, l, span, step * kTile, key0);
     all_see = span.same && span.q + kTile <= l.q_len && l.Last(span.q) >= key0 + kTile * N - 1;
@@ -1106,7 +1128,8 @@ __global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardKeysKernel(Args
       my_delta = 0.f;
       if (w.last >= 0) {
         my_lse = Lse<BIAS>(a.lse[flat]);
-        my_delta = -s.delta[flat];
+        if constexpr (!ALONE)
+          my_delta = -s.delta[flat];
         if constexpr (BIAS != kNoBias)
           my_rest = s.rest[flat];
       }
@@ -1119,12 +1142,15 @@ __global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardKeysKernel(Args
   while (step < end) {
     qt.Store(qs);
     dt.Store(dos);
+    if constexpr (ALONE)
+      dt.StoreDots(ot, info.delta);
     if constexpr (BIAS == kHalves)
       bt.Store(bs);
     if (threadIdx.x < kTile) {
       info.last[threadIdx.x] = my_last;
       info.lse[threadIdx.x] = my_lse;
-      info.delta[threadIdx.x] = my_delta;
+      if constexpr (!ALONE)
+        info.delta[threadIdx.x] = my_delta;
       info.rest[threadIdx.x] = my_rest;
       info.bias[threadIdx.x] = my_bias;
     }
@@ -1232,6 +1258,38 @@ __global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardKeysKernel(Args
       StoreHead<DT, DP>(Out<DT>(a.dk, l.b, l.kv, j[n]), lane, a.dim, dk[n], a.scale);
     if (a.dv.p)
       StoreHead<DT, DP>(Out<DT>(a.dv, l.b, l.kv, j[n]), lane, a.dim, dv[n], 1.f);
+  }
+}
+template <int DT, int DP, int N, int BIAS>
+__global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardKeysKernel(Args s) {
+  __shared__ __attribute__((aligned(16))) typename Mat<DT>::T tiles[2][kTile * kLd<DT, DP>];
+  __shared__ RowInfo info;
+  // A bias of 16 bits goes through LDS too: read from memory value by value, a key a
+  // lane, the backward pass of 4 x 16 bf16 heads of 64 over 1024 tokens took 295 us,
+  // so 198.
+  __shared__ __attribute__((aligned(16)))
+  std::uint16_t bs[BIAS == kHalves ? kTile * BiasStage<kTile * N>::kLd : 1];
+  Part part;
+  if (PartOf(s, &part))
+    BackwardKeys<DT, DP, N, BIAS, false>(s, part, tiles[0], tiles[1], info, bs);
+}
+
+// Both in one launch (BothAtOnce): the first key_groups workgroups have keys and
+// form delta themselves from out, the others rows.
+template <int DT, int DP>
+__global__ __launch_bounds__(256, (kWaves<DT, DP>)) void BackwardBothKernel(Args rows, Args keys,
+                                                                            int key_groups) {
+  __shared__ __attribute__((aligned(16))) typename Mat<DT>::T tiles[2][kTile * kLd<DT, DP>];
+  __shared__ RowInfo info;
+  Part part;
+  const int id = static_cast<int>(blockIdx.x);
+  if (id < key_groups) {
+    if (PartOf(keys, id % keys.across, keys.across, id / keys.across, &part))
+      BackwardKeys<DT, DP, 1, kNoBias, true>(keys, part, tiles[0], tiles[1], info, nullptr);
+  } else {
+    const int at = id - key_groups;
+    if (PartOf(rows, at % rows.across, rows.across, at / rows.across, &part))
+      BackwardRows<DT, DP, 1, kNoBias>(rows, part, tiles[0], tiles[1]);
   }
 }
 
@@ -1548,6 +1606,35 @@ template <class K> hipError_t Run(K kernel, Args s, hipStream_t stream) {
     }
   return e;
 }
+// A pass's workgroups as a part of one launch along x.
+inline std::int64_t GroupsOf(Args *s) {
+  const bool ragged = s->a.q_lengths || s->a.k_lengths;
+  s->lines_now = s->lines;
+  if (s->splits > 1) {
+    s->turn = ragged;
+    s->spread = !ragged;
+    s->down = 0;
+    s->across = (s->lines * s->tiles * s->splits + 7) / 8 * 8;
+    return s->across;
+  }
+  s->spread = s->lines >= 64;
+  s->turn = ragged && !s->spread;
+  s->across = s->spread ? (s->lines + 7) / 8 * 8 : s->lines;
+  const int tiles = s->down ? (s->tiles + s->down - 1) / s->down * s->down : s->tiles;
+  return static_cast<std::int64_t>(s->across) * tiles;
+}
+// Whether a backward pass does rows and keys in one launch: the one's last workgroups
+// run beside the other's, and a launch is saved.  bf16, causal: 1 x 4 over 4096 tokens of
+// 64 99 us, apart 120; four lines of up to 1021, 16 heads over 4, 57.8 and 64.4; 2 x 4 over
+// 116 8.5 and 13.2.  Heads of 128 leave a SIMD two waves and gain less: 37 x 8 over 2, 66
+// tokens (700 workgroups) 28 and 37, 2 x 16 over 2048 (2048) 221 and 214.  With a bias the
+// keys need what the rows find out (Coarse).
+inline bool BothAtOnce(const Args &rows, const Args &keys) {
+  const std::int64_t most = rows.a.dim > 64 ? 1024 : 4096;
+  return !rows.a.bias && rows.wide == 1 && keys.wide == 1 && rows.a.q_len > 0 && rows.a.k_len > 0 &&
+         (static_cast<std::int64_t>(rows.tiles) * rows.splits +
+          static_cast<std::int64_t>(keys.tiles) * keys.splits) * rows.lines <= most;
+}
 // Splits have few rows.
 template <class K> hipError_t RunJoin(K kernel, const Args &s, std::int64_t groups, hipStream_t stream) {
   if (groups == 0)
@@ -1601,6 +1688,28 @@ hipError_t Backward(const TrainAttention &a, hipStream_t stream) {
     if (square) {
       s.tiles = 1;
       e = Run(SquareBackwardKernel<DT, DP, BIAS>, s, stream);
+    }
+  }
+  if constexpr (BIAS == kNoBias) {
+    Args k = ArgsOf(a, true);
+    if (!square && BothAtOnce(s, k) && (a.dk.p || a.dv.p)) {
+      s.delta = nullptr;
+      k.partials = s.partials + RowsBytes(s) / sizeof(float);
+      // Whole rounds of the dies, so that the rows' workgroups begin on the first; what
+      // is added is behind the last tile of keys.
+      const std::int64_t key_groups = (GroupsOf(&k) + 7) / 8 * 8,
+                         row_groups = a.dq.p ? GroupsOf(&s) : 0;
+      hipLaunchKernelGGL((BackwardBothKernel<DT, DP>),
+                         dim3(static_cast<unsigned>(key_groups + row_groups)), dim3(256), 0, stream, s,
+                         k, static_cast<int>(key_groups));
+      e = hipGetLastError();
+      if (e == hipSuccess && s.splits > 1 && a.dq.p)
+        e = RunJoin(JoinBackwardKernel<DT, false>, s,
+                    joins(static_cast<std::int64_t>(s.lines) * s.rows), stream);
+      if (e == hipSuccess && k.splits > 1)
+        e = RunJoin(JoinBackwardKernel<DT, true>, k,
+                    joins(2 * static_cast<std::int64_t>(k.lines) * a.k_len), stream);
+      return e;
     }
   }
   if (!square)

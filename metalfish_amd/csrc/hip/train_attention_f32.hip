@@ -37,8 +37,9 @@ std::uint64_t AttentionForwardWorkspace(const TrainAttention &a) {
 
 std::uint64_t AttentionBackwardWorkspace(const TrainAttention &a) {
   const attend::Args rows = attend::ArgsOf(a, false), keys = attend::ArgsOf(a, true);
+  const std::uint64_t r = attend::RowsBytes(rows), k = attend::KeysBytes(keys);
   return attend::RowValuesBytes(rows) +
-         std::max(attend::RowsBytes(rows), attend::KeysBytes(keys));
+         (attend::BothAtOnce(rows, keys) ? r + k : std::max(r, k));
 }
 
 hipError_t LaunchAttentionForward(const TrainAttention &a, hipStream_t stream, std::string *err) {

@@ -210,6 +210,27 @@ def test_two_sets_of_columns_with_an_odd_bias(dev, q_len, k_len, bias_dtype):
              k_lengths=[k_len, 1, 77, 0, 64, 138, 130, k_len - 1], seed=k_len).check()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [24, 64, 120])
+@pytest.mark.parametrize("batch,heads,kv_heads,q_len,k_len", [
+    (1, 1, 1, 1, 65), (3, 5, 5, 66, 66), (2, 8, 2, 130, 70), (1, 2, 1, 900, 65), (5, 4, 4, 65, 700),
+    (9, 8, 8, 70, 129), (1, 3, 3, 1100, 1100)])
+def test_rows_and_keys_in_one_launch(dev, batch, heads, kv_heads, q_len, k_len, dim, dtype):
+    """Little work without a bias: odd numbers of lines and tiles, either side split,
+    lengths; an output does not depend on which others are asked for."""
+    rng = np.random.default_rng(q_len + k_len)
+    for causal in (False, True):
+        lengths = {}
+        if causal and batch > 1:
+            lengths = dict(q_lengths=rng.integers(0, q_len + 1, batch),
+                           k_lengths=rng.integers(0, k_len + 1, batch))
+        c = Case(dev, batch, heads, q_len, k_len, dim, dtype, kv_heads=kv_heads, causal=causal,
+                 seed=dim, **lengths)
+        every = c.check()
+        for n in every:
+            assert np.array_equal(c.backward(only=(n,))[n], every[n]), n
+
+
 def test_a_bias_shared_by_queries(dev):
     c = Case(dev, 2, 2, 20, 70, 16, "f32", bias="random", shared=(2,))
     (q, k, v), rest = c.oracle()
