@@ -238,7 +238,7 @@ __device__ __forceinline__ int Uniform(int v) { return __builtin_amdgcn_readfirs
 // queries over 20011 keys, four lines, 10.9 us; one line after another along x, 18.4.
 // Few lines that may differ in length take turns with the tiles, or a long one's
 // parts meet on the same CUs: backward of four lines of up to 1021 tokens with four
-// key heads 67 us, 87 without.  Equal lines stay where they are, for the cache: 2 x 16
+// key heads, rows and keys launched apart, 67 us, 87 without.  Equal lines stay where they are, for the cache: 2 x 16
 // heads of 128 over 2048 tokens forward 58 us, 77 in turns.
 struct Part {
   int line, tile, split;
@@ -264,7 +264,7 @@ __device__ __forceinline__ bool PartOf(const Args &s, int x, int across, int dow
   }
   if (s.turn) {
     // One further a tile, and a step aside after each 256 workgroups (the CUs): 67
-    // us; one further a tile alone, 72.
+    // us in that case; one further a tile alone, 72.
     const unsigned aside = (static_cast<unsigned>(y) * s.lines_now >> 8) * (s.a.kv_heads + 1);
     line = static_cast<int>((line + y + aside) % static_cast<unsigned>(s.lines_now));
   }
@@ -1070,7 +1070,8 @@ struct RowInfo {
 // dk and dv of a tile of keys over the rows that share them; each wave has N
 // times 16 keys and holds them, and rows go through LDS.  Bound by LDS: a step of 64
 // rows of 64 elements reads 32 KB a wave, for 32 matrix instructions at N = 1 and 64 at
-// N = 2 (four lines of up to 1021 tokens, 16 heads over 4: 38 us).
+// N = 2 (four lines of up to 1021 tokens, 16 heads over 4: 38 us, with the rows' beside it
+// 50).
 template <int DT, int DP, int N, int BIAS, bool ALONE>
 __device__ __forceinline__ void BackwardKeys(const Args &s, const Part &part,
                                              typename Mat<DT>::T *qs, typename Mat<DT>::T *dos,
@@ -1506,8 +1507,10 @@ __global__ __launch_bounds__(256) void BiasGradKernel(Args s, int plane_heads, s
 }
 
 // Workgroups that fill the card twice, a split of two tiles at least; six times where
-// each still loops over ten: causal bf16 heads of 64, backward of 8 over 2048 tokens 65
-// us (four times, over sixteen: 75; eight, over eight: 83), of 4 over 4096 121 (128, 134).
+// each still loops over ten: causal bf16, 8 heads of 64 over 2048 tokens 24 us and
+// backward 54.5 (four times, over sixteen: 27.5 and 56.8), 8 heads of 128 over 2 and 4000
+// tokens 89 and 364 (107 and 381); some lines lose (8 x 4 over 1, up to 2000 tokens,
+// backward 103 and 95).  Eight times, over eight, lost everywhere.
 inline int SplitsOf(std::int64_t groups, int steps) {
   const std::int64_t g = std::max<std::int64_t>(groups, 1);
   const std::int64_t want = std::min<std::int64_t>(
