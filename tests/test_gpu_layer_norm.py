@@ -132,6 +132,43 @@ def test_more_rows_than_the_workgroups_have(dev, rows, width, dtype):
     run(dev, rows, width, dtype, seed=width)
 
 
+@pytest.mark.parametrize("width", [5, 40, 1030])
+def test_rows_beyond_32_bits(dev, width):
+    """Three rows 2^30 elements apart, every array's row in columns of one buffer."""
+    rng = np.random.default_rng(8)
+    rows, stride, at = 3, 1 << 30, 2048
+    x, r, dy = (lu.values(rng, (rows, width), "bf16") for _ in range(3))
+    far = dev.alloc(2 * ((rows - 1) * stride + 8 * at))
+
+    def row(k, i):
+        return far + 2 * (i * stride + k * at)
+
+    for k, t in enumerate((x, r, dy)):
+        for i in range(rows):
+            dev.write(row(k, i), lu.to_bits(t[i], "bf16"))
+    stats = [dev.put(np.zeros(rows, np.float32)) for _ in range(2)]
+    p = backend.norm_rows(row(0, 0), rows, width, dtype="bf16", x_stride=stride,
+                          d_residual=row(1, 0), residual_stride=stride, alpha=0.5)
+    backend.layer_norm_device(p, row(3, 0), y_stride=stride, d_mean=stats[0], d_rstd=stats[1])
+    backend.layer_norm_backward_device(p, row(2, 0), *stats, d_dx=row(4, 0), d_dresidual=row(5, 0),
+                                       dy_stride=stride, dx_stride=stride, dresidual_stride=stride)
+    dev.sync()
+
+    def get(k):
+        host = np.zeros(width, np.uint16)
+        return np.stack([lu.from_bits(dev.get(row(k, i), host), "bf16") for i in range(rows)])
+
+    eps = float(np.float32(1e-3))
+    want = layers.layer_norm(x, r, 0.5, None, None, eps)
+    tol = lu.norm_bounds(x, r, 0.5, None, None, eps, want, "bf16")
+    lu.check(get(3), want["y"], tol["y"], "y")
+    mean, rstd = (dev.get(d, np.zeros(rows, np.float32)).astype(np.float64) for d in stats)
+    want = layers.layer_norm_backward(x, dy, mean, rstd, r, 0.5, None)
+    tol = lu.norm_backward_bounds(x, r, 0.5, None, dy, mean, rstd, want, "bf16")
+    lu.check(get(4), want["dx"], tol["dx"], "dx")
+    lu.check(get(5), want["dresidual"], tol["dresidual"], "dresidual")
+
+
 def test_large_means_keep_their_variance(dev):
     # The variance is 1e-6 of the mean's square: a difference of mean squares
     # would hold no digit of it.
