@@ -519,7 +519,8 @@ typedef struct {
  * over the keys j that query i sees: with m = d_q_lengths[b] and n =
  * d_k_lengths[b] (NULL: q_len, k_len; clamped to 0 .. those) j < n, and with
  * `causal` j <= i + n - m, so the last query sees the last key.  What lies
- * behind a length is not read.  A query that sees nothing (i >= m among them), or
+ * behind a length is not read, and a bias of what a query does not see has no
+ * effect, whatever it is.  A query that sees nothing (i >= m among them), or
  * only keys of bias -inf, has out 0, lse -inf, and gradients of 0.  The bias is
  * p[b * bias_batch + h * bias_head + i * bias_query + j]; a stride of 0 shares
  * it.  Scores, statistics and sums are in 32 bits; with bf16 or fp16 inputs the

@@ -1,5 +1,5 @@
 // Which bytes the arrays of a call hold, and whether two of them share any
-// (host only; learn_api.cpp).
+// (host only; learn_api.cpp, train_api.cpp).
 #pragma once
 
 #include <algorithm>

@@ -170,6 +170,25 @@ def test_ragged_lines(dev, causal, order, dtype):
          k_lengths=[90, 13, 0, 64, 65], order=order, spoil=True, bias="random").check()
 
 
+@pytest.mark.parametrize("bias_dtype", DTYPES)
+@pytest.mark.parametrize("q_len,k_len", [(64, 64), (57, 61), (100, 90), (70, 203), (5, 900)])
+def test_a_bias_of_what_is_not_seen_has_no_effect(dev, q_len, k_len, bias_dtype):
+    """NaN there: behind the lengths and right of the diagonal."""
+    m, n = [q_len, 1, q_len - 2], [k_len, k_len - 3, 9]
+    rng = np.random.default_rng(14)
+    ok = np.stack([layers.seen(q_len, k_len, a, b, True) for a, b in zip(m, n)])[:, None]
+    bias = np.where(ok, rng.normal(size=(3, 2, q_len, k_len)), 0.0)
+    for dtype in DTYPES:
+        c = Case(dev, 3, 2, q_len, k_len, 32, dtype, bias=bias, bias_dtype=bias_dtype, causal=True,
+                 q_lengths=m, k_lengths=n)
+        unseen = np.broadcast_to(~ok, bias.shape).reshape(-1)
+        at = c.d_bias.lead + np.flatnonzero(unseen)
+        c.d_bias.flat[at] = lu.NAN[bias_dtype]
+        dev.write(c.d_bias.base, c.d_bias.flat)
+        got = c.check()
+        assert not got["dbias"].reshape(-1)[unseen].any()
+
+
 def test_lengths_outside_their_arrays_are_clamped(dev):
     Case(dev, 3, 2, 20, 30, 16, "f32", q_lengths=[50, -4, 20], k_lengths=[31, 5, -1]).check()
 
