@@ -1332,11 +1332,13 @@ __global__ __launch_bounds__(256) void JoinBackwardKernel(Args s) {
 
 // The whole backward pass of a head of up to 64 queries and 64 keys, none of
 // them shared: one workgroup, each input read once.  Bound by memory: 256 x 32 heads
-// of 32 elements, bf16 with a bias, 93.7 us (4.3 TB/s).  A wave has 16 queries while
+// of 32 elements, bf16 with a bias, 88.3 us (4.2 TB/s).  delta is the sum of p dp over
+// the keys, which are all here: out is not read, and a query that sees one key has
+// gradients of exactly 0.  A wave has 16 queries while
 // scores, probabilities, dS and dq are formed, and 16 keys for dk and dv; P and
 // then dS change hands through a tile of LDS that held V before (256 x 16 heads of
-// 64 elements: 79 us; with tiles of their own, and so two workgroups a CU instead
-// of four, 84).
+// 64 elements: 75 us; with tiles of their own, and so two workgroups a CU instead
+// of four, 5 more).
 template <int DT, int DP, int BIAS>
 __global__ __launch_bounds__(256, 2) void SquareBackwardKernel(Args s) {
   using M = Mat<DT>;
@@ -1353,14 +1355,13 @@ __global__ __launch_bounds__(256, 2) void SquareBackwardKernel(Args s) {
   const int mine = 16 * wave + fr;  // a query, and later a key
   const RowOfWave w = RowFor(s, l, mine);
   const std::int64_t flat = static_cast<std::int64_t>(part.line) * s.rows + mine;
-  typename M::Frag qf[1][DP / 32], df[1][DP / 32], of[DP / 32];
+  typename M::Frag qf[1][DP / 32], df[1][DP / 32];
   {
     typename M::Frag kf[DP / 32], vf[DP / 32];
     LoadKey<DT, DP>(s, a.k, l, mine, lane, kf);
     LoadRow<DT, DP>(s, a.q, l, w, lane, qf[0]);
     LoadKey<DT, DP>(s, a.v, l, mine, lane, vf);
     LoadRow<DT, DP>(s, a.dout, l, w, lane, df[0]);
-    LoadRow<DT, DP>(s, a.out, l, w, lane, of);
 #pragma unroll
     for (int c = 0; c < DP / 32; ++c) {
       const int at = mine * LD + 32 * c + 8 * g;
@@ -1370,18 +1371,16 @@ __global__ __launch_bounds__(256, 2) void SquareBackwardKernel(Args s) {
       ToRow<DT>(dos + at, df[0][c]);
     }
   }
-  const float delta = Delta<DT, DP>(of, df[0]);
-  if (w.live && g == 0)
-    s.delta[flat] = delta;
   const float lse = w.last >= 0 ? Lse<BIAS>(a.lse[flat]) : __builtin_inff();
   const std::int64_t bias_at = BIAS ? BiasAt(a, l.b, w.head, w.q) : 0;
   __syncthreads();
   f32x4 xs[1][4], dps[1][4], *x = xs[0], *dp = dps[0];
-  Fill(dp, 4, -delta);
   Products<DT, DP, 1, false>(ks, qf, lane, xs);
-  Products<DT, DP, 1, true>(vs, df, lane, dps);
+  Products<DT, DP, 1, false>(vs, df, lane, dps);
   ToScores<BIAS>(a, bias_at, 8 * g, w.last, lse, x);
-  float rest = 0.f;
+  // dp of the key that has more than half of the row, if one has: delta is summed
+  // about it.
+  float rest = 0.f, delta = 0.f, near = -__builtin_inff();
   if constexpr (BIAS != kNoBias) {
     if (__any(Coarse(lse))) {
       float sum = 0.f;
@@ -1401,8 +1400,21 @@ __global__ __launch_bounds__(256, 2) void SquareBackwardKernel(Args s) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       x[t][e] = Probability<BIAS>(x[t][e], rest);
-      dp[t][e] *= x[t][e];
+      near = x[t][e] > 0.5f ? dp[t][e] : near;
     }
+  near = OverRows(near, true);
+  near = near == -__builtin_inff() ? 0.f : near;
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      delta += x[t][e] * (dp[t][e] - near);
+  delta = near + OverRows(delta, false);
+  if (w.live && g == 0)
+    s.delta[flat] = delta;
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+    dp[t] = (dp[t] - delta) * x[t];
   if (BIAS && a.dbias && w.live) {
 #pragma unroll
     for (int u = 0; u < 2; ++u)

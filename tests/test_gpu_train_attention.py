@@ -250,6 +250,17 @@ def test_rows_and_keys_in_one_launch(dev, batch, heads, kv_heads, q_len, k_len, 
             assert np.array_equal(c.backward(only=(n,))[n], every[n]), n
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("q_len,k_len,bias", [(1, 1, None), (7, 1, None), (64, 1, "random"),
+                                              (1, 64, None)])
+def test_a_query_of_one_key_has_gradients_of_exactly_0(dev, q_len, k_len, bias, dtype):
+    """p is 1 and delta the same dp: nothing is left of their difference."""
+    k_lengths = [1, 0, 1]
+    c = Case(dev, 3, 4, q_len, k_len, 32, dtype, bias=bias, k_lengths=k_lengths, seed=3)
+    got = c.check()
+    assert not any(got[n].any() for n in got if n != "dv") and got["dv"].any()
+
+
 def test_a_bias_shared_by_queries(dev):
     c = Case(dev, 2, 2, 20, 70, 16, "f32", bias="random", shared=(2,))
     (q, k, v), rest = c.oracle()
