@@ -229,6 +229,23 @@ struct Args {
 
 __device__ __forceinline__ int Uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
+// Causal rows' tiles from the last to the first, in interleaved runs of tiles, one a
+// head where heads have tiles of their own.  More runs than tiles would launch workgroups
+// for nothing (1024 lines of one query of 128 heads over one key head, 64 keys of 64, bf16:
+// 128 a line, 76 us and backward 158; so 2, 11.7 and 46).  The tile at place `at`; behind
+// the last tile there is none.
+inline int RunsDown(int tiles, int heads) {
+  const int each = (tiles + heads - 1) / heads;
+  return each > 0 ? (tiles + each - 1) / each : 0;
+}
+inline int PlacesDown(int tiles, int runs) {
+  return runs ? (tiles + runs - 1) / runs * runs : tiles;
+}
+__host__ __device__ inline int TileDown(int at, int tiles, int runs) {
+  const int each = (tiles + runs - 1) / runs;
+  return at % runs * each + (each - 1 - at / runs);
+}
+
 // Which part a workgroup does.  Workgroups go round the eight dies by their
 // number, and round a die's CUs.  Without splits blockIdx.x is the line and y the
 // tile; with many lines (spread) x is a multiple of eight, so that the parts of one
@@ -268,10 +285,8 @@ __device__ __forceinline__ bool PartOf(const Args &s, int x, int across, int dow
     const unsigned aside = (static_cast<unsigned>(y) * s.lines_now >> 8) * (s.a.kv_heads + 1);
     line = static_cast<int>((line + y + aside) % static_cast<unsigned>(s.lines_now));
   }
-  if (s.down) {
-    const int each = (s.tiles + s.down - 1) / s.down;
-    tile = tile % s.down * each + (each - 1 - tile / s.down);
-  }
+  if (s.down)
+    tile = TileDown(tile, s.tiles, s.down);
   p->line = s.line0 + line;
   p->tile = tile;
   return mine && tile < s.tiles;
@@ -1560,7 +1575,7 @@ inline Args ArgsOf(const TrainAttention &a, bool keys) {
   s.steps = keys ? Tiles(s.rows) : Tiles(a.k_len);
   s.splits = SplitsOf(static_cast<std::int64_t>(s.lines) * s.tiles, s.steps);
   if (!keys && a.causal)
-    s.down = a.group;
+    s.down = RunsDown(s.tiles, s.a.group);
   return s;
 }
 // Whether the bias is shared by lines or heads.
@@ -1602,8 +1617,7 @@ template <class K> hipError_t Run(K kernel, Args s, hipStream_t stream) {
                        s);
     return hipGetLastError();
   }
-  const std::int64_t tiles =
-      s.down ? static_cast<std::int64_t>((s.tiles + s.down - 1) / s.down) * s.down : s.tiles;
+  const std::int64_t tiles = PlacesDown(s.tiles, s.down);
   const std::int64_t most_tiles = std::min<std::int64_t>(tiles, 65535);
   const std::int64_t most_lines = std::max<std::int64_t>(8, kMostGroups / most_tiles / 8 * 8);
   hipError_t e = hipSuccess;
@@ -1635,8 +1649,7 @@ inline std::int64_t GroupsOf(Args *s) {
   s->spread = s->lines >= 64;
   s->turn = ragged && !s->spread;
   s->across = s->spread ? (s->lines + 7) / 8 * 8 : s->lines;
-  const int tiles = s->down ? (s->tiles + s->down - 1) / s->down * s->down : s->tiles;
-  return static_cast<std::int64_t>(s->across) * tiles;
+  return static_cast<std::int64_t>(s->across) * PlacesDown(s->tiles, s->down);
 }
 // Whether a backward pass does rows and keys in one launch: the one's last workgroups
 // run beside the other's, and a launch is saved.  bf16, causal: 1 x 4 over 4096 tokens of
@@ -1670,6 +1683,7 @@ hipError_t Forward(const TrainAttention &a, hipStream_t stream) {
   if (s.steps <= 1) {
     s.wide = 1;
     s.tiles = Tiles(s.rows);
+    s.down = s.down ? RunsDown(s.tiles, a.group) : 0;
     e = Run(ForwardKernel<DT, DP, 1, BIAS, true>, s, stream);
   } else if (s.wide == 2) {
     e = Run(ForwardKernel<DT, DP, kWide, BIAS, false>, s, stream);
