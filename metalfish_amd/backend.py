@@ -774,12 +774,21 @@ class GradSet:
                                           stream), "mfh_grad_clip_device")
 
 
+def _int32(**values):
+    """Refuses what a 32-bit field would cut off: ctypes keeps the low bits."""
+    for name, v in values.items():
+        if not -2 ** 31 <= v < 2 ** 31:
+            raise ValueError(f"{name} must fit 32 bits")
+
+
 def norm_rows(d_x, rows, width, dtype="f32", x_stride=None, d_residual=None,
               residual_stride=None, alpha=1.0, d_gamma=None, d_beta=None, eps=1e-3, device=-1):
     """Rows h = residual + alpha x in device memory for the layer norms below:
     [rows, width] of ``dtype`` "f32", "bf16" or "f16", strides in elements
     (``width``); ``d_gamma`` and ``d_beta`` float32 [width], None for 1 and 0.
     Holds addresses only."""
+    if (width | device + 1) >> 31:
+        _int32(width=width, device=device)
     return MfhNormRows(d_x, width if x_stride is None else x_stride, d_residual,
                        width if residual_stride is None else residual_stride, rows, width,
                        DTYPE[dtype], alpha, eps, d_gamma, d_beta, device)
@@ -795,6 +804,7 @@ def layer_norm_device(rows, d_y, y_stride=None, d_mean=None, d_rstd=None, stream
 
 def layer_norm_workspace_bytes(rows: int, width: int) -> int:
     """Bytes of device memory a layer norm's backward pass works in."""
+    _int32(width=width)
     n = ctypes.c_uint64(0)
     _check(lib().mfh_layer_norm_workspace_bytes(rows, width, ctypes.byref(n)),
            "mfh_layer_norm_workspace_bytes")
@@ -834,9 +844,14 @@ def attention_problem(d_q, d_k, d_v, batch, heads, q_len, k_len, dim, dtype="f32
     q_len, k_len].  ``scale`` defaults to 1 / sqrt(dim); ``causal``: the last
     query sees the last key; lengths int32 [batch].  Holds addresses only."""
     kv = heads if kv_heads is None else kv_heads
+    if (batch | heads | kv | q_len | k_len | dim | device + 1) >> 31:
+        _int32(batch=batch, heads=heads, kv_heads=kv, q_len=q_len, k_len=k_len, dim=dim,
+               device=device)
+    if scale is None:
+        scale = dim ** -0.5 if dim > 0 else 1.0  # the call refuses such a dim
     bias = (heads * q_len * k_len, q_len * k_len, k_len) if bias_strides is None else bias_strides
     return MfhAttention(batch, heads, kv, q_len, k_len, dim, DTYPE[dtype], 1 if causal else 0,
-                        dim ** -0.5 if scale is None else scale,
+                        scale,
                         _heads(d_q, q_strides, q_len, heads, dim),
                         _heads(d_k, k_strides, k_len, kv, dim),
                         _heads(d_v, v_strides, k_len, kv, dim), d_bias, DTYPE[bias_dtype], *bias,
