@@ -521,7 +521,8 @@ typedef struct {
  * `causal` j <= i + n - m, so the last query sees the last key.  What lies
  * behind a length is not read, and a bias of what a query does not see has no
  * effect, whatever it is.  A query that sees nothing (i >= m among them), or
- * only keys of bias -inf, has out 0, lse -inf, and gradients of 0.  The bias is
+ * only keys of bias -inf, has out 0, lse -inf, and gradients of 0, and a key behind
+ * its line's end gradients of 0, whatever the other values are.  The bias is
  * p[b * bias_batch + h * bias_head + i * bias_query + j]; a stride of 0 shares
  * it.  Scores, statistics and sums are in 32 bits; with bf16 or fp16 inputs the
  * probabilities and dS are rounded to that type before they are multiplied (in

@@ -791,6 +791,9 @@ __global__ __launch_bounds__(256, (kWaves<DT, DP>)) void ForwardKernel(Args s) {
       }
       continue;
     }
+    // A row that sees nothing has 0 times every value, which may be infinite.
+    if (total[n] == 0.f)
+      Fill(acc[n], DP / 16, 0.f);
     StoreHead<DT, DP>(Out<DT>(a.out, l.b, w[n].head, w[n].q), lane, a.dim, acc[n],
                       total[n] == 0.f ? 0.f : 1.f / total[n]);
     if (a.lse && g == 0)
@@ -836,7 +839,8 @@ __global__ __launch_bounds__(256) void JoinFewKernel(Args s) {
     }
   const int line = static_cast<int>(flat / s.rows), r = static_cast<int>(flat % s.rows);
   const int b = line / s.a.kv_heads, head = line % s.a.kv_heads * s.a.group + r / s.a.q_len;
-  ToMemory<DT>(Out<DT>(s.a.out, b, head, r % s.a.q_len) + 4 * c, o * (sum == 0.f ? 0.f : 1.f / sum));
+  ToMemory<DT>(Out<DT>(s.a.out, b, head, r % s.a.q_len) + 4 * c,
+               sum == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : o * (1.f / sum));
   if (s.a.lse && c == 0)
     s.a.lse[flat] = sum == 0.f ? -__builtin_inff() : top + kLn2 * __builtin_amdgcn_logf(sum);
 }
@@ -888,7 +892,7 @@ __global__ __launch_bounds__(256) void JoinForwardKernel(Args s) {
   const int line = static_cast<int>(flat / s.rows), r = static_cast<int>(flat % s.rows);
   const int b = line / s.a.kv_heads, head = line % s.a.kv_heads * s.a.group + r / s.a.q_len;
   ToMemory<DT>(Out<DT>(s.a.out, b, head, r % s.a.q_len) + 4 * k,
-               o * (total == 0.f ? 0.f : 1.f / total));
+               total == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : o * (1.f / total));
   if (s.a.lse && k == 0)
     s.a.lse[flat] = total == 0.f ? -__builtin_inff() : most + kLn2 * __builtin_amdgcn_logf(total);
 }
@@ -900,6 +904,9 @@ template <int BIAS> __device__ __forceinline__ float Lse(float v) {
     return __builtin_inff();
   return BIAS ? v : v * kLog2e;
 }
+// Such a row's gradients are stored as 0: 0 times a key or value that is not finite
+// is not.
+__device__ __forceinline__ bool SeesNothing(float lse) { return lse == __builtin_inff(); }
 // A row's probabilities from a bias as large as this are too coarse by its
 // log-sum-exp alone: ln(sum) is below a rounding of it, and where a mask of the
 // type's lowest value takes every key, each would have probability 1.  Such rows
@@ -1030,6 +1037,8 @@ __device__ __forceinline__ void BackwardRows(const Args &s, const Part &part,
         for (int e = 0; e < 4; ++e)
           x[n][t][e] = Probability<BIAS>(x[n][t][e], rest[n]) * dp[n][t][e];
       if (BIAS && a.dbias && w[n].live) {
+        if (SeesNothing(lse[n]))
+          Fill(x[n], 4, 0.f);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
           StoreBias8<BIAS>(a, bias_at[n], j0 + 32 * u, x[n] + 2 * u);
@@ -1055,6 +1064,8 @@ __device__ __forceinline__ void BackwardRows(const Args &s, const Part &part,
   for (int n = 0; n < N; ++n) {
     if (!w[n].live || !a.dq.p)
       continue;
+    if (SeesNothing(lse[n]))
+      Fill(acc[n], DP / 16, 0.f);
     if (s.splits > 1) {
       if (w[n].last < 0)
         continue;
@@ -1270,6 +1281,10 @@ __device__ __forceinline__ void BackwardKeys(const Args &s, const Part &part,
       StorePartial<DP>(o + all * s.a.dim, lane, s.a.dim, dv[n]);
       continue;
     }
+    if (j[n] >= l.k_len) {
+      Fill(dk[n], DP / 16, 0.f);
+      Fill(dv[n], DP / 16, 0.f);
+    }
     if (a.dk.p)
       StoreHead<DT, DP>(Out<DT>(a.dk, l.b, l.kv, j[n]), lane, a.dim, dk[n], a.scale);
     if (a.dv.p)
@@ -1430,6 +1445,8 @@ __global__ __launch_bounds__(256, 2) void SquareBackwardKernel(Args s) {
 #pragma unroll
   for (int t = 0; t < 4; ++t)
     dp[t] = (dp[t] - delta) * x[t];
+  if (SeesNothing(lse))
+    Fill(dp, 4, 0.f);
   if (BIAS && a.dbias && w.live) {
 #pragma unroll
     for (int u = 0; u < 2; ++u)
@@ -1447,6 +1464,8 @@ __global__ __launch_bounds__(256, 2) void SquareBackwardKernel(Args s) {
     for (int i = 0; i < DP / 16; ++i)
       acc[i] = M::Mul(HeadColumns<DT, DP, LD>(ks, 32 * u, i, lane), ds[u], acc[i]);
   }
+  if (SeesNothing(lse))
+    Fill(acc, DP / 16, 0.f);
   if (w.live && a.dq.p)
     StoreHead<DT, DP>(Out<DT>(a.dq, l.b, w.head, w.q), lane, a.dim, acc, a.scale);
   if (!a.dk.p && !a.dv.p)
@@ -1462,6 +1481,8 @@ __global__ __launch_bounds__(256, 2) void SquareBackwardKernel(Args s) {
       for (int i = 0; i < DP / 16; ++i)
         acc[i] = M::Mul(HeadColumns<DT, DP, LD>(tile, 32 * u, i, lane), p, acc[i]);
     }
+    if (mine >= l.k_len)
+      Fill(acc, DP / 16, 0.f);
     if (mine < a.k_len && out.p)
       StoreHead<DT, DP>(Out<DT>(out, l.b, l.kv, mine), lane, a.dim, acc, scale);
   };
@@ -1507,6 +1528,7 @@ __global__ __launch_bounds__(256) void BiasGradKernel(Args s, int plane_heads, s
       LoadRow<DT, DP>(s, a.dout, l, w, lane, df);
       const float lse = w.last >= 0 ? Lse<BIAS>(a.lse[flat]) : __builtin_inff();
       const float delta = w.last >= 0 ? s.delta[flat] : 0.f, rest = w.last >= 0 ? s.rest[flat] : 0.f;
+      const int last = SeesNothing(lse) ? -1 : w.last;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         f32x4 x{0.f, 0.f, 0.f, 0.f}, dp{-delta, -delta, -delta, -delta};
@@ -1522,7 +1544,7 @@ __global__ __launch_bounds__(256) void BiasGradKernel(Args s, int plane_heads, s
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float p = Probability<BIAS>(x[e] * a.scale + bias[t][e] - lse, rest);
-          acc[t][e] += j + e <= w.last ? p * dp[e] : 0.f;
+          acc[t][e] += j + e <= last ? p * dp[e] : 0.f;
         }
       }
     }
