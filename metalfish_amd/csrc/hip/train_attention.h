@@ -206,7 +206,6 @@ __device__ __forceinline__ float OverRows(float v, bool most) {
   return most ? fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]))
               : __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
-__device__ __forceinline__ float Exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // One launch's problem: a part of the work is (line and key head, tile, split
 // of the axis that it loops over).
