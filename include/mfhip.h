@@ -552,7 +552,8 @@ int mfh_attention_forward_device(const mfh_attention *a, const mfh_heads *out, f
                                  void *d_workspace, uint64_t workspace_bytes, void *stream);
 
 /* The gradients from dout and the forward pass's out and lse; with p_ij =
- * exp(s_ij - lse_i) formed again and dS_ij = p_ij (dout_i . v_j - dout_i . out_i):
+ * exp(s_ij - lse_i) formed again and dS_ij = p_ij (dout_i . v_j - delta_i), delta_i =
+ * dout_i . out_i = sum_j p_ij dout_i . v_j, taken from the one or the other:
  *   dq_i = scale sum_j dS_ij k_j,  dk_j = scale sum_i dS_ij q_i,
  *   dv_j = sum_i p_ij dout_i,      dbias_ij = dS_ij,
  * dk and dv summed over the heads that share them, dbias over what shares the
@@ -561,7 +562,7 @@ int mfh_attention_forward_device(const mfh_attention *a, const mfh_heads *out, f
  * be NULL (p of a mfh_heads).  No sum depends on the order in which the device
  * runs. */
 typedef struct {
-  mfh_heads out, dout; /* read */
+  mfh_heads out, dout; /* read (out not always, but it has to be given) */
   const float *d_lse;
   mfh_heads dq, dk, dv;
   void *d_dbias;

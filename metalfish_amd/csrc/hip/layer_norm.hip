@@ -7,8 +7,10 @@
 // Bound by memory: the forward pass reads x (and the residual) and writes y,
 // the backward pass reads dy, x (and the residual) and writes dx (and
 // dresidual); 16384 x 1024 with a residual: bf16 18.0 us (5.6 TB/s) and 38.8 (4.3
-// TB/s, the second kernel's 4.6 us with it), fp32 34.4 and 66.2.  A row is held in the registers of 16, 32, 64, 256 or 1024 lanes, so
-// every pass over it after the first costs no memory; the variance is summed
+// TB/s, the second kernel's 4.6 us with it), fp32 34.4 and 64.6.  A row of up to 32768
+// columns (16384 in the fp32 backward pass, MaxHeld) is held in the registers of 16,
+// 32, 64, 256 or 1024 lanes, so every pass over it after the first costs no memory, but
+// for the weights' gradients of rows above 8192 columns; the variance is summed
 // about the mean.  Workgroups loop over rows: gamma stays in registers, and in the
 // backward pass each lane sums dy n and dy of its own columns over all rows of
 // its workgroup.  Those partial sums (one row of 2 width a workgroup) are
@@ -532,8 +534,9 @@ __device__ __forceinline__ void LoadSum(const NormParams &p, std::int64_t row, i
   Sums<DT, 1>(p, &x, &r, h);
 }
 
-// Rows too long for registers, read three times by 1024 lanes: 300 x 40000 bf16 with a
-// residual 88 us, backward 120.
+// Rows too long for registers, read three times by 1024 lanes, a vector of a lane on
+// its way at a time, and the weights value by value once a row: 300 x 40000 bf16 with a
+// residual 88 us (0.8 TB/s), backward 120.
 template <int DT>
 __global__ __launch_bounds__(1024) void LongNormKernel(NormParams p) {
   constexpr int VE = Elem<DT>::kPerVec;
@@ -592,7 +595,8 @@ __device__ __forceinline__ void StoreGrads(const NormParams &p, std::int64_t row
   }
 }
 
-// Rows too long for registers: dh alone, read twice.
+// Rows too long for registers: dh alone, read twice.  1000 x 16385 fp32 with a residual
+// 138 us with the column sums; of 16384 columns, in registers, 90.
 template <int DT>
 __global__ __launch_bounds__(1024) void LongNormBackwardKernel(NormParams p) {
   constexpr int VE = Elem<DT>::kPerVec;
@@ -627,8 +631,8 @@ __global__ __launch_bounds__(1024) void LongNormBackwardKernel(NormParams p) {
   }
 }
 
-// The weights' partial sums of wide rows: 256 lanes take a vector of columns
-// each, a workgroup the rows blockIdx.y, blockIdx.y + gridDim.y, ...
+// The weights' partial sums of wide rows, which are read once more for them: 256
+// lanes take a vector of columns each, a workgroup the rows blockIdx.y, blockIdx.y + gridDim.y, ...
 template <int DT>
 __global__ __launch_bounds__(256) void ColumnSumsKernel(NormParams p) {
   constexpr int VE = Elem<DT>::kPerVec;

@@ -15,6 +15,12 @@
 // elements of a head.
 //
 // fp32 runs the same code on the 16 x 16 x 4 instruction, eight times.
+//
+// With 16-bit inputs probabilities and dS are rounded to the inputs' type where they
+// become operands (Mat::Pack): the instruction takes no wider ones beside them, and
+// the fp32 one has an eighth of the rate that products reach (154 of 1216 TFLOP/s).
+// That is at most 2^-8 (bf16) or 2^-11 (fp16) of each; scores, maxima, sums, delta and
+// every accumulator are fp32.
 #pragma once
 
 #include "learn_device.h"
@@ -682,8 +688,8 @@ template <int DT, int DP> constexpr int kWaves = DT == DT_F32 && DP == 128 ? 1 :
 // the running maximum and sum of its rows; out is scaled once at the end.  ONE: all
 // keys in one tile.  Squares are bound by memory (256 x 32 heads of 64 x 64 x 32, bf16
 // with a bias 43.7 us, 4.7 TB/s), long lines by LDS reads, exponentials and matrix
-// instructions together (4 x 32 x 2048 x 64 bf16 215 us, 639 TFLOP/s; causal 4 x 16 58.5,
-// 588; fp32, whose matrix instruction has a sixteenth of the rate, 95 TFLOP/s).
+// instructions together (4 x 32 x 2048 x 64 bf16 202 us, 681 TFLOP/s; causal 4 x 16 66,
+// 519; fp32, where products reach 154 TFLOP/s, 2 x 16 causal 184, 93).
 template <int DT, int DP, int N, int BIAS, bool ONE>
 __global__ __launch_bounds__(256, (kWaves<DT, DP>)) void ForwardKernel(Args s) {
   using M = Mat<DT>;
@@ -932,7 +938,7 @@ __device__ __forceinline__ float Delta(const typename Mat<DT>::Frag *out,
 
 // delta of each row, then dq (and dbias) of a tile of rows over the keys: three
 // products a step, and with the keys' kernel seven where five would do, but each sum
-// stays in the registers of one wave.  4 x 32 x 2048 x 64 bf16 570 us for both (603
+// stays in the registers of one wave.  4 x 32 x 2048 x 64 bf16 559 us for both (615
 // TFLOP/s of the five).
 template <int DT, int DP, int N, int BIAS>
 __device__ __forceinline__ void BackwardRows(const Args &s, const Part &part,
@@ -1360,8 +1366,11 @@ __global__ __launch_bounds__(256) void JoinBackwardKernel(Args s) {
 }
 
 // The whole backward pass of a head of up to 64 queries and 64 keys, none of
-// them shared: one workgroup, each input read once.  Bound by memory: 256 x 32 heads
-// of 32 elements, bf16 with a bias, 88.3 us (4.2 TB/s).  delta is the sum of p dp over
+// them shared: one workgroup, each input read once.  Bound by the latency of memory,
+// since a workgroup loads, waits, computes and stores once, with nothing of another
+// head on its way: 256 x 32 heads of 32 elements, bf16 with a bias, 88.3 us (4.2 TB/s,
+// the vector unit a third busy); 256 x 16 of 64 elements, whose rows are whole cache
+// lines, 72.6 (4.2 too).  delta is the sum of p dp over
 // the keys, which are all here: out is not read, and a query that sees one key has
 // gradients of exactly 0.  A wave has 16 queries while
 // scores, probabilities, dS and dq are formed, and 16 keys for dk and dv; P and
@@ -1494,7 +1503,10 @@ __global__ __launch_bounds__(256, 2) void SquareBackwardKernel(Args s) {
 }
 
 // The gradient of a bias that lines or heads share: a workgroup has 64 queries
-// and 64 keys of one of its planes and loops over what shares it.
+// and 64 keys of one of its planes and loops over what shares it, so a small plane
+// that much shares leaves most of the card idle: 256 x 32 heads of 64 x 64 x 32, bf16,
+// backward 741 us with a bias shared by the lines (32 workgroups of 256 rounds, 2.6 us
+// each) and 17400 shared by the heads too (one of 8192); 88 with one of its own.
 template <int DT, int DP, int BIAS>
 __global__ __launch_bounds__(256) void BiasGradKernel(Args s, int plane_heads, std::int64_t first) {
   using M = Mat<DT>;
